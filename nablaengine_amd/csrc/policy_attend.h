@@ -1,0 +1,141 @@
+// What the attention kernels share: the arguments, the packed sequences, the matrix instructions and the LDS tiles.
+//
+// Layouts. The matrix instruction v_mfma_f32_32x32x16 takes A (32 x 16) and B (16 x 32), lane l holding row (column)
+// l % 32 and the eight products k = 8 (l / 32) + 0..7, and gives C (32 x 32) with lane l holding column l % 32 and its
+// register r row r % 4 + 8 (r / 4) + 4 (l / 32). Every product here is arranged so that one product's C is the next
+// one's B as it stands: scores are computed transposed, S^T = K Q^T, so that a lane holds 16 keys of ONE query. Its
+// softmax needs no exchange but one with lane l ^ 32, a rescaling is a product with the lane's own number, and the 16
+// probabilities, packed to 16 bits, are the B operand of O^T = V^T P^T for two instructions, whose k then runs over the
+// keys in the order 4 h + {0..3}, 8 + 4 h + {0..3} (h = l / 32). The A operand follows the same order: it is read from
+// the row-major LDS tile with ds_read_b64_tr_b16, which gives each lane four consecutive rows of its column.
+#pragma once
+#include "policy_device.h"
+
+namespace pol {
+
+typedef float F16x __attribute__((ext_vector_type(16)));
+typedef short S4 __attribute__((ext_vector_type(4)));
+template <typename T> struct Frag { typedef T V8 __attribute__((ext_vector_type(8))); };
+template <typename T> using V8 = typename Frag<T>::V8;
+
+__device__ __forceinline__ F16x mfma(V8<__bf16> a, V8<__bf16> b, F16x c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ F16x mfma(V8<_Float16> a, V8<_Float16> b, F16x c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int QROWS = 128;  // query rows a workgroup: 32 a wave
+constexpr int KROWS = 128;  // keys a workgroup of the key gradients: 32 a wave
+constexpr int TILE = 64;    // rows of an LDS tile
+
+struct Attend {
+  const void *q, *k, *v;
+  long long q_t, q_h, k_t, k_h, v_t, v_h;  // elements from token to token, and from head to head
+  int heads, kv_heads, group, dim, seqs, tq, tk;
+  const int *starts_q, *starts_k;
+  float scale;
+  void* out;   // (tq, heads, dim)
+  float* lse;  // (heads, tq): log2 of the row's sum of exponentials, +inf for a row without keys; NULL: not kept
+  const int* order;
+  // the backward's
+  const void* dout;
+  long long do_t, do_h;
+  float* delta;  // (heads, tq): the row's dout . out
+  void *dq, *dk, *dv;
+};
+
+// The order: two lists of tiles, (sequence, tile of it), heaviest first: the query tiles (QROWS rows of a key/value
+// head's queries, row = token * group + head of the group) and the key tiles.
+constexpr int ORDER_HEAD = 16;  // ints before the lists: their lengths
+__host__ __device__ inline long long order_queries(int seqs, int tq, int group) {
+  return (long long)tq * group / QROWS + seqs + 1;
+}
+__host__ __device__ inline long long order_keys(int seqs, int tk) { return (long long)tk / KROWS + seqs + 1; }
+
+// Sequence s of the packed tokens [0, total): its first token and length, kept inside the tokens whatever `starts`
+// holds. Sequence `seqs` is what lies past the last one: its queries have no keys and its keys no queries.
+__device__ __forceinline__ void sequence(const int* starts, int s, int seqs, int total, int& first, int& length) {
+  auto in = [&](int x) { return x < 0 ? 0 : x > total ? total : x; };
+  first = s == 0 ? 0 : in(starts[s]);
+  const int end = s == seqs ? total : in(starts[s + 1]);
+  length = end > first ? end - first : 0;
+}
+
+// An LDS tile of TILE rows of DP elements in 16-byte chunks. Chunk c of row r lies at chunk c ^ swizzle(r), so that
+// both reads are free of bank conflicts: 16 rows of one chunk (A operands, 16 bytes a lane) and 4 rows of 4 chunks
+// (transposed reads, 8 bytes a lane, 32 lanes at a time). A row of 64 elements is half of the 64 banks, one of 128 all.
+template <int DP>
+__device__ __forceinline__ int swizzle(int r) {
+  if constexpr (DP == 64) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
+  else return (r & 3) << 2 | ((r >> 2) & 3);
+}
+template <int DP>
+__device__ __forceinline__ int chunk_at(int r, int c) { return r * DP + ((c ^ swizzle<DP>(r)) << 3); }
+
+// rows of A (row n of the 32 from r0, products 16 s + 8 h ..)
+template <int DP, typename T>
+__device__ __forceinline__ V8<T> read_rows(const T* tile, int r0, int s, int n, int h) {
+  return *(const V8<T>*)(tile + chunk_at<DP>(r0 + n, 2 * s + h));
+}
+// columns 32 t + l % 32 as rows of A, products over the tile's rows r0 + 4 h + {0..3}, r0 + 8 + 4 h + {0..3}
+template <int DP, typename T>
+__device__ __forceinline__ V8<T> read_columns(const T* tile, int r0, int t, int l) {
+  typedef __attribute__((address_space(3))) S4 L4;
+  const int r = r0 + 4 * (l >> 5) + ((l & 15) >> 2), d = 32 * t + (l & 16) + 4 * (l & 3);
+  const S4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L4*)(tile + chunk_at<DP>(r, d >> 3) + (d & 7)));
+  const S4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L4*)(tile + chunk_at<DP>(r + 8, d >> 3) + (d & 7)));
+  typedef short S8 __attribute__((ext_vector_type(8)));
+  const S8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(V8<T>, both);
+}
+// registers 8 s .. 8 s + 7 of a C, packed: products k of B
+template <typename T>
+__device__ __forceinline__ V8<T> pack(const F16x& c, int s) {
+  V8<T> r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = (T)c[8 * s + j];
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ V8<T> zero8() { return V8<T>{}; }
+
+template <typename T>
+__device__ __forceinline__ V8<T> load8(const T* p) {
+  V8<T> r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+
+// 32 rows' B operands straight from memory: lane's row p (NULL: none), products 16 s + 8 h ..
+template <int DP, typename T>
+__device__ __forceinline__ void load_rows(const T* p, int dim, int h, V8<T>* f) {
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int d = 16 * s + 8 * h;
+    f[s] = p && d < dim ? load8(p + d) : zero8<T>();
+  }
+}
+
+// A C of columns = rows of a result (transposed result), d = 32 t + register's row, to p (NULL: none), times f
+template <int DP, typename T>
+__device__ __forceinline__ void store_rows(T* p, int dim, int h, const F16x* acc, float f) {
+  if (!p) return;
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = 32 * t + 8 * j + 4 * h;
+      if (d < dim) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (T)(acc[t][4 * j + e] * f);
+        __builtin_memcpy(p + d, &o, 8);
+      }
+    }
+}
+
+}  // namespace pol

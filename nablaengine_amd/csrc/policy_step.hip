@@ -1,0 +1,257 @@
+// Attention of one new query a world over that world's cached history: the control loop's form.
+//
+//   o = sum_j softmax_j(scale q . k_j) v_j over the world's first `length` cached tokens; zeros where there are none
+//
+// Memory bounds it: each cached key and value is read once, for all the query heads that share it. A workgroup takes
+// one world, one key/value head and one stretch of the history. A key's 16-byte chunks lie across LPR lanes, so that a
+// wave reads 64 / LPR keys at once in whole lines; the scores come from two-element dot products in 16 bits with
+// float32 sums and DPP adds over the LPR lanes, and each group of LPR lanes keeps its own running maximum, sum and
+// output in float32 over the keys it reads. The groups are joined at the end in registers and LDS, and stretches (long
+// histories of few worlds) by a second kernel in a fixed order.
+#include "../../include/nablaengine_policy.h"
+#include "policy_device.h"
+
+namespace pol {
+
+struct Step {
+  const void *q, *k, *v;
+  long long q_w, q_h, k_w, k_t, k_h, v_w, v_t, v_h;  // elements from world to world, token to token, head to head
+  int worlds, heads, kv_heads, group, dim, capacity;
+  const int* lengths;
+  float scale;
+  void* out;  // (worlds, heads, dim)
+  int stretches, stretch;
+  float* part;  // (stretches, worlds, heads, dim + 2): output sums, running maximum, sum
+};
+
+typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+typedef _Float16 H2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float dot2(const __bf16* a, const __bf16* b, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(*(const B2*)a, *(const B2*)b, c, false);
+}
+__device__ __forceinline__ float dot2(const _Float16* a, const _Float16* b, float c) {
+  return __builtin_amdgcn_fdot2(*(const H2*)a, *(const H2*)b, c, false);
+}
+
+constexpr float LOG2E_STEP = 1.4426950408889634f;
+constexpr int UNROLL = 4;
+
+template <typename T, int LPR, int GC>
+__global__ __launch_bounds__(256) void k_step(Step a) {
+  constexpr int RPW = 64 / LPR, ROWS = 4 * RPW * UNROLL;  // keys a wave reads at once; keys a turn of the workgroup
+  __shared__ float wm[4][GC], wl[4][GC];
+  __shared__ float wo[4][GC][LPR * 8];
+  const int chunks = (a.group + GC - 1) / GC;
+  int id = blockIdx.x;
+  const int g0 = id % chunks * GC;
+  id /= chunks;
+  const int kv = id % a.kv_heads;
+  id /= a.kv_heads;
+  const int stretch = id % a.stretches, world = id / a.stretches;
+  int length = a.lengths[world];
+  length = length < 0 ? 0 : length > a.capacity ? a.capacity : length;
+  const long long from = (long long)stretch * a.stretch, to = from + a.stretch;
+  const int begin = from < length ? (int)from : length, end = to < length ? (int)to : length;
+  const int l = threadIdx.x % 64, w = threadIdx.x / 64, part = l % LPR, rg = l / LPR, d0 = part * 8;
+  const bool in_row = d0 < a.dim;
+  const T* kp = (const T*)a.k + (long long)world * a.k_w + (long long)kv * a.k_h + d0;
+  const T* vp = (const T*)a.v + (long long)world * a.v_w + (long long)kv * a.v_h + d0;
+
+  Vec<T> q[GC];
+#pragma unroll
+  for (int g = 0; g < GC; ++g) {
+    q[g] = Vec<T>{};
+    if (in_row && g0 + g < a.group)
+      q[g] = load16((const T*)a.q + (long long)world * a.q_w + (long long)(kv * a.group + g0 + g) * a.q_h + d0);
+  }
+  const float c = a.scale * LOG2E_STEP;
+  float m[GC], sum[GC], o[GC][8];
+#pragma unroll
+  for (int g = 0; g < GC; ++g) {
+    m[g] = -INFINITY;
+    sum[g] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[g][e] = 0.0f;
+  }
+  for (int key0 = begin + w * RPW * UNROLL + rg; key0 - rg < end; key0 += ROWS) {
+    Vec<T> k[UNROLL], v[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const bool in = in_row && key0 + u * RPW < end;
+      k[u] = in ? load16(kp + (long long)(key0 + u * RPW) * a.k_t) : Vec<T>{};
+      v[u] = in ? load16(vp + (long long)(key0 + u * RPW) * a.v_t) : Vec<T>{};
+    }
+    float s[GC][UNROLL];
+#pragma unroll
+    for (int g = 0; g < GC; ++g) {
+      float top = m[g];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        float d = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) d = dot2(&q[g].v[e], &k[u].v[e], d);
+        d = sum_lanes<LPR>(d) * c;
+        s[g][u] = key0 + u * RPW < end ? d : -INFINITY;
+        top = fmaxf(top, s[g][u]);
+      }
+      const float base = top == -INFINITY ? 0.0f : top, f = exp2f(m[g] - base);
+      m[g] = top;
+      sum[g] *= f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[g][e] *= f;
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        s[g][u] = exp2f(s[g][u] - base);
+        sum[g] += s[g][u];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = (float)v[u].v[e];
+#pragma unroll
+        for (int g = 0; g < GC; ++g) o[g][e] += s[g][u] * x;
+      }
+  }
+  // join the row groups of the wave, then the waves
+#pragma unroll
+  for (int g = 0; g < GC; ++g) {
+    float top = m[g];
+#pragma unroll
+    for (int d = LPR; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    const float f = m[g] == -INFINITY ? 0.0f : exp2f(m[g] - top);
+    sum[g] *= f;
+#pragma unroll
+    for (int d = LPR; d < 64; d *= 2) sum[g] += __shfl_xor(sum[g], d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      o[g][e] *= f;
+#pragma unroll
+      for (int d = LPR; d < 64; d *= 2) o[g][e] += __shfl_xor(o[g][e], d);
+    }
+    if (rg == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wo[w][g][d0 + e] = o[g][e];
+      if (part == 0) {
+        wm[w][g] = top;
+        wl[w][g] = sum[g];
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < GC * LPR * 8; i += 256) {
+    const int g = i / (LPR * 8), d = i % (LPR * 8);
+    if (g0 + g >= a.group || d >= a.dim) continue;
+    const float top = fmaxf(fmaxf(wm[0][g], wm[1][g]), fmaxf(wm[2][g], wm[3][g]));
+    float total = 0.0f, x = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float f = wm[j][g] == -INFINITY ? 0.0f : exp2f(wm[j][g] - top);
+      total += f * wl[j][g];
+      x += f * wo[j][g][d];
+    }
+    const long long head = (long long)world * a.heads + kv * a.group + g0 + g;
+    if (a.stretches == 1) {
+      ((T*)a.out)[head * a.dim + d] = (T)(total == 0.0f ? 0.0f : x / total);
+    } else {
+      float* to_part = a.part + ((long long)stretch * a.worlds * a.heads + head) * (a.dim + 2);
+      to_part[d] = x;
+      if (d == 0) {
+        to_part[a.dim] = top;
+        to_part[a.dim + 1] = total;
+      }
+    }
+  }
+}
+
+// one wave a head: the stretches' sums, each scaled to the largest maximum, in their order
+template <typename T>
+__global__ __launch_bounds__(256) void k_step_join(Step a) {
+  const long long all = (long long)a.worlds * a.heads, head = blockIdx.x * 4LL + threadIdx.x / 64;
+  if (head >= all) return;
+  const int l = threadIdx.x % 64, n = a.dim + 2;
+  float top = -INFINITY;
+  for (int s = 0; s < a.stretches; ++s) top = fmaxf(top, a.part[(s * all + head) * n + a.dim]);
+  float total = 0.0f, x0 = 0.0f, x1 = 0.0f;
+  for (int s = 0; s < a.stretches; ++s) {
+    const float* p = a.part + (s * all + head) * n;
+    const float f = p[a.dim] == -INFINITY ? 0.0f : exp2f(p[a.dim] - top);
+    total += f * p[a.dim + 1];
+    if (l < a.dim) x0 += f * p[l];
+    if (l + 64 < a.dim) x1 += f * p[l + 64];
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  T* out = (T*)a.out + head * a.dim;
+  if (l < a.dim) out[l] = (T)(x0 * inv);
+  if (l + 64 < a.dim) out[l + 64] = (T)(x1 * inv);
+}
+
+// Stretches: enough workgroups for the 256 CUs where worlds and heads alone are too few, none under 256 keys.
+int step_heads_a_group(int group) { return group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8; }
+int step_stretches(int worlds, int kv_heads, int group, int capacity) {
+  const int gc = step_heads_a_group(group);
+  const long long blocks = (long long)worlds * kv_heads * ((group + gc - 1) / gc);
+  const long long want = (2048 + blocks - 1) / blocks, most = (capacity + 255) / 256;
+  const long long n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n);
+}
+size_t step_work_bytes(int worlds, int heads, int kv_heads, int dim, int capacity) {
+  if (worlds <= 0) return 0;
+  const int n = step_stretches(worlds, kv_heads, heads / kv_heads, capacity);
+  return n == 1 ? 0 : sizeof(float) * (size_t)n * worlds * heads * (dim + 2);
+}
+
+template <typename T, int LPR>
+int step(hipStream_t st, Step a) {
+  const int gc = step_heads_a_group(a.group);
+  const long long blocks = (long long)a.worlds * a.kv_heads * ((a.group + gc - 1) / gc) * a.stretches;
+  if (blocks >= 1LL << 24) return (int)hipErrorInvalidValue;
+  switch (gc) {
+    case 1: k_step<T, LPR, 1><<<(unsigned)blocks, 256, 0, st>>>(a); break;
+    case 2: k_step<T, LPR, 2><<<(unsigned)blocks, 256, 0, st>>>(a); break;
+    case 4: k_step<T, LPR, 4><<<(unsigned)blocks, 256, 0, st>>>(a); break;
+    default: k_step<T, LPR, 8><<<(unsigned)blocks, 256, 0, st>>>(a);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.stretches == 1) return (int)e;
+  k_step_join<T><<<(unsigned)(((long long)a.worlds * a.heads + 3) / 4), 256, 0, st>>>(a);
+  return (int)hipGetLastError();
+}
+
+int launch_step(hipStream_t st, int type, Step a) {
+  a.stretches = step_stretches(a.worlds, a.kv_heads, a.group, a.capacity);
+  a.stretch = (a.capacity + a.stretches - 1) / a.stretches;
+  if (type == BF16) return a.dim <= 64 ? step<__bf16, 8>(st, a) : step<__bf16, 16>(st, a);
+  return a.dim <= 64 ? step<_Float16, 8>(st, a) : step<_Float16, 16>(st, a);
+}
+
+}  // namespace pol
+
+extern "C" {
+
+int dk_attention_step(hipStream_t st, int type, int worlds, int heads, int kv_heads, int dim, int capacity,
+                      const void* q, long long q_w, long long q_h, const void* k, long long k_w, long long k_t,
+                      long long k_h, const void* v, long long v_w, long long v_t, long long v_h, const int* lengths,
+                      float scale, void* out, void* work) {
+  if ((type != pol::BF16 && type != pol::F16) || worlds < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 8 ||
+      dim > 128 || dim % 8 || capacity < 0 || capacity >= 1 << 30 || !(scale > 0.0f))
+    return (int)hipErrorInvalidValue;
+  if (worlds == 0) return 0;
+  if (!q || !lengths || !out || (capacity && (!k || !v)) ||
+      (!work && pol::step_work_bytes(worlds, heads, kv_heads, dim, capacity)))
+    return (int)hipErrorInvalidValue;
+  pol::Step a = {};
+  a.q = q, a.k = k, a.v = v, a.q_w = q_w, a.q_h = q_h;
+  a.k_w = k_w, a.k_t = k_t, a.k_h = k_h, a.v_w = v_w, a.v_t = v_t, a.v_h = v_h;
+  a.worlds = worlds, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim;
+  a.capacity = capacity, a.lengths = lengths, a.scale = scale, a.out = out, a.part = (float*)work;
+  return pol::launch_step(st, type, a);
+}
+
+long long dk_attention_step_work_bytes(int worlds, int heads, int kv_heads, int dim, int capacity) {
+  if (worlds < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 1 || capacity < 0) return 0;
+  return (long long)pol::step_work_bytes(worlds, heads, kv_heads, dim, capacity);
+}
+
+}  // extern "C"

@@ -105,6 +105,17 @@ _PROTOTYPES = {
     "dk_torch_diag_bwd": "i:ppi" + "p" * 6,
     "dk_prof_read": "i:pi",
     "dk_prof_read_adj": "i:pi",
+    # the policy operators (policy.py)
+    "dk_layer_norm": "i:pqiipqippfpp",
+    "dk_layer_norm_vjp": "i:pqiipqpqi" + "p" * 6,
+    "dk_layer_norm_work_bytes": "q:qii",
+    "dk_clip": "i:pi" + "p" * 5 + "fpp",
+    "dk_clip_work_bytes": "q:i",
+    "dk_attention": "i:piiiiiii" + "pqq" * 3 + "ppfppp",
+    "dk_attention_vjp": "i:piiiiiii" + "pqq" * 3 + "ppfppp" + "pqq" + "pppp",
+    "dk_attention_work_bytes": "q:iiiii",
+    "dk_attention_step": "i:piiiiii" + "pqq" + "pqqq" * 2 + "pfpp",
+    "dk_attention_step_work_bytes": "q:iiiii",
 }
 _CTYPE = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float, "q": ctypes.c_longlong, "-": None}
 

@@ -1,0 +1,102 @@
+"""The policy operators without a GPU: the library exports every entry of include/nablaengine_policy.h, the C entries
+refuse bad arguments before any launch, the Python calls refuse what is not on a ROCm device, and the operators' fake
+implementations give the library's output shapes and types."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+from nablaengine_amd import policy, torch_ffi
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "nablaengine_policy.h")
+
+
+def _prototypes():
+    """{name: result and arguments, one letter a value} of the header's declarations."""
+    txt = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    letter = lambda a: "p" if "*" in a or "hipStream_t" in a else {"long long": "q", "int": "i", "float": "f"}[  # noqa: E731
+        a.rsplit(" ", 1)[0]]
+    return {m[2]: {"long long": "q", "int": "i"}[m[1]] + ":" + "".join(letter(" ".join(a.split())) for a in m[3].split(","))
+            for m in re.finditer(r"(long long|int) (dk_\w+)\(([^;]*?)\);", txt, re.S)}
+
+
+def test_bindings_are_the_headers():
+    protos = _prototypes()
+    assert len(protos) == 10
+    for name, proto in protos.items():
+        assert torch_ffi._PROTOTYPES[name] == proto, name
+    dll = torch_ffi.load_library()
+    for name in protos:
+        assert hasattr(dll, name)
+
+
+def test_c_entries_refuse_before_any_launch():
+    dll = torch_ffi.load_library()
+    X = 0x1000  # never dereferenced
+    norm = lambda rows=3, n=8, t=0, wt=0, x=X, y=X: dll.dk_layer_norm(None, rows, n, t, x, n, wt, None, None, 1e-5, y, None)  # noqa: E731
+    assert norm(rows=0) == 0
+    assert norm(rows=-1) == norm(n=0) == norm(t=3) == norm(t=1, wt=2) == norm(x=None) == norm(y=None) == 1
+    vjp = lambda rows=3, n=8, t=0, stats=X, dw=X, work=X: dll.dk_layer_norm_vjp(  # noqa: E731
+        None, rows, n, t, X, n, X, n, 0, None, stats, None, dw, None, work)
+    assert vjp(rows=-1) == vjp(n=0) == vjp(t=-1) == vjp(stats=None) == vjp(work=None) == 1
+    assert dll.dk_layer_norm_work_bytes(0, 8, 0) == 0 and dll.dk_layer_norm_work_bytes(3, 8, 0) >= 2 * 8 * 4
+
+    def clip(n=(5,), types=(0,), outs=(0,), g=X, norm=X, work=X, out=X):
+        k = len(n)
+        ptr = (ctypes.c_void_p * k)(*[g] * k)
+        return dll.dk_clip(None, k, ptr, (ctypes.c_longlong * k)(*n), (ctypes.c_int * k)(*types),
+                           (ctypes.c_void_p * k)(*[out] * k), (ctypes.c_int * k)(*outs), 1.0, norm, work)
+    assert clip(n=(-1,)) == clip(types=(3,)) == clip(outs=(1,)) == clip(g=None) == clip(norm=None) == clip(work=None) == 1
+    assert clip(out=None) == clip(n=(5, 5), types=(1, 1), outs=(1, 2)) == 1
+    assert dll.dk_clip(None, -1, None, None, None, None, None, 1.0, X, X) == 1
+
+    def attention(t=1, heads=4, kv=2, dim=64, seqs=1, tq=5, tk=5, q=X, starts=X, scale=0.1, work=X):
+        return dll.dk_attention(None, t, heads, kv, dim, seqs, tq, tk, q, 1, 1, X, 1, 1, X, 1, 1, starts, X, scale, X, None, work)
+    for bad in (dict(t=0), dict(heads=3), dict(kv=0), dict(dim=7), dict(dim=136), dict(seqs=-1), dict(tq=-1), dict(tk=1 << 30),
+                dict(tq=1 << 29), dict(q=None), dict(starts=None), dict(scale=0.0), dict(scale=float("nan")), dict(work=None)):
+        assert attention(**bad) == 1, bad
+    assert dll.dk_attention_work_bytes(4, 2, 1, 5, 5) > 0
+
+    def step(t=1, worlds=2, heads=4, kv=2, dim=64, cap=9, q=X, lengths=X, scale=0.1, work=X):
+        return dll.dk_attention_step(None, t, worlds, heads, kv, dim, cap, q, 1, 1, X, 1, 1, 1, X, 1, 1, 1, lengths, scale, X, work)
+    assert step(worlds=0) == 0
+    for bad in (dict(t=0), dict(worlds=-1), dict(heads=3), dict(dim=9), dict(cap=-1), dict(q=None), dict(lengths=None),
+                dict(scale=-1.0), dict(cap=100000, work=None)):
+        assert step(**bad) == 1, bad
+
+
+def test_no_cpu_path():
+    x = torch.randn(3, 8)
+    a = torch.tensor([0, 3], dtype=torch.int32)
+    h = torch.randn(3, 2, 8).bfloat16()
+    for call in (lambda: policy.layer_norm(x), lambda: policy.layer_norm(x.requires_grad_()), lambda: policy.grad_norm([a.float()]),
+                 lambda: policy.clip_grads_([a.float()], 1.0), lambda: policy.attention(h, h, h, a),
+                 lambda: policy.attention_step(h, h[:, None], h[:, None], a[:1]), lambda: policy.layer_norm(None),
+                 lambda: policy.grad_norm([None]), lambda: policy.attention(None, h, h, a)):
+        with pytest.raises(TypeError):
+            call()
+    for eps in (-1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            policy.layer_norm(x, eps=eps)
+
+
+def test_fake_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = policy._ops()
+    with FakeTensorMode():
+        x, w = torch.empty((4, 5, 9), dtype=torch.bfloat16), torch.empty(9)
+        y, stats = ops.layer_norm(x, w, None, 1e-5, True)
+        assert y.shape == x.shape and y.dtype == x.dtype and stats.shape == (2, 20) and stats.dtype == torch.float32
+        assert ops.layer_norm(x, w, None, 1e-5, False)[1].shape == (2, 0)
+        dx, dw, db = ops.layer_norm_backward(x, x, w, None, stats, True, True, False)
+        assert dx.shape == x.shape and dw.shape == (9,) and dw.dtype == torch.float32 and db.shape == (0,)
+        assert ops.grad_norm([x, w]).shape == () and ops.clip_grads_out([x], [x.float()], 1.0).dtype == torch.float32
+        q, k = torch.empty((7, 4, 64), dtype=torch.float16), torch.empty((9, 2, 64), dtype=torch.float16)
+        a = torch.empty(4, dtype=torch.int32)
+        out, lse, work = ops.attention(q, k, k, a, a, 0.125, True)
+        assert out.shape == q.shape and lse.shape == (4, 7) and work.dtype == torch.int32
+        assert [t.shape for t in ops.attention_backward(q, q, k, k, a, a, out, lse, work, 0.125)] == [q.shape, k.shape, k.shape]
+        assert ops.attention_step(q, k[:7, None], k[:7, None], a, 0.125).shape == q.shape
