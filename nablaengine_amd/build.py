@@ -1,5 +1,6 @@
 """Build the HIP library libnablaengine_g1.so in-tree for gfx950 (hipcc; one shared library, the C ABI of
-include/nablaengine_g1.h). `python -m nablaengine_amd.build`."""
+include/nablaengine_g1.h and nablaengine_policy.h), and beside it the policy operators' torch side (g++).
+`python -m nablaengine_amd.build`."""
 import os
 import subprocess
 import sys
@@ -9,6 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libnablaengine_g1.so")
 PROF_LIB = os.path.join(HERE, "libnablaengine_g1_prof.so")
+TORCH_LIB, TORCH_SOURCE = os.path.join(HERE, "libnablaengine_policy_torch.so"), "policy_torch.cpp"
 SOURCES = ["g1_forward.hip", "g1_adjoint.hip", "g1_order.hip", "g1_kinematics.hip", "g1_diag.hip", "g1_capi.hip",
            "policy_norm.hip", "policy_clip.hip", "policy_attend.hip", "policy_step.hip"]
 ARCH = os.environ.get("NABLA_OFFLOAD_ARCH", "gfx950")
@@ -20,6 +22,27 @@ FLAGS = ["-O3", f"--offload-arch={ARCH}", "-std=c++17", "-fPIC", "-shared", "-Xc
          "-packed-fp32-ops", "-ffp-contract=fast", "-mllvm", "-disable-machine-licm",
          "-Wno-unused-command-line-argument", "-Werror=return-type",
          "-Werror=uninitialized", "-Werror=sometimes-uninitialized", "-Werror=array-bounds"]
+
+
+def build_torch(verbose=False):
+    """Compile the policy operators' torch side (C++, no device code) into TORCH_LIB."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    fd, tmp = tempfile.mkstemp(prefix="libnablaengine_policy_torch.", suffix=".so.tmp", dir=HERE)
+    os.close(fd)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-Wall", "-Wno-sign-compare"]
+    cmd += [f"-I{p}" for p in include_paths()] + ["-I/opt/rocm/include", "-o", tmp, os.path.join(CSRC, TORCH_SOURCE)]
+    cmd += [f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}", "-lc10", "-ltorch_cpu", "-lc10_hip", "-lamdhip64"]
+    if verbose:
+        print(" ".join(cmd))
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        os.unlink(tmp)
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError(f"g++ failed ({r.returncode})")
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
 
 
 def build(verbose=False, profile=False):
@@ -44,3 +67,4 @@ def build(verbose=False, profile=False):
 
 if __name__ == "__main__":
     print(build(verbose=True, profile="--profile" in sys.argv))
+    print(build_torch(verbose=True))

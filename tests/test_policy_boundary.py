@@ -88,15 +88,16 @@ def test_fake_shapes():
     ops = policy._ops()
     with FakeTensorMode():
         x, w = torch.empty((4, 5, 9), dtype=torch.bfloat16), torch.empty(9)
-        y, stats = ops.layer_norm(x, w, None, 1e-5, True)
+        assert ops.layer_norm(x, w, None, 1e-5).shape == x.shape
+        y, stats = ops.layer_norm_forward(x, w, None, 1e-5, True)
         assert y.shape == x.shape and y.dtype == x.dtype and stats.shape == (2, 20) and stats.dtype == torch.float32
-        assert ops.layer_norm(x, w, None, 1e-5, False)[1].shape == (2, 0)
+        assert ops.layer_norm_forward(x, w, None, 1e-5, False)[1].shape == (2, 0)
         dx, dw, db = ops.layer_norm_backward(x, x, w, None, stats, True, True, False)
         assert dx.shape == x.shape and dw.shape == (9,) and dw.dtype == torch.float32 and db.shape == (0,)
         assert ops.grad_norm([x, w]).shape == () and ops.clip_grads_out([x], [x.float()], 1.0).dtype == torch.float32
         q, k = torch.empty((7, 4, 64), dtype=torch.float16), torch.empty((9, 2, 64), dtype=torch.float16)
         a = torch.empty(4, dtype=torch.int32)
-        out, lse, work = ops.attention(q, k, k, a, a, 0.125, True)
+        out, lse, work = ops.attention_forward(q, k, k, a, a, 0.125, True)
         assert out.shape == q.shape and lse.shape == (4, 7) and work.dtype == torch.int32
         assert [t.shape for t in ops.attention_backward(q, q, k, k, a, a, out, lse, work, 0.125)] == [q.shape, k.shape, k.shape]
         assert ops.attention_step(q, k[:7, None], k[:7, None], a, 0.125).shape == q.shape
