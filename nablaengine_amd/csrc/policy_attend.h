@@ -27,13 +27,13 @@ __device__ __forceinline__ F16x mfma(V8<_Float16> a, V8<_Float16> b, F16x c) {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int QROWS = 128;  // query rows a workgroup: 32 a wave
-constexpr int KROWS = 128;  // keys a workgroup of the key gradients: 32 a wave
-constexpr int TILE = 64;    // rows of an LDS tile
+constexpr int TILE = 64;    // keys of an LDS tile of the forward and the queries' gradient
 
 struct Attend {
   const void *q, *k, *v;
   long long q_t, q_h, k_t, k_h, v_t, v_h;  // elements from token to token, and from head to head
   int heads, kv_heads, group, dim, seqs, tq, tk;
+  int key_waves;  // waves of a workgroup of the keys' gradients that differ in their 32 keys: 1, 2 or 4
   const int *starts_q, *starts_k;
   float scale;
   void* out;   // (tq, heads, dim)
@@ -47,12 +47,14 @@ struct Attend {
 };
 
 // The order: two lists of tiles, (sequence, tile of it), heaviest first: the query tiles (QROWS rows of a key/value
-// head's queries, row = token * group + head of the group) and the key tiles.
+// head's queries, row = token * group + head of the group) and the key tiles (32 * key_waves keys).
 constexpr int ORDER_HEAD = 16;  // ints before the lists: their lengths
 __host__ __device__ inline long long order_queries(int seqs, int tq, int group) {
   return (long long)tq * group / QROWS + seqs + 1;
 }
-__host__ __device__ inline long long order_keys(int seqs, int tk) { return (long long)tk / KROWS + seqs + 1; }
+__host__ __device__ inline long long order_keys(int seqs, int tk, int key_waves) {
+  return (long long)tk / (32 * key_waves) + seqs + 1;
+}
 
 // Sequence s of the packed tokens [0, total): its first token and length, kept inside the tokens whatever `starts`
 // holds. Sequence `seqs` is what lies past the last one: its queries have no keys and its keys no queries.
@@ -93,11 +95,25 @@ __device__ __forceinline__ V8<T> read_columns(const T* tile, int r0, int t, int 
 // registers 8 s .. 8 s + 7 of a C, packed: products k of B
 template <typename T>
 __device__ __forceinline__ V8<T> pack(const F16x& c, int s) {
-  V8<T> r;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) r[j] = (T)c[8 * s + j];
-  return r;
+  typedef float F8 __attribute__((ext_vector_type(8)));
+  const F8 f = s ? __builtin_shufflevector(c, c, 8, 9, 10, 11, 12, 13, 14, 15) : __builtin_shufflevector(c, c, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_convertvector(f, V8<T>);
 }
+
+// 2^x in one instruction: results below 2^-126 become 0, which a sum of exponentials up to 1 does not notice
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A tile on its way from memory to LDS without passing registers: each lane gives the address of its 16 bytes, which
+// land lane after lane; a lane without any gives that of zeros. All of a wave's are there after loads_done().
+__device__ __align__(16) const unsigned no_row[4] = {0, 0, 0, 0};
+template <typename T>
+__device__ __forceinline__ void to_lds(const T* from, bool valid, T* wave_at) {
+  typedef __attribute__((address_space(1))) const void* G;
+  typedef __attribute__((address_space(3))) void* L;
+  const T* p = valid ? from : (const T*)no_row;
+  __builtin_amdgcn_global_load_lds((G)p, (L)wave_at, 16, 0, 0);
+}
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
 template <typename T>
 __device__ __forceinline__ V8<T> zero8() { return V8<T>{}; }

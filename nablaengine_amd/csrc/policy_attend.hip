@@ -14,7 +14,8 @@ namespace pol {
 
 // One workgroup lists the tiles, heaviest first (a counting sort by the tiles of the other side that each one reads;
 // its place among equals is free, results do not depend on the order). seqs + 1 sequences, LS lanes on each.
-__global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk, int group, const int* __restrict__ starts_q,
+__global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk, int group, int key_waves,
+                                                       const int* __restrict__ starts_q,
                                                        const int* __restrict__ starts_k, int* __restrict__ order) {
   constexpr int BUCKETS = 1024;
   __shared__ int count[BUCKETS];
@@ -22,7 +23,8 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   int ls = 1;
   while (ls < 1024 && ls * 2 * (long long)(seqs + 1) <= 1024) ls *= 2;
   const int lane = threadIdx.x % ls, first_seq = threadIdx.x / ls, stride = 1024 / ls;
-  const long long caps[2] = {order_queries(seqs, tq, group), order_keys(seqs, tk)};
+  const int keys_a_tile = 32 * key_waves;
+  const long long caps[2] = {order_queries(seqs, tq, group), order_keys(seqs, tk, key_waves)};
   int* list = order + ORDER_HEAD;
   for (int which = 0; which < 2; ++which) {
     auto each_tile = [&](auto f) {
@@ -31,11 +33,11 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
         sequence(starts_q, s, seqs, tq, q0, nq);
         sequence(starts_k, s, seqs, tk, k0, nk);
         if (s == seqs) (which ? nq : nk) = 0;
-        const int rows = which ? nk : nq * group, per = which ? KROWS : QROWS, tiles = (rows + per - 1) / per;
+        const int rows = which ? nk : nq * group, per = which ? keys_a_tile : QROWS, tiles = (rows + per - 1) / per;
         for (int t = lane; t < tiles; t += ls) {
           int cost;
           if (which) {  // the query rows that see the tile's first key
-            const int from = t * KROWS - (nk - nq);
+            const int from = t * keys_a_tile - (nk - nq);
             cost = nq - (from > 0 ? from : 0);
             cost = (int)(((long long)(cost > 0 ? cost : 0) * group + TILE - 1) / TILE);
           } else {  // the keys that the tile's last row sees
@@ -84,38 +86,68 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
 struct Place {
   int tile, kv, q0, nq, k0, nk;
 };
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ bool place(const Attend& a, int which, Place& p) {
   const int entry = blockIdx.x / a.kv_heads;
-  if (entry >= a.order[which]) return false;
+  if (entry >= uniform(a.order[which])) return false;
   const int* list = a.order + ORDER_HEAD + (which ? 2 * order_queries(a.seqs, a.tq, a.group) : 0) + 2LL * entry;
-  const int s = list[0];
-  p.tile = list[1];
+  const int s = uniform(list[0]);
+  p.tile = uniform(list[1]);
   p.kv = blockIdx.x % a.kv_heads;
   sequence(a.starts_q, s, a.seqs, a.tq, p.q0, p.nq);
   sequence(a.starts_k, s, a.seqs, a.tk, p.k0, p.nk);
+  p.q0 = uniform(p.q0), p.nq = uniform(p.nq), p.k0 = uniform(p.k0), p.nk = uniform(p.nk);
   if (s == a.seqs) (which ? p.nq : p.nk) = 0;
   return true;
 }
 
-// A tile of TILE rows on its way from memory to LDS: 16-byte chunks, the same for each thread of the 256.
+// The keys' side of the forward and of the queries' gradient: tiles of TILE keys and their values, one tile ahead.
 template <int DP, typename T>
-struct Stage {
-  static constexpr int CH = DP / 8, N = TILE * CH / 256;
-  V8<T> x[N];
-  // row r of the tile is at base + r * stride; rows past `rows` and columns past `dim` are zeros
-  __device__ __forceinline__ void load(const T* base, long long stride, int rows, int dim) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = i * 256 + threadIdx.x, r = at / CH, c = at % CH;
-      x[i] = r < rows && 8 * c < dim ? load8(base + r * stride + 8 * c) : zero8<T>();
-    }
+struct Keys {
+  static constexpr int CH = DP / 8, STEP = 256 / CH, N = TILE / STEP;  // chunks a row; rows a turn of the workgroup
+  const T *k, *v;  // this thread's chunk of the tile's first rows
+  long long k_t, v_t;
+  int row, at, left;  // this thread's row; its wave's place in LDS; keys from the tile's first on
+  bool in_row;
+  __device__ __forceinline__ Keys(const Attend& a, const Place& p) {
+    row = threadIdx.x / CH;
+    const int c = threadIdx.x % CH ^ swizzle<DP>(row);  // LDS is filled in order: the swizzle is the source's
+    in_row = 8 * c < a.dim;
+    k_t = a.k_t, v_t = a.v_t;
+    k = (const T*)a.k + (long long)p.k0 * k_t + (long long)p.kv * a.k_h + row * k_t + 8 * c;
+    v = (const T*)a.v + (long long)p.k0 * v_t + (long long)p.kv * a.v_h + row * v_t + 8 * c;
+    at = threadIdx.x / 64 * 64 * 8;
+    left = p.nk;
   }
-  __device__ __forceinline__ void write(T* tile) const {
+  __device__ __forceinline__ void next(T* ks, T* vs) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = i * 256 + threadIdx.x;
-      *(V8<T>*)(tile + chunk_at<DP>(at / CH, at % CH)) = x[i];
+      const bool valid = in_row && row + i * STEP < left;
+      to_lds(k + i * STEP * k_t, valid, ks + i * 2048 + at);
+      to_lds(v + i * STEP * v_t, valid, vs + i * 2048 + at);
     }
+    k += TILE * k_t;
+    v += TILE * v_t;
+    left -= TILE;
+  }
+};
+
+// The rows' side: a wave's 32 query rows of a workgroup's 128
+struct Rows {
+  int pos, head, limit, all_see, any_sees, tiles;
+  bool valid;
+  __device__ __forceinline__ Rows(const Attend& a, const Place& p) {
+    const int rows = p.nq * a.group, off = p.nk - p.nq, w = uniform(threadIdx.x / 64);
+    const int row0 = p.tile * QROWS + 32 * w, row = row0 + threadIdx.x % 32;
+    valid = row < rows;
+    pos = row / a.group;
+    head = p.kv * a.group + row % a.group;
+    limit = valid ? pos + off : -1;  // the row's last key (below 0: none)
+    // of the wave's rows: the last key that all see, and the last that any sees; the workgroup's tiles of keys
+    all_see = row0 < rows ? row0 / a.group + off : -1;
+    any_sees = row0 < rows ? (row0 + 31 < rows ? row0 + 31 : rows - 1) / a.group + off : -1;
+    const int end = p.tile * QROWS + QROWS < rows ? p.tile * QROWS + QROWS : rows, last = (end - 1) / a.group + off;
+    tiles = last < 0 ? 0 : last / TILE + 1;
   }
 };
 
@@ -124,98 +156,79 @@ struct Stage {
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
   constexpr int KS = DP / 16, DT = DP / 32;
-  __shared__ __align__(16) T ks[TILE * DP];
-  __shared__ __align__(16) T vs[TILE * DP];
+  __shared__ __align__(16) T ks[2][TILE * DP];
+  __shared__ __align__(16) T vs[2][TILE * DP];
   Place p;
   if (!place(a, 0, p)) return;
-  const int l = threadIdx.x % 64, n = l % 32, h = l / 32, w = threadIdx.x / 64;
-  const int rows = p.nq * a.group, off = p.nk - p.nq, dim = a.dim;
-  const int row0 = p.tile * QROWS + 32 * w, row = row0 + n;
-  const bool valid = row < rows;
-  const int pos = row / a.group, head = p.kv * a.group + row % a.group;
-  const int limit = valid ? pos + off : -1;  // the row's last key (below 0: none)
-  // of the wave's rows: the last key that all see, and the last that any sees; of the workgroup's
-  const int all_see = row0 < rows ? row0 / a.group + off : -1;
-  const int any_sees = row0 < rows ? (row0 + 31 < rows ? row0 + 31 : rows - 1) / a.group + off : -1;
-  const int end0 = p.tile * QROWS + QROWS < rows ? p.tile * QROWS + QROWS : rows;
-  const int last = (end0 - 1) / a.group + off;
-  const int tiles = last < 0 ? 0 : last / TILE + 1;
-
+  const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
+  const Rows r(a, p);
+  Keys<DP, T> keys(a, p);
+  if (r.tiles) keys.next(ks[0], vs[0]);
   V8<T> q[KS];
-  load_rows<DP>(valid ? (const T*)a.q + (long long)(p.q0 + pos) * a.q_t + (long long)head * a.q_h : nullptr, dim, h, q);
-  const T* kb = (const T*)a.k + (long long)p.k0 * a.k_t + (long long)p.kv * a.k_h;
-  const T* vb = (const T*)a.v + (long long)p.k0 * a.v_t + (long long)p.kv * a.v_h;
-
+  load_rows<DP>(r.valid ? (const T*)a.q + (long long)(p.q0 + r.pos) * a.q_t + (long long)r.head * a.q_h : nullptr, dim, h,
+                q);
   F16x acc[DT] = {};
   float m = -INFINITY, sum = 0.0f;
   const float c = a.scale * LOG2E;
-  Stage<DP, T> ksg, vsg;
-  if (tiles) {
-    ksg.load(kb, a.k_t, p.nk, dim);
-    vsg.load(vb, a.v_t, p.nk, dim);
-  }
-  for (int t = 0; t < tiles; ++t) {
+  for (int t = 0; t < r.tiles; ++t) {
     const int key0 = t * TILE;
-    __syncthreads();
-    ksg.write(ks);
-    vsg.write(vs);
-    __syncthreads();
-    if (t + 1 < tiles) {
-      ksg.load(kb + (long long)(key0 + TILE) * a.k_t, a.k_t, p.nk - key0 - TILE, dim);
-      vsg.load(vb + (long long)(key0 + TILE) * a.v_t, a.v_t, p.nk - key0 - TILE, dim);
-    }
-    if (key0 > any_sees) continue;
-    const bool second = key0 + 32 <= any_sees;
+    const T *kt = ks[t & 1], *vt = vs[t & 1];
+    loads_done();
+    __syncthreads();  // this tile is there for all, and all are done with the one before
+    if (t + 1 < r.tiles) keys.next(ks[(t + 1) & 1], vs[(t + 1) & 1]);
+    if (key0 > r.any_sees) continue;
+    const bool second = key0 + 32 <= r.any_sees;
     F16x s[2] = {};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (i == 1 && !second) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[1][r] = -INFINITY;
+        for (int j = 0; j < 16; ++j) s[1][j] = -INFINITY;
         break;
       }
 #pragma unroll
-      for (int x = 0; x < KS; ++x) s[i] = mfma(read_rows<DP>(ks, 32 * i, x, n, h), q[x], s[i]);
-      if (key0 + 32 * i + 31 > all_see)
+      for (int x = 0; x < KS; ++x) s[i] = mfma(read_rows<DP>(kt, 32 * i, x, n, h), q[x], s[i]);
+      if (key0 + 32 * i + 31 > r.all_see)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (key0 + 32 * i + r % 4 + 8 * (r / 4) + 4 * h > limit) s[i][r] = -INFINITY;
+        for (int j = 0; j < 16; ++j)
+          if (key0 + 32 * i + j % 4 + 8 * (j / 4) + 4 * h > r.limit) s[i][j] = -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[0][r]);
+    for (int j = 1; j < 16; ++j) top = fmaxf(top, s[0][j]);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[1][r]);
+    for (int j = 0; j < 16; ++j) top = fmaxf(top, s[1][j]);
     const float m1 = fmaxf(m, max_halves(top));
     const float base = m1 == -INFINITY ? 0.0f : m1 * c;  // a row that has seen no key yet
     if (__any(m1 != m)) {
-      const float f = m == -INFINITY ? 0.0f : exp2f(m * c - base);
+      const float f = m == -INFINITY ? 0.0f : exp2_fast(m * c - base);
       sum *= f;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+        for (int j = 0; j < 16; ++j) acc[d][j] *= f;
       m = m1;
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[i][r] = exp2f(fmaf(s[i][r], c, -base));
-        sum += s[i][r];
+      for (int j = 0; j < 16; ++j) {
+        s[i][j] = exp2_fast(fmaf(s[i][j], c, -base));
+        sum += s[i][j];
       }
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       if (x == 2 && !second) break;
       const V8<T> pr = pack<T>(s[x / 2], x % 2);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) acc[d] = mfma(read_columns<DP>(vs, 16 * x, d, l), pr, acc[d]);
+      for (int d = 0; d < DT; ++d) acc[d] = mfma(read_columns<DP>(vt, 16 * x, d, l), pr, acc[d]);
     }
   }
   sum = add_halves(sum);
-  if (a.lse && valid && h == 0)
-    a.lse[(long long)head * a.tq + p.q0 + pos] = sum == 0.0f ? INFINITY : m * c + log2f(sum);
-  store_rows<DP>(valid ? (T*)a.out + ((long long)(p.q0 + pos) * a.heads + head) * dim : nullptr, dim, h, acc,
+  const long long token = p.q0 + r.pos;
+  if (a.lse && r.valid && h == 0)
+    a.lse[(long long)r.head * a.tq + token] = sum == 0.0f ? INFINITY : m * c + log2f(sum);
+  store_rows<DP>(r.valid ? (T*)a.out + (token * a.heads + r.head) * dim : nullptr, dim, h, acc,
                  sum == 0.0f ? 0.0f : 1.0f / sum);
 }
 
@@ -224,175 +237,208 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
   constexpr int KS = DP / 16, DT = DP / 32;
-  __shared__ __align__(16) T ks[TILE * DP];
-  __shared__ __align__(16) T vs[TILE * DP];
+  __shared__ __align__(16) T ks[2][TILE * DP];
+  __shared__ __align__(16) T vs[2][TILE * DP];
   Place p;
   if (!place(a, 0, p)) return;
-  const int l = threadIdx.x % 64, n = l % 32, h = l / 32, w = threadIdx.x / 64;
-  const int rows = p.nq * a.group, off = p.nk - p.nq, dim = a.dim;
-  const int row0 = p.tile * QROWS + 32 * w, row = row0 + n;
-  const bool valid = row < rows;
-  const int pos = row / a.group, head = p.kv * a.group + row % a.group;
-  const int limit = valid ? pos + off : -1;
-  const int all_see = row0 < rows ? row0 / a.group + off : -1;
-  const int any_sees = row0 < rows ? (row0 + 31 < rows ? row0 + 31 : rows - 1) / a.group + off : -1;
-  const int end0 = p.tile * QROWS + QROWS < rows ? p.tile * QROWS + QROWS : rows;
-  const int last = (end0 - 1) / a.group + off;
-  const int tiles = last < 0 ? 0 : last / TILE + 1;
-
+  const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
+  const Rows r(a, p);
+  Keys<DP, T> keys(a, p);
+  if (r.tiles) keys.next(ks[0], vs[0]);
+  const long long token = p.q0 + r.pos;
   V8<T> q[KS], g[KS];
-  const long long token = p.q0 + pos;
-  load_rows<DP>(valid ? (const T*)a.q + token * a.q_t + (long long)head * a.q_h : nullptr, dim, h, q);
-  load_rows<DP>(valid ? (const T*)a.dout + token * a.do_t + (long long)head * a.do_h : nullptr, dim, h, g);
-  float delta = 0.0f, lse = INFINITY;
-  {
+  load_rows<DP>(r.valid ? (const T*)a.q + token * a.q_t + (long long)r.head * a.q_h : nullptr, dim, h, q);
+  load_rows<DP>(r.valid ? (const T*)a.dout + token * a.do_t + (long long)r.head * a.do_h : nullptr, dim, h, g);
+  const float lse = r.valid ? a.lse[(long long)r.head * a.tq + token] : INFINITY;
+  const float c = a.scale * LOG2E;
+  // the row's 32 scores and dP of subtile i; masked probabilities are 0
+  auto products = [&](const T* kt, const T* vt, int key0, int i, F16x& s, F16x& dp) {
+    s = F16x{}, dp = F16x{};
+#pragma unroll
+    for (int x = 0; x < KS; ++x) {
+      s = mfma(read_rows<DP>(kt, 32 * i, x, n, h), q[x], s);
+      dp = mfma(read_rows<DP>(vt, 32 * i, x, n, h), g[x], dp);
+    }
+    if (key0 + 32 * i + 31 > r.all_see)
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (key0 + 32 * i + j % 4 + 8 * (j / 4) + 4 * h > r.limit) s[j] = -INFINITY, dp[j] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[j] = exp2_fast(fmaf(s[j], c, -lse));
+  };
+  // delta = dout . out from the stored output, whose rounding is felt where few keys share a row: rows whose keys all
+  // lie in the first tile take it from that tile's products instead, sum P dP in float32, below
+  float delta = 0.0f;
+  const bool few = r.any_sees < TILE;
+  if (!few) {
     V8<T> o[KS];
-    load_rows<DP>(valid ? (const T*)a.out + (token * a.heads + head) * dim : nullptr, dim, h, o);
+    load_rows<DP>(r.valid ? (const T*)a.out + (token * a.heads + r.head) * dim : nullptr, dim, h, o);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta += (float)o[s][e] * (float)g[s][e];
     delta = add_halves(delta);
-    if (valid) {
-      lse = a.lse[(long long)head * a.tq + token];
-      if (h == 0) a.delta[(long long)head * a.tq + token] = delta;
-    }
   }
-  const T* kb = (const T*)a.k + (long long)p.k0 * a.k_t + (long long)p.kv * a.k_h;
-  const T* vb = (const T*)a.v + (long long)p.k0 * a.v_t + (long long)p.kv * a.v_h;
   F16x acc[DT] = {};
-  const float c = a.scale * LOG2E;
-  Stage<DP, T> ksg, vsg;
-  if (tiles) {
-    ksg.load(kb, a.k_t, p.nk, dim);
-    vsg.load(vb, a.v_t, p.nk, dim);
-  }
-  for (int t = 0; t < tiles; ++t) {
+  for (int t = 0; t < r.tiles; ++t) {
     const int key0 = t * TILE;
+    const T *kt = ks[t & 1], *vt = vs[t & 1];
+    loads_done();
     __syncthreads();
-    ksg.write(ks);
-    vsg.write(vs);
-    __syncthreads();
-    if (t + 1 < tiles) {
-      ksg.load(kb + (long long)(key0 + TILE) * a.k_t, a.k_t, p.nk - key0 - TILE, dim);
-      vsg.load(vb + (long long)(key0 + TILE) * a.v_t, a.v_t, p.nk - key0 - TILE, dim);
+    if (t + 1 < r.tiles) keys.next(ks[(t + 1) & 1], vs[(t + 1) & 1]);
+    if (t == 0 && few) {
+#pragma unroll 1
+      for (int i = 0; 32 * i <= r.any_sees; ++i) {
+        F16x s, dp;
+        products(kt, vt, 0, i, s, dp);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) delta += s[j] * dp[j];
+      }
+      delta = add_halves(delta);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (key0 + 32 * i > any_sees) break;
-      F16x s = {}, dp = {};
+      if (key0 + 32 * i > r.any_sees) break;
+      F16x s, dp;
+      products(kt, vt, key0, i, s, dp);
 #pragma unroll
-      for (int x = 0; x < KS; ++x) {
-        s = mfma(read_rows<DP>(ks, 32 * i, x, n, h), q[x], s);
-        dp = mfma(read_rows<DP>(vs, 32 * i, x, n, h), g[x], dp);
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
-      if (key0 + 32 * i + 31 > all_see)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (key0 + 32 * i + r % 4 + 8 * (r / 4) + 4 * h > limit) s[r] = 0.0f;
+      for (int j = 0; j < 16; ++j) s[j] *= dp[j] - delta;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const V8<T> ds = pack<T>(s, x);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] = mfma(read_columns<DP>(ks, 32 * i + 16 * x, d, l), ds, acc[d]);
+        for (int d = 0; d < DT; ++d) acc[d] = mfma(read_columns<DP>(kt, 32 * i + 16 * x, d, l), ds, acc[d]);
       }
     }
   }
-  store_rows<DP>(valid ? (T*)a.dq + (token * a.heads + head) * dim : nullptr, dim, h, acc, a.scale);
+  if (r.valid && h == 0) a.delta[(long long)r.head * a.tq + token] = delta;
+  store_rows<DP>(r.valid ? (T*)a.dq + (token * a.heads + r.head) * dim : nullptr, dim, h, acc, a.scale);
 }
 
 // ---- backward: the keys' and values' gradients ----------------------------------------------------------------------
 
-// A wave keeps 32 keys and their values as B operands and walks over the rows that see them; rows lie in LDS. S = Q K^T
-// here, so that a lane holds 16 rows of ONE key and P, dS are the B operands of dV^T = dO^T P and dK^T = Q^T dS.
-template <typename T, int DP>
-__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void k_attend_dkv(Attend a) {
-  constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, N = TILE * CH / 256;
-  __shared__ __align__(16) T qs[TILE * DP];
-  __shared__ __align__(16) T gs[TILE * DP];
-  __shared__ __align__(16) float lses[TILE], deltas[TILE];
-  __shared__ __align__(16) int limits[TILE];
+// A wave keeps 32 keys and their values as B operands and walks over the rows that see them; rows lie in LDS, RT at a
+// time. S = Q K^T here, so that a lane holds 16 rows of ONE key and P, dS are the B operands of dV^T = dO^T P and dK^T =
+// Q^T dS. KW of the four waves differ in their keys, the others take every 4/KW-th subtile of 32 rows of the same keys,
+// and their sums are added at the end, in order. Heads of 128 hold three quarters of the values in LDS: with all of them
+// in registers a SIMD has room for one wave only.
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(256, 2) void k_attend_dkv(Attend a) {
+  constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 256 / CH, SPLIT = 4 / KW;
+  constexpr int RT = DP == 64 ? (KW == 1 ? 128 : 64) : (KW == 4 ? 32 : 64), SUB = RT / 32, N = RT / STEP;
+  constexpr int VR = DP == 64 ? KS : KS / 4;  // of a value row's KS operands, those in registers
+  __shared__ __align__(16) T tiles[2][2][RT * DP];  // (turn, q or dout)
+  __shared__ __align__(16) V8<T> vl[VR < KS ? KW * (KS - VR) * 64 : 1];
+  __shared__ __align__(16) float lses[2][RT], deltas[2][RT];
+  __shared__ __align__(16) int limits[2][RT];
   Place p;
   if (!place(a, 1, p)) return;
-  const int l = threadIdx.x % 64, n = l % 32, h = l / 32, w = threadIdx.x / 64;
-  const int rows = p.nq * a.group, off = p.nk - p.nq, dim = a.dim;
-  const int key0 = p.tile * KROWS + 32 * w, key = key0 + n;
+  const int l = threadIdx.x % 64, n = l % 32, h = l / 32, w = uniform(threadIdx.x / 64), dim = a.dim, group = a.group;
+  const int kw = w % KW, split = w / KW;
+  const int rows = p.nq * group, off = p.nk - p.nq;
+  const int key0 = p.tile * 32 * KW + 32 * kw, key = key0 + n;
   const bool valid = key < p.nk;
-  V8<T> k[KS], v[KS];
-  load_rows<DP>(valid ? (const T*)a.k + (long long)(p.k0 + key) * a.k_t + (long long)p.kv * a.k_h : nullptr, dim, h, k);
-  load_rows<DP>(valid ? (const T*)a.v + (long long)(p.k0 + key) * a.v_t + (long long)p.kv * a.v_h : nullptr, dim, h, v);
-  F16x dk[DT] = {}, dv[DT] = {};
   const float c = a.scale * LOG2E;
-  const int from = p.tile * KROWS - off;  // the first token that sees the tile's first key
-  const int first = (from > 0 ? from : 0) * a.group;
 
-  V8<T> qx[N], gx[N];
-  float lse = INFINITY, delta = 0.0f;
-  int limit = -1;
-  auto load = [&](int r0) {
+  // Row tiles start at whole tokens (but for groups above RT, whose rows' places are computed anew for each tile), so
+  // that a thread's rows keep their distance from the tile's first token: RT or a little less rows are used of each.
+  const int used = group <= RT ? RT / group * group : RT;
+  const int from = p.tile * 32 * KW - off;  // the first token that sees the tile's first key
+  const int first = (from > 0 ? from : 0) * group;
+  const int chunk = threadIdx.x % CH ^ swizzle<DP>(threadIdx.x / CH);
+  const bool in_row = 8 * chunk < dim;
+  long long qo[N], go[N];
+  auto offsets = [&](int r0) {  // of this thread's rows from the first token of r0
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = i * 256 + threadIdx.x, r = r0 + at / CH, d = at % CH * 8;
-      const bool in = r < rows && d < dim;
-      const int pos = r / a.group, head = p.kv * a.group + r % a.group;
-      qx[i] = in ? load8((const T*)a.q + (long long)(p.q0 + pos) * a.q_t + (long long)head * a.q_h + d) : zero8<T>();
-      gx[i] = in ? load8((const T*)a.dout + (long long)(p.q0 + pos) * a.do_t + (long long)head * a.do_h + d) : zero8<T>();
-    }
-    if (threadIdx.x < TILE) {
-      const int r = r0 + threadIdx.x, pos = r / a.group;
-      const long long at = (long long)(p.kv * a.group + r % a.group) * a.tq + p.q0 + pos;
-      lse = r < rows ? a.lse[at] : INFINITY;
-      delta = r < rows ? a.delta[at] : 0.0f;
-      limit = r < rows ? pos + off : -1;
+      const int r = r0 % group + (int)threadIdx.x / CH + i * STEP, pos = r / group, head = r % group;
+      qo[i] = pos * a.q_t + head * a.q_h + 8 * chunk;
+      go[i] = pos * a.do_t + head * a.do_h + 8 * chunk;
     }
   };
-  if (first < rows) load(first);
-  for (int r0 = first; r0 < rows; r0 += TILE) {
-    __syncthreads();
+  offsets(first);
+  const T* qb = (const T*)a.q + (long long)p.q0 * a.q_t + (long long)p.kv * group * a.q_h;
+  const T* gb = (const T*)a.dout + (long long)p.q0 * a.do_t + (long long)p.kv * group * a.do_h;
+  float lse = INFINITY, delta = 0.0f;
+  int limit = -1;
+  auto load = [&](int r0, int turn) {
+    if (group > RT) offsets(r0);
+    const long long token = r0 / group;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = i * 256 + threadIdx.x;
-      *(V8<T>*)(qs + chunk_at<DP>(at / CH, at % CH)) = qx[i];
-      *(V8<T>*)(gs + chunk_at<DP>(at / CH, at % CH)) = gx[i];
+      const int row = threadIdx.x / CH + i * STEP;
+      const bool there = in_row && row < used && r0 + row < rows;
+      to_lds(qb + token * a.q_t + qo[i], there, tiles[turn][0] + i * 2048 + w * 512);
+      to_lds(gb + token * a.do_t + go[i], there, tiles[turn][1] + i * 2048 + w * 512);
     }
-    if (threadIdx.x < TILE) {
-      lses[threadIdx.x] = lse;
-      deltas[threadIdx.x] = delta;
-      limits[threadIdx.x] = limit;
+    if (threadIdx.x < RT) {
+      const int r = r0 + threadIdx.x, pos = r / group;
+      const bool there = threadIdx.x < used && r < rows;
+      const long long at = (long long)(p.kv * group + r % group) * a.tq + p.q0 + pos;
+      lse = there ? a.lse[at] : INFINITY;
+      delta = there ? a.delta[at] : 0.0f;
+      limit = there ? pos + off : -1;
     }
-    __syncthreads();
-    if (r0 + TILE < rows) load(r0 + TILE);
-    if (key0 >= p.nk) continue;
+  };
+  // From the last rows, which every key tile of the sequence reads, to the tile's first: workgroups that run side by
+  // side then read the same rows at about the same time, from the L2 cache of their XCD.
+  const int start = first + (rows > first ? (rows - 1 - first) / used * used : -used);
+  if (start >= first) load(start, 0);
+  V8<T> k[KS], v[VR];
+  load_rows<DP>(valid ? (const T*)a.k + (long long)(p.k0 + key) * a.k_t + (long long)p.kv * a.k_h : nullptr, dim, h, k);
+  {
+    V8<T> all[KS];
+    load_rows<DP>(valid ? (const T*)a.v + (long long)(p.k0 + key) * a.v_t + (long long)p.kv * a.v_h : nullptr, dim, h, all);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int ra = r0 + 32 * i, rb = ra + 31 < rows ? ra + 31 : rows - 1;
-      if (ra >= rows || rb / a.group + off < key0) continue;  // no row sees a key of the wave
+    for (int x = 0; x < VR; ++x) v[x] = all[x];
+#pragma unroll
+    for (int x = VR; x < KS; ++x)
+      if (split == 0) vl[(kw * (KS - VR) + x - VR) * 64 + l] = all[x];
+  }
+  F16x dk[DT] = {}, dv[DT] = {};
+  int turn = 0, sub0 = 0, token0 = start / group;
+  for (int r0 = start; r0 >= first; r0 -= used, turn ^= 1, sub0 += SUB) {
+    if (threadIdx.x < RT) {
+      lses[turn][threadIdx.x] = lse;
+      deltas[turn][threadIdx.x] = delta;
+      limits[turn][threadIdx.x] = limit;
+    }
+    loads_done();
+    __syncthreads();
+    if (r0 - used >= first) load(r0 - used, turn ^ 1);
+    if (key0 >= p.nk) continue;
+    const int token = group <= RT ? token0 : r0 / group, inside = group <= RT ? 0 : r0 % group;
+    token0 -= used / group;
+    const T *qt = tiles[turn][0], *gt = tiles[turn][1];
+#pragma unroll
+    for (int i = 0; i < SUB; ++i) {
+      if (SPLIT > 1 && (sub0 + i) % SPLIT != split) continue;
+      // the last keys that the subtile's first row and (at most) its last one see
+      const int low = token + (32 * i) / group + off, most = ((32 * i + 31 < used ? 32 * i + 31 : used - 1) + inside) / group;
+      if (32 * i >= used || r0 + 32 * i >= rows || token + most + off < key0) continue;
       F16x s = {}, dp = {};
 #pragma unroll
       for (int x = 0; x < KS; ++x) {
-        s = mfma(read_rows<DP>(qs, 32 * i, x, n, h), k[x], s);
-        dp = mfma(read_rows<DP>(gs, 32 * i, x, n, h), v[x], dp);
+        s = mfma(read_rows<DP>(qt, 32 * i, x, n, h), k[x], s);
+        dp = mfma(read_rows<DP>(gt, 32 * i, x, n, h), x < VR ? v[x < VR ? x : 0] : vl[(kw * (KS - VR) + x - VR) * 64 + l], dp);
       }
-      const bool masked = ra / a.group + off < key0 + 31;
+      const bool masked = low < key0 + 31;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int at = 32 * i + 8 * j + 4 * h;
-        const float4 ls = *(const float4*)(lses + at), de = *(const float4*)(deltas + at);
-        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dev[4] = {de.x, de.y, de.z, de.w};
+        typedef float F4 __attribute__((ext_vector_type(4)));
+        typedef int I4 __attribute__((ext_vector_type(4)));
+        const F4 ls = *(const F4*)(lses[turn] + at), de = *(const F4*)(deltas[turn] + at);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int r = 4 * j + e;
-          s[r] = exp2f(fmaf(s[r], c, -lsv[e]));
-          dp[r] = s[r] * (dp[r] - dev[e]);
+          s[4 * j + e] = exp2_fast(fmaf(s[4 * j + e], c, -ls[e]));
+          dp[4 * j + e] = s[4 * j + e] * (dp[4 * j + e] - de[e]);
         }
         if (masked) {
-          const int4 li = *(const int4*)(limits + at);
-          const int liv[4] = {li.x, li.y, li.z, li.w};
+          const I4 li = *(const I4*)(limits[turn] + at);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (key > liv[e]) s[4 * j + e] = dp[4 * j + e] = 0.0f;
+            if (key > li[e]) s[4 * j + e] = dp[4 * j + e] = 0.0f;
         }
       }
 #pragma unroll
@@ -400,11 +446,35 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void k_attend_dkv(Attend a) 
         const V8<T> pr = pack<T>(s, x), ds = pack<T>(dp, x);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          dv[d] = mfma(read_columns<DP>(gs, 32 * i + 16 * x, d, l), pr, dv[d]);
-          dk[d] = mfma(read_columns<DP>(qs, 32 * i + 16 * x, d, l), ds, dk[d]);
+          dv[d] = mfma(read_columns<DP>(gt, 32 * i + 16 * x, d, l), pr, dv[d]);
+          dk[d] = mfma(read_columns<DP>(qt, 32 * i + 16 * x, d, l), ds, dk[d]);
         }
       }
     }
+  }
+  // the waves of the same keys: split 0 adds the others' sums, one after another
+  if constexpr (SPLIT > 1) {
+    float* mine = (float*)&tiles[0][0][0];  // (KW, 16 DT, 64) a turn: dk, then dv; within the tiles
+    static_assert(sizeof(tiles) >= sizeof(float) * KW * 16 * DT * 64, "");
+#pragma unroll
+    for (int o = 1; o < SPLIT; ++o)
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        F16x* acc = which ? dv : dk;
+        __syncthreads();
+        if (split == o)
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mine[((kw * DT + d) * 16 + j) * 64 + l] = acc[d][j];
+        __syncthreads();
+        if (split == 0)
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[d][j] += mine[((kw * DT + d) * 16 + j) * 64 + l];
+      }
+    if (split) return;
   }
   const long long at = ((long long)(p.k0 + key) * a.kv_heads + p.kv) * dim;
   store_rows<DP>(valid ? (T*)a.dk + at : nullptr, dim, h, dk, a.scale);
@@ -413,8 +483,16 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void k_attend_dkv(Attend a) 
 
 // ---- launches -------------------------------------------------------------------------------------------------------
 
-size_t attend_work_bytes(int seqs, int tq, int tk, int group) {
-  return sizeof(int) * (ORDER_HEAD + 2 * (size_t)(order_queries(seqs, tq, group) + order_keys(seqs, tk)));
+// Keys a workgroup of the keys' gradients: 128, or fewer where sequences are short (the waves would have none) or tiles
+// few (a causal tile's work goes from all rows to none: several a CU even that out).
+int key_waves(int kv_heads, int seqs, int tk) {
+  const long long tiles = (long long)tk / 128 * kv_heads;
+  if (tk <= 48LL * seqs) return 1;
+  return tk <= 96LL * seqs || tiles < 2048 ? 2 : 4;
+}
+size_t attend_work_bytes(int kv_heads, int seqs, int tq, int tk, int group) {
+  return sizeof(int) * (ORDER_HEAD + 2 * (size_t)(order_queries(seqs, tq, group) +
+                                                  order_keys(seqs, tk, key_waves(kv_heads, seqs, tk))));
 }
 
 template <typename T, int DP>
@@ -428,12 +506,18 @@ int attend_vjp(hipStream_t st, const Attend& a) {
   if (a.tq) k_attend_dq<T, DP><<<(unsigned)(order_queries(a.seqs, a.tq, a.group) * a.kv_heads), 256, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  if (a.tk) k_attend_dkv<T, DP><<<(unsigned)(order_keys(a.seqs, a.tk) * a.kv_heads), 256, 0, st>>>(a);
+  if (!a.tk) return 0;
+  const unsigned blocks = (unsigned)(order_keys(a.seqs, a.tk, a.key_waves) * a.kv_heads);
+  switch (a.key_waves) {
+    case 1: k_attend_dkv<T, DP, 1><<<blocks, 256, 0, st>>>(a); break;
+    case 2: k_attend_dkv<T, DP, 2><<<blocks, 256, 0, st>>>(a); break;
+    default: k_attend_dkv<T, DP, 4><<<blocks, 256, 0, st>>>(a);
+  }
   return (int)hipGetLastError();
 }
 
 int launch_attend(hipStream_t st, int type, const Attend& a) {
-  k_attend_order<<<1, 1024, 0, st>>>(a.seqs, a.tq, a.tk, a.group, a.starts_q, a.starts_k, (int*)a.order);
+  k_attend_order<<<1, 1024, 0, st>>>(a.seqs, a.tq, a.tk, a.group, a.key_waves, a.starts_q, a.starts_k, (int*)a.order);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.tq) return (int)e;
   if (type == BF16) return a.dim <= 64 ? attend<__bf16, 64>(st, a) : attend<__bf16, 128>(st, a);
@@ -453,7 +537,7 @@ bool attention_takes(int type, int heads, int kv_heads, int dim, int seqs, int t
       dim % 8 || seqs < 0 || tq < 0 || tk < 0 || tk >= 1 << 30 || (long long)tq * (heads / kv_heads) >= 1 << 30)
     return false;
   const long long most = (1LL << 24) - 1;  // workgroups of 256 work-items a launch
-  return pol::order_queries(seqs, tq, heads / kv_heads) * kv_heads <= most && pol::order_keys(seqs, tk) * kv_heads <= most;
+  return pol::order_queries(seqs, tq, heads / kv_heads) * kv_heads <= most && pol::order_keys(seqs, tk, 1) * kv_heads <= most;
 }
 }  // namespace
 
@@ -470,6 +554,7 @@ int dk_attention(hipStream_t st, int type, int heads, int kv_heads, int dim, int
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
+  a.key_waves = pol::key_waves(kv_heads, seqs, tk);
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.out = out, a.lse = lse, a.order = (const int*)work;
   return pol::launch_attend(st, type, a);
 }
@@ -486,6 +571,7 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
+  a.key_waves = pol::key_waves(kv_heads, seqs, tk);
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.order = (const int*)work;
   a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse);
   a.dout = dout, a.do_t = do_t, a.do_h = do_h, a.delta = delta, a.dq = dq, a.dk = dk, a.dv = dv;
@@ -494,7 +580,7 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
 
 long long dk_attention_work_bytes(int heads, int kv_heads, int seqs, int tq, int tk) {
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || seqs < 0 || tq < 0 || tk < 0) return 0;
-  return (long long)pol::attend_work_bytes(seqs, tq, tk, heads / kv_heads);
+  return (long long)pol::attend_work_bytes(kv_heads, seqs, tq, tk, heads / kv_heads);
 }
 
 }  // extern "C"
