@@ -1,6 +1,7 @@
 """Build the HIP library libnablaengine_g1.so in-tree for gfx950 (hipcc; one shared library, the C ABI of
 include/nablaengine_g1.h and nablaengine_policy.h), and beside it the policy operators' torch side (g++).
 `python -m nablaengine_amd.build`."""
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -22,6 +23,13 @@ FLAGS = ["-O3", f"--offload-arch={ARCH}", "-std=c++17", "-fPIC", "-shared", "-Xc
          "-packed-fp32-ops", "-ffp-contract=fast", "-mllvm", "-disable-machine-licm",
          "-Wno-unused-command-line-argument", "-Werror=return-type",
          "-Werror=uninitialized", "-Werror=sometimes-uninitialized", "-Werror=array-bounds"]
+
+
+def flags_of(source):
+    """The flags a source is compiled with. The policy operators' kernels have registers to spare, and LDS addresses that
+    machine LICM keeps out of their loops."""
+    policy = source.startswith("policy_")
+    return [f for f in FLAGS if not (policy and f in ("-mllvm", "-disable-machine-licm")) and f != "-shared"]
 
 
 def build_torch(verbose=False):
@@ -53,14 +61,23 @@ def build(verbose=False, profile=False):
     target = PROF_LIB if profile else LIB
     fd, tmp = tempfile.mkstemp(prefix="libnablaengine_g1.", suffix=".so.tmp", dir=HERE)
     os.close(fd)
-    cmd = [hipcc] + FLAGS + (["-DG1_PROFILE"] if profile else []) + ["-o", tmp] + [os.path.join(CSRC, s) for s in SOURCES]
-    if verbose:
-        print(" ".join(cmd))
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
+    with tempfile.TemporaryDirectory() as objects, concurrent.futures.ThreadPoolExecutor(8) as pool:
+        def one(source):
+            obj = os.path.join(objects, source + ".o")
+            cmd = [hipcc] + flags_of(source) + (["-DG1_PROFILE"] if profile else []) + ["-c", "-o", obj,
+                                                                                         os.path.join(CSRC, source)]
+            if verbose:
+                print(" ".join(cmd))
+            return obj, subprocess.run(cmd, capture_output=True, text=True)
+        done = list(pool.map(one, SOURCES))
+        link = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp] + [obj for obj, _ in done]
+        runs = [r for _, r in done]
+        if all(r.returncode == 0 for r in runs):
+            runs.append(subprocess.run(link, capture_output=True, text=True))
+    if any(r.returncode for r in runs):
         os.unlink(tmp)
-        sys.stderr.write(r.stdout + r.stderr)
-        raise RuntimeError(f"hipcc failed ({r.returncode})")
+        sys.stderr.write("".join(r.stdout + r.stderr for r in runs if r.returncode))
+        raise RuntimeError(f"hipcc failed ({[r.returncode for r in runs]})")
     os.replace(tmp, target)
     return target
 

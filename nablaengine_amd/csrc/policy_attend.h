@@ -33,6 +33,7 @@ struct Attend {
   const void *q, *k, *v;
   long long q_t, q_h, k_t, k_h, v_t, v_h;  // elements from token to token, and from head to head
   int heads, kv_heads, group, dim, seqs, tq, tk;
+  int by_sequence;  // the order of the tiles, see below
   int key_waves;  // waves of a workgroup of the keys' gradients that differ in their 32 keys: 1, 2 or 4
   const int *starts_q, *starts_k;
   float scale;
@@ -46,8 +47,14 @@ struct Attend {
   void *dq, *dk, *dv;
 };
 
-// The order: two lists of tiles, (sequence, tile of it), heaviest first: the query tiles (QROWS rows of a key/value
-// head's queries, row = token * group + head of the group) and the key tiles (32 * key_waves keys).
+// The order: two lists of tiles, (sequence, tile of it): the query tiles (QROWS rows of a key/value head's queries, row =
+// token * group + head of the group) and the key tiles (32 * key_waves keys). A list is heaviest first, by the tiles of
+// the other side that each one reads: over all tiles where sequences are long; over sequences, each one's tiles one after
+// another, where they are not (by_sequence). Workgroups go to the XCDs in turn, and each XCD has an L2 cache of its own:
+// in the second case WINDOW neighbours of the list go to one XCD, so that a sequence's tiles find what they share in one
+// cache; in the first a list's neighbours are tiles of different sequences and heads anyway.
+constexpr int WINDOW = 64, XCDS = 8;
+constexpr int LONG = 2048;  // tokens a sequence, in the mean: from there on single tiles are ordered
 constexpr int ORDER_HEAD = 16;  // ints before the lists: their lengths
 __host__ __device__ inline long long order_queries(int seqs, int tq, int group) {
   return (long long)tq * group / QROWS + seqs + 1;

@@ -12,93 +12,125 @@ namespace pol {
 
 // ---- the order ------------------------------------------------------------------------------------------------------
 
-// One workgroup lists the tiles, heaviest first (a counting sort by the tiles of the other side that each one reads;
-// its place among equals is free, results do not depend on the order). seqs + 1 sequences, LS lanes on each.
-__global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk, int group, int key_waves,
+// One workgroup lists the tiles by a counting sort (a tile's place among equals is free, results do not depend on the
+// order). seqs + 1 sequences, LS lanes on each.
+__global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk, int group, int key_waves, int by_sequence,
                                                        const int* __restrict__ starts_q,
                                                        const int* __restrict__ starts_k, int* __restrict__ order) {
   constexpr int BUCKETS = 1024;
-  __shared__ int count[BUCKETS];
-  __shared__ int wave_sum[16];
+  __shared__ int count[2][BUCKETS];
+  __shared__ int wave_sum[2][16];
   int ls = 1;
-  while (ls < 1024 && ls * 2 * (long long)(seqs + 1) <= 1024) ls *= 2;
+  if (!by_sequence)
+    while (ls < 1024 && ls * 2 * (long long)(seqs + 1) <= 1024) ls *= 2;
   const int lane = threadIdx.x % ls, first_seq = threadIdx.x / ls, stride = 1024 / ls;
-  const int keys_a_tile = 32 * key_waves;
+  const int per[2] = {QROWS, 32 * key_waves};
   const long long caps[2] = {order_queries(seqs, tq, group), order_keys(seqs, tk, key_waves)};
-  int* list = order + ORDER_HEAD;
-  for (int which = 0; which < 2; ++which) {
-    auto each_tile = [&](auto f) {
-      for (int s = first_seq; s <= seqs; s += stride) {
-        int q0, k0, nq, nk;
-        sequence(starts_q, s, seqs, tq, q0, nq);
-        sequence(starts_k, s, seqs, tk, k0, nk);
-        if (s == seqs) (which ? nq : nk) = 0;
-        const int rows = which ? nk : nq * group, per = which ? keys_a_tile : QROWS, tiles = (rows + per - 1) / per;
-        for (int t = lane; t < tiles; t += ls) {
-          int cost;
+  int* const lists[2] = {order + ORDER_HEAD, order + ORDER_HEAD + 2 * caps[0]};
+  // f(list, sequence, first tile, tiles, bucket) for every stretch of tiles that stays together
+  auto each = [&](auto f) {
+    for (int s = first_seq; s <= seqs; s += stride) {
+      int q0, k0, nq, nk;
+      sequence(starts_q, s, seqs, tq, q0, nq);
+      sequence(starts_k, s, seqs, tk, k0, nk);
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const int mq = which && s == seqs ? 0 : nq, mk = !which && s == seqs ? 0 : nk;
+        const int rows = which ? mk : mq * group, tiles = (rows + per[which] - 1) / per[which];
+        auto bucket = [&](int t) {
+          long long cost;
           if (which) {  // the query rows that see the tile's first key
-            const int from = t * keys_a_tile - (nk - nq);
-            cost = nq - (from > 0 ? from : 0);
-            cost = (int)(((long long)(cost > 0 ? cost : 0) * group + TILE - 1) / TILE);
+            const int from = t * per[1] - (mk - mq);
+            cost = mq - (from > 0 ? from : 0);
+            cost = (cost > 0 ? cost : 0) * group;
           } else {  // the keys that the tile's last row sees
-            const int last = ((t + 1) * QROWS < rows ? (t + 1) * QROWS : rows) - 1, keys = last / group + nk - nq + 1;
-            cost = keys > 0 ? (keys + TILE - 1) / TILE : 0;
+            const int last = ((t + 1) * QROWS < rows ? (t + 1) * QROWS : rows) - 1;
+            cost = last / group + mk - mq + 1;
           }
-          f(s, t, BUCKETS - 1 - (cost < BUCKETS ? cost : BUCKETS - 1));
+          cost = cost > 0 ? (cost + TILE - 1) / TILE : 0;
+          return (int)(BUCKETS - 1 - (cost < BUCKETS ? cost : BUCKETS - 1));
+        };
+        if (by_sequence) {
+          if (tiles) f(which, s, 0, tiles, bucket(which ? 0 : tiles - 1));
+        } else {
+          for (int t = lane; t < tiles; t += ls) f(which, s, t, 1, bucket(t));
         }
       }
-    };
-    count[threadIdx.x] = 0;
-    __syncthreads();
-    each_tile([&](int, int, int b) { atomicAdd(&count[b], 1); });
-    __syncthreads();
-    // exclusive prefix over the buckets
-    const int mine = count[threadIdx.x];
-    int sum = mine;
+    }
+  };
+  count[0][threadIdx.x] = count[1][threadIdx.x] = 0;
+  __syncthreads();
+  each([&](int which, int, int, int n, int b) { atomicAdd(&count[which][b], n); });
+  __syncthreads();
+  // exclusive prefixes over the buckets
+  int mine[2], sum[2];
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    sum[which] = mine[which] = count[which][threadIdx.x];
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-      const int x = __shfl_up(sum, d);
-      if (threadIdx.x % 64 >= d) sum += x;
+      const int x = __shfl_up(sum[which], d);
+      if (threadIdx.x % 64 >= d) sum[which] += x;
     }
-    if (threadIdx.x % 64 == 63) wave_sum[threadIdx.x / 64] = sum;
-    __syncthreads();
+    if (threadIdx.x % 64 == 63) wave_sum[which][threadIdx.x / 64] = sum[which];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
     int before = 0, total = 0;
     for (int w = 0; w < 16; ++w) {
-      if (w < (int)threadIdx.x / 64) before += wave_sum[w];
-      total += wave_sum[w];
+      if (w < (int)threadIdx.x / 64) before += wave_sum[which][w];
+      total += wave_sum[which][w];
     }
-    count[threadIdx.x] = before + sum - mine;
+    count[which][threadIdx.x] = before + sum[which] - mine[which];
     if (threadIdx.x == 0) order[which] = total < caps[which] ? total : (int)caps[which];
-    __syncthreads();
-    each_tile([&](int s, int t, int b) {
-      const int at = atomicAdd(&count[b], 1);
-      if (at < caps[which]) {
-        list[2 * at] = s;
-        list[2 * at + 1] = t;
-      }
-    });
-    __syncthreads();
-    list += 2 * caps[0];
   }
+  __syncthreads();
+  each([&](int which, int s, int t, int n, int b) {
+    int at = atomicAdd(&count[which][b], n);
+    for (int i = 0; i < n; ++i, ++at)  // the heaviest of the sequence first
+      if (at < caps[which]) {
+        lists[which][2 * at] = s;
+        lists[which][2 * at + 1] = t + (which ? i : n - 1 - i);
+      }
+  });
 }
 
 // what a workgroup works on
 struct Place {
-  int tile, kv, q0, nq, k0, nk;
+  int tile, kv, part, q0, nq, k0, nk;
 };
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ bool place(const Attend& a, int which, Place& p) {
-  const int entry = blockIdx.x / a.kv_heads;
+// of `parts` workgroups a tile and key/value head
+__device__ __forceinline__ bool place(const Attend& a, int which, int parts, Place& p) {
+  const int all = uniform(a.order[which]) * a.kv_heads * parts, b = blockIdx.x;
+  int at = b;
+  if (a.by_sequence) {
+    const int base = b / (WINDOW * XCDS) * (WINDOW * XCDS), left = all - base;
+    const int mine = left < WINDOW * XCDS ? (left + XCDS - 1) / XCDS : WINDOW, r = b - base;
+    if (left <= 0 || r / XCDS >= mine) return false;
+    at = base + r % XCDS * mine + r / XCDS;
+    p.part = at % parts, at /= parts;
+  } else {  // the parts take turns on each XCD
+    p.part = b / XCDS % parts;
+    at = b / (XCDS * parts) * XCDS + b % XCDS;
+  }
+  const int entry = at / a.kv_heads;
   if (entry >= uniform(a.order[which])) return false;
   const int* list = a.order + ORDER_HEAD + (which ? 2 * order_queries(a.seqs, a.tq, a.group) : 0) + 2LL * entry;
   const int s = uniform(list[0]);
   p.tile = uniform(list[1]);
-  p.kv = blockIdx.x % a.kv_heads;
+  p.kv = at % a.kv_heads;
   sequence(a.starts_q, s, a.seqs, a.tq, p.q0, p.nq);
   sequence(a.starts_k, s, a.seqs, a.tk, p.k0, p.nk);
   p.q0 = uniform(p.q0), p.nq = uniform(p.nq), p.k0 = uniform(p.k0), p.nk = uniform(p.nk);
   if (s == a.seqs) (which ? p.nq : p.nk) = 0;
   return true;
+}
+// workgroups that cover a list of at most `most` tiles
+unsigned blocks_of(const Attend& a, long long most, int parts) {
+  constexpr long long turn = WINDOW * XCDS;
+  return (unsigned)((most * a.kv_heads * parts + turn - 1) / turn * turn);
 }
 
 // The keys' side of the forward and of the queries' gradient: tiles of TILE keys and their values, one tile ahead.
@@ -159,7 +191,7 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
   __shared__ __align__(16) T ks[2][TILE * DP];
   __shared__ __align__(16) T vs[2][TILE * DP];
   Place p;
-  if (!place(a, 0, p)) return;
+  if (!place(a, 0, 1, p)) return;
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
   const Rows r(a, p);
   Keys<DP, T> keys(a, p);
@@ -240,7 +272,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
   __shared__ __align__(16) T ks[2][TILE * DP];
   __shared__ __align__(16) T vs[2][TILE * DP];
   Place p;
-  if (!place(a, 0, p)) return;
+  if (!place(a, 0, 1, p)) return;
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
   const Rows r(a, p);
   Keys<DP, T> keys(a, p);
@@ -323,16 +355,20 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
 // and their sums are added at the end, in order. Heads of 128 hold three quarters of the values in LDS: with all of them
 // in registers a SIMD has room for one wave only.
 template <typename T, int DP, int KW>
-__global__ __launch_bounds__(256, 2) void k_attend_dkv(Attend a) {
+struct DkvTiles {
+  static constexpr int RT = DP == 64 && KW == 1 ? 128 : 64;
+  alignas(16) T tiles[2][2][RT * DP];  // (turn, q or dout)
+  alignas(16) float lses[2][RT], deltas[2][RT];
+  alignas(16) int places_of[2][RT];  // a row's token from its tile's first
+};
+enum Role { BOTH, KEYS, VALUES };
+template <typename T, int DP, int KW, int ROLE>
+__device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, KW>& lds) {
   constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 256 / CH, SPLIT = 4 / KW;
-  constexpr int RT = DP == 64 ? (KW == 1 ? 128 : 64) : (KW == 4 ? 32 : 64), SUB = RT / 32, N = RT / STEP;
-  constexpr int VR = DP == 64 ? KS : KS / 4;  // of a value row's KS operands, those in registers
-  __shared__ __align__(16) T tiles[2][2][RT * DP];  // (turn, q or dout)
-  __shared__ __align__(16) V8<T> vl[VR < KS ? KW * (KS - VR) * 64 : 1];
-  __shared__ __align__(16) float lses[2][RT], deltas[2][RT];
-  __shared__ __align__(16) int limits[2][RT];
-  Place p;
-  if (!place(a, 1, p)) return;
+  constexpr int RT = DkvTiles<T, DP, KW>::RT, SUB = RT / 32, N = RT / STEP;
+  auto& tiles = lds.tiles;
+  auto &lses = lds.lses, &deltas = lds.deltas;
+  auto& places_of = lds.places_of;
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, w = uniform(threadIdx.x / 64), dim = a.dim, group = a.group;
   const int kw = w % KW, split = w / KW;
   const int rows = p.nq * group, off = p.nk - p.nq;
@@ -343,72 +379,69 @@ __global__ __launch_bounds__(256, 2) void k_attend_dkv(Attend a) {
   // Row tiles start at whole tokens (but for groups above RT, whose rows' places are computed anew for each tile), so
   // that a thread's rows keep their distance from the tile's first token: RT or a little less rows are used of each.
   const int used = group <= RT ? RT / group * group : RT;
+  const int back = used / group;  // tokens of a tile
   const int from = p.tile * 32 * KW - off;  // the first token that sees the tile's first key
   const int first = (from > 0 ? from : 0) * group;
   const int chunk = threadIdx.x % CH ^ swizzle<DP>(threadIdx.x / CH);
   const bool in_row = 8 * chunk < dim;
-  long long qo[N], go[N];
-  auto offsets = [&](int r0) {  // of this thread's rows from the first token of r0
+  const T *qp[N], *gp[N];  // this thread's rows of the next tile to load, and its row's place in lse and delta
+  long long stat = 0;
+  auto places = [&](int r0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int r = r0 % group + (int)threadIdx.x / CH + i * STEP, pos = r / group, head = r % group;
-      qo[i] = pos * a.q_t + head * a.q_h + 8 * chunk;
-      go[i] = pos * a.do_t + head * a.do_h + 8 * chunk;
+      const int r = r0 + (int)threadIdx.x / CH + i * STEP, pos = r / group, head = p.kv * group + r % group;
+      qp[i] = (const T*)a.q + (long long)(p.q0 + pos) * a.q_t + (long long)head * a.q_h + 8 * chunk;
+      gp[i] = (const T*)a.dout + (long long)(p.q0 + pos) * a.do_t + (long long)head * a.do_h + 8 * chunk;
     }
+    const int r = r0 + threadIdx.x;
+    stat = (long long)(p.kv * group + r % group) * a.tq + p.q0 + r / group;
   };
-  offsets(first);
-  const T* qb = (const T*)a.q + (long long)p.q0 * a.q_t + (long long)p.kv * group * a.q_h;
-  const T* gb = (const T*)a.dout + (long long)p.q0 * a.do_t + (long long)p.kv * group * a.do_h;
   float lse = INFINITY, delta = 0.0f;
-  int limit = -1;
-  auto load = [&](int r0, int turn) {
-    if (group > RT) offsets(r0);
-    const long long token = r0 / group;
+  auto load = [&](int r0, int turn) {  // the rows from r0, then the places of those before them
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int row = threadIdx.x / CH + i * STEP;
       const bool there = in_row && row < used && r0 + row < rows;
-      to_lds(qb + token * a.q_t + qo[i], there, tiles[turn][0] + i * 2048 + w * 512);
-      to_lds(gb + token * a.do_t + go[i], there, tiles[turn][1] + i * 2048 + w * 512);
+      to_lds(qp[i], there, tiles[turn][0] + i * 2048 + w * 512);
+      to_lds(gp[i], there, tiles[turn][1] + i * 2048 + w * 512);
     }
     if (threadIdx.x < RT) {
-      const int r = r0 + threadIdx.x, pos = r / group;
-      const bool there = threadIdx.x < used && r < rows;
-      const long long at = (long long)(p.kv * group + r % group) * a.tq + p.q0 + pos;
-      lse = there ? a.lse[at] : INFINITY;
-      delta = there ? a.delta[at] : 0.0f;
-      limit = there ? pos + off : -1;
+      const bool there = threadIdx.x < used && r0 + (int)threadIdx.x < rows;
+      lse = there ? a.lse[stat] : INFINITY;
+      if (ROLE != VALUES) delta = there ? a.delta[stat] : 0.0f;
+    }
+    if (group > RT) {
+      if (r0 >= used) places(r0 - used);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) qp[i] -= back * a.q_t, gp[i] -= back * a.do_t;
+      stat -= back;
     }
   };
   // From the last rows, which every key tile of the sequence reads, to the tile's first: workgroups that run side by
   // side then read the same rows at about the same time, from the L2 cache of their XCD.
   const int start = first + (rows > first ? (rows - 1 - first) / used * used : -used);
+  places(start >= first ? start : 0);
   if (start >= first) load(start, 0);
-  V8<T> k[KS], v[VR];
+  V8<T> k[KS], v[KS];
   load_rows<DP>(valid ? (const T*)a.k + (long long)(p.k0 + key) * a.k_t + (long long)p.kv * a.k_h : nullptr, dim, h, k);
-  {
-    V8<T> all[KS];
-    load_rows<DP>(valid ? (const T*)a.v + (long long)(p.k0 + key) * a.v_t + (long long)p.kv * a.v_h : nullptr, dim, h, all);
-#pragma unroll
-    for (int x = 0; x < VR; ++x) v[x] = all[x];
-#pragma unroll
-    for (int x = VR; x < KS; ++x)
-      if (split == 0) vl[(kw * (KS - VR) + x - VR) * 64 + l] = all[x];
-  }
+  if (ROLE != VALUES)
+    load_rows<DP>(valid ? (const T*)a.v + (long long)(p.k0 + key) * a.v_t + (long long)p.kv * a.v_h : nullptr, dim, h, v);
   F16x dk[DT] = {}, dv[DT] = {};
+  if (threadIdx.x < RT && group <= RT) places_of[0][threadIdx.x] = places_of[1][threadIdx.x] = threadIdx.x / group;
   int turn = 0, sub0 = 0, token0 = start / group;
   for (int r0 = start; r0 >= first; r0 -= used, turn ^= 1, sub0 += SUB) {
     if (threadIdx.x < RT) {
       lses[turn][threadIdx.x] = lse;
       deltas[turn][threadIdx.x] = delta;
-      limits[turn][threadIdx.x] = limit;
+      if (group > RT) places_of[turn][threadIdx.x] = (r0 % group + (int)threadIdx.x) / group;
     }
     loads_done();
     __syncthreads();
     if (r0 - used >= first) load(r0 - used, turn ^ 1);
     if (key0 >= p.nk) continue;
     const int token = group <= RT ? token0 : r0 / group, inside = group <= RT ? 0 : r0 % group;
-    token0 -= used / group;
+    token0 -= back;
     const T *qt = tiles[turn][0], *gt = tiles[turn][1];
 #pragma unroll
     for (int i = 0; i < SUB; ++i) {
@@ -420,7 +453,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_dkv(Attend a) {
 #pragma unroll
       for (int x = 0; x < KS; ++x) {
         s = mfma(read_rows<DP>(qt, 32 * i, x, n, h), k[x], s);
-        dp = mfma(read_rows<DP>(gt, 32 * i, x, n, h), x < VR ? v[x < VR ? x : 0] : vl[(kw * (KS - VR) + x - VR) * 64 + l], dp);
+        if (ROLE != VALUES) dp = mfma(read_rows<DP>(gt, 32 * i, x, n, h), v[x], dp);
       }
       const bool masked = low < key0 + 31;
 #pragma unroll
@@ -432,10 +465,10 @@ __global__ __launch_bounds__(256, 2) void k_attend_dkv(Attend a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[4 * j + e] = exp2_fast(fmaf(s[4 * j + e], c, -ls[e]));
-          dp[4 * j + e] = s[4 * j + e] * (dp[4 * j + e] - de[e]);
+          if (ROLE != VALUES) dp[4 * j + e] = s[4 * j + e] * (dp[4 * j + e] - de[e]);
         }
         if (masked) {
-          const I4 li = *(const I4*)(limits[turn] + at);
+          const I4 li = *(const I4*)(places_of[turn] + at) + (token + off);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (key > li[e]) s[4 * j + e] = dp[4 * j + e] = 0.0f;
@@ -446,8 +479,8 @@ __global__ __launch_bounds__(256, 2) void k_attend_dkv(Attend a) {
         const V8<T> pr = pack<T>(s, x), ds = pack<T>(dp, x);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          dv[d] = mfma(read_columns<DP>(gt, 32 * i + 16 * x, d, l), pr, dv[d]);
-          dk[d] = mfma(read_columns<DP>(qt, 32 * i + 16 * x, d, l), ds, dk[d]);
+          if (ROLE != KEYS) dv[d] = mfma(read_columns<DP>(gt, 32 * i + 16 * x, d, l), pr, dv[d]);
+          if (ROLE != VALUES) dk[d] = mfma(read_columns<DP>(qt, 32 * i + 16 * x, d, l), ds, dk[d]);
         }
       }
     }
@@ -460,6 +493,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_dkv(Attend a) {
     for (int o = 1; o < SPLIT; ++o)
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
+        if (ROLE == (which ? KEYS : VALUES)) continue;
         F16x* acc = which ? dv : dk;
         __syncthreads();
         if (split == o)
@@ -477,8 +511,27 @@ __global__ __launch_bounds__(256, 2) void k_attend_dkv(Attend a) {
     if (split) return;
   }
   const long long at = ((long long)(p.k0 + key) * a.kv_heads + p.kv) * dim;
-  store_rows<DP>(valid ? (T*)a.dk + at : nullptr, dim, h, dk, a.scale);
-  store_rows<DP>(valid ? (T*)a.dv + at : nullptr, dim, h, dv, 1.0f);
+  if (ROLE != VALUES) store_rows<DP>(valid ? (T*)a.dk + at : nullptr, dim, h, dk, a.scale);
+  if (ROLE != KEYS) store_rows<DP>(valid ? (T*)a.dv + at : nullptr, dim, h, dv, 1.0f);
+}
+
+#ifndef W64
+#define W64 2
+#endif
+#ifndef W128
+#define W128 2
+#endif
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? W64 : W128, DP == 64 ? W64 : W128))) void k_attend_dkv(Attend a) {
+  __shared__ DkvTiles<T, DP, KW> lds;
+  Place p;
+  if constexpr (DP == 64) {
+    if (place(a, 1, 1, p)) dkv_tile<T, DP, KW, BOTH>(a, p, lds);
+  } else {
+    if (!place(a, 1, 2, p)) return;
+    if (p.part) dkv_tile<T, DP, KW, VALUES>(a, p, lds);
+    else dkv_tile<T, DP, KW, KEYS>(a, p, lds);
+  }
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------
@@ -486,6 +539,9 @@ __global__ __launch_bounds__(256, 2) void k_attend_dkv(Attend a) {
 // Keys a workgroup of the keys' gradients: 128, or fewer where sequences are short (the waves would have none) or tiles
 // few (a causal tile's work goes from all rows to none: several a CU even that out).
 int key_waves(int kv_heads, int seqs, int tk) {
+#ifdef FORCE
+  return FORCE;
+#endif
   const long long tiles = (long long)tk / 128 * kv_heads;
   if (tk <= 48LL * seqs) return 1;
   return tk <= 96LL * seqs || tiles < 2048 ? 2 : 4;
@@ -497,17 +553,16 @@ size_t attend_work_bytes(int kv_heads, int seqs, int tq, int tk, int group) {
 
 template <typename T, int DP>
 int attend(hipStream_t st, const Attend& a) {
-  const long long blocks = order_queries(a.seqs, a.tq, a.group) * a.kv_heads;
-  k_attend<T, DP><<<(unsigned)blocks, 256, 0, st>>>(a);
+  k_attend<T, DP><<<blocks_of(a, order_queries(a.seqs, a.tq, a.group), 1), 256, 0, st>>>(a);
   return (int)hipGetLastError();
 }
 template <typename T, int DP>
 int attend_vjp(hipStream_t st, const Attend& a) {
-  if (a.tq) k_attend_dq<T, DP><<<(unsigned)(order_queries(a.seqs, a.tq, a.group) * a.kv_heads), 256, 0, st>>>(a);
+  if (a.tq) k_attend_dq<T, DP><<<blocks_of(a, order_queries(a.seqs, a.tq, a.group), 1), 256, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (!a.tk) return 0;
-  const unsigned blocks = (unsigned)(order_keys(a.seqs, a.tk, a.key_waves) * a.kv_heads);
+  const unsigned blocks = blocks_of(a, order_keys(a.seqs, a.tk, a.key_waves), DP == 64 ? 1 : 2);
   switch (a.key_waves) {
     case 1: k_attend_dkv<T, DP, 1><<<blocks, 256, 0, st>>>(a); break;
     case 2: k_attend_dkv<T, DP, 2><<<blocks, 256, 0, st>>>(a); break;
@@ -517,7 +572,8 @@ int attend_vjp(hipStream_t st, const Attend& a) {
 }
 
 int launch_attend(hipStream_t st, int type, const Attend& a) {
-  k_attend_order<<<1, 1024, 0, st>>>(a.seqs, a.tq, a.tk, a.group, a.key_waves, a.starts_q, a.starts_k, (int*)a.order);
+  k_attend_order<<<1, 1024, 0, st>>>(a.seqs, a.tq, a.tk, a.group, a.key_waves, a.by_sequence, a.starts_q, a.starts_k,
+                                  (int*)a.order);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.tq) return (int)e;
   if (type == BF16) return a.dim <= 64 ? attend<__bf16, 64>(st, a) : attend<__bf16, 128>(st, a);
@@ -536,7 +592,7 @@ bool attention_takes(int type, int heads, int kv_heads, int dim, int seqs, int t
   if ((type != pol::BF16 && type != pol::F16) || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 8 || dim > 128 ||
       dim % 8 || seqs < 0 || tq < 0 || tk < 0 || tk >= 1 << 30 || (long long)tq * (heads / kv_heads) >= 1 << 30)
     return false;
-  const long long most = (1LL << 24) - 1;  // workgroups of 256 work-items a launch
+  const long long most = (1LL << 23) - 1024;  // workgroups of 256 work-items a launch, two for a key tile of large heads
   return pol::order_queries(seqs, tq, heads / kv_heads) * kv_heads <= most && pol::order_keys(seqs, tk, 1) * kv_heads <= most;
 }
 }  // namespace
@@ -555,6 +611,7 @@ int dk_attention(hipStream_t st, int type, int heads, int kv_heads, int dim, int
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
   a.key_waves = pol::key_waves(kv_heads, seqs, tk);
+  a.by_sequence = tq <= (long long)pol::LONG * seqs;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.out = out, a.lse = lse, a.order = (const int*)work;
   return pol::launch_attend(st, type, a);
 }
@@ -572,6 +629,7 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
   a.key_waves = pol::key_waves(kv_heads, seqs, tk);
+  a.by_sequence = tq <= (long long)pol::LONG * seqs;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.order = (const int*)work;
   a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse);
   a.dout = dout, a.do_t = do_t, a.do_h = do_h, a.delta = delta, a.dq = dq, a.dk = dk, a.dv = dv;
