@@ -34,7 +34,7 @@ struct Attend {
   long long q_t, q_h, k_t, k_h, v_t, v_h;  // elements from token to token, and from head to head
   int heads, kv_heads, group, dim, seqs, tq, tk;
   int by_sequence;  // the order of the tiles, see below
-  int key_waves;  // waves of a workgroup of the keys' gradients that differ in their 32 keys: 1, 2 or 4
+  int key_waves;  // waves of a workgroup of the keys' gradients that differ in their 32 keys: 2 or 4
   const int *starts_q, *starts_k;
   float scale;
   void* out;   // (tq, heads, dim)
@@ -121,6 +121,10 @@ __device__ __forceinline__ void to_lds(const T* from, bool valid, T* wave_at) {
   __builtin_amdgcn_global_load_lds((G)p, (L)wave_at, 16, 0, 0);
 }
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+
+// The compiler moves nothing across: LDS reads that a phase issues ahead of the next one's use stay ahead. Left to
+// itself it puts each read just before its product, and waits for every one.
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
 
 template <typename T>
 __device__ __forceinline__ V8<T> zero8() { return V8<T>{}; }

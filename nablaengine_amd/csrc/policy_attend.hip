@@ -351,21 +351,26 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
 
 // A wave keeps 32 keys and their values as B operands and walks over the rows that see them; rows lie in LDS, RT at a
 // time. S = Q K^T here, so that a lane holds 16 rows of ONE key and P, dS are the B operands of dV^T = dO^T P and dK^T =
-// Q^T dS. KW of the four waves differ in their keys, the others take every 4/KW-th subtile of 32 rows of the same keys,
-// and their sums are added at the end, in order. Heads of 128 hold three quarters of the values in LDS: with all of them
-// in registers a SIMD has room for one wave only.
-template <typename T, int DP, int KW>
+// Q^T dS. KW of the waves differ in their keys, the others take every SPLIT-th subtile of 32 rows of the same keys, and
+// their sums are added at the end, in order.
+template <typename T, int DP>
 struct DkvTiles {
-  static constexpr int RT = DP == 64 && KW == 1 ? 128 : 64;
+  static constexpr int WAVES = DP == 64 ? 4 : 8, RT = DP == 64 ? 64 : 128;
   alignas(16) T tiles[2][2][RT * DP];  // (turn, q or dout)
   alignas(16) float lses[2][RT], deltas[2][RT];
   alignas(16) int places_of[2][RT];  // a row's token from its tile's first
 };
+// Heads of 128: dk and dv together take 128 registers a lane, with the keys and values more than two waves a SIMD have.
+// One workgroup takes dk and another dv (a fourth more products, the scores twice): 1150 us at 2 x (8192 and 2800) tokens
+// of 16 heads against 1480 us with both in one and part of the operands in LDS or scratch. Eight waves share a tile of
+// 128 rows there: with four, the tiles that all rows read are one round's length each.
 enum Role { BOTH, KEYS, VALUES };
 template <typename T, int DP, int KW, int ROLE>
-__device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, KW>& lds) {
-  constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 256 / CH, SPLIT = 4 / KW;
-  constexpr int RT = DkvTiles<T, DP, KW>::RT, SUB = RT / 32, N = RT / STEP;
+__device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP>& lds) {
+  constexpr int WAVES = DkvTiles<T, DP>::WAVES, RT = DkvTiles<T, DP>::RT;
+  constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 64 * WAVES / CH, SPLIT = WAVES / KW;
+  constexpr int AHEAD = DP == 64 ? 2 : 1;  // of a subtile's two column operands, those read during the exponentials
+  constexpr int SUB = RT / 32, N = RT / STEP;
   auto& tiles = lds.tiles;
   auto &lses = lds.lses, &deltas = lds.deltas;
   auto& places_of = lds.places_of;
@@ -402,8 +407,8 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
     for (int i = 0; i < N; ++i) {
       const int row = threadIdx.x / CH + i * STEP;
       const bool there = in_row && row < used && r0 + row < rows;
-      to_lds(qp[i], there, tiles[turn][0] + i * 2048 + w * 512);
-      to_lds(gp[i], there, tiles[turn][1] + i * 2048 + w * 512);
+      to_lds(qp[i], there, tiles[turn][0] + (i * WAVES + w) * 512);
+      to_lds(gp[i], there, tiles[turn][1] + (i * WAVES + w) * 512);
     }
     if (threadIdx.x < RT) {
       const bool there = threadIdx.x < used && r0 + (int)threadIdx.x < rows;
@@ -429,6 +434,10 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
     load_rows<DP>(valid ? (const T*)a.v + (long long)(p.k0 + key) * a.v_t + (long long)p.kv * a.v_h : nullptr, dim, h, v);
   F16x dk[DT] = {}, dv[DT] = {};
   if (threadIdx.x < RT && group <= RT) places_of[0][threadIdx.x] = places_of[1][threadIdx.x] = threadIdx.x / group;
+  int low_of[SUB], most_of[SUB];  // from a tile's first token to those of a subtile's first row and, at most, its last
+#pragma unroll
+  for (int i = 0; i < SUB; ++i)
+    low_of[i] = 32 * i / group, most_of[i] = group <= RT ? (32 * i + 31 < used ? 32 * i + 31 : used - 1) / group : 1;
   int turn = 0, sub0 = 0, token0 = start / group;
   for (int r0 = start; r0 >= first; r0 -= used, turn ^= 1, sub0 += SUB) {
     if (threadIdx.x < RT) {
@@ -440,21 +449,40 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
     __syncthreads();
     if (r0 - used >= first) load(r0 - used, turn ^ 1);
     if (key0 >= p.nk) continue;
-    const int token = group <= RT ? token0 : r0 / group, inside = group <= RT ? 0 : r0 % group;
+    const int token = group <= RT ? token0 : r0 / group;
     token0 -= back;
     const T *qt = tiles[turn][0], *gt = tiles[turn][1];
 #pragma unroll
     for (int i = 0; i < SUB; ++i) {
       if (SPLIT > 1 && (sub0 + i) % SPLIT != split) continue;
       // the last keys that the subtile's first row and (at most) its last one see
-      const int low = token + (32 * i) / group + off, most = ((32 * i + 31 < used ? 32 * i + 31 : used - 1) + inside) / group;
-      if (32 * i >= used || r0 + 32 * i >= rows || token + most + off < key0) continue;
+      const int low = token + low_of[i] + off;
+      if (32 * i >= used || r0 + 32 * i >= rows || token + most_of[i] + off < key0) continue;
       F16x s = {}, dp = {};
 #pragma unroll
-      for (int x = 0; x < KS; ++x) {
-        s = mfma(read_rows<DP>(qt, 32 * i, x, n, h), k[x], s);
-        if (ROLE != VALUES) dp = mfma(read_rows<DP>(gt, 32 * i, x, n, h), v[x], dp);
+      for (int y = 0; y < KS; y += 4) {
+        V8<T> qr[4], gr[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          qr[x] = read_rows<DP>(qt, 32 * i, y + x, n, h);
+          if (ROLE != VALUES) gr[x] = read_rows<DP>(gt, 32 * i, y + x, n, h);
+        }
+        phase();
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          s = mfma(qr[x], k[y + x], s);
+          if (ROLE != VALUES) dp = mfma(gr[x], v[y + x], dp);
+        }
       }
+      V8<T> qc[2][DT], gc[2][DT];  // on their way during the exponentials
+#pragma unroll
+      for (int x = 0; x < AHEAD; ++x)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          if (ROLE != KEYS) gc[x][d] = read_columns<DP>(gt, 32 * i + 16 * x, d, l);
+          if (ROLE != VALUES) qc[x][d] = read_columns<DP>(qt, 32 * i + 16 * x, d, l);
+        }
+      phase();
       const bool masked = low < key0 + 31;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -479,8 +507,8 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
         const V8<T> pr = pack<T>(s, x), ds = pack<T>(dp, x);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          if (ROLE != KEYS) dv[d] = mfma(read_columns<DP>(gt, 32 * i + 16 * x, d, l), pr, dv[d]);
-          if (ROLE != VALUES) dk[d] = mfma(read_columns<DP>(qt, 32 * i + 16 * x, d, l), ds, dk[d]);
+          if (ROLE != KEYS) dv[d] = mfma(x < AHEAD ? gc[x][d] : read_columns<DP>(gt, 32 * i + 16 * x, d, l), pr, dv[d]);
+          if (ROLE != VALUES) dk[d] = mfma(x < AHEAD ? qc[x][d] : read_columns<DP>(qt, 32 * i + 16 * x, d, l), ds, dk[d]);
         }
       }
     }
@@ -515,15 +543,9 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
   if (ROLE != KEYS) store_rows<DP>(valid ? (T*)a.dv + at : nullptr, dim, h, dv, 1.0f);
 }
 
-#ifndef W64
-#define W64 2
-#endif
-#ifndef W128
-#define W128 2
-#endif
 template <typename T, int DP, int KW>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? W64 : W128, DP == 64 ? W64 : W128))) void k_attend_dkv(Attend a) {
-  __shared__ DkvTiles<T, DP, KW> lds;
+__global__ __launch_bounds__(DP == 64 ? 256 : 512) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_dkv(Attend a) {
+  __shared__ DkvTiles<T, DP> lds;
   Place p;
   if constexpr (DP == 64) {
     if (place(a, 1, 1, p)) dkv_tile<T, DP, KW, BOTH>(a, p, lds);
@@ -536,19 +558,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 
 
 // ---- launches -------------------------------------------------------------------------------------------------------
 
-// Keys a workgroup of the keys' gradients: 128, or fewer where sequences are short (the waves would have none) or tiles
-// few (a causal tile's work goes from all rows to none: several a CU even that out).
-int key_waves(int kv_heads, int seqs, int tk) {
-#ifdef FORCE
-  return FORCE;
-#endif
-  const long long tiles = (long long)tk / 128 * kv_heads;
-  if (tk <= 48LL * seqs) return 1;
-  return tk <= 96LL * seqs || tiles < 2048 ? 2 : 4;
+// Keys a workgroup of the keys' gradients: 128, or 64 where sequences are short (half of the waves would have none).
+int key_waves(int seqs, int tk) {
+  return tk <= 96LL * seqs ? 2 : 4;
 }
-size_t attend_work_bytes(int kv_heads, int seqs, int tq, int tk, int group) {
+size_t attend_work_bytes(int seqs, int tq, int tk, int group) {
   return sizeof(int) * (ORDER_HEAD + 2 * (size_t)(order_queries(seqs, tq, group) +
-                                                  order_keys(seqs, tk, key_waves(kv_heads, seqs, tk))));
+                                                  order_keys(seqs, tk, key_waves(seqs, tk))));
 }
 
 template <typename T, int DP>
@@ -563,11 +579,9 @@ int attend_vjp(hipStream_t st, const Attend& a) {
   if (e != hipSuccess) return (int)e;
   if (!a.tk) return 0;
   const unsigned blocks = blocks_of(a, order_keys(a.seqs, a.tk, a.key_waves), DP == 64 ? 1 : 2);
-  switch (a.key_waves) {
-    case 1: k_attend_dkv<T, DP, 1><<<blocks, 256, 0, st>>>(a); break;
-    case 2: k_attend_dkv<T, DP, 2><<<blocks, 256, 0, st>>>(a); break;
-    default: k_attend_dkv<T, DP, 4><<<blocks, 256, 0, st>>>(a);
-  }
+  constexpr int threads = 64 * DkvTiles<T, DP>::WAVES;
+  if (a.key_waves == 2) k_attend_dkv<T, DP, 2><<<blocks, threads, 0, st>>>(a);
+  else k_attend_dkv<T, DP, 4><<<blocks, threads, 0, st>>>(a);
   return (int)hipGetLastError();
 }
 
@@ -592,8 +606,8 @@ bool attention_takes(int type, int heads, int kv_heads, int dim, int seqs, int t
   if ((type != pol::BF16 && type != pol::F16) || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 8 || dim > 128 ||
       dim % 8 || seqs < 0 || tq < 0 || tk < 0 || tk >= 1 << 30 || (long long)tq * (heads / kv_heads) >= 1 << 30)
     return false;
-  const long long most = (1LL << 23) - 1024;  // workgroups of 256 work-items a launch, two for a key tile of large heads
-  return pol::order_queries(seqs, tq, heads / kv_heads) * kv_heads <= most && pol::order_keys(seqs, tk, 1) * kv_heads <= most;
+  const long long most = (1LL << 22) - 1024;  // workgroups of 256 or 512 work-items a launch
+  return pol::order_queries(seqs, tq, heads / kv_heads) * kv_heads <= most && pol::order_keys(seqs, tk, 2) * kv_heads <= most;
 }
 }  // namespace
 
@@ -610,7 +624,7 @@ int dk_attention(hipStream_t st, int type, int heads, int kv_heads, int dim, int
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
-  a.key_waves = pol::key_waves(kv_heads, seqs, tk);
+  a.key_waves = pol::key_waves(seqs, tk);
   a.by_sequence = tq <= (long long)pol::LONG * seqs;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.out = out, a.lse = lse, a.order = (const int*)work;
   return pol::launch_attend(st, type, a);
@@ -628,7 +642,7 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
-  a.key_waves = pol::key_waves(kv_heads, seqs, tk);
+  a.key_waves = pol::key_waves(seqs, tk);
   a.by_sequence = tq <= (long long)pol::LONG * seqs;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.order = (const int*)work;
   a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse);
@@ -638,7 +652,7 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
 
 long long dk_attention_work_bytes(int heads, int kv_heads, int seqs, int tq, int tk) {
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || seqs < 0 || tq < 0 || tk < 0) return 0;
-  return (long long)pol::attend_work_bytes(kv_heads, seqs, tq, tk, heads / kv_heads);
+  return (long long)pol::attend_work_bytes(seqs, tq, tk, heads / kv_heads);
 }
 
 }  // extern "C"
