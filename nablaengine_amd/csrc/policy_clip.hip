@@ -36,7 +36,7 @@ struct Grads {
 };
 static_assert(sizeof(Grads) <= 4000, "kernel arguments");
 
-// f(tensor, first element, element past the last) for each unit of this workgroup's share
+// f(tensor, first element, element past the last) for each tensor of this workgroup's share of the units
 template <typename F>
 __device__ __forceinline__ void my_units(const Grads& a, F f) {
   int u = (int)((long long)blockIdx.x * a.units / gridDim.x);
@@ -46,34 +46,45 @@ __device__ __forceinline__ void my_units(const Grads& a, F f) {
     const int mid = (lo + hi) / 2;
     if (a.t[mid].unit <= u) lo = mid; else hi = mid;
   }
-  for (; u < end; ++u) {
-    while (lo + 1 < a.count && a.t[lo + 1].unit <= u) ++lo;
-    const long long at = (long long)(u - a.t[lo].unit) * UNIT, n = a.t[lo].n;
-    f(a.t[lo], at, at + UNIT < n ? at + UNIT : n);
+  for (; u < end; ++lo) {
+    const int next = lo + 1 < a.count && a.t[lo + 1].unit < end ? a.t[lo + 1].unit : end;
+    const long long at = (long long)(u - a.t[lo].unit) * UNIT, to = (long long)(next - a.t[lo].unit) * UNIT;
+    f(a.t[lo], at, to < a.t[lo].n ? to : a.t[lo].n);
+    u = next;
   }
+}
+
+// f(first element, elements) for steps of `most` vectors a thread, then of one, then of single elements
+template <int E, int MOST, typename F>
+__device__ __forceinline__ void steps(long long at, long long end, F f) {
+  for (; end - at >= (long long)MOST * E * BLOCK; at += MOST * E * BLOCK)
+    f(at + threadIdx.x * E, std::integral_constant<int, MOST>{});
+  for (; end - at >= E * BLOCK; at += E * BLOCK) f(at + threadIdx.x * E, std::integral_constant<int, 1>{});
+  for (at += threadIdx.x; at < end; at += BLOCK) f(at, std::integral_constant<int, 0>{});
 }
 
 template <typename T>
 __device__ __forceinline__ double squares(const T* g, long long at, long long end) {
-  constexpr int E = Vec<T>::E, PER = UNIT / (E * BLOCK);  // vectors a thread
+  constexpr int E = Vec<T>::E;
   double s = 0.0;
-  if (end - at == UNIT) {
-    Vec<T> v[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = load16(g + at + (i * BLOCK + (int)threadIdx.x) * E);
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const double d = (double)(float)v[i].v[e];
-        s = fma(d, d, s);
-      }
-  } else {
-    for (long long i = at + threadIdx.x; i < end; i += BLOCK) {
+  steps<E, 8>(at, end, [&](long long i, auto count) {
+    constexpr int N = decltype(count)::value;
+    if constexpr (N == 0) {
       const double d = (double)(float)g[i];
       s = fma(d, d, s);
+    } else {
+      Vec<T> v[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = load16(g + i + k * BLOCK * E);
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const double d = (double)(float)v[k].v[e];
+          s = fma(d, d, s);
+        }
     }
-  }
+  });
   return s;
 }
 
@@ -113,30 +124,30 @@ __global__ __launch_bounds__(BLOCK) void k_grad_norm(const double* __restrict__ 
   if (threadIdx.x == 0) *norm = (float)r;
 }
 
-// an in-place call loads what another thread never writes: g and out are the same elements, or do not overlap
+// in place every thread reads what it writes itself, and reads it first
 template <typename T, typename O>
 __device__ __forceinline__ void scale(const T* g, O* out, long long at, long long end, float f) {
-  constexpr int E = Vec<T>::E, PER = UNIT / (E * BLOCK), OE = Vec<O>::E, K = E > OE ? E : OE;  // elements a step
-  static_assert(PER >= 1 && K % E == 0 && K % OE == 0, "");
-  if (end - at == UNIT) {
-    constexpr int STEPS = UNIT / (K * BLOCK);
-    Vec<T> v[STEPS][K / E];
+  constexpr int E = Vec<T>::E, OE = Vec<O>::E;
+  static_assert(E % OE == 0, "an output element has as many bytes as the gradient's, or more");
+  steps<E, 4>(at, end, [&](long long i, auto count) {
+    constexpr int N = decltype(count)::value;
+    if constexpr (N == 0) {
+      out[i] = (O)((float)g[i] * f);
+    } else {
+      Vec<T> v[N];
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i)
+      for (int k = 0; k < N; ++k) v[k] = load16(g + i + k * BLOCK * E);
 #pragma unroll
-      for (int j = 0; j < K / E; ++j) v[i][j] = load16(g + at + (i * BLOCK + (int)threadIdx.x) * K + j * E);
+      for (int k = 0; k < N; ++k)
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i)
+        for (int j = 0; j < E / OE; ++j) {
+          Vec<O> o;
 #pragma unroll
-      for (int j = 0; j < K / OE; ++j) {
-        Vec<O> o;
-#pragma unroll
-        for (int e = 0; e < OE; ++e) o.v[e] = (O)((float)v[i][(j * OE + e) / E].v[(j * OE + e) % E] * f);
-        store16(out + at + (i * BLOCK + (int)threadIdx.x) * K + j * OE, o);
-      }
-  } else {
-    for (long long i = at + threadIdx.x; i < end; i += BLOCK) out[i] = (O)((float)g[i] * f);
-  }
+          for (int e = 0; e < OE; ++e) o.v[e] = (O)((float)v[k].v[j * OE + e] * f);
+          store16(out + i + k * BLOCK * E + j * OE, o);
+        }
+    }
+  });
 }
 
 __global__ __launch_bounds__(BLOCK) void k_clip(Grads a, const double* __restrict__ sums, int count, float limit,

@@ -310,8 +310,10 @@ __global__ __launch_bounds__(1024) void k_norm_params(int blocks, int n, const f
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   const long long col = (long long)blockIdx.x * 64 + lane;  // of the 2 n columns
   float s = 0.0f;
-  if (col < 2LL * n)
+  if (col < 2LL * n) {
+#pragma unroll 8
     for (int i = wave; i < blocks; i += 16) s += part[(long long)i * 2 * n + col];
+  }
   add[wave][lane] = s;
   __syncthreads();
   if (wave == 0 && col < 2LL * n) {
@@ -337,18 +339,22 @@ bool by_width(int nv, F f) {
 #undef POL_CASE
   return false;
 }
-int lanes_of(int nv) {
-  int lanes = WIDE;
-  by_width(nv, [&](auto l, auto) { lanes = decltype(l)::value; });
-  return lanes;
+// lanes a row, and vectors a lane
+void group_of(int nv, int& lanes, int& vectors) {
+  lanes = WIDE, vectors = 2;
+  by_width(nv, [&](auto l, auto c) { lanes = decltype(l)::value, vectors = decltype(c)::value; });
 }
 int vectors_of(int n, int type) { const int e = 16 / bytes_of(type); return (n + e - 1) / e; }
 
-// the backward's workgroups: each row in flight at once at most, two workgroups a CU
+// The backward's workgroups: each row in flight at once at most, and what the CUs hold at once (of 8 waves: three with one
+// vector a lane, two with two; more would only write more partial rows). 524288 x 256 bfloat16: 174 us with two a CU, 151
+// with three, 194 with four, which take a second round.
 int vjp_blocks(long long rows, int n, int type) {
-  const int lanes = lanes_of(vectors_of(n, type)), groups = vjp_block(lanes) / lanes;
-  const long long need = (rows + groups - 1) / groups;
-  return (int)(need < 2 * CUS ? need : 2 * CUS);
+  int lanes, vectors;
+  group_of(vectors_of(n, type), lanes, vectors);
+  const int groups = vjp_block(lanes) / lanes;
+  const long long need = (rows + groups - 1) / groups, most = (vectors == 1 && lanes <= 512 ? 3 : 2) * CUS;
+  return (int)(need < most ? need : most);
 }
 
 template <typename T, typename W>

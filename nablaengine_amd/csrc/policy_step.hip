@@ -20,7 +20,7 @@ struct Step {
   const int* lengths;
   float scale;
   void* out;  // (worlds, heads, dim)
-  int stretches, stretch;
+  int stretches, stretch, units;
   float* part;  // (stretches, worlds, heads, dim + 2): output sums, running maximum, sum
 };
 
@@ -34,29 +34,47 @@ __device__ __forceinline__ float dot2(const _Float16* a, const _Float16* b, floa
 }
 
 constexpr float LOG2E_STEP = 1.4426950408889634f;
-constexpr int UNROLL = 4;
+constexpr int UNROLL = 2;
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }  // below 2^-126: 0
 
-template <typename T, int LPR, int GC>
+// W of a workgroup's four waves share a unit (one world, key/value head, up to GC of its query heads and stretch)
+template <typename T, int LPR, int GC, int W>
 __global__ __launch_bounds__(256) void k_step(Step a) {
-  constexpr int RPW = 64 / LPR, ROWS = 4 * RPW * UNROLL;  // keys a wave reads at once; keys a turn of the workgroup
+  constexpr int RPW = 64 / LPR, BATCH = RPW * UNROLL;  // keys a wave reads at once, and in one turn
   __shared__ float wm[4][GC], wl[4][GC];
   __shared__ float wo[4][GC][LPR * 8];
+  const int l = threadIdx.x % 64, w = threadIdx.x / 64, part = l % LPR, rg = l / LPR, d0 = part * 8;
   const int chunks = (a.group + GC - 1) / GC;
-  int id = blockIdx.x;
+  int id = blockIdx.x * (4 / W) + w / W;
+  const bool exists = id < a.units;
+  if (W == 1 && !exists) return;
+  if (!exists) id = 0;
   const int g0 = id % chunks * GC;
   id /= chunks;
   const int kv = id % a.kv_heads;
   id /= a.kv_heads;
   const int stretch = id % a.stretches, world = id / a.stretches;
-  int length = a.lengths[world];
+  int length = exists ? a.lengths[world] : 0;
   length = length < 0 ? 0 : length > a.capacity ? a.capacity : length;
   const long long from = (long long)stretch * a.stretch, to = from + a.stretch;
   const int begin = from < length ? (int)from : length, end = to < length ? (int)to : length;
-  const int l = threadIdx.x % 64, w = threadIdx.x / 64, part = l % LPR, rg = l / LPR, d0 = part * 8;
   const bool in_row = d0 < a.dim;
-  const T* kp = (const T*)a.k + (long long)world * a.k_w + (long long)kv * a.k_h + d0;
-  const T* vp = (const T*)a.v + (long long)world * a.v_w + (long long)kv * a.v_h + d0;
-
+  int key = begin + w % W * BATCH + rg;  // this lane's next key to read
+  const T* kp = (const T*)a.k + (long long)world * a.k_w + (long long)kv * a.k_h + key * a.k_t + d0;
+  const T* vp = (const T*)a.v + (long long)world * a.v_w + (long long)kv * a.v_h + key * a.v_t + d0;
+  Vec<T> kn[UNROLL], vn[UNROLL];  // one turn ahead
+  auto read = [&] {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const bool in = in_row && key + u * RPW < end;
+      kn[u] = in ? load16(kp + u * RPW * a.k_t) : Vec<T>{};
+      vn[u] = in ? load16(vp + u * RPW * a.v_t) : Vec<T>{};
+    }
+    key += W * BATCH;
+    kp += W * BATCH * a.k_t;
+    vp += W * BATCH * a.v_t;
+  };
+  read();
   Vec<T> q[GC];
 #pragma unroll
   for (int g = 0; g < GC; ++g) {
@@ -73,14 +91,11 @@ __global__ __launch_bounds__(256) void k_step(Step a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[g][e] = 0.0f;
   }
-  for (int key0 = begin + w * RPW * UNROLL + rg; key0 - rg < end; key0 += ROWS) {
+  for (int key0 = begin + w % W * BATCH; key0 < end; key0 += W * BATCH) {
     Vec<T> k[UNROLL], v[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const bool in = in_row && key0 + u * RPW < end;
-      k[u] = in ? load16(kp + (long long)(key0 + u * RPW) * a.k_t) : Vec<T>{};
-      v[u] = in ? load16(vp + (long long)(key0 + u * RPW) * a.v_t) : Vec<T>{};
-    }
+    for (int u = 0; u < UNROLL; ++u) k[u] = kn[u], v[u] = vn[u];
+    read();
     float s[GC][UNROLL];
 #pragma unroll
     for (int g = 0; g < GC; ++g) {
@@ -91,17 +106,17 @@ __global__ __launch_bounds__(256) void k_step(Step a) {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) d = dot2(&q[g].v[e], &k[u].v[e], d);
         d = sum_lanes<LPR>(d) * c;
-        s[g][u] = key0 + u * RPW < end ? d : -INFINITY;
+        s[g][u] = key0 + rg + u * RPW < end ? d : -INFINITY;
         top = fmaxf(top, s[g][u]);
       }
-      const float base = top == -INFINITY ? 0.0f : top, f = exp2f(m[g] - base);
+      const float base = top == -INFINITY ? 0.0f : top, f = exp2_fast(m[g] - base);
       m[g] = top;
       sum[g] *= f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[g][e] *= f;
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
-        s[g][u] = exp2f(s[g][u] - base);
+        s[g][u] = exp2_fast(s[g][u] - base);
         sum[g] += s[g][u];
       }
     }
@@ -115,42 +130,7 @@ __global__ __launch_bounds__(256) void k_step(Step a) {
       }
   }
   // join the row groups of the wave, then the waves
-#pragma unroll
-  for (int g = 0; g < GC; ++g) {
-    float top = m[g];
-#pragma unroll
-    for (int d = LPR; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    const float f = m[g] == -INFINITY ? 0.0f : exp2f(m[g] - top);
-    sum[g] *= f;
-#pragma unroll
-    for (int d = LPR; d < 64; d *= 2) sum[g] += __shfl_xor(sum[g], d);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      o[g][e] *= f;
-#pragma unroll
-      for (int d = LPR; d < 64; d *= 2) o[g][e] += __shfl_xor(o[g][e], d);
-    }
-    if (rg == 0) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) wo[w][g][d0 + e] = o[g][e];
-      if (part == 0) {
-        wm[w][g] = top;
-        wl[w][g] = sum[g];
-      }
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < GC * LPR * 8; i += 256) {
-    const int g = i / (LPR * 8), d = i % (LPR * 8);
-    if (g0 + g >= a.group || d >= a.dim) continue;
-    const float top = fmaxf(fmaxf(wm[0][g], wm[1][g]), fmaxf(wm[2][g], wm[3][g]));
-    float total = 0.0f, x = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float f = wm[j][g] == -INFINITY ? 0.0f : exp2f(wm[j][g] - top);
-      total += f * wl[j][g];
-      x += f * wo[j][g][d];
-    }
+  auto put = [&](int g, int d, float top, float total, float x) {
     const long long head = (long long)world * a.heads + kv * a.group + g0 + g;
     if (a.stretches == 1) {
       ((T*)a.out)[head * a.dim + d] = (T)(total == 0.0f ? 0.0f : x / total);
@@ -162,39 +142,115 @@ __global__ __launch_bounds__(256) void k_step(Step a) {
         to_part[a.dim + 1] = total;
       }
     }
+  };
+#pragma unroll
+  for (int g = 0; g < GC; ++g) {
+    float top = m[g];
+#pragma unroll
+    for (int d = LPR; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    const float f = m[g] == -INFINITY ? 0.0f : exp2_fast(m[g] - top);
+    sum[g] *= f;
+    if (LPR <= 8) sum[g] += __shfl_xor(sum[g], 8);
+    sum[g] = add_halves(add_rows(sum[g]));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      o[g][e] *= f;
+      if (LPR <= 8) o[g][e] += __shfl_xor(o[g][e], 8);
+      o[g][e] = add_halves(add_rows(o[g][e]));
+    }
+    if (rg == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wo[w][g][d0 + e] = o[g][e];
+      if (part == 0) {
+        wm[w][g] = top;
+        wl[w][g] = sum[g];
+      }
+    }
+  }
+  if constexpr (W == 1) {  // the wave's own LDS: what it wrote it reads
+    __builtin_amdgcn_wave_barrier();
+    for (int i = l; i < GC * LPR * 8; i += 64) {
+      const int g = i / (LPR * 8), d = i % (LPR * 8);
+      if (g0 + g < a.group && d < a.dim) put(g, d, wm[w][g], wl[w][g], wo[w][g][d]);
+    }
+  } else {
+    __syncthreads();
+    if (!exists) return;
+    for (int i = threadIdx.x; i < GC * LPR * 8; i += 256) {
+      const int g = i / (LPR * 8), d = i % (LPR * 8);
+      if (g0 + g >= a.group || d >= a.dim) continue;
+      const float top = fmaxf(fmaxf(wm[0][g], wm[1][g]), fmaxf(wm[2][g], wm[3][g]));
+      float total = 0.0f, x = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float f = wm[j][g] == -INFINITY ? 0.0f : exp2_fast(wm[j][g] - top);
+        total += f * wl[j][g];
+        x += f * wo[j][g][d];
+      }
+      put(g, d, top, total, x);
+    }
   }
 }
 
-// one wave a head: the stretches' sums, each scaled to the largest maximum, in their order
-template <typename T>
-__global__ __launch_bounds__(256) void k_step_join(Step a) {
-  const long long all = (long long)a.worlds * a.heads, head = blockIdx.x * 4LL + threadIdx.x / 64;
-  if (head >= all) return;
-  const int l = threadIdx.x % 64, n = a.dim + 2;
+// One workgroup a head: the stretches' factors from their maxima, then their sums in their order, JW of them at once and
+// those joined at the end. With one wave a head, one stretch after another, the join took as long as the reading.
+constexpr int MOST_STRETCHES = 2048;
+template <typename T, int LPR>
+__global__ __launch_bounds__(1024) void k_step_join(Step a) {
+  constexpr int D = LPR * 8, JW = 1024 / D;
+  __shared__ float factor[MOST_STRETCHES];
+  __shared__ float red[16];
+  __shared__ float sums[JW][D];
+  const long long all = (long long)a.worlds * a.heads, head = blockIdx.x;
+  const int n = a.dim + 2, wave = threadIdx.x / 64;
+  const float* p = a.part + head * n;
+  const long long step = all * n;
   float top = -INFINITY;
-  for (int s = 0; s < a.stretches; ++s) top = fmaxf(top, a.part[(s * all + head) * n + a.dim]);
-  float total = 0.0f, x0 = 0.0f, x1 = 0.0f;
-  for (int s = 0; s < a.stretches; ++s) {
-    const float* p = a.part + (s * all + head) * n;
-    const float f = p[a.dim] == -INFINITY ? 0.0f : exp2f(p[a.dim] - top);
-    total += f * p[a.dim + 1];
-    if (l < a.dim) x0 += f * p[l];
-    if (l + 64 < a.dim) x1 += f * p[l + 64];
+  for (int s = threadIdx.x; s < a.stretches; s += 1024) {
+    factor[s] = p[s * step + a.dim];
+    top = fmaxf(top, factor[s]);
   }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  T* out = (T*)a.out + head * a.dim;
-  if (l < a.dim) out[l] = (T)(x0 * inv);
-  if (l + 64 < a.dim) out[l + 64] = (T)(x1 * inv);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if (threadIdx.x % 64 == 0) red[wave] = top;
+  __syncthreads();
+  for (int w = 0; w < 16; ++w) top = fmaxf(top, red[w]);
+  __syncthreads();
+  float total = 0.0f;
+  for (int s = threadIdx.x; s < a.stretches; s += 1024) {
+    factor[s] = factor[s] == -INFINITY ? 0.0f : exp2_fast(factor[s] - top);
+    total += factor[s] * p[s * step + a.dim + 1];
+  }
+  total = sum_lanes<64>(total);
+  if (threadIdx.x % 64 == 0) red[wave] = total;
+  __syncthreads();
+  total = 0.0f;
+  for (int w = 0; w < 16; ++w) total += red[w];
+  const int d = threadIdx.x % D, j = threadIdx.x / D;
+  float x = 0.0f;
+  if (d < a.dim) {
+#pragma unroll 8
+    for (int s = j; s < a.stretches; s += JW) x += factor[s] * p[s * step + d];
+  }
+  sums[j][d] = x;
+  __syncthreads();
+  if (j == 0 && d < a.dim) {
+    x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < JW; ++i) x += sums[i][d];
+    ((T*)a.out)[head * a.dim + d] = (T)(total == 0.0f ? 0.0f : x / total);
+  }
 }
 
-// Stretches: enough workgroups for the 256 CUs where worlds and heads alone are too few, none under 256 keys.
+// Stretches: enough workgroups for the 256 CUs where worlds and heads alone are too few, none under 512 keys (joining
+// takes a second launch: 3.4 us beside 4.7 us at 257 keys).
 int step_heads_a_group(int group) { return group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8; }
 int step_stretches(int worlds, int kv_heads, int group, int capacity) {
   const int gc = step_heads_a_group(group);
   const long long blocks = (long long)worlds * kv_heads * ((group + gc - 1) / gc);
-  const long long want = (2048 + blocks - 1) / blocks, most = (capacity + 255) / 256;
+  const long long want = (2048 + blocks - 1) / blocks, most = (capacity + 511) / 512;
   const long long n = want < most ? want : most;
-  return (int)(n < 1 ? 1 : n);
+  return (int)(n < 1 ? 1 : n < MOST_STRETCHES ? n : MOST_STRETCHES);
 }
 size_t step_work_bytes(int worlds, int heads, int kv_heads, int dim, int capacity) {
   if (worlds <= 0) return 0;
@@ -202,20 +258,29 @@ size_t step_work_bytes(int worlds, int heads, int kv_heads, int dim, int capacit
   return n == 1 ? 0 : sizeof(float) * (size_t)n * worlds * heads * (dim + 2);
 }
 
+// Where there are units for every wave the GPU holds, a wave takes one alone: nothing is joined over LDS, and short
+// histories do not leave three waves of four idle.
+constexpr int ALONE = 4096;
+template <typename T, int LPR, int GC>
+void step_units(hipStream_t st, const Step& a) {
+  if (a.units >= ALONE) k_step<T, LPR, GC, 1><<<(a.units + 3) / 4, 256, 0, st>>>(a);
+  else k_step<T, LPR, GC, 4><<<a.units, 256, 0, st>>>(a);
+}
 template <typename T, int LPR>
 int step(hipStream_t st, Step a) {
   const int gc = step_heads_a_group(a.group);
-  const long long blocks = (long long)a.worlds * a.kv_heads * ((a.group + gc - 1) / gc) * a.stretches;
-  if (blocks >= 1LL << 24) return (int)hipErrorInvalidValue;
+  const long long units = (long long)a.worlds * a.kv_heads * ((a.group + gc - 1) / gc) * a.stretches;
+  if (units >= 1LL << 24) return (int)hipErrorInvalidValue;
+  a.units = (int)units;
   switch (gc) {
-    case 1: k_step<T, LPR, 1><<<(unsigned)blocks, 256, 0, st>>>(a); break;
-    case 2: k_step<T, LPR, 2><<<(unsigned)blocks, 256, 0, st>>>(a); break;
-    case 4: k_step<T, LPR, 4><<<(unsigned)blocks, 256, 0, st>>>(a); break;
-    default: k_step<T, LPR, 8><<<(unsigned)blocks, 256, 0, st>>>(a);
+    case 1: step_units<T, LPR, 1>(st, a); break;
+    case 2: step_units<T, LPR, 2>(st, a); break;
+    case 4: step_units<T, LPR, 4>(st, a); break;
+    default: step_units<T, LPR, 8>(st, a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.stretches == 1) return (int)e;
-  k_step_join<T><<<(unsigned)(((long long)a.worlds * a.heads + 3) / 4), 256, 0, st>>>(a);
+  k_step_join<T, LPR><<<(unsigned)(a.worlds * a.heads), 1024, 0, st>>>(a);
   return (int)hipGetLastError();
 }
 
