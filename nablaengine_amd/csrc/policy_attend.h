@@ -27,6 +27,7 @@ __device__ __forceinline__ F16x mfma(V8<_Float16> a, V8<_Float16> b, F16x c) {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int QROWS = 128;  // query rows a workgroup: 32 a wave
+constexpr float SLACK = 8.0f;  // log2
 constexpr int TILE = 64;    // keys of an LDS tile of the forward and the queries' gradient
 
 struct Attend {

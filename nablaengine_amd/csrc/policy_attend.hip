@@ -230,10 +230,11 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
     for (int j = 1; j < 16; ++j) top = fmaxf(top, s[0][j]);
 #pragma unroll
     for (int j = 0; j < 16; ++j) top = fmaxf(top, s[1][j]);
-    const float m1 = fmaxf(m, max_halves(top));
-    const float base = m1 == -INFINITY ? 0.0f : m1 * c;  // a row that has seen no key yet
-    if (__any(m1 != m)) {
-      const float f = m == -INFINITY ? 0.0f : exp2_fast(m * c - base);
+    top = max_halves(top);
+    // The subtracted maximum may lag behind the true one by 2^SLACK: sums and products stay far inside float32 and the
+    // probabilities inside float16, and the quotient at the end is the same. The outputs are then hardly ever rescaled.
+    if (__any(top * c > m * c + SLACK)) {
+      const float m1 = fmaxf(m, top), f = m == -INFINITY ? 0.0f : exp2_fast((m - m1) * c);
       sum *= f;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -241,6 +242,7 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
         for (int j = 0; j < 16; ++j) acc[d][j] *= f;
       m = m1;
     }
+    const float base = m == -INFINITY ? 0.0f : m * c;  // a row that has seen no key yet
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
