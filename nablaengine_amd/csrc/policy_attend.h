@@ -108,6 +108,64 @@ __device__ __forceinline__ V8<T> pack(const F16x& c, int s) {
   return __builtin_convertvector(f, V8<T>);
 }
 
+// Infinities and NaN under the mask. A masked probability is 0, but 0 times an infinity in a row that the mask hides is
+// NaN: such sums are not what the mask asks for. The kernels do not look for them; they look at their results, and compute
+// a row (a key) whose sums are not finite once more, over what it sees alone, one product after another in float32. That
+// takes long, and nothing where all is finite.
+// 0, or NaN where a register is not finite
+template <int N>
+__device__ __forceinline__ float not_finite(const F16x* acc) {
+  float t = 0.0f;
+#pragma unroll
+  for (int d = 0; d < N; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) t = fmaf(acc[d][j], 0.0f, t);
+  return t;
+}
+// columns for which `bad` holds in either half of the wave
+__device__ __forceinline__ unsigned bad_columns(bool bad) {
+  const unsigned long long b = __ballot(bad);
+  return (unsigned)b | (unsigned)(b >> 32);
+}
+// a row's elements l and l + 64 of up to DP
+template <int DP>
+struct Row {
+  float x[DP / 64];
+  Row() = default;
+  template <typename T>
+  __device__ __forceinline__ Row(const T* p, int dim) {
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i) {
+      const int d = threadIdx.x % 64 + 64 * i;
+      x[i] = d < dim ? (float)p[d] : 0.0f;
+    }
+  }
+  __device__ __forceinline__ float dot(const Row& o) const {
+    float s = x[0] * o.x[0];
+#pragma unroll
+    for (int i = 1; i < DP / 64; ++i) s += x[i] * o.x[i];
+    return sum_lanes<64>(s);
+  }
+  __device__ __forceinline__ void add(float f, const Row& o) {
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i) x[i] += f * o.x[i];
+  }
+  __device__ __forceinline__ bool all_nan(int dim) const {  // nothing more changes it
+    bool nan = true;
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i) nan &= (int)threadIdx.x % 64 + 64 * i >= dim || x[i] != x[i];
+    return __all(nan);
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* p, int dim, float f) const {
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i) {
+      const int d = threadIdx.x % 64 + 64 * i;
+      if (d < dim) p[d] = (T)(x[i] * f);
+    }
+  }
+};
+
 // 2^x in one instruction: results below 2^-126 become 0, which a sum of exponentials up to 1 does not notice
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -183,6 +183,17 @@ struct Rows {
   }
 };
 
+// one row of a wave's 32, for all its lanes
+struct Sight {
+  long long token, head;
+  int limit;
+  __device__ __forceinline__ Sight(const Attend& a, const Place& p, const Rows& r, int n) {
+    token = p.q0 + __builtin_amdgcn_readlane(r.pos, n);
+    head = __builtin_amdgcn_readlane(r.head, n);
+    limit = __builtin_amdgcn_readlane(r.limit, n);
+  }
+};
+
 // ---- forward --------------------------------------------------------------------------------------------------------
 
 template <typename T, int DP>
@@ -262,8 +273,25 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
   const long long token = p.q0 + r.pos;
   if (a.lse && r.valid && h == 0)
     a.lse[(long long)r.head * a.tq + token] = sum == 0.0f ? INFINITY : m * c + log2f(sum);
-  store_rows<DP>(r.valid ? (T*)a.out + (token * a.heads + r.head) * dim : nullptr, dim, h, acc,
+  const unsigned bad = bad_columns(r.valid && not_finite<DT>(acc) != 0.0f);
+  store_rows<DP>(r.valid && !(bad >> n & 1) ? (T*)a.out + (token * a.heads + r.head) * dim : nullptr, dim, h, acc,
                  sum == 0.0f ? 0.0f : 1.0f / sum);
+  for (unsigned left = bad; left; left &= left - 1) {
+    const Sight one(a, p, r, __builtin_ctz(left));
+    const Row<DP> qr((const T*)a.q + one.token * a.q_t + one.head * a.q_h, dim);
+    Row<DP> o = {};
+    float top = -INFINITY, total = 0.0f;
+    for (int j = 0; j <= one.limit && total == total; ++j) {
+      const float x = qr.dot(Row<DP>((const T*)a.k + (p.k0 + j) * a.k_t + p.kv * a.k_h, dim)) * c, top1 = fmaxf(top, x);
+      const float base1 = top1 == -INFINITY ? 0.0f : top1, f = exp2_fast(top - base1), pr = exp2_fast(x - base1);
+      total = total * f + pr;
+#pragma unroll
+      for (int i = 0; i < DP / 64; ++i) o.x[i] *= f;
+      o.add(pr, Row<DP>((const T*)a.v + (p.k0 + j) * a.v_t + p.kv * a.v_h, dim));
+      top = top1;
+    }
+    o.store((T*)a.out + (one.token * a.heads + one.head) * dim, dim, total == 0.0f ? 0.0f : 1.0f / total);
+  }
 }
 
 // ---- backward: the queries' gradient --------------------------------------------------------------------------------
@@ -346,7 +374,22 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
     }
   }
   if (r.valid && h == 0) a.delta[(long long)r.head * a.tq + token] = delta;
-  store_rows<DP>(r.valid ? (T*)a.dq + (token * a.heads + r.head) * dim : nullptr, dim, h, acc, a.scale);
+  const unsigned bad = bad_columns(r.valid && not_finite<DT>(acc) != 0.0f);
+  store_rows<DP>(r.valid && !(bad >> n & 1) ? (T*)a.dq + (token * a.heads + r.head) * dim : nullptr, dim, h, acc, a.scale);
+  for (unsigned left = bad; left; left &= left - 1) {
+    const int i = __builtin_ctz(left);
+    const Sight one(a, p, r, i);
+    const Row<DP> qr((const T*)a.q + one.token * a.q_t + one.head * a.q_h, dim);
+    const Row<DP> gr((const T*)a.dout + one.token * a.do_t + one.head * a.do_h, dim);
+    const float lse1 = __shfl(lse, i), delta1 = __shfl(delta, i);
+    Row<DP> o = {};
+    for (int j = 0; j <= one.limit && !o.all_nan(dim); ++j) {
+      const Row<DP> kr((const T*)a.k + (p.k0 + j) * a.k_t + p.kv * a.k_h, dim);
+      const float dp = gr.dot(Row<DP>((const T*)a.v + (p.k0 + j) * a.v_t + p.kv * a.v_h, dim));
+      o.add(exp2_fast(qr.dot(kr) * c - lse1) * (dp - delta1), kr);
+    }
+    o.store((T*)a.dq + (one.token * a.heads + one.head) * dim, dim, a.scale);
+  }
 }
 
 // ---- backward: the keys' and values' gradients ----------------------------------------------------------------------
@@ -371,7 +414,7 @@ template <typename T, int DP, int KW, int ROLE>
 __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP>& lds) {
   constexpr int WAVES = DkvTiles<T, DP>::WAVES, RT = DkvTiles<T, DP>::RT;
   constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 64 * WAVES / CH, SPLIT = WAVES / KW;
-  constexpr int AHEAD = DP == 64 ? 2 : 1;  // of a subtile's two column operands, those read during the exponentials
+  constexpr int AHEAD = DP == 64 ? 2 : KW == 4 ? 1 : 0;  // of a subtile's two column operands, those read during the exponentials
   constexpr int SUB = RT / 32, N = RT / STEP;
   auto& tiles = lds.tiles;
   auto &lses = lds.lses, &deltas = lds.deltas;
@@ -436,10 +479,9 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
     load_rows<DP>(valid ? (const T*)a.v + (long long)(p.k0 + key) * a.v_t + (long long)p.kv * a.v_h : nullptr, dim, h, v);
   F16x dk[DT] = {}, dv[DT] = {};
   if (threadIdx.x < RT && group <= RT) places_of[0][threadIdx.x] = places_of[1][threadIdx.x] = threadIdx.x / group;
-  int low_of[SUB], most_of[SUB];  // from a tile's first token to those of a subtile's first row and, at most, its last
-#pragma unroll
-  for (int i = 0; i < SUB; ++i)
-    low_of[i] = 32 * i / group, most_of[i] = group <= RT ? (32 * i + 31 < used ? 32 * i + 31 : used - 1) / group : 1;
+  // tokens from a tile's first to those of a subtile's first row and, at most, its last: x / group for x < RT as a product
+  const int inverse = 65535 / group + 1;
+  auto tokens = [&](int x) { return x * inverse >> 16; };
   int turn = 0, sub0 = 0, token0 = start / group;
   for (int r0 = start; r0 >= first; r0 -= used, turn ^= 1, sub0 += SUB) {
     if (threadIdx.x < RT) {
@@ -458,8 +500,9 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
     for (int i = 0; i < SUB; ++i) {
       if (SPLIT > 1 && (sub0 + i) % SPLIT != split) continue;
       // the last keys that the subtile's first row and (at most) its last one see
-      const int low = token + low_of[i] + off;
-      if (32 * i >= used || r0 + 32 * i >= rows || token + most_of[i] + off < key0) continue;
+      const int low = token + (group <= RT ? tokens(32 * i) : 0) + off;
+      const int most = token + (group <= RT ? tokens(32 * i + 31 < used ? 32 * i + 31 : used - 1) : 1) + off;
+      if (32 * i >= used || r0 + 32 * i >= rows || most < key0) continue;
       F16x s = {}, dp = {};
 #pragma unroll
       for (int y = 0; y < KS; y += 4) {
@@ -540,9 +583,30 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
       }
     if (split) return;
   }
+  const float off_dv = ROLE != KEYS ? not_finite<DT>(dv) : 0.0f, off_dk = ROLE != VALUES ? not_finite<DT>(dk) : 0.0f;
+  const unsigned bad = bad_columns(valid && off_dv + off_dk != 0.0f);
+  const bool put = valid && !(bad >> n & 1);
   const long long at = ((long long)(p.k0 + key) * a.kv_heads + p.kv) * dim;
-  if (ROLE != VALUES) store_rows<DP>(valid ? (T*)a.dk + at : nullptr, dim, h, dk, a.scale);
-  if (ROLE != KEYS) store_rows<DP>(valid ? (T*)a.dv + at : nullptr, dim, h, dv, 1.0f);
+  if (ROLE != VALUES) store_rows<DP>(put ? (T*)a.dk + at : nullptr, dim, h, dk, a.scale);
+  if (ROLE != KEYS) store_rows<DP>(put ? (T*)a.dv + at : nullptr, dim, h, dv, 1.0f);
+  for (unsigned left = bad; left; left &= left - 1) {
+    const int one = key0 + __builtin_ctz(left);
+    const Row<DP> kr((const T*)a.k + (long long)(p.k0 + one) * a.k_t + p.kv * a.k_h, dim);
+    const Row<DP> vr((const T*)a.v + (long long)(p.k0 + one) * a.v_t + p.kv * a.v_h, dim);
+    Row<DP> ok = {}, ov = {};
+    for (int r = (one - off > 0 ? one - off : 0) * group;
+         r < rows && !((ROLE == VALUES || ok.all_nan(dim)) && (ROLE == KEYS || ov.all_nan(dim))); ++r) {
+      const long long token = p.q0 + r / group, head = p.kv * group + r % group;
+      const Row<DP> qr((const T*)a.q + token * a.q_t + head * a.q_h, dim);
+      const Row<DP> gr((const T*)a.dout + token * a.do_t + head * a.do_h, dim);
+      const float pr = exp2_fast(qr.dot(kr) * c - a.lse[head * a.tq + token]);
+      if (ROLE != KEYS) ov.add(pr, gr);
+      if (ROLE != VALUES) ok.add(pr * (gr.dot(vr) - a.delta[head * a.tq + token]), qr);
+    }
+    const long long to = ((long long)(p.k0 + one) * a.kv_heads + p.kv) * dim;
+    if (ROLE != VALUES) ok.store((T*)a.dk + to, dim, a.scale);
+    if (ROLE != KEYS) ov.store((T*)a.dv + to, dim, 1.0f);
+  }
 }
 
 template <typename T, int DP, int KW>

@@ -342,7 +342,8 @@ def check_attention(q, k, v, lq, lk, scale=None, dout=None, same=False):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("heads,kv,dim", [(1, 1, 64), (4, 2, 64), (6, 2, 128), (5, 5, 40), (8, 1, 8), (3, 1, 72), (7, 1, 120)])
+@pytest.mark.parametrize("heads,kv,dim", [(1, 1, 64), (4, 2, 64), (6, 2, 128), (5, 5, 40), (8, 1, 8), (3, 1, 72), (7, 1, 120), (70, 1, 64),
+                                           (130, 1, 128)])
 def test_attention_heads(dtype, heads, kv, dim):
     print("attention", dtype, heads, kv, dim, flush=True)
     lq = [1, 33, 70, 0, 129, 5]
@@ -450,6 +451,61 @@ def test_attention_keeps_sequences_apart():
     q[50], k[60], v[70], dout[45] = math.nan, math.inf, -math.inf, math.nan
     for a, b in zip(clean, run(q, k, v)):
         assert torch.equal(a[:40], b[:40]) and torch.equal(a[80:], b[80:])
+
+
+@pytest.mark.parametrize("dtype,dim,heads", [(BF16, 64, 2), (F16, 64, 6), (BF16, 128, 4), (F16, 40, 2)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_attention_what_the_mask_hides(dtype, dim, heads, bad):
+    """A value, key, query or cotangent that is not finite reaches the rows and keys that the mask lets see it, and no
+    other of its sequence; an infinite value element reaches its own column only, as itself."""
+    print("hidden", dtype, dim, heads, bad, flush=True)
+    lq, lk = [150, 70], [150, 75]
+    q, dout = rand((220, heads, dim), dtype, 1), rand((220, heads, dim), dtype, 4)
+    k, v = rand((225, 2, dim), dtype, 2), rand((225, 2, dim), dtype, 3)
+    want = attend64(q, k, v, lq, lk, 1 / math.sqrt(dim), dout)
+
+    def run(q, k, v, dout):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        out = policy.attention(*leaves, starts(lq), starts(lk))
+        return dict(zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, dout))))
+
+    def same(got, name, rows, cols=slice(None)):
+        w, b = want[name]
+        within(f"{name} {rows}", got[name][rows, :, cols], w[rows, :, cols], b[rows, :, cols])
+    early, late, other = slice(0, 100), slice(100, 150), slice(150, None)
+    v2 = v.clone()
+    v2[100, :, 7] = bad
+    got = run(q, k, v2, dout)
+    for name in ("out", "dq"):
+        same(got, name, early), same(got, name, other)
+    same(got, "out", late, slice(0, 7)), same(got, "out", late, slice(8, None))
+    late7 = got["out"][late, :, 7]
+    assert torch.isnan(late7).all() if math.isnan(bad) else (late7 == bad).all()
+    same(got, "dv", slice(None))  # no value has a part in the values' gradient
+    same(got, "dk", other)
+    k2 = k.clone()
+    k2[100] = bad
+    got = run(q, k2, v, dout)
+    for name in ("out", "dq"):
+        same(got, name, early), same(got, name, other)
+    for name in ("dk", "dv"):
+        same(got, name, other)
+    d2 = dout.clone()
+    d2[40, :, 5] = bad  # row 40 sees keys 0 to 40
+    got = run(q, k, v, d2)
+    same(got, "out", slice(None))
+    for name, rows in (("dq", slice(0, 40)), ("dq", slice(41, None)), ("dk", slice(41, None)), ("dv", slice(41, None))):
+        same(got, name, rows)
+    same(got, "dv", slice(0, 41), slice(0, 5)), same(got, "dv", slice(0, 41), slice(6, None))
+    seen = got["dv"][0:41, :, 5]
+    assert torch.isnan(seen).all() if math.isnan(bad) else (seen == bad).all()
+    q2 = q.clone()
+    q2[40] = bad
+    got = run(q2, k, v, dout)
+    for name in ("out", "dq"):
+        same(got, name, slice(0, 40)), same(got, name, slice(41, None))
+    for name in ("dk", "dv"):
+        same(got, name, slice(41, None))
 
 
 def test_attention_is_the_same_every_time():
