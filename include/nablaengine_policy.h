@@ -53,7 +53,7 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
                      const void* v, long long v_t, long long v_h, const int* starts_q, const int* starts_k,
                      float scale, const void* out, const float* lse, const void* work, const void* dout,
                      long long do_t, long long do_h, float* delta, void* dq, void* dk, void* dv);
-long long dk_attention_work_bytes(int heads, int kv_heads, int seqs, int tq, int tk);
+long long dk_attention_work_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk);
 
 /* Attention of one query a world over that world's cache: q (worlds, heads, dim), k, v (worlds, capacity, kv_heads,
  * dim) with elements from world to world (_w), token to token (_t) and head to head (_h); lengths: worlds int32 on the

@@ -35,7 +35,7 @@ struct Attend {
   long long q_t, q_h, k_t, k_h, v_t, v_h;  // elements from token to token, and from head to head
   int heads, kv_heads, group, dim, seqs, tq, tk;
   int by_sequence;  // the order of the tiles, see below
-  int key_waves;  // waves of a workgroup of the keys' gradients that differ in their 32 keys: 2 or 4
+  int key_waves;  // 32 keys each: a tile of the keys' gradients (1, 2 or 4)
   const int *starts_q, *starts_k;
   float scale;
   void* out;   // (tq, heads, dim)

@@ -27,16 +27,19 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   const int per[2] = {QROWS, 32 * key_waves};
   const long long caps[2] = {order_queries(seqs, tq, group), order_keys(seqs, tk, key_waves)};
   int* const lists[2] = {order + ORDER_HEAD, order + ORDER_HEAD + 2 * caps[0]};
-  // f(list, sequence, first tile, tiles, bucket) for every stretch of tiles that stays together
+  // f(list, sequence, first tile, tiles, bucket) for every stretch of tiles that stays together; every lane of a wave takes
+  // part each time, with 0 tiles where it has none
   auto each = [&](auto f) {
-    for (int s = first_seq; s <= seqs; s += stride) {
+    for (int s0 = 0; s0 <= seqs; s0 += stride) {
+      const int s = s0 + first_seq < seqs ? s0 + first_seq : seqs;
+      const bool mine = s0 + first_seq <= seqs;
       int q0, k0, nq, nk;
       sequence(starts_q, s, seqs, tq, q0, nq);
       sequence(starts_k, s, seqs, tk, k0, nk);
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         const int mq = which && s == seqs ? 0 : nq, mk = !which && s == seqs ? 0 : nk;
-        const int rows = which ? mk : mq * group, tiles = (rows + per[which] - 1) / per[which];
+        const int rows = which ? mk : mq * group, tiles = mine ? (rows + per[which] - 1) / per[which] : 0;
         auto bucket = [&](int t) {
           long long cost;
           if (which) {  // the query rows that see the tile's first key
@@ -51,16 +54,33 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
           return (int)(BUCKETS - 1 - (cost < BUCKETS ? cost : BUCKETS - 1));
         };
         if (by_sequence) {
-          if (tiles) f(which, s, 0, tiles, bucket(which ? 0 : tiles - 1));
+          f(which, s, 0, tiles, bucket(which || !tiles ? 0 : tiles - 1));
         } else {
-          for (int t = lane; t < tiles; t += ls) f(which, s, t, 1, bucket(t));
+          for (int t = lane; __any(t < tiles); t += ls) f(which, s, t, t < tiles ? 1 : 0, bucket(t));
         }
       }
     }
   };
+  // adds n to a bucket's count and returns what it was; lanes that all add to one bucket (short sequences mostly cost the
+  // same) add at once: one after another they took half of this kernel's time
+  auto add = [&](int which, int n, int b) {
+    const unsigned long long some = __ballot(n > 0);
+    if (!some) return 0;
+    const int lead = __builtin_ctzll(some), me = threadIdx.x % 64, b0 = __shfl(b, lead);
+    if (!__all(n == 0 || b == b0)) return n ? atomicAdd(&count[which][b], n) : 0;
+    int before = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int x = __shfl_up(before, d);
+      if (me >= d) before += x;
+    }
+    const int all = __shfl(before, 63);
+    const int base = __shfl(me == lead ? atomicAdd(&count[which][b0], all) : 0, lead);
+    return base + before - n;
+  };
   count[0][threadIdx.x] = count[1][threadIdx.x] = 0;
   __syncthreads();
-  each([&](int which, int, int, int n, int b) { atomicAdd(&count[which][b], n); });
+  each([&](int which, int, int, int n, int b) { add(which, n, b); });
   __syncthreads();
   // exclusive prefixes over the buckets
   int mine[2], sum[2];
@@ -87,7 +107,7 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   }
   __syncthreads();
   each([&](int which, int s, int t, int n, int b) {
-    int at = atomicAdd(&count[which][b], n);
+    int at = add(which, n, b);
     for (int i = 0; i < n; ++i, ++at)  // the heaviest of the sequence first
       if (at < caps[which]) {
         lists[which][2 * at] = s;
@@ -101,20 +121,8 @@ struct Place {
   int tile, kv, part, q0, nq, k0, nk;
 };
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-// of `parts` workgroups a tile and key/value head
-__device__ __forceinline__ bool place(const Attend& a, int which, int parts, Place& p) {
-  const int all = uniform(a.order[which]) * a.kv_heads * parts, b = blockIdx.x;
-  int at = b;
-  if (a.by_sequence) {
-    const int base = b / (WINDOW * XCDS) * (WINDOW * XCDS), left = all - base;
-    const int mine = left < WINDOW * XCDS ? (left + XCDS - 1) / XCDS : WINDOW, r = b - base;
-    if (left <= 0 || r / XCDS >= mine) return false;
-    at = base + r % XCDS * mine + r / XCDS;
-    p.part = at % parts, at /= parts;
-  } else {  // the parts take turns on each XCD
-    p.part = b / XCDS % parts;
-    at = b / (XCDS * parts) * XCDS + b % XCDS;
-  }
+// entry `at` of a list times its key/value heads
+__device__ __forceinline__ bool place(const Attend& a, int which, int at, Place& p) {
   const int entry = at / a.kv_heads;
   if (entry >= uniform(a.order[which])) return false;
   const int* list = a.order + ORDER_HEAD + (which ? 2 * order_queries(a.seqs, a.tq, a.group) : 0) + 2LL * entry;
@@ -126,6 +134,22 @@ __device__ __forceinline__ bool place(const Attend& a, int which, int parts, Pla
   p.q0 = uniform(p.q0), p.nq = uniform(p.nq), p.k0 = uniform(p.k0), p.nk = uniform(p.nk);
   if (s == a.seqs) (which ? p.nq : p.nk) = 0;
   return true;
+}
+// this workgroup's, of `parts` a tile and key/value head
+__device__ __forceinline__ bool place_of_block(const Attend& a, int which, int parts, Place& p) {
+  const int b = blockIdx.x;
+  int at;
+  if (a.by_sequence) {
+    const int all = uniform(a.order[which]) * a.kv_heads * parts, base = b / (WINDOW * XCDS) * (WINDOW * XCDS);
+    const int left = all - base, mine = left < WINDOW * XCDS ? (left + XCDS - 1) / XCDS : WINDOW, r = b - base;
+    if (left <= 0 || r / XCDS >= mine) return false;
+    at = base + r % XCDS * mine + r / XCDS;
+    p.part = at % parts, at /= parts;
+  } else {  // the parts take turns on each XCD
+    p.part = b / XCDS % parts;
+    at = b / (XCDS * parts) * XCDS + b % XCDS;
+  }
+  return place(a, which, at, p);
 }
 // workgroups that cover a list of at most `most` tiles
 unsigned blocks_of(const Attend& a, long long most, int parts) {
@@ -202,7 +226,7 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
   __shared__ __align__(16) T ks[2][TILE * DP];
   __shared__ __align__(16) T vs[2][TILE * DP];
   Place p;
-  if (!place(a, 0, 1, p)) return;
+  if (!place_of_block(a, 0, 1, p)) return;
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
   const Rows r(a, p);
   Keys<DP, T> keys(a, p);
@@ -302,7 +326,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
   __shared__ __align__(16) T ks[2][TILE * DP];
   __shared__ __align__(16) T vs[2][TILE * DP];
   Place p;
-  if (!place(a, 0, 1, p)) return;
+  if (!place_of_block(a, 0, 1, p)) return;
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
   const Rows r(a, p);
   Keys<DP, T> keys(a, p);
@@ -398,9 +422,9 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
 // time. S = Q K^T here, so that a lane holds 16 rows of ONE key and P, dS are the B operands of dV^T = dO^T P and dK^T =
 // Q^T dS. KW of the waves differ in their keys, the others take every SPLIT-th subtile of 32 rows of the same keys, and
 // their sums are added at the end, in order.
-template <typename T, int DP>
+template <typename T, int DP, int WAVES>
 struct DkvTiles {
-  static constexpr int WAVES = DP == 64 ? 4 : 8, RT = DP == 64 ? 64 : 128;
+  static constexpr int RT = WAVES == 1 ? 32 : DP == 64 ? 64 : 128;
   alignas(16) T tiles[2][2][RT * DP];  // (turn, q or dout)
   alignas(16) float lses[2][RT], deltas[2][RT];
   alignas(16) int places_of[2][RT];  // a row's token from its tile's first
@@ -410,16 +434,25 @@ struct DkvTiles {
 // of 16 heads against 1480 us with both in one and part of the operands in LDS or scratch. Eight waves share a tile of
 // 128 rows there: with four, the tiles that all rows read are one round's length each.
 enum Role { BOTH, KEYS, VALUES };
-template <typename T, int DP, int KW, int ROLE>
-__device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP>& lds) {
-  constexpr int WAVES = DkvTiles<T, DP>::WAVES, RT = DkvTiles<T, DP>::RT;
+template <typename T, int DP, int KW, int WAVES, int ROLE>
+__device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, WAVES>& lds) {
+  constexpr int RT = DkvTiles<T, DP, WAVES>::RT;
   constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 64 * WAVES / CH, SPLIT = WAVES / KW;
   constexpr int AHEAD = DP == 64 ? 2 : KW == 4 ? 1 : 0;  // of a subtile's two column operands, those read during the exponentials
   constexpr int SUB = RT / 32, N = RT / STEP;
   auto& tiles = lds.tiles;
   auto &lses = lds.lses, &deltas = lds.deltas;
   auto& places_of = lds.places_of;
-  const int l = threadIdx.x % 64, n = l % 32, h = l / 32, w = uniform(threadIdx.x / 64), dim = a.dim, group = a.group;
+  const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim, group = a.group;
+  const int tid = threadIdx.x % (64 * WAVES), w = uniform(tid / 64);
+  auto meet = [] {  // the waves of the tile; one alone only keeps its own LDS accesses in order
+    if constexpr (WAVES > 1) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
   const int kw = w % KW, split = w / KW;
   const int rows = p.nq * group, off = p.nk - p.nq;
   const int key0 = p.tile * 32 * KW + 32 * kw, key = key0 + n;
@@ -432,31 +465,30 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
   const int back = used / group;  // tokens of a tile
   const int from = p.tile * 32 * KW - off;  // the first token that sees the tile's first key
   const int first = (from > 0 ? from : 0) * group;
-  const int chunk = threadIdx.x % CH ^ swizzle<DP>(threadIdx.x / CH);
-  const bool in_row = 8 * chunk < dim;
+  auto chunk = [&](int i) { return tid % CH ^ swizzle<DP>(tid / CH + i * STEP); };
   const T *qp[N], *gp[N];  // this thread's rows of the next tile to load, and its row's place in lse and delta
   long long stat = 0;
   auto places = [&](int r0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int r = r0 + (int)threadIdx.x / CH + i * STEP, pos = r / group, head = p.kv * group + r % group;
-      qp[i] = (const T*)a.q + (long long)(p.q0 + pos) * a.q_t + (long long)head * a.q_h + 8 * chunk;
-      gp[i] = (const T*)a.dout + (long long)(p.q0 + pos) * a.do_t + (long long)head * a.do_h + 8 * chunk;
+      const int r = r0 + tid / CH + i * STEP, pos = r / group, head = p.kv * group + r % group;
+      qp[i] = (const T*)a.q + (long long)(p.q0 + pos) * a.q_t + (long long)head * a.q_h + 8 * chunk(i);
+      gp[i] = (const T*)a.dout + (long long)(p.q0 + pos) * a.do_t + (long long)head * a.do_h + 8 * chunk(i);
     }
-    const int r = r0 + threadIdx.x;
+    const int r = r0 + tid;
     stat = (long long)(p.kv * group + r % group) * a.tq + p.q0 + r / group;
   };
   float lse = INFINITY, delta = 0.0f;
   auto load = [&](int r0, int turn) {  // the rows from r0, then the places of those before them
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int row = threadIdx.x / CH + i * STEP;
-      const bool there = in_row && row < used && r0 + row < rows;
+      const int row = tid / CH + i * STEP;
+      const bool there = 8 * chunk(i) < dim && row < used && r0 + row < rows;
       to_lds(qp[i], there, tiles[turn][0] + (i * WAVES + w) * 512);
       to_lds(gp[i], there, tiles[turn][1] + (i * WAVES + w) * 512);
     }
-    if (threadIdx.x < RT) {
-      const bool there = threadIdx.x < used && r0 + (int)threadIdx.x < rows;
+    if (tid < RT) {
+      const bool there = tid < used && r0 + tid < rows;
       lse = there ? a.lse[stat] : INFINITY;
       if (ROLE != VALUES) delta = there ? a.delta[stat] : 0.0f;
     }
@@ -478,19 +510,19 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
   if (ROLE != VALUES)
     load_rows<DP>(valid ? (const T*)a.v + (long long)(p.k0 + key) * a.v_t + (long long)p.kv * a.v_h : nullptr, dim, h, v);
   F16x dk[DT] = {}, dv[DT] = {};
-  if (threadIdx.x < RT && group <= RT) places_of[0][threadIdx.x] = places_of[1][threadIdx.x] = threadIdx.x / group;
+  if (tid < RT && group <= RT) places_of[0][tid] = places_of[1][tid] = tid / group;
   // tokens from a tile's first to those of a subtile's first row and, at most, its last: x / group for x < RT as a product
   const int inverse = 65535 / group + 1;
   auto tokens = [&](int x) { return x * inverse >> 16; };
   int turn = 0, sub0 = 0, token0 = start / group;
   for (int r0 = start; r0 >= first; r0 -= used, turn ^= 1, sub0 += SUB) {
-    if (threadIdx.x < RT) {
-      lses[turn][threadIdx.x] = lse;
-      deltas[turn][threadIdx.x] = delta;
-      if (group > RT) places_of[turn][threadIdx.x] = (r0 % group + (int)threadIdx.x) / group;
+    if (tid < RT) {
+      lses[turn][tid] = lse;
+      deltas[turn][tid] = delta;
+      if (group > RT) places_of[turn][tid] = (r0 % group + tid) / group;
     }
     loads_done();
-    __syncthreads();
+    meet();
     if (r0 - used >= first) load(r0 - used, turn ^ 1);
     if (key0 >= p.nk) continue;
     const int token = group <= RT ? token0 : r0 / group;
@@ -568,13 +600,13 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
       for (int which = 0; which < 2; ++which) {
         if (ROLE == (which ? KEYS : VALUES)) continue;
         F16x* acc = which ? dv : dk;
-        __syncthreads();
+        meet();
         if (split == o)
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int j = 0; j < 16; ++j) mine[((kw * DT + d) * 16 + j) * 64 + l] = acc[d][j];
-        __syncthreads();
+        meet();
         if (split == 0)
 #pragma unroll
           for (int d = 0; d < DT; ++d)
@@ -609,28 +641,33 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
   }
 }
 
-template <typename T, int DP, int KW>
-__global__ __launch_bounds__(DP == 64 ? 256 : 512) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_dkv(Attend a) {
-  __shared__ DkvTiles<T, DP> lds;
+template <typename T, int DP, int KW, int WAVES>
+__global__ __launch_bounds__(WAVES == 8 ? 512 : 256) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_dkv(Attend a) {
+  __shared__ DkvTiles<T, DP, WAVES> lds[WAVES == 1 ? 4 : 1];
   Place p;
-  if constexpr (DP == 64) {
-    if (place(a, 1, 1, p)) dkv_tile<T, DP, KW, BOTH>(a, p, lds);
+  if constexpr (WAVES == 1) {  // each wave a tile of its own
+    const int w = uniform(threadIdx.x / 64);
+    if (place(a, 1, blockIdx.x * 4 + w, p)) dkv_tile<T, DP, KW, WAVES, BOTH>(a, p, lds[w]);
+  } else if constexpr (DP == 64) {
+    if (place_of_block(a, 1, 1, p)) dkv_tile<T, DP, KW, WAVES, BOTH>(a, p, lds[0]);
   } else {
-    if (!place(a, 1, 2, p)) return;
-    if (p.part) dkv_tile<T, DP, KW, VALUES>(a, p, lds);
-    else dkv_tile<T, DP, KW, KEYS>(a, p, lds);
+    if (!place_of_block(a, 1, 2, p)) return;
+    if (p.part) dkv_tile<T, DP, KW, WAVES, VALUES>(a, p, lds[0]);
+    else dkv_tile<T, DP, KW, WAVES, KEYS>(a, p, lds[0]);
   }
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------
 
-// Keys a workgroup of the keys' gradients: 128, or 64 where sequences are short (half of the waves would have none).
-int key_waves(int seqs, int tk) {
+// Keys a tile of the keys' gradients: 128; where sequences are short (most of a workgroup's waves would have no keys) 32,
+// a wave each, for heads up to 64, and 64 for larger ones.
+int key_waves(int dim, int seqs, int tk) {
+  if (dim <= 64) return tk <= 64LL * seqs ? 1 : 4;
   return tk <= 96LL * seqs ? 2 : 4;
 }
-size_t attend_work_bytes(int seqs, int tq, int tk, int group) {
+size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group) {
   return sizeof(int) * (ORDER_HEAD + 2 * (size_t)(order_queries(seqs, tq, group) +
-                                                  order_keys(seqs, tk, key_waves(seqs, tk))));
+                                                  order_keys(seqs, tk, key_waves(dim, seqs, tk))));
 }
 
 template <typename T, int DP>
@@ -644,10 +681,14 @@ int attend_vjp(hipStream_t st, const Attend& a) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (!a.tk) return 0;
-  const unsigned blocks = blocks_of(a, order_keys(a.seqs, a.tk, a.key_waves), DP == 64 ? 1 : 2);
-  constexpr int threads = 64 * DkvTiles<T, DP>::WAVES;
-  if (a.key_waves == 2) k_attend_dkv<T, DP, 2><<<blocks, threads, 0, st>>>(a);
-  else k_attend_dkv<T, DP, 4><<<blocks, threads, 0, st>>>(a);
+  const long long tiles = order_keys(a.seqs, a.tk, a.key_waves);
+  if constexpr (DP == 64) {
+    if (a.key_waves == 1) k_attend_dkv<T, 64, 1, 1><<<(unsigned)((tiles * a.kv_heads + 3) / 4), 256, 0, st>>>(a);
+    else k_attend_dkv<T, 64, 4, 4><<<blocks_of(a, tiles, 1), 256, 0, st>>>(a);
+  } else {
+    if (a.key_waves == 2) k_attend_dkv<T, 128, 2, 8><<<blocks_of(a, tiles, 2), 512, 0, st>>>(a);
+    else k_attend_dkv<T, 128, 4, 8><<<blocks_of(a, tiles, 2), 512, 0, st>>>(a);
+  }
   return (int)hipGetLastError();
 }
 
@@ -673,7 +714,7 @@ bool attention_takes(int type, int heads, int kv_heads, int dim, int seqs, int t
       dim % 8 || seqs < 0 || tq < 0 || tk < 0 || tk >= 1 << 30 || (long long)tq * (heads / kv_heads) >= 1 << 30)
     return false;
   const long long most = (1LL << 22) - 1024;  // workgroups of 256 or 512 work-items a launch
-  return pol::order_queries(seqs, tq, heads / kv_heads) * kv_heads <= most && pol::order_keys(seqs, tk, 2) * kv_heads <= most;
+  return pol::order_queries(seqs, tq, heads / kv_heads) * kv_heads <= most && pol::order_keys(seqs, tk, 1) * kv_heads <= most;
 }
 }  // namespace
 
@@ -690,7 +731,7 @@ int dk_attention(hipStream_t st, int type, int heads, int kv_heads, int dim, int
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
-  a.key_waves = pol::key_waves(seqs, tk);
+  a.key_waves = pol::key_waves(dim, seqs, tk);
   a.by_sequence = tq <= (long long)pol::LONG * seqs;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.out = out, a.lse = lse, a.order = (const int*)work;
   return pol::launch_attend(st, type, a);
@@ -708,7 +749,7 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
-  a.key_waves = pol::key_waves(seqs, tk);
+  a.key_waves = pol::key_waves(dim, seqs, tk);
   a.by_sequence = tq <= (long long)pol::LONG * seqs;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.order = (const int*)work;
   a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse);
@@ -716,9 +757,9 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
   return pol::launch_attend_vjp(st, type, a);
 }
 
-long long dk_attention_work_bytes(int heads, int kv_heads, int seqs, int tq, int tk) {
+long long dk_attention_work_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk) {
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || seqs < 0 || tq < 0 || tk < 0) return 0;
-  return (long long)pol::attend_work_bytes(seqs, tq, tk, heads / kv_heads);
+  return (long long)pol::attend_work_bytes(dim, seqs, tq, tk, heads / kv_heads);
 }
 
 }  // extern "C"

@@ -276,7 +276,7 @@ int sequences_checks(const Tensor& q, const Tensor& k, const Tensor& starts_q, c
   return (int)seqs;
 }
 long long order_words(const Heads& h, int seqs, const Tensor& q, const Tensor& k) {
-  return lib.dk_attention_work_bytes(h.heads, h.kv, seqs, (int)q.size(0), (int)k.size(0)) / 4;
+  return lib.dk_attention_work_bytes(h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0)) / 4;
 }
 
 std::vector<Tensor> attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& starts_q,

@@ -98,8 +98,8 @@ def _fake_norm(grads, *_):
 
 
 def _fake_attention_forward(q, k, v, starts_q, starts_k, scale, train):
-    words = int(torch_ffi._load().dll.dk_attention_work_bytes(q.shape[1], k.shape[1], starts_q.shape[0] - 1, q.shape[0],
-                                                              k.shape[0])) // 4
+    words = int(torch_ffi._load().dll.dk_attention_work_bytes(q.shape[1], k.shape[1], q.shape[2], starts_q.shape[0] - 1,
+                                                              q.shape[0], k.shape[0])) // 4
     return [q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0] if train else 0), dtype=torch.float32),
             starts_q.new_empty((words,))]
 

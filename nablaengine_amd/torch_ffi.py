@@ -113,7 +113,7 @@ _PROTOTYPES = {
     "dk_clip_work_bytes": "q:i",
     "dk_attention": "i:piiiiiii" + "pqq" * 3 + "ppfppp",
     "dk_attention_vjp": "i:piiiiiii" + "pqq" * 3 + "ppfppp" + "pqq" + "pppp",
-    "dk_attention_work_bytes": "q:iiiii",
+    "dk_attention_work_bytes": "q:iiiiii",
     "dk_attention_step": "i:piiiiii" + "pqq" + "pqqq" * 2 + "pfpp",
     "dk_attention_step_work_bytes": "q:iiiii",
 }

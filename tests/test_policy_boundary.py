@@ -58,7 +58,7 @@ def test_c_entries_refuse_before_any_launch():
     for bad in (dict(t=0), dict(heads=3), dict(kv=0), dict(dim=7), dict(dim=136), dict(seqs=-1), dict(tq=-1), dict(tk=1 << 30),
                 dict(tq=1 << 29), dict(q=None), dict(starts=None), dict(scale=0.0), dict(scale=float("nan")), dict(work=None)):
         assert attention(**bad) == 1, bad
-    assert dll.dk_attention_work_bytes(4, 2, 1, 5, 5) > 0
+    assert dll.dk_attention_work_bytes(4, 2, 64, 1, 5, 5) > 0
 
     def step(t=1, worlds=2, heads=4, kv=2, dim=64, cap=9, q=X, lengths=X, scale=0.1, work=X):
         return dll.dk_attention_step(None, t, worlds, heads, kv, dim, cap, q, 1, 1, X, 1, 1, 1, X, 1, 1, 1, lengths, scale, X, work)
