@@ -10,23 +10,37 @@
 
 namespace pol {
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // ---- the order ------------------------------------------------------------------------------------------------------
 
 // One workgroup lists the tiles by a counting sort (a tile's place among equals is free, results do not depend on the
 // order). seqs + 1 sequences, LS lanes on each.
 __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk, int group, int key_waves, int by_sequence,
-                                                       const int* __restrict__ starts_q,
-                                                       const int* __restrict__ starts_k, int* __restrict__ order) {
+                                                       const int* starts_q, const int* starts_k,
+                                                       int* __restrict__ order) {
   constexpr int BUCKETS = 1024;
   __shared__ int count[2][BUCKETS];
   __shared__ int wave_sum[2][16];
+  constexpr int STAGED = 8192;  // sequences whose offsets are read to LDS, all at once: the passes below wait for none
+  __shared__ int staged[2][STAGED + 1];
+  if (seqs <= STAGED) {
+    for (int s = threadIdx.x; s <= seqs; s += 1024) staged[0][s] = starts_q[s], staged[1][s] = starts_k[s];
+    starts_q = staged[0], starts_k = staged[1];
+    __syncthreads();
+  }
   int ls = 1;
   if (!by_sequence)
     while (ls < 1024 && ls * 2 * (long long)(seqs + 1) <= 1024) ls *= 2;
   const int lane = threadIdx.x % ls, first_seq = threadIdx.x / ls, stride = 1024 / ls;
-  const int per[2] = {QROWS, 32 * key_waves};
+  const int bits[2] = {7, key_waves == 1 ? 5 : key_waves == 2 ? 6 : 7};  // of a tile's rows
+  static_assert(QROWS == 128, "");
   const long long caps[2] = {order_queries(seqs, tq, group), order_keys(seqs, tk, key_waves)};
   int* const lists[2] = {order + ORDER_HEAD, order + ORDER_HEAD + 2 * caps[0]};
+  auto bucket_of = [](long long cost) {  // rows or keys of the other side
+    cost = cost > 0 ? (cost + TILE - 1) / TILE : 0;
+    return (int)(BUCKETS - 1 - (cost < BUCKETS ? cost : BUCKETS - 1));
+  };
   // f(list, sequence, first tile, tiles, bucket) for every stretch of tiles that stays together; every lane of a wave takes
   // part each time, with 0 tiles where it has none
   auto each = [&](auto f) {
@@ -39,22 +53,21 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         const int mq = which && s == seqs ? 0 : nq, mk = !which && s == seqs ? 0 : nk;
-        const int rows = which ? mk : mq * group, tiles = mine ? (rows + per[which] - 1) / per[which] : 0;
+        const int rows = which ? mk : mq * group, tiles = mine ? (rows + (1 << bits[which]) - 1) >> bits[which] : 0;
         auto bucket = [&](int t) {
           long long cost;
           if (which) {  // the query rows that see the tile's first key
-            const int from = t * per[1] - (mk - mq);
+            const int from = (t << bits[1]) - (mk - mq);
             cost = mq - (from > 0 ? from : 0);
             cost = (cost > 0 ? cost : 0) * group;
           } else {  // the keys that the tile's last row sees
             const int last = ((t + 1) * QROWS < rows ? (t + 1) * QROWS : rows) - 1;
             cost = last / group + mk - mq + 1;
           }
-          cost = cost > 0 ? (cost + TILE - 1) / TILE : 0;
-          return (int)(BUCKETS - 1 - (cost < BUCKETS ? cost : BUCKETS - 1));
+          return bucket_of(cost);
         };
-        if (by_sequence) {
-          f(which, s, 0, tiles, bucket(which || !tiles ? 0 : tiles - 1));
+        if (by_sequence) {  // its heaviest tile: the last row sees every key, the first key almost every row
+          f(which, s, 0, tiles, bucket_of(which ? (long long)(mq < mk ? mq : mk) * group : mk));
         } else {
           for (int t = lane; __any(t < tiles); t += ls) f(which, s, t, t < tiles ? 1 : 0, bucket(t));
         }
@@ -66,17 +79,12 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   auto add = [&](int which, int n, int b) {
     const unsigned long long some = __ballot(n > 0);
     if (!some) return 0;
-    const int lead = __builtin_ctzll(some), me = threadIdx.x % 64, b0 = __shfl(b, lead);
+    const int lead = uniform(__builtin_ctzll(some)), b0 = __builtin_amdgcn_readlane(b, lead);
     if (!__all(n == 0 || b == b0)) return n ? atomicAdd(&count[which][b], n) : 0;
-    int before = n;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int x = __shfl_up(before, d);
-      if (me >= d) before += x;
-    }
-    const int all = __shfl(before, 63);
-    const int base = __shfl(me == lead ? atomicAdd(&count[which][b0], all) : 0, lead);
-    return base + before - n;
+    const int before = scan_wave(n), all = __builtin_amdgcn_readlane(before, 63);
+    int base = 0;
+    if ((int)threadIdx.x % 64 == lead) base = atomicAdd(&count[which][b0], all);
+    return __builtin_amdgcn_readlane(base, lead) + before - n;
   };
   count[0][threadIdx.x] = count[1][threadIdx.x] = 0;
   __syncthreads();
@@ -86,12 +94,8 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   int mine[2], sum[2];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    sum[which] = mine[which] = count[which][threadIdx.x];
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int x = __shfl_up(sum[which], d);
-      if (threadIdx.x % 64 >= d) sum[which] += x;
-    }
+    mine[which] = count[which][threadIdx.x];
+    sum[which] = scan_wave(mine[which]);
     if (threadIdx.x % 64 == 63) wave_sum[which][threadIdx.x / 64] = sum[which];
   }
   __syncthreads();
@@ -120,7 +124,6 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
 struct Place {
   int tile, kv, part, q0, nq, k0, nk;
 };
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 // entry `at` of a list times its key/value heads
 __device__ __forceinline__ bool place(const Attend& a, int which, int at, Place& p) {
   const int entry = at / a.kv_heads;
@@ -145,9 +148,9 @@ __device__ __forceinline__ bool place_of_block(const Attend& a, int which, int p
     if (left <= 0 || r / XCDS >= mine) return false;
     at = base + r % XCDS * mine + r / XCDS;
     p.part = at % parts, at /= parts;
-  } else {  // the parts take turns on each XCD
-    p.part = b / XCDS % parts;
-    at = b / (XCDS * parts) * XCDS + b % XCDS;
+  } else {  // the heavier part first
+    const int n = uniform(a.order[which]) * a.kv_heads;
+    p.part = parts > 1 && b >= n, at = b - p.part * n;
   }
   return place(a, which, at, p);
 }
