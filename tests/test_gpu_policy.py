@@ -720,3 +720,37 @@ def test_operators_in_a_graph():
         torch.cuda.synchronize()
         for i, (a, b) in enumerate(zip(want, held)):
             assert torch.equal(a, b), (turn, i)
+
+
+def test_operators_compiled():
+    """torch.compile keeps each operator as one node of a full graph, forward and backward, with eager's results."""
+    x, w, b = rand((300, 64), F32, 1), rand((64,), F32, 2), rand((64,), F32, 3)
+    lq = [20, 0, 44, 11]
+    a, heads = starts(lq), rand((75, 6, 64), BF16, 4)
+
+    def loss(x, w, b, heads):
+        y = policy.layer_norm(torch.sin(x), w, b)
+        o = policy.attention(heads[:, :2], heads[:, 2:4], heads[:, 4:], a)
+        return (y * y).sum() + (o.float() * 3).sum()
+
+    def run(f):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, heads)]
+        value = f(*leaves)
+        return [value.detach(), *torch.autograd.grad(value, leaves)]
+    eager, compiled = run(loss), run(torch.compile(loss, fullgraph=True, backend="aot_eager"))
+    for i, (e, c) in enumerate(zip(eager, compiled)):
+        assert torch.equal(e, c), i
+    grads = [rand((50, 3), F32, 5), rand((7,), F32, 6)]
+    clip = torch.compile(lambda g: policy.clip_grads_(g, 0.5) * 2, fullgraph=True, backend="aot_eager")
+    one, two = [g.clone() for g in grads], [g.clone() for g in grads]
+    assert torch.equal(clip(one), policy.clip_grads_(two, 0.5) * 2) and all(torch.equal(p, q) for p, q in zip(one, two))
+
+
+def test_clipping_marks_what_it_writes():
+    """A graph that saved a tensor which clipping then overwrites notices."""
+    w = rand((8,), F32, 1).requires_grad_()
+    g = rand((8,), F32, 2)
+    y = (w * g).sum()
+    policy.clip_grads_([g], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
