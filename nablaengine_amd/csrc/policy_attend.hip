@@ -37,9 +37,9 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   static_assert(QROWS == 128, "");
   const long long caps[2] = {order_queries(seqs, tq, group), order_keys(seqs, tk, key_waves)};
   int* const lists[2] = {order + ORDER_HEAD, order + ORDER_HEAD + 2 * caps[0]};
-  auto bucket_of = [](long long cost) {  // rows or keys of the other side
-    cost = cost > 0 ? (cost + TILE - 1) / TILE : 0;
-    return (int)(BUCKETS - 1 - (cost < BUCKETS ? cost : BUCKETS - 1));
+  auto bucket_of = [](int cost) {  // rows or keys of the other side, below 2^30
+    const int tiles = cost > 0 ? (int)((unsigned)(cost + TILE - 1) / TILE) : 0;
+    return BUCKETS - 1 - (tiles < BUCKETS ? tiles : BUCKETS - 1);
   };
   // f(list, sequence, first tile, tiles, bucket) for every stretch of tiles that stays together; every lane of a wave takes
   // part each time, with 0 tiles where it has none
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
         const int mq = which && s == seqs ? 0 : nq, mk = !which && s == seqs ? 0 : nk;
         const int rows = which ? mk : mq * group, tiles = mine ? (rows + (1 << bits[which]) - 1) >> bits[which] : 0;
         auto bucket = [&](int t) {
-          long long cost;
+          int cost;
           if (which) {  // the query rows that see the tile's first key
             const int from = (t << bits[1]) - (mk - mq);
             cost = mq - (from > 0 ? from : 0);
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
           return bucket_of(cost);
         };
         if (by_sequence) {  // its heaviest tile: the last row sees every key, the first key almost every row
-          f(which, s, 0, tiles, bucket_of(which ? (long long)(mq < mk ? mq : mk) * group : mk));
+          f(which, s, 0, tiles, bucket_of(which ? (mq < mk ? mq : mk) * group : mk));
         } else {
           for (int t = lane; __any(t < tiles); t += ls) f(which, s, t, t < tiles ? 1 : 0, bucket(t));
         }
@@ -548,12 +548,14 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
           if (ROLE != VALUES) gr[x] = read_rows<DP>(gt, 32 * i, y + x, n, h);
         }
         phase();
+        if (WAVES == 8) __builtin_amdgcn_s_setprio(1);  // products first: 965 us for 993 without
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           s = mfma(qr[x], k[y + x], s);
           if (ROLE != VALUES) dp = mfma(gr[x], v[y + x], dp);
         }
       }
+      if (WAVES == 8) __builtin_amdgcn_s_setprio(0);
       V8<T> qc[2][DT], gc[2][DT];  // on their way during the exponentials
 #pragma unroll
       for (int x = 0; x < AHEAD; ++x)
@@ -585,11 +587,13 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const V8<T> pr = pack<T>(s, x), ds = pack<T>(dp, x);
+        if (WAVES == 8) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           if (ROLE != KEYS) dv[d] = mfma(x < AHEAD ? gc[x][d] : read_columns<DP>(gt, 32 * i + 16 * x, d, l), pr, dv[d]);
           if (ROLE != VALUES) dk[d] = mfma(x < AHEAD ? qc[x][d] : read_columns<DP>(qt, 32 * i + 16 * x, d, l), ds, dk[d]);
         }
+        if (WAVES == 8) __builtin_amdgcn_s_setprio(0);
       }
     }
   }
