@@ -40,20 +40,24 @@ long long dk_clip_work_bytes(int count);
  * kv_heads) and tk below 2^30. starts_q, starts_k: seqs + 1 int32 on the device, 0 first: sequence s has the tokens
  * starts[s] .. starts[s + 1] - 1. Query i of a sequence of nq queries and nk keys sees its keys 0 .. i + nk - nq; one
  * that sees none gives zeros, as do tokens past the last sequence. out (tq, heads, dim) contiguous; lse (heads, tq)
- * float32 for the backward, or NULL; work: dk_attention_work_bytes bytes, which the backward reads again. scale > 0.
+ * float32 for the backward, or NULL; work: dk_attention_work_bytes bytes, which the backward reads again; scratch:
+ * dk_attention_scratch_bytes bytes (vjp 0), or NULL when 0. scale > 0.
  * Offsets outside the tokens are moved inside them; they never make the call read or write out of bounds. */
 int dk_attention(hipStream_t st, int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk, const void* q,
                  long long q_t, long long q_h, const void* k, long long k_t, long long k_h, const void* v,
                  long long v_t, long long v_h, const int* starts_q, const int* starts_k, float scale, void* out,
-                 float* lse, void* work);
+                 float* lse, void* work, void* scratch);
 /* Its VJP, from the forward's arguments, out, lse and work: dout (strides do_t, do_h) -> dq (tq, heads, dim), dk, dv
- * (tk, kv_heads, dim), contiguous. delta: (heads, tq) float32 scratch. */
+ * (tk, kv_heads, dim), contiguous. delta: (heads, tq) float32 scratch; scratch:
+ * dk_attention_scratch_bytes bytes (vjp 1), or NULL when 0. */
 int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk,
                      const void* q, long long q_t, long long q_h, const void* k, long long k_t, long long k_h,
                      const void* v, long long v_t, long long v_h, const int* starts_q, const int* starts_k,
                      float scale, const void* out, const float* lse, const void* work, const void* dout,
-                     long long do_t, long long do_h, float* delta, void* dq, void* dk, void* dv);
+                     long long do_t, long long do_h, float* delta, void* dq, void* dk, void* dv,
+                     void* scratch);
 long long dk_attention_work_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk);
+long long dk_attention_scratch_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk, int vjp);
 
 /* Attention of one query a world over that world's cache: q (worlds, heads, dim), k, v (worlds, capacity, kv_heads,
  * dim) with elements from world to world (_w), token to token (_t) and head to head (_h); lengths: worlds int32 on the

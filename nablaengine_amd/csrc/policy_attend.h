@@ -36,8 +36,10 @@ struct Attend {
   int heads, kv_heads, group, dim, seqs, tq, tk;
   int by_sequence;  // the order of the tiles, see below
   int key_waves;  // 32 keys each: a tile of the keys' gradients (1, 2 or 4)
+  int parts_q, parts_k;  // workgroups (of a role) among which a query tile's keys, a key tile's rows are split
   const int *starts_q, *starts_k;
   float scale;
+  float* scratch;  // their sums, one slot each
   void* out;   // (tq, heads, dim)
   float* lse;  // (heads, tq): log2 of the row's sum of exponentials, +inf for a row without keys; NULL: not kept
   const int* order;
@@ -63,6 +65,18 @@ __host__ __device__ inline long long order_queries(int seqs, int tq, int group) 
 __host__ __device__ inline long long order_keys(int seqs, int tk, int key_waves) {
   return (long long)tk / (32 * key_waves) + seqs + 1;
 }
+
+// A tile's loop over `tiles` tiles of the other side, split among `parts` workgroups (at least LEAST each): this one's.
+constexpr int LEAST = 4;
+struct Slice {
+  int first, end, parts;  // parts: those that have any, and one where none has
+  __host__ __device__ __forceinline__ Slice(int tiles, int most, int part) {
+    const int split = (tiles + most - 1) / most, each = split > LEAST ? split : LEAST;
+    first = part * each < tiles ? part * each : tiles;
+    end = first + each < tiles ? first + each : tiles;
+    parts = tiles > each ? (tiles + each - 1) / each : 1;
+  }
+};
 
 // Sequence s of the packed tokens [0, total): its first token and length, kept inside the tokens whatever `starts`
 // holds. Sequence `seqs` is what lies past the last one: its queries have no keys and its keys no queries.
@@ -157,11 +171,11 @@ struct Row {
     return __all(nan);
   }
   template <typename T>
-  __device__ __forceinline__ void store(T* p, int dim, float f) const {
+  __device__ __forceinline__ void store(T* p, int from, int to, float f) const {  // elements from .. to - 1
 #pragma unroll
     for (int i = 0; i < DP / 64; ++i) {
       const int d = threadIdx.x % 64 + 64 * i;
-      if (d < dim) p[d] = (T)(x[i] * f);
+      if (d >= from && d < to) p[d] = (T)(x[i] * f);
     }
   }
 };
@@ -205,15 +219,15 @@ __device__ __forceinline__ void load_rows(const T* p, int dim, int h, V8<T>* f) 
   }
 }
 
-// A C of columns = rows of a result (transposed result), d = 32 t + register's row, to p (NULL: none), times f
-template <int DP, typename T>
-__device__ __forceinline__ void store_rows(T* p, int dim, int h, const F16x* acc, float f) {
+// A C of columns = rows of a result (transposed result), d = d0 + 32 t + register's row, to p (NULL: none), times f
+template <int N, typename T>
+__device__ __forceinline__ void store_rows(T* p, int d0, int dim, int h, const F16x* acc, float f) {
   if (!p) return;
 #pragma unroll
-  for (int t = 0; t < DP / 32; ++t)
+  for (int t = 0; t < N; ++t)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int d = 32 * t + 8 * j + 4 * h;
+      const int d = d0 + 32 * t + 8 * j + 4 * h;
       if (d < dim) {
         typedef T T4 __attribute__((ext_vector_type(4)));
         T4 o;

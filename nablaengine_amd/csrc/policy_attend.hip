@@ -122,7 +122,7 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
 
 // what a workgroup works on
 struct Place {
-  int tile, kv, part, q0, nq, k0, nk;
+  int at, tile, kv, part, q0, nq, k0, nk;
 };
 // entry `at` of a list times its key/value heads
 __device__ __forceinline__ bool place(const Attend& a, int which, int at, Place& p) {
@@ -130,6 +130,7 @@ __device__ __forceinline__ bool place(const Attend& a, int which, int at, Place&
   if (entry >= uniform(a.order[which])) return false;
   const int* list = a.order + ORDER_HEAD + (which ? 2 * order_queries(a.seqs, a.tq, a.group) : 0) + 2LL * entry;
   const int s = uniform(list[0]);
+  p.at = at;
   p.tile = uniform(list[1]);
   p.kv = at % a.kv_heads;
   sequence(a.starts_q, s, a.seqs, a.tq, p.q0, p.nq);
@@ -150,14 +151,14 @@ __device__ __forceinline__ bool place_of_block(const Attend& a, int which, int p
     p.part = at % parts, at /= parts;
   } else {  // the heavier part first
     const int n = uniform(a.order[which]) * a.kv_heads;
-    p.part = parts > 1 && b >= n, at = b - p.part * n;
+    if (b >= n * parts) return false;
+    p.part = parts > 1 ? b / n : 0, at = b - p.part * n;
   }
   return place(a, which, at, p);
 }
 // workgroups that cover a list of at most `most` tiles
 unsigned blocks_of(const Attend& a, long long most, int parts) {
-  constexpr long long turn = WINDOW * XCDS;
-  return (unsigned)((most * a.kv_heads * parts + turn - 1) / turn * turn);
+  return (unsigned)((most * a.kv_heads * parts + XCDS - 1) / XCDS * XCDS);
 }
 
 // The keys' side of the forward and of the queries' gradient: tiles of TILE keys and their values, one tile ahead.
@@ -168,15 +169,15 @@ struct Keys {
   long long k_t, v_t;
   int row, at, left;  // this thread's row; its wave's place in LDS; keys from the tile's first on
   bool in_row;
-  __device__ __forceinline__ Keys(const Attend& a, const Place& p) {
+  __device__ __forceinline__ Keys(const Attend& a, const Place& p, int first) {  // from tile `first` on
     row = threadIdx.x / CH;
     const int c = threadIdx.x % CH ^ swizzle<DP>(row);  // LDS is filled in order: the swizzle is the source's
     in_row = 8 * c < a.dim;
     k_t = a.k_t, v_t = a.v_t;
-    k = (const T*)a.k + (long long)p.k0 * k_t + (long long)p.kv * a.k_h + row * k_t + 8 * c;
-    v = (const T*)a.v + (long long)p.k0 * v_t + (long long)p.kv * a.v_h + row * v_t + 8 * c;
+    k = (const T*)a.k + (long long)(p.k0 + first * TILE) * k_t + (long long)p.kv * a.k_h + row * k_t + 8 * c;
+    v = (const T*)a.v + (long long)(p.k0 + first * TILE) * v_t + (long long)p.kv * a.v_h + row * v_t + 8 * c;
     at = threadIdx.x / 64 * 64 * 8;
-    left = p.nk;
+    left = p.nk - first * TILE;
   }
   __device__ __forceinline__ void next(T* ks, T* vs) {
 #pragma unroll
@@ -195,8 +196,8 @@ struct Keys {
 struct Rows {
   int pos, head, limit, all_see, any_sees, tiles;
   bool valid;
-  __device__ __forceinline__ Rows(const Attend& a, const Place& p) {
-    const int rows = p.nq * a.group, off = p.nk - p.nq, w = uniform(threadIdx.x / 64);
+  __device__ __forceinline__ Rows(const Attend& a, const Place& p, int w) {
+    const int rows = p.nq * a.group, off = p.nk - p.nq;
     const int row0 = p.tile * QROWS + 32 * w, row = row0 + threadIdx.x % 32;
     valid = row < rows;
     pos = row / a.group;
@@ -223,29 +224,106 @@ struct Sight {
 
 // ---- forward --------------------------------------------------------------------------------------------------------
 
-template <typename T, int DP>
+// What a tile's parts hand to the join, in the order of the registers: each lane's N sums, and for N + 2 a row's maximum and
+// its sum of probabilities.
+template <int N>
+struct Part {
+  static constexpr size_t SIZE = 256 * N;  // floats of a slot: four waves
+  float* at;
+  __device__ __forceinline__ Part(const Attend& a, size_t slot, int wave) {
+    at = a.scratch + slot * SIZE + wave * 64 * N + threadIdx.x % 64;
+  }
+  __device__ __forceinline__ void put(int first, const F16x* acc, int n) const {
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) at[64 * (16 * (first + i) + j)] = acc[i][j];
+  }
+};
+template <int DP>
+using RowsPart = Part<DP / 2 + 2>;
+// One block of the join: 32 rows (keys) and 32 of their elements. Its four waves take every fourth part, f(part) times it,
+// and wave 0 gets the sum of all.
+template <int N, typename F>
+__device__ __forceinline__ F16x add_parts(const Attend& a, size_t slot, int parts, int wave, int block, F f) {
+  __shared__ float sums[3][16][64];
+  const int w = uniform(threadIdx.x / 64), l = threadIdx.x % 64;
+  F16x acc = {};
+#pragma unroll 4
+  for (int i = w; i < parts; i += 4) {
+    const float* from = Part<N>(a, slot + i, wave).at + 64 * 16 * block;
+    const float times = f(i);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[j] = fmaf(times, from[64 * j], acc[j]);
+  }
+  if (w)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sums[w - 1][j][l] = acc[j];
+  __syncthreads();
+  if (!w)
+#pragma unroll
+    for (int o = 0; o < 3; ++o)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[j] += sums[o][j][l];
+  return acc;
+}
+
+// what a wave's rows come to, from their outputs' sums, the maximum that these lack and the probabilities' sum
+template <typename T, int DP, int N>
+__device__ __forceinline__ void finish_rows(const Attend& a, const Place& p, const Rows& r, int d0, const F16x* acc, float m,
+                                            float sum) {
+  const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
+  const float c = a.scale * LOG2E;
+  const long long token = p.q0 + r.pos;
+  if (a.lse && r.valid && h == 0 && d0 == 0)
+    a.lse[(long long)r.head * a.tq + token] = sum == 0.0f ? INFINITY : m * c + log2f(sum);
+  const unsigned bad = bad_columns(r.valid && not_finite<N>(acc) != 0.0f);
+  store_rows<N>(r.valid && !(bad >> n & 1) ? (T*)a.out + (token * a.heads + r.head) * dim : nullptr, d0, dim, h, acc,
+                sum == 0.0f ? 0.0f : 1.0f / sum);
+  for (unsigned left = bad; left; left &= left - 1) {
+    const Sight one(a, p, r, __builtin_ctz(left));
+    const Row<DP> qr((const T*)a.q + one.token * a.q_t + one.head * a.q_h, dim);
+    Row<DP> o = {};
+    float top = -INFINITY, total = 0.0f;
+    for (int j = 0; j <= one.limit && total == total; ++j) {
+      const float x = qr.dot(Row<DP>((const T*)a.k + (p.k0 + j) * a.k_t + p.kv * a.k_h, dim)) * c, top1 = fmaxf(top, x);
+      const float base1 = top1 == -INFINITY ? 0.0f : top1, f = exp2_fast(top - base1), pr = exp2_fast(x - base1);
+      total = total * f + pr;
+#pragma unroll
+      for (int i = 0; i < DP / 64; ++i) o.x[i] *= f;
+      o.add(pr, Row<DP>((const T*)a.v + (p.k0 + j) * a.v_t + p.kv * a.v_h, dim));
+      top = top1;
+    }
+    o.store((T*)a.out + (one.token * a.heads + one.head) * dim, d0, d0 + 32 * N < dim ? d0 + 32 * N : dim, total == 0.0f ? 0.0f : 1.0f / total);
+  }
+}
+
+template <typename T, int DP, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
   constexpr int KS = DP / 16, DT = DP / 32;
   __shared__ __align__(16) T ks[2][TILE * DP];
   __shared__ __align__(16) T vs[2][TILE * DP];
   Place p;
-  if (!place_of_block(a, 0, 1, p)) return;
+  if (!place_of_block(a, 0, SPLIT ? a.parts_q : 1, p)) return;
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
-  const Rows r(a, p);
-  Keys<DP, T> keys(a, p);
-  if (r.tiles) keys.next(ks[0], vs[0]);
+  const Rows r(a, p, uniform(threadIdx.x / 64));
+  const Slice my(r.tiles, SPLIT ? a.parts_q : 1, SPLIT ? p.part : 0);
+  const int first = SPLIT ? my.first : 0, end = SPLIT ? my.end : r.tiles;
+  if (SPLIT && p.part >= my.parts) return;
+  Keys<DP, T> keys(a, p, first);
+  if (first < end) keys.next(ks[first & 1], vs[first & 1]);
   V8<T> q[KS];
   load_rows<DP>(r.valid ? (const T*)a.q + (long long)(p.q0 + r.pos) * a.q_t + (long long)r.head * a.q_h : nullptr, dim, h,
                 q);
   F16x acc[DT] = {};
   float m = -INFINITY, sum = 0.0f;
   const float c = a.scale * LOG2E;
-  for (int t = 0; t < r.tiles; ++t) {
+  for (int t = first; t < end; ++t) {
     const int key0 = t * TILE;
     const T *kt = ks[t & 1], *vt = vs[t & 1];
     loads_done();
     __syncthreads();  // this tile is there for all, and all are done with the one before
-    if (t + 1 < r.tiles) keys.next(ks[(t + 1) & 1], vs[(t + 1) & 1]);
+    if (t + 1 < end) keys.next(ks[(t + 1) & 1], vs[(t + 1) & 1]);
     if (key0 > r.any_sees) continue;
     const bool second = key0 + 32 <= r.any_sees;
     F16x s[2] = {};
@@ -297,43 +375,77 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
     }
   }
   sum = add_halves(sum);
-  const long long token = p.q0 + r.pos;
-  if (a.lse && r.valid && h == 0)
-    a.lse[(long long)r.head * a.tq + token] = sum == 0.0f ? INFINITY : m * c + log2f(sum);
-  const unsigned bad = bad_columns(r.valid && not_finite<DT>(acc) != 0.0f);
-  store_rows<DP>(r.valid && !(bad >> n & 1) ? (T*)a.out + (token * a.heads + r.head) * dim : nullptr, dim, h, acc,
-                 sum == 0.0f ? 0.0f : 1.0f / sum);
-  for (unsigned left = bad; left; left &= left - 1) {
-    const Sight one(a, p, r, __builtin_ctz(left));
-    const Row<DP> qr((const T*)a.q + one.token * a.q_t + one.head * a.q_h, dim);
-    Row<DP> o = {};
-    float top = -INFINITY, total = 0.0f;
-    for (int j = 0; j <= one.limit && total == total; ++j) {
-      const float x = qr.dot(Row<DP>((const T*)a.k + (p.k0 + j) * a.k_t + p.kv * a.k_h, dim)) * c, top1 = fmaxf(top, x);
-      const float base1 = top1 == -INFINITY ? 0.0f : top1, f = exp2_fast(top - base1), pr = exp2_fast(x - base1);
-      total = total * f + pr;
-#pragma unroll
-      for (int i = 0; i < DP / 64; ++i) o.x[i] *= f;
-      o.add(pr, Row<DP>((const T*)a.v + (p.k0 + j) * a.v_t + p.kv * a.v_h, dim));
-      top = top1;
-    }
-    o.store((T*)a.out + (one.token * a.heads + one.head) * dim, dim, total == 0.0f ? 0.0f : 1.0f / total);
+  if (SPLIT && my.parts > 1) {
+    const RowsPart<DP> mine(a, (size_t)p.at * a.parts_q + p.part, uniform(threadIdx.x / 64));
+    mine.put(0, acc, DT);
+    mine.at[64 * 16 * DT] = m, mine.at[64 * (16 * DT + 1)] = sum;
+    return;
   }
+  finish_rows<T, DP, DT>(a, p, r, 0, acc, m, sum);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_attend_join(Attend a) {
+  constexpr int DT = DP / 32, N = DP / 2 + 2;
+  const int wave = blockIdx.y / DT, block = blockIdx.y % DT;
+  Place p;
+  if (!place_of_block(a, 0, 1, p)) return;
+  const Rows r(a, p, wave);
+  const int parts = Slice(r.tiles, a.parts_q, 0).parts;
+  if (parts == 1) return;
+  const size_t slot = (size_t)p.at * a.parts_q;
+  auto stat = [&](int part, int which) { return Part<N>(a, slot + part, wave).at[64 * (N - 2 + which)]; };
+  const float c = a.scale * LOG2E;
+  float m = -INFINITY, sum = 0.0f;
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, stat(i, 0));
+  const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i) sum += exp2_fast((stat(i, 0) - base) * c) * stat(i, 1);
+  const F16x acc = add_parts<N>(a, slot, parts, wave, block, [&](int i) { return exp2_fast((stat(i, 0) - base) * c); });
+  if (threadIdx.x < 64) finish_rows<T, DP, 1>(a, p, r, 32 * block, &acc, m, sum);
 }
 
 // ---- backward: the queries' gradient --------------------------------------------------------------------------------
 
-template <typename T, int DP>
+template <typename T, int DP, int N>
+__device__ __forceinline__ void finish_dq(const Attend& a, const Place& p, const Rows& r, int d0, const F16x* acc, float lse,
+                                          float delta) {
+  const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
+  const float c = a.scale * LOG2E;
+  const long long token = p.q0 + r.pos;
+  const unsigned bad = bad_columns(r.valid && not_finite<N>(acc) != 0.0f);
+  store_rows<N>(r.valid && !(bad >> n & 1) ? (T*)a.dq + (token * a.heads + r.head) * dim : nullptr, d0, dim, h, acc, a.scale);
+  for (unsigned left = bad; left; left &= left - 1) {
+    const int i = __builtin_ctz(left);
+    const Sight one(a, p, r, i);
+    const Row<DP> qr((const T*)a.q + one.token * a.q_t + one.head * a.q_h, dim);
+    const Row<DP> gr((const T*)a.dout + one.token * a.do_t + one.head * a.do_h, dim);
+    const float lse1 = __shfl(lse, i), delta1 = __shfl(delta, i);
+    Row<DP> o = {};
+    for (int j = 0; j <= one.limit && !o.all_nan(dim); ++j) {
+      const Row<DP> kr((const T*)a.k + (p.k0 + j) * a.k_t + p.kv * a.k_h, dim);
+      const float dp = gr.dot(Row<DP>((const T*)a.v + (p.k0 + j) * a.v_t + p.kv * a.v_h, dim));
+      o.add(exp2_fast(qr.dot(kr) * c - lse1) * (dp - delta1), kr);
+    }
+    o.store((T*)a.dq + (one.token * a.heads + one.head) * dim, d0, d0 + 32 * N < dim ? d0 + 32 * N : dim, a.scale);
+  }
+}
+
+template <typename T, int DP, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
   constexpr int KS = DP / 16, DT = DP / 32;
   __shared__ __align__(16) T ks[2][TILE * DP];
   __shared__ __align__(16) T vs[2][TILE * DP];
   Place p;
-  if (!place_of_block(a, 0, 1, p)) return;
+  if (!place_of_block(a, 0, SPLIT ? a.parts_q : 1, p)) return;
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
-  const Rows r(a, p);
-  Keys<DP, T> keys(a, p);
-  if (r.tiles) keys.next(ks[0], vs[0]);
+  const Rows r(a, p, uniform(threadIdx.x / 64));
+  const Slice my(r.tiles, SPLIT ? a.parts_q : 1, SPLIT ? p.part : 0);
+  const int first = SPLIT ? my.first : 0, end = SPLIT ? my.end : r.tiles;
+  if (SPLIT && p.part >= my.parts) return;
+  Keys<DP, T> keys(a, p, first);
+  if (first < end) keys.next(ks[first & 1], vs[first & 1]);
   const long long token = p.q0 + r.pos;
   V8<T> q[KS], g[KS];
   load_rows<DP>(r.valid ? (const T*)a.q + token * a.q_t + (long long)r.head * a.q_h : nullptr, dim, h, q);
@@ -369,12 +481,12 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
     delta = add_halves(delta);
   }
   F16x acc[DT] = {};
-  for (int t = 0; t < r.tiles; ++t) {
+  for (int t = first; t < end; ++t) {
     const int key0 = t * TILE;
     const T *kt = ks[t & 1], *vt = vs[t & 1];
     loads_done();
     __syncthreads();
-    if (t + 1 < r.tiles) keys.next(ks[(t + 1) & 1], vs[(t + 1) & 1]);
+    if (t + 1 < end) keys.next(ks[(t + 1) & 1], vs[(t + 1) & 1]);
     if (t == 0 && few) {
 #pragma unroll 1
       for (int i = 0; 32 * i <= r.any_sees; ++i) {
@@ -400,23 +512,28 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
       }
     }
   }
-  if (r.valid && h == 0) a.delta[(long long)r.head * a.tq + token] = delta;
-  const unsigned bad = bad_columns(r.valid && not_finite<DT>(acc) != 0.0f);
-  store_rows<DP>(r.valid && !(bad >> n & 1) ? (T*)a.dq + (token * a.heads + r.head) * dim : nullptr, dim, h, acc, a.scale);
-  for (unsigned left = bad; left; left &= left - 1) {
-    const int i = __builtin_ctz(left);
-    const Sight one(a, p, r, i);
-    const Row<DP> qr((const T*)a.q + one.token * a.q_t + one.head * a.q_h, dim);
-    const Row<DP> gr((const T*)a.dout + one.token * a.do_t + one.head * a.do_h, dim);
-    const float lse1 = __shfl(lse, i), delta1 = __shfl(delta, i);
-    Row<DP> o = {};
-    for (int j = 0; j <= one.limit && !o.all_nan(dim); ++j) {
-      const Row<DP> kr((const T*)a.k + (p.k0 + j) * a.k_t + p.kv * a.k_h, dim);
-      const float dp = gr.dot(Row<DP>((const T*)a.v + (p.k0 + j) * a.v_t + p.kv * a.v_h, dim));
-      o.add(exp2_fast(qr.dot(kr) * c - lse1) * (dp - delta1), kr);
-    }
-    o.store((T*)a.dq + (one.token * a.heads + one.head) * dim, dim, a.scale);
+  if (r.valid && h == 0 && (!SPLIT || p.part == 0)) a.delta[(long long)r.head * a.tq + token] = delta;
+  if (SPLIT && my.parts > 1) {
+    RowsPart<DP>(a, (size_t)p.at * a.parts_q + p.part, uniform(threadIdx.x / 64)).put(0, acc, DT);
+    return;
   }
+  finish_dq<T, DP, DT>(a, p, r, 0, acc, lse, delta);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_attend_dq_join(Attend a) {
+  constexpr int DT = DP / 32;
+  const int wave = blockIdx.y / DT, block = blockIdx.y % DT;
+  Place p;
+  if (!place_of_block(a, 0, 1, p)) return;
+  const Rows r(a, p, wave);
+  const int parts = Slice(r.tiles, a.parts_q, 0).parts;
+  if (parts == 1) return;
+  const F16x acc =
+      add_parts<DP / 2 + 2>(a, (size_t)p.at * a.parts_q, parts, wave, block, [](int) { return 1.0f; });
+  const long long at = (long long)r.head * a.tq + p.q0 + r.pos;
+  if (threadIdx.x < 64)
+    finish_dq<T, DP, 1>(a, p, r, 32 * block, &acc, r.valid ? a.lse[at] : INFINITY, r.valid ? a.delta[at] : 0.0f);
 }
 
 // ---- backward: the keys' and values' gradients ----------------------------------------------------------------------
@@ -437,11 +554,57 @@ struct DkvTiles {
 // of 16 heads against 1480 us with both in one and part of the operands in LDS or scratch. Eight waves share a tile of
 // 128 rows there: with four, the tiles that all rows read are one round's length each.
 enum Role { BOTH, KEYS, VALUES };
-template <typename T, int DP, int KW, int WAVES, int ROLE>
+struct RowTiles {  // the rows that see a key tile, in tiles of RT rows or a little less
+  int used, first, tiles;
+  __device__ __forceinline__ RowTiles(const Attend& a, const Place& p, int kw, int rt) {
+    used = a.group <= rt ? rt / a.group * a.group : rt;
+    const int rows = p.nq * a.group, from = p.tile * 32 * kw - (p.nk - p.nq);  // the first token that sees the tile's first key
+    first = (from > 0 ? from : 0) * a.group;
+    tiles = rows > first ? (rows - 1 - first) / used + 1 : 0;
+  }
+};
+// a key tile's part: dk and dv of its 32 keys a wave in turn (heads of 64), or one of them
+constexpr int KEY_PART = 64;
+__device__ __forceinline__ size_t key_slot(const Attend& a, const Place& p, int role) {
+  return ((size_t)p.at * (role == BOTH ? 1 : 2) + (role == VALUES)) * a.parts_k;
+}
+template <typename T, int DP, int N, int ROLE>
+__device__ __forceinline__ void finish_dkv(const Attend& a, const Place& p, int key0, int d0, const F16x* dk, const F16x* dv) {
+  const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim, group = a.group;
+  const int rows = p.nq * group, off = p.nk - p.nq, key = key0 + n;
+  const bool valid = key < p.nk;
+  const float c = a.scale * LOG2E;
+  const float off_dv = ROLE != KEYS ? not_finite<N>(dv) : 0.0f, off_dk = ROLE != VALUES ? not_finite<N>(dk) : 0.0f;
+  const unsigned bad = bad_columns(valid && off_dv + off_dk != 0.0f);
+  const bool put = valid && !(bad >> n & 1);
+  const long long at = ((long long)(p.k0 + key) * a.kv_heads + p.kv) * dim;
+  if (ROLE != VALUES) store_rows<N>(put ? (T*)a.dk + at : nullptr, d0, dim, h, dk, a.scale);
+  if (ROLE != KEYS) store_rows<N>(put ? (T*)a.dv + at : nullptr, d0, dim, h, dv, 1.0f);
+  for (unsigned left = bad; left; left &= left - 1) {
+    const int one = key0 + __builtin_ctz(left);
+    const Row<DP> kr((const T*)a.k + (long long)(p.k0 + one) * a.k_t + p.kv * a.k_h, dim);
+    const Row<DP> vr((const T*)a.v + (long long)(p.k0 + one) * a.v_t + p.kv * a.v_h, dim);
+    Row<DP> ok = {}, ov = {};
+    for (int r = (one - off > 0 ? one - off : 0) * group;
+         r < rows && !((ROLE == VALUES || ok.all_nan(dim)) && (ROLE == KEYS || ov.all_nan(dim))); ++r) {
+      const long long token = p.q0 + r / group, head = p.kv * group + r % group;
+      const Row<DP> qr((const T*)a.q + token * a.q_t + head * a.q_h, dim);
+      const Row<DP> gr((const T*)a.dout + token * a.do_t + head * a.do_h, dim);
+      const float pr = exp2_fast(qr.dot(kr) * c - a.lse[head * a.tq + token]);
+      if (ROLE != KEYS) ov.add(pr, gr);
+      if (ROLE != VALUES) ok.add(pr * (gr.dot(vr) - a.delta[head * a.tq + token]), qr);
+    }
+    const long long to = ((long long)(p.k0 + one) * a.kv_heads + p.kv) * dim;
+    const int d1 = d0 + 32 * N < dim ? d0 + 32 * N : dim;
+    if (ROLE != VALUES) ok.store((T*)a.dk + to, d0, d1, a.scale);
+    if (ROLE != KEYS) ov.store((T*)a.dv + to, d0, d1, 1.0f);
+  }
+}
+template <typename T, int DP, int KW, int WAVES, int ROLE, bool PARTS>
 __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, WAVES>& lds) {
   constexpr int RT = DkvTiles<T, DP, WAVES>::RT;
   constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 64 * WAVES / CH, SPLIT = WAVES / KW;
-  constexpr int AHEAD = DP == 64 ? 2 : KW == 4 ? 1 : 0;  // of a subtile's two column operands, those read during the exponentials
+  constexpr int AHEAD = DP == 64 ? 2 : KW == 4 && !PARTS ? 1 : 0;  // of a subtile's two column operands, those read during the exponentials
   constexpr int SUB = RT / 32, N = RT / STEP;
   auto& tiles = lds.tiles;
   auto &lses = lds.lses, &deltas = lds.deltas;
@@ -464,10 +627,8 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
 
   // Row tiles start at whole tokens (but for groups above RT, whose rows' places are computed anew for each tile), so
   // that a thread's rows keep their distance from the tile's first token: RT or a little less rows are used of each.
-  const int used = group <= RT ? RT / group * group : RT;
-  const int back = used / group;  // tokens of a tile
-  const int from = p.tile * 32 * KW - off;  // the first token that sees the tile's first key
-  const int first = (from > 0 ? from : 0) * group;
+  const RowTiles all(a, p, KW, RT);
+  const int used = all.used, first = all.first, back = used / group;  // back: tokens of a tile
   auto chunk = [&](int i) { return tid % CH ^ swizzle<DP>(tid / CH + i * STEP); };
   const T *qp[N], *gp[N];  // this thread's rows of the next tile to load, and its row's place in lse and delta
   long long stat = 0;
@@ -505,9 +666,12 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
   };
   // From the last rows, which every key tile of the sequence reads, to the tile's first: workgroups that run side by
   // side then read the same rows at about the same time, from the L2 cache of their XCD.
-  const int start = first + (rows > first ? (rows - 1 - first) / used * used : -used);
-  places(start >= first ? start : 0);
-  if (start >= first) load(start, 0);
+  const Slice my(all.tiles, PARTS ? a.parts_k : 1, PARTS ? p.part % a.parts_k : 0);
+  const int start = first + (all.tiles - 1 - (PARTS ? my.first : 0)) * used;
+  const int last = PARTS ? first + (all.tiles - my.end) * used : first;
+  if (PARTS && p.part % a.parts_k >= my.parts) return;
+  places(start >= last ? start : 0);
+  if (start >= last) load(start, 0);
   V8<T> k[KS], v[KS];
   load_rows<DP>(valid ? (const T*)a.k + (long long)(p.k0 + key) * a.k_t + (long long)p.kv * a.k_h : nullptr, dim, h, k);
   if (ROLE != VALUES)
@@ -518,7 +682,7 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
   const int inverse = 65535 / group + 1;
   auto tokens = [&](int x) { return x * inverse >> 16; };
   int turn = 0, sub0 = 0, token0 = start / group;
-  for (int r0 = start; r0 >= first; r0 -= used, turn ^= 1, sub0 += SUB) {
+  for (int r0 = start; r0 >= last; r0 -= used, turn ^= 1, sub0 += SUB) {
     if (tid < RT) {
       lses[turn][tid] = lse;
       deltas[turn][tid] = delta;
@@ -526,7 +690,7 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
     }
     loads_done();
     meet();
-    if (r0 - used >= first) load(r0 - used, turn ^ 1);
+    if (r0 - used >= last) load(r0 - used, turn ^ 1);
     if (key0 >= p.nk) continue;
     const int token = group <= RT ? token0 : r0 / group;
     token0 -= back;
@@ -622,46 +786,46 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
       }
     if (split) return;
   }
-  const float off_dv = ROLE != KEYS ? not_finite<DT>(dv) : 0.0f, off_dk = ROLE != VALUES ? not_finite<DT>(dk) : 0.0f;
-  const unsigned bad = bad_columns(valid && off_dv + off_dk != 0.0f);
-  const bool put = valid && !(bad >> n & 1);
-  const long long at = ((long long)(p.k0 + key) * a.kv_heads + p.kv) * dim;
-  if (ROLE != VALUES) store_rows<DP>(put ? (T*)a.dk + at : nullptr, dim, h, dk, a.scale);
-  if (ROLE != KEYS) store_rows<DP>(put ? (T*)a.dv + at : nullptr, dim, h, dv, 1.0f);
-  for (unsigned left = bad; left; left &= left - 1) {
-    const int one = key0 + __builtin_ctz(left);
-    const Row<DP> kr((const T*)a.k + (long long)(p.k0 + one) * a.k_t + p.kv * a.k_h, dim);
-    const Row<DP> vr((const T*)a.v + (long long)(p.k0 + one) * a.v_t + p.kv * a.v_h, dim);
-    Row<DP> ok = {}, ov = {};
-    for (int r = (one - off > 0 ? one - off : 0) * group;
-         r < rows && !((ROLE == VALUES || ok.all_nan(dim)) && (ROLE == KEYS || ov.all_nan(dim))); ++r) {
-      const long long token = p.q0 + r / group, head = p.kv * group + r % group;
-      const Row<DP> qr((const T*)a.q + token * a.q_t + head * a.q_h, dim);
-      const Row<DP> gr((const T*)a.dout + token * a.do_t + head * a.do_h, dim);
-      const float pr = exp2_fast(qr.dot(kr) * c - a.lse[head * a.tq + token]);
-      if (ROLE != KEYS) ov.add(pr, gr);
-      if (ROLE != VALUES) ok.add(pr * (gr.dot(vr) - a.delta[head * a.tq + token]), qr);
-    }
-    const long long to = ((long long)(p.k0 + one) * a.kv_heads + p.kv) * dim;
-    if (ROLE != VALUES) ok.store((T*)a.dk + to, dim, a.scale);
-    if (ROLE != KEYS) ov.store((T*)a.dv + to, dim, 1.0f);
+  if (PARTS && my.parts > 1) {
+    const Part<KEY_PART> mine(a, key_slot(a, p, ROLE) + p.part % a.parts_k, w);
+    if (ROLE != VALUES) mine.put(0, dk, DT);
+    if (ROLE != KEYS) mine.put(ROLE == BOTH ? DT : 0, dv, DT);
+    return;
   }
+  finish_dkv<T, DP, DT, ROLE>(a, p, key0, 0, dk, dv);
 }
 
-template <typename T, int DP, int KW, int WAVES>
+template <typename T, int DP, int KW, int WAVES, bool PARTS>
 __global__ __launch_bounds__(WAVES == 8 ? 512 : 256) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_dkv(Attend a) {
   __shared__ DkvTiles<T, DP, WAVES> lds[WAVES == 1 ? 4 : 1];
+  const int parts = PARTS ? a.parts_k : 1;
   Place p;
   if constexpr (WAVES == 1) {  // each wave a tile of its own
     const int w = uniform(threadIdx.x / 64);
-    if (place(a, 1, blockIdx.x * 4 + w, p)) dkv_tile<T, DP, KW, WAVES, BOTH>(a, p, lds[w]);
+    if (place(a, 1, blockIdx.x * 4 + w, p)) dkv_tile<T, DP, KW, WAVES, BOTH, false>(a, p, lds[w]);
   } else if constexpr (DP == 64) {
-    if (place_of_block(a, 1, 1, p)) dkv_tile<T, DP, KW, WAVES, BOTH>(a, p, lds[0]);
+    if (place_of_block(a, 1, parts, p)) dkv_tile<T, DP, KW, WAVES, BOTH, PARTS>(a, p, lds[0]);
   } else {
-    if (!place_of_block(a, 1, 2, p)) return;
-    if (p.part) dkv_tile<T, DP, KW, WAVES, VALUES>(a, p, lds[0]);
-    else dkv_tile<T, DP, KW, WAVES, KEYS>(a, p, lds[0]);
+    if (!place_of_block(a, 1, 2 * parts, p)) return;
+    if (p.part >= parts) dkv_tile<T, DP, KW, WAVES, VALUES, PARTS>(a, p, lds[0]);
+    else dkv_tile<T, DP, KW, WAVES, KEYS, PARTS>(a, p, lds[0]);
   }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_attend_dkv_join(Attend a) {
+  constexpr int DT = DP / 32;
+  const int role = blockIdx.y / (4 * DT) ? VALUES : KEYS, wave = blockIdx.y / DT % 4, block = blockIdx.y % DT;
+  Place p;
+  if (!place_of_block(a, 1, 1, p)) return;
+  const int parts = Slice(RowTiles(a, p, 4, DkvTiles<T, DP, DP / 16>::RT).tiles, a.parts_k, 0).parts;
+  if (parts == 1) return;
+  const F16x acc = add_parts<KEY_PART>(a, key_slot(a, p, DP == 64 ? BOTH : role), parts, wave,
+                                       (DP == 64 && role == VALUES ? DT : 0) + block, [](int) { return 1.0f; });
+  if (threadIdx.x >= 64) return;
+  const int key0 = p.tile * 128 + wave * 32;
+  if (role == KEYS) finish_dkv<T, DP, 1, KEYS>(a, p, key0, 32 * block, &acc, nullptr);
+  else finish_dkv<T, DP, 1, VALUES>(a, p, key0, 32 * block, nullptr, &acc);
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------
@@ -672,29 +836,78 @@ int key_waves(int dim, int seqs, int tk) {
   if (dim <= 64) return tk <= 64LL * seqs ? 1 : 4;
   return tk <= 96LL * seqs ? 2 : 4;
 }
+// Few tiles leave compute units idle while each walks over all keys (rows) alone. Their loops are then split among as many
+// workgroups as fill the GPU, but with LEAST tiles a part for a sequence of twice the mean length.
+constexpr int FILL = 512;
+int parts_of(long long blocks, long long others, int tile, int seqs) {
+  if (blocks > FILL / 2) return 1;
+  const long long most = 2 * others / ((long long)(seqs > 0 ? seqs : 1) * LEAST * tile), fill = FILL / (blocks > 0 ? blocks : 1);
+  return most < 4 || fill < 2 ? 1 : (int)(fill < most ? fill : most);
+}
+int query_parts(int kv_heads, int seqs, int tq, int tk, int group) {
+  return parts_of(order_queries(seqs, tq, group) * kv_heads, tk, TILE, seqs);
+}
+int key_parts(int kv_heads, int dim, int seqs, int tq, int tk, int group) {
+  const int kw = key_waves(dim, seqs, tk);
+  return kw < 4 ? 1 : parts_of(order_keys(seqs, tk, kw) * kv_heads * (dim <= 64 ? 1 : 2), (long long)tq * group, dim <= 64 ? 64 : 128, seqs);
+}
 size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group) {
   return sizeof(int) * (ORDER_HEAD + 2 * (size_t)(order_queries(seqs, tq, group) +
                                                   order_keys(seqs, tk, key_waves(dim, seqs, tk))));
 }
+size_t attend_scratch_bytes(int kv_heads, int dim, int seqs, int tq, int tk, int group, bool vjp) {
+  const size_t pq = query_parts(kv_heads, seqs, tq, tk, group), pk = vjp ? key_parts(kv_heads, dim, seqs, tq, tk, group) : 1;
+  const size_t q = pq == 1 ? 0 : pq * order_queries(seqs, tq, group) * kv_heads * (dim <= 64 ? RowsPart<64>::SIZE : RowsPart<128>::SIZE);
+  const size_t k = pk == 1 ? 0 : pk * order_keys(seqs, tk, 4) * kv_heads * (dim <= 64 ? 1 : 2) * Part<KEY_PART>::SIZE;
+  return sizeof(float) * (q > k ? q : k);
+}
 
 template <typename T, int DP>
 int attend(hipStream_t st, const Attend& a) {
-  k_attend<T, DP><<<blocks_of(a, order_queries(a.seqs, a.tq, a.group), 1), 256, 0, st>>>(a);
+  const long long tiles = order_queries(a.seqs, a.tq, a.group);
+  if (a.parts_q == 1) {
+    k_attend<T, DP, false><<<blocks_of(a, tiles, 1), 256, 0, st>>>(a);
+  } else {
+    k_attend<T, DP, true><<<blocks_of(a, tiles, a.parts_q), 256, 0, st>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    k_attend_join<T, DP><<<dim3(blocks_of(a, tiles, 1), 4 * (DP / 32)), 256, 0, st>>>(a);
+  }
+  return (int)hipGetLastError();
+}
+template <typename T, int DP>
+int attend_dq(hipStream_t st, const Attend& a) {
+  const long long tiles = order_queries(a.seqs, a.tq, a.group);
+  if (a.parts_q == 1) {
+    k_attend_dq<T, DP, false><<<blocks_of(a, tiles, 1), 256, 0, st>>>(a);
+  } else {
+    k_attend_dq<T, DP, true><<<blocks_of(a, tiles, a.parts_q), 256, 0, st>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    k_attend_dq_join<T, DP><<<dim3(blocks_of(a, tiles, 1), 4 * (DP / 32)), 256, 0, st>>>(a);
+  }
   return (int)hipGetLastError();
 }
 template <typename T, int DP>
 int attend_vjp(hipStream_t st, const Attend& a) {
-  if (a.tq) k_attend_dq<T, DP><<<blocks_of(a, order_queries(a.seqs, a.tq, a.group), 1), 256, 0, st>>>(a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return (int)e;
+  if (a.tq) {
+    const int e = attend_dq<T, DP>(st, a);
+    if (e) return e;
+  }
   if (!a.tk) return 0;
   const long long tiles = order_keys(a.seqs, a.tk, a.key_waves);
-  if constexpr (DP == 64) {
-    if (a.key_waves == 1) k_attend_dkv<T, 64, 1, 1><<<(unsigned)((tiles * a.kv_heads + 3) / 4), 256, 0, st>>>(a);
-    else k_attend_dkv<T, 64, 4, 4><<<blocks_of(a, tiles, 1), 256, 0, st>>>(a);
+  constexpr int ROLES = DP == 64 ? 1 : 2, THREADS = DP == 64 ? 256 : 512;
+  if (a.parts_k > 1) {
+    k_attend_dkv<T, DP, 4, DP / 16, true><<<blocks_of(a, tiles, ROLES * a.parts_k), THREADS, 0, st>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    k_attend_dkv_join<T, DP><<<dim3(blocks_of(a, tiles, 1), 8 * (DP / 32)), 256, 0, st>>>(a);
+  } else if (a.key_waves == 4) {
+    k_attend_dkv<T, DP, 4, DP / 16, false><<<blocks_of(a, tiles, ROLES), THREADS, 0, st>>>(a);
+  } else if constexpr (DP == 64) {
+    k_attend_dkv<T, 64, 1, 1, false><<<(unsigned)((tiles * a.kv_heads + 3) / 4), 256, 0, st>>>(a);
   } else {
-    if (a.key_waves == 2) k_attend_dkv<T, 128, 2, 8><<<blocks_of(a, tiles, 2), 512, 0, st>>>(a);
-    else k_attend_dkv<T, 128, 4, 8><<<blocks_of(a, tiles, 2), 512, 0, st>>>(a);
+    k_attend_dkv<T, 128, 2, 8, false><<<blocks_of(a, tiles, 2), 512, 0, st>>>(a);
   }
   return (int)hipGetLastError();
 }
@@ -730,16 +943,18 @@ extern "C" {
 int dk_attention(hipStream_t st, int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk, const void* q,
                  long long q_t, long long q_h, const void* k, long long k_t, long long k_h, const void* v,
                  long long v_t, long long v_h, const int* starts_q, const int* starts_k, float scale, void* out,
-                 float* lse, void* work) {
+                 float* lse, void* work, void* scratch) {
   if (!attention_takes(type, heads, kv_heads, dim, seqs, tq, tk) || !(scale > 0.0f) || !starts_q || !starts_k || !work ||
-      (tq && (!q || !out)) || (tk && (!k || !v)))
+      (tq && (!q || !out)) || (tk && (!k || !v)) ||
+      (!scratch && dk_attention_scratch_bytes(heads, kv_heads, dim, seqs, tq, tk, 0)))
     return (int)hipErrorInvalidValue;
   pol::Attend a = {};
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
   a.key_waves = pol::key_waves(dim, seqs, tk);
-  a.by_sequence = tq <= (long long)pol::LONG * seqs;
+  a.by_sequence = (tq > tk ? tq : tk) <= (long long)pol::LONG * seqs;
+  a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group), a.scratch = (float*)scratch;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.out = out, a.lse = lse, a.order = (const int*)work;
   return pol::launch_attend(st, type, a);
 }
@@ -748,16 +963,20 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
                      const void* q, long long q_t, long long q_h, const void* k, long long k_t, long long k_h,
                      const void* v, long long v_t, long long v_h, const int* starts_q, const int* starts_k,
                      float scale, const void* out, const float* lse, const void* work, const void* dout,
-                     long long do_t, long long do_h, float* delta, void* dq, void* dk, void* dv) {
+                     long long do_t, long long do_h, float* delta, void* dq, void* dk, void* dv,
+                     void* scratch) {
   if (!attention_takes(type, heads, kv_heads, dim, seqs, tq, tk) || !(scale > 0.0f) || !starts_q || !starts_k || !work ||
-      (tq && (!q || !out || !lse || !dout || !delta || !dq)) || (tk && (!k || !v || !dk || !dv)))
+      (tq && (!q || !out || !lse || !dout || !delta || !dq)) || (tk && (!k || !v || !dk || !dv)) ||
+      (!scratch && dk_attention_scratch_bytes(heads, kv_heads, dim, seqs, tq, tk, 1)))
     return (int)hipErrorInvalidValue;
   pol::Attend a = {};
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
   a.key_waves = pol::key_waves(dim, seqs, tk);
-  a.by_sequence = tq <= (long long)pol::LONG * seqs;
+  a.by_sequence = (tq > tk ? tq : tk) <= (long long)pol::LONG * seqs;
+  a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group), a.scratch = (float*)scratch;
+  a.parts_k = pol::key_parts(kv_heads, dim, seqs, tq, tk, a.group);
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.order = (const int*)work;
   a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse);
   a.dout = dout, a.do_t = do_t, a.do_h = do_h, a.delta = delta, a.dq = dq, a.dk = dk, a.dv = dv;
@@ -767,6 +986,11 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
 long long dk_attention_work_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk) {
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || seqs < 0 || tq < 0 || tk < 0) return 0;
   return (long long)pol::attend_work_bytes(dim, seqs, tq, tk, heads / kv_heads);
+}
+
+long long dk_attention_scratch_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk, int vjp) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads || seqs < 0 || tq < 0 || tk < 0) return 0;
+  return (long long)pol::attend_scratch_bytes(kv_heads, dim, seqs, tq, tk, heads / kv_heads, vjp != 0);
 }
 
 }  // extern "C"

@@ -29,7 +29,8 @@ using torch::autograd::variable_list;
 
 #define ENTRIES(X)                                                                                             \
   X(dk_layer_norm) X(dk_layer_norm_vjp) X(dk_layer_norm_work_bytes) X(dk_clip) X(dk_clip_work_bytes)           \
-  X(dk_attention) X(dk_attention_vjp) X(dk_attention_work_bytes) X(dk_attention_step) X(dk_attention_step_work_bytes)
+  X(dk_attention) X(dk_attention_vjp) X(dk_attention_work_bytes) X(dk_attention_scratch_bytes)                  \
+  X(dk_attention_step) X(dk_attention_step_work_bytes)
 struct Entries {
 #define X(name) decltype(&::name) name;
   ENTRIES(X)
@@ -279,6 +280,13 @@ long long order_words(const Heads& h, int seqs, const Tensor& q, const Tensor& k
   return lib.dk_attention_work_bytes(h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0)) / 4;
 }
 
+// what a call's kernels hand to one another, or an undefined tensor where they hand nothing
+Tensor attention_scratch(const Heads& h, int seqs, const Tensor& q, const Tensor& k, int vjp) {
+  const long long bytes =
+      lib.dk_attention_scratch_bytes(h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0), vjp);
+  return bytes ? at::empty({bytes}, q.options().dtype(at::kByte)) : Tensor();
+}
+
 std::vector<Tensor> attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& starts_q,
                                       const Tensor& starts_k, double scale, bool train) {
   const Heads h = heads_checks(q, k, v, 3);
@@ -287,11 +295,13 @@ std::vector<Tensor> attention_forward(const Tensor& q, const Tensor& k, const Te
   const Tensor out = at::empty(q.sizes(), q.options());
   const Tensor lse = at::empty({h.heads, train ? q.size(0) : 0}, q.options().dtype(at::kFloat));
   const Tensor work = at::empty({order_words(h, seqs, q, k)}, q.options().dtype(at::kInt));
+  const Tensor scratch = attention_scratch(h, seqs, q, k, 0);
   call("the attention launch", q, [&](hipStream_t st) {
     return lib.dk_attention(st, h.type, h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0), q.data_ptr(), q.stride(0),
                             q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
                             starts_q.data_ptr<int>(), starts_k.data_ptr<int>(), (float)scale, out.data_ptr(),
-                            train ? lse.data_ptr<float>() : nullptr, work.data_ptr());
+                            train ? lse.data_ptr<float>() : nullptr, work.data_ptr(),
+                            scratch.defined() ? scratch.data_ptr() : nullptr);
   });
   return {out, lse, work};
 }
@@ -311,12 +321,14 @@ std::vector<Tensor> attention_backward(const Tensor& dout, const Tensor& q, cons
   const Tensor delta = at::empty(lse.sizes(), lse.options());
   const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), q.options()),
                dv = at::empty(k.sizes(), q.options());
+  const Tensor scratch = attention_scratch(h, seqs, q, k, 1);
   call("the attention VJP launch", q, [&](hipStream_t st) {
     return lib.dk_attention_vjp(st, h.type, h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0), q.data_ptr(),
                                 q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
                                 v.stride(1), starts_q.data_ptr<int>(), starts_k.data_ptr<int>(), (float)scale,
                                 out.data_ptr(), lse.data_ptr<float>(), work.data_ptr(), dout.data_ptr(), dout.stride(0),
-                                dout.stride(1), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr());
+                                dout.stride(1), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                scratch.defined() ? scratch.data_ptr() : nullptr);
   });
   return {dq, dk, dv};
 }
@@ -421,6 +433,12 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
 }  // namespace
 
 // addresses: those of ENTRIES, in that order
+// the entries' names, in the order in which dk_policy_torch_bind takes their addresses
+extern "C" const char* dk_policy_torch_entries() {
+#define X(name) #name " "
+  return ENTRIES(X);
+#undef X
+}
 extern "C" void dk_policy_torch_bind(void* const* addresses) {
   size_t i = 0;
 #define X(name) lib.name = (decltype(lib.name))addresses[i++];

@@ -32,9 +32,6 @@ from .torch_ffi import _wants_grad
 
 EPS = 1e-5
 TORCH_LIB = os.path.join(torch_ffi.HERE, "libnablaengine_policy_torch.so")
-# the kernels' entries that the operators call, in the order in which dk_policy_torch_bind takes them
-_ENTRIES = ("dk_layer_norm", "dk_layer_norm_vjp", "dk_layer_norm_work_bytes", "dk_clip", "dk_clip_work_bytes", "dk_attention",
-            "dk_attention_vjp", "dk_attention_work_bytes", "dk_attention_step", "dk_attention_step_work_bytes")
 
 
 def _err(msg, kind=TypeError):
@@ -75,9 +72,10 @@ def _bind():
         if not hasattr(torch.ops.nablaengine, "attention_step"):
             _define()
         dll = torch_ffi._load().dll
-        entries = (ctypes.c_void_p * len(_ENTRIES))(*(ctypes.cast(getattr(dll, n), ctypes.c_void_p).value for n in _ENTRIES))
         lib = ctypes.CDLL(TORCH_LIB)
-        lib.dk_policy_torch_bind.restype = None
+        lib.dk_policy_torch_entries.restype, lib.dk_policy_torch_bind.restype = ctypes.c_char_p, None
+        names = lib.dk_policy_torch_entries().decode().split()
+        entries = (ctypes.c_void_p * len(names))(*(ctypes.cast(getattr(dll, n), ctypes.c_void_p).value for n in names))
         lib.dk_policy_torch_bind(entries)
         _bound.append(lib)
 

@@ -111,9 +111,10 @@ _PROTOTYPES = {
     "dk_layer_norm_work_bytes": "q:qii",
     "dk_clip": "i:pi" + "p" * 5 + "fpp",
     "dk_clip_work_bytes": "q:i",
-    "dk_attention": "i:piiiiiii" + "pqq" * 3 + "ppfppp",
-    "dk_attention_vjp": "i:piiiiiii" + "pqq" * 3 + "ppfppp" + "pqq" + "pppp",
+    "dk_attention": "i:piiiiiii" + "pqq" * 3 + "ppfpppp",
+    "dk_attention_vjp": "i:piiiiiii" + "pqq" * 3 + "ppfppp" + "pqq" + "ppppp",
     "dk_attention_work_bytes": "q:iiiiii",
+    "dk_attention_scratch_bytes": "q:iiiiiii",
     "dk_attention_step": "i:piiiiii" + "pqq" + "pqqq" * 2 + "pfpp",
     "dk_attention_step_work_bytes": "q:iiiii",
 }

@@ -376,6 +376,40 @@ def test_attention_drawn_lengths():
         check_attention(q, k, v, lq, lk, scale=0.3)
 
 
+@pytest.mark.parametrize("dtype,dim,heads", [(BF16, 64, 2), (F16, 128, 6), (BF16, 40, 8)])
+@pytest.mark.parametrize("lq,lk", [([1], [4000]), ([5, 60], [1800, 2100]), ([70, 0, 9], [1100, 900, 0]), ([1500], [1500]),
+                                   ([1300, 700], [257, 1900]), ([300], [256]), ([129], [5000])])
+def test_attention_few_sequences(dtype, dim, heads, lq, lk):
+    """Few tiles, long sequences: a tile's keys (rows) are split among workgroups, whose sums a second kernel adds."""
+    print("attention few", dtype, dim, heads, lq, lk, flush=True)
+    q = rand((sum(lq), heads, dim), dtype, 1)
+    k, v = rand((sum(lk), 2, dim), dtype, 2), rand((sum(lk), 2, dim), dtype, 3)
+    check_attention(q, k, v, lq, lk)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_few_sequences_what_the_mask_hides(dim, bad):
+    """As below for a tile's parts: the last key, which the last row alone sees, and the first row, which sees one key. The
+    last row sees every key: what the last key holds reaches every key's gradient, so those are read without it."""
+    print("attention few hidden", dim, bad, flush=True)
+    n = 1200
+    q, dout = rand((n, 2, dim), BF16, 1), rand((n, 2, dim), BF16, 4)
+    k, v = rand((n, 1, dim), BF16, 2), rand((n, 1, dim), BF16, 3)
+    want = attend64(q, k, v, [n], [n], 1 / math.sqrt(dim), dout)
+    q[0], dout[0] = bad, bad
+
+    def check(names):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        out = policy.attention(*leaves, starts([n]))
+        got = dict(zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, dout))))
+        for name in names:
+            within(name, got[name][1:n - 1], want[name][0][1:n - 1], want[name][1][1:n - 1])
+    check(("out", "dq", "dk", "dv"))
+    k[-1], v[-1] = bad, bad
+    check(("out", "dq"))
+
+
 def test_attention_strides():
     """Slices of one projection at odd offsets, heads before tokens, a cotangent with its own strides."""
     lq = [40, 0, 77]

@@ -25,7 +25,7 @@ def _prototypes():
 
 def test_bindings_are_the_headers():
     protos = _prototypes()
-    assert len(protos) == 10
+    assert len(protos) == 11
     for name, proto in protos.items():
         assert torch_ffi._PROTOTYPES[name] == proto, name
     dll = torch_ffi.load_library()
@@ -53,12 +53,14 @@ def test_c_entries_refuse_before_any_launch():
     assert clip(out=None) == clip(n=(5, 5), types=(1, 1), outs=(1, 2)) == 1
     assert dll.dk_clip(None, -1, None, None, None, None, None, 1.0, X, X) == 1
 
-    def attention(t=1, heads=4, kv=2, dim=64, seqs=1, tq=5, tk=5, q=X, starts=X, scale=0.1, work=X):
-        return dll.dk_attention(None, t, heads, kv, dim, seqs, tq, tk, q, 1, 1, X, 1, 1, X, 1, 1, starts, X, scale, X, None, work)
+    def attention(t=1, heads=4, kv=2, dim=64, seqs=1, tq=5, tk=5, q=X, starts=X, scale=0.1, work=X, scratch=None):
+        return dll.dk_attention(None, t, heads, kv, dim, seqs, tq, tk, q, 1, 1, X, 1, 1, X, 1, 1, starts, X, scale, X, None, work,
+                                scratch)
     for bad in (dict(t=0), dict(heads=3), dict(kv=0), dict(dim=7), dict(dim=136), dict(seqs=-1), dict(tq=-1), dict(tk=1 << 30),
-                dict(tq=1 << 29), dict(q=None), dict(starts=None), dict(scale=0.0), dict(scale=float("nan")), dict(work=None)):
+                dict(tq=1 << 29), dict(q=None), dict(starts=None), dict(scale=0.0), dict(scale=float("nan")), dict(work=None), dict(tq=300, tk=3000)):
         assert attention(**bad) == 1, bad
-    assert dll.dk_attention_work_bytes(4, 2, 64, 1, 5, 5) > 0
+    assert dll.dk_attention_work_bytes(4, 2, 64, 1, 5, 5) > 0 and dll.dk_attention_scratch_bytes(4, 2, 64, 1, 5, 5, 1) == 0
+    assert dll.dk_attention_scratch_bytes(4, 2, 64, 1, 300, 5000, 0) > 0
 
     def step(t=1, worlds=2, heads=4, kv=2, dim=64, cap=9, q=X, lengths=X, scale=0.1, work=X):
         return dll.dk_attention_step(None, t, worlds, heads, kv, dim, cap, q, 1, 1, X, 1, 1, 1, X, 1, 1, 1, lengths, scale, X, work)
