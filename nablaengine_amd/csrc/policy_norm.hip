@@ -9,6 +9,11 @@
 // is rounded once. The backward's groups walk over rows and keep their columns' dw and db sums in registers; at the end
 // a workgroup adds its groups' sums in LDS and writes one partial row, and a second small kernel adds the partial rows
 // in a fixed order (no atomics: bitwise the same on every run).
+//
+// Measured, 2^27 elements, of the 5.2 TB/s of a large copy: forward 5.0 to 5.6 TB/s in float32 at widths 32 to 8192, odd
+// ones (99, 331, 1331) among them, and in bfloat16 at 64 to 4096 (4.1 to 5.0 at odd ones); backward 4.8 to 5.4 TB/s in
+// float32, in bfloat16 4.5 to 5.2 at powers of two and 3.5 to 4.4 at odd widths, where a vector's conversions bound it.
+// Up to a few thousand rows a call is bound by its launch (2 us a kernel).
 #include "../../include/nablaengine_policy.h"
 #include "policy_device.h"
 
@@ -17,41 +22,42 @@ namespace pol {
 // Rows that no register variant holds: each pass reads the row again (it stays in the L2 cache: at most a few MB).
 constexpr int WIDE = 1024;  // lanes of the largest groups, and of the wide rows'
 
-template <typename T>
-__device__ __forceinline__ void row_load(const T* p, int v, int n, float* f) {  // vector v of a row of n elements
-  constexpr int E = Vec<T>::E;
-  const int at = v * E;
-  if (at + E <= n) {
-    load_floats<E>(f, p + at);
+// A row of n elements in vectors of E. The last one ends with the row: where n is no multiple of E it holds elements of the
+// one before again, which both write, with the same values, and only the first counts in sums. A tail of single elements
+// cost the waves that hold it as much again as the row: 2^27 elements in rows of 99 bfloat16 211 us forward and 307
+// backward, now 107 and 182.
+template <int E>
+__device__ __forceinline__ int first_of(int v, int n) { return v * E + E <= n || n < E ? v * E : n - E; }
+// whether element e of vector v counts
+template <int E>
+__device__ __forceinline__ bool own(int v, int n, int e) {
+  const int at = first_of<E>(v, n) + e;
+  return at >= v * E && at < n;
+}
+
+// vector v of a row (of parameters), `none` where there is no row, vector or element
+template <int E, typename T>
+__device__ __forceinline__ void row_load(const T* p, int v, int n, float none, float* f) {
+  if (p && v * E < n && n >= E) {
+    load_floats<E>(f, p + first_of<E>(v, n));
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = at + e < n ? (float)p[at + e] : 0.0f;
+    for (int e = 0; e < E; ++e) f[e] = p && n < E && v == 0 && e < n ? (float)p[e] : none;
   }
 }
 template <typename T>
 __device__ __forceinline__ void row_store(T* p, int v, int n, const float* f) {
   constexpr int E = Vec<T>::E;
-  const int at = v * E;
-  if (at + E <= n) {
+  if (v * E >= n) return;
+  if (n >= E) {
     Vec<T> o;
 #pragma unroll
     for (int e = 0; e < E; ++e) o.v[e] = (T)f[e];
-    store16(p + at, o);
+    store16(p + first_of<E>(v, n), o);
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (at + e < n) p[at + e] = (T)f[e];
-  }
-}
-// the E parameters of vector v (`none` where there is no such parameter, and past the row's end)
-template <int E, typename W>
-__device__ __forceinline__ void param_load(const W* p, int v, int n, float none, float* f) {
-  const int at = v * E;
-  if (p && at + E <= n) {
-    load_floats<E>(f, p + at);
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = p && at + e < n ? (float)p[at + e] : none;
+      if (e < n) p[e] = (T)f[e];
   }
 }
 
@@ -80,14 +86,25 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void k_norm(long long rows, int 
   constexpr int E = Vec<T>::E, BLOCK = L > 256 ? L : 256, GROUPS = BLOCK / L;
   __shared__ float red[BLOCK / 64];
   const int lane = threadIdx.x % L, group = threadIdx.x / L;
+  // A lane's parameters, the same for all its rows, stay in registers and are read beside its first row, not after the
+  // sums: rows of 4096 float32 193 us for 317. For 16 and more too few waves would fit.
+  constexpr bool KEEP = C * E <= 8;
+  float wf[KEEP ? C : 1][E], bf[KEEP ? C : 1][E];
+  auto params = [&](int c, int to) {
+    row_load<E>(w, lane + c * L, n, 1.0f, wf[to]);
+    row_load<E>(b, lane + c * L, n, 0.0f, bf[to]);
+  };
+  if (KEEP)
+#pragma unroll
+    for (int c = 0; c < C; ++c) params(c, c);
   for (long long row = (long long)blockIdx.x * GROUPS + group; row < rows; row += (long long)gridDim.x * GROUPS) {
     float f[C][E];
     float s = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      row_load(x + row * xs, lane + c * L, n, f[c]);
+      row_load<E>(x + row * xs, lane + c * L, n, 0.0f, f[c]);
 #pragma unroll
-      for (int e = 0; e < E; ++e) s += f[c][e];
+      for (int e = 0; e < E; ++e) s += own<E>(lane + c * L, n, e) ? f[c][e] : 0.0f;
     }
     const float mu = group_sum<L>(s, red) / (float)n;
     float q = 0.0f;
@@ -95,8 +112,9 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void k_norm(long long rows, int 
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        f[c][e] = (lane + c * L) * E + e < n ? f[c][e] - mu : 0.0f;
-        q += f[c][e] * f[c][e];
+        f[c][e] -= mu;
+        const float d = own<E>(lane + c * L, n, e) ? f[c][e] : 0.0f;
+        q += d * d;
       }
     const float r = 1.0f / sqrtf(group_sum<L>(q, red) / (float)n + eps);
     if (stats && lane == 0) {
@@ -106,11 +124,10 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void k_norm(long long rows, int 
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       if ((lane + c * L) * E >= n) continue;
-      float wf[E], bf[E];
-      param_load<E>(w, lane + c * L, n, 1.0f, wf);
-      param_load<E>(b, lane + c * L, n, 0.0f, bf);
+      const int at = KEEP ? c : 0;
+      if (!KEEP) params(c, at);
 #pragma unroll
-      for (int e = 0; e < E; ++e) f[c][e] = f[c][e] * r * wf[e] + bf[e];
+      for (int e = 0; e < E; ++e) f[c][e] = f[c][e] * r * wf[at][e] + bf[at][e];
       row_store(y + row * n, lane + c * L, n, f[c]);
     }
   }
@@ -127,19 +144,19 @@ __global__ __launch_bounds__(WIDE) void k_norm_wide(long long rows, int n, const
     const T* xr = x + row * xs;
     float f[E], s = 0.0f, q = 0.0f;
     for (int v = threadIdx.x; v < nv; v += WIDE) {
-      row_load(xr, v, n, f);
+      row_load<E>(xr, v, n, 0.0f, f);
       float t = 0.0f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) t += f[e];
+      for (int e = 0; e < E; ++e) t += own<E>(v, n, e) ? f[e] : 0.0f;
       s += t;
     }
     const float mu = group_sum<WIDE>(s, red) / (float)n;
     for (int v = threadIdx.x; v < nv; v += WIDE) {
-      row_load(xr, v, n, f);
+      row_load<E>(xr, v, n, 0.0f, f);
       float t = 0.0f;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float d = v * E + e < n ? f[e] - mu : 0.0f;
+        const float d = own<E>(v, n, e) ? f[e] - mu : 0.0f;
         t += d * d;
       }
       q += t;
@@ -151,9 +168,9 @@ __global__ __launch_bounds__(WIDE) void k_norm_wide(long long rows, int n, const
     }
     for (int v = threadIdx.x; v < nv; v += WIDE) {
       float wf[E], bf[E];
-      row_load(xr, v, n, f);
-      param_load<E>(w, v, n, 1.0f, wf);
-      param_load<E>(b, v, n, 0.0f, bf);
+      row_load<E>(xr, v, n, 0.0f, f);
+      row_load<E>(w, v, n, 1.0f, wf);
+      row_load<E>(b, v, n, 0.0f, bf);
 #pragma unroll
       for (int e = 0; e < E; ++e) f[e] = (f[e] - mu) * r * wf[e] + bf[e];
       row_store(y + row * n, v, n, f);
@@ -179,6 +196,13 @@ __global__ __launch_bounds__(vjp_block(L)) void k_norm_vjp(long long rows, int n
   float aw[CE], ab[CE];
 #pragma unroll
   for (int i = 0; i < CE; ++i) aw[i] = ab[i] = 0.0f;
+  // as the forward (rows of 331 float32 316 us for 365), but for 16-bit rows of several waves, which have the registers for
+  // three workgroups a CU only without: rows of 4096 bfloat16 180 us for 248
+  constexpr bool KEEP = CE <= 8 && (E == 4 || L <= 64);
+  float wf[KEEP ? C : 1][E];
+  if (KEEP)
+#pragma unroll
+    for (int c = 0; c < C; ++c) row_load<E>(w, lane + c * L, n, 1.0f, wf[c]);
   // groups of several waves meet at barriers: the workgroup stays together, a group past the last row has none of it
   for (long long row = (long long)blockIdx.x * GROUPS + group;; row += (long long)gridDim.x * GROUPS) {
     if (L > 64 ? row - group >= rows : row >= rows) break;
@@ -186,24 +210,25 @@ __global__ __launch_bounds__(vjp_block(L)) void k_norm_vjp(long long rows, int n
     float f[CE], g[CE];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      row_load(x + row * xs, lane + c * L, m, f + c * E);
-      row_load(dy + row * dys, lane + c * L, m, g + c * E);
+      row_load<E>(x + row * xs, lane + c * L, m, 0.0f, f + c * E);
+      row_load<E>(dy + row * dys, lane + c * L, m, 0.0f, g + c * E);
     }
     const float mu = m ? stats[row] : 0.0f, r = m ? stats[rows + row] : 0.0f;
     float s = 0.0f, q = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      float wf[E];
-      param_load<E>(w, lane + c * L, n, 1.0f, wf);
+      const int at = KEEP ? c : 0;
+      if (!KEEP) row_load<E>(w, lane + c * L, n, 1.0f, wf[at]);
 #pragma unroll
       for (int e = 0; e < E; ++e) {  // past the row's end x and dy were read as 0: g stays 0 there, xh is not used
         const int i = c * E + e;
         f[i] = (f[i] - mu) * r;
         aw[i] += g[i] * f[i];
         ab[i] += g[i];
-        g[i] *= wf[e];
-        s += g[i];
-        q += g[i] * f[i];
+        g[i] *= wf[at][e];
+        const float t = own<E>(lane + c * L, n, e) ? g[i] : 0.0f;
+        s += t;
+        q += t * f[i];
       }
     }
     if (dx) {
@@ -247,8 +272,7 @@ __global__ __launch_bounds__(vjp_block(L)) void k_norm_vjp(long long rows, int n
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const int col = (lane + c * L) * E + e;
-          if (col < n) out[which * n + col] = a[c * E + e];
+          if (own<E>(lane + c * L, n, e)) out[which * n + first_of<E>(lane + c * L, n) + e] = a[c * E + e];
         }
   }
 }
@@ -270,15 +294,16 @@ __global__ __launch_bounds__(WIDE) void k_norm_vjp_wide(long long rows, int n, c
     float s = 0.0f, q = 0.0f;
     for (int v = threadIdx.x; v < nv; v += WIDE) {
       float f[E], g[E], wf[E];
-      row_load(x + row * xs, v, n, f);
-      row_load(dy + row * dys, v, n, g);
-      param_load<E>(w, v, n, 1.0f, wf);
+      row_load<E>(x + row * xs, v, n, 0.0f, f);
+      row_load<E>(dy + row * dys, v, n, 0.0f, g);
+      row_load<E>(w, v, n, 1.0f, wf);
       float ts = 0.0f, tq = 0.0f;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         f[e] = (f[e] - mu) * r;
-        const int col = v * E + e;
-        if (out && col < n) {
+        if (!own<E>(v, n, e)) continue;
+        const int col = first_of<E>(v, n) + e;
+        if (out) {
           out[col] = (first ? 0.0f : out[col]) + g[e] * f[e];
           out[n + col] = (first ? 0.0f : out[n + col]) + g[e];
         }
@@ -292,9 +317,9 @@ __global__ __launch_bounds__(WIDE) void k_norm_vjp_wide(long long rows, int n, c
     const float ms = group_sum<WIDE>(s, red) / (float)n, mq = group_sum<WIDE>(q, red) / (float)n;
     for (int v = threadIdx.x; v < nv; v += WIDE) {
       float f[E], g[E], wf[E];
-      row_load(x + row * xs, v, n, f);
-      row_load(dy + row * dys, v, n, g);
-      param_load<E>(w, v, n, 1.0f, wf);
+      row_load<E>(x + row * xs, v, n, 0.0f, f);
+      row_load<E>(dy + row * dys, v, n, 0.0f, g);
+      row_load<E>(w, v, n, 1.0f, wf);
 #pragma unroll
       for (int e = 0; e < E; ++e) f[e] = r * (g[e] * wf[e] - ms - (f[e] - mu) * r * mq);
       row_store(dx + row * n, v, n, f);
@@ -329,20 +354,31 @@ __global__ __launch_bounds__(1024) void k_norm_params(int blocks, int n, const f
 
 constexpr int CUS = 256;
 
-// f(L, C) for a row of nv vectors: the smallest group that holds it. Returns false where none does.
-template <typename F>
+// f(L, C) for a row of nv vectors of E elements: the smallest group that holds it. Returns false where none does. Two vectors
+// a lane save barriers where a vector is 4 float32 (rows of 2048: 203 us forward and 304 backward for 233 and 327 with one);
+// with 8 elements of 16 bits they take the registers of other waves (rows of 4096 bfloat16: 180 us backward with one a lane,
+// 270 with two; of 768: 109 forward for 132), but where only groups of 1024, two a CU, would hold the row with one (8192:
+// 126 and 198 us for 167 and 252).
+template <int E, typename F>
 bool by_width(int nv, F f) {
 #define POL_CASE(L, C) \
   if (nv <= L * C) { f(std::integral_constant<int, L>{}, std::integral_constant<int, C>{}); return true; }
-  POL_CASE(8, 1) POL_CASE(16, 1) POL_CASE(32, 1) POL_CASE(64, 1) POL_CASE(64, 2) POL_CASE(256, 1) POL_CASE(256, 2)
+  POL_CASE(8, 1) POL_CASE(16, 1) POL_CASE(32, 1) POL_CASE(64, 1)
+  if constexpr (E == 8) {
+    POL_CASE(128, 1) POL_CASE(256, 1) POL_CASE(512, 1) POL_CASE(512, 2)
+  } else {
+    POL_CASE(64, 2) POL_CASE(256, 1) POL_CASE(256, 2)
+  }
   POL_CASE(1024, 1) POL_CASE(1024, 2)
 #undef POL_CASE
   return false;
 }
 // lanes a row, and vectors a lane
-void group_of(int nv, int& lanes, int& vectors) {
+void group_of(int nv, int type, int& lanes, int& vectors) {
   lanes = WIDE, vectors = 2;
-  by_width(nv, [&](auto l, auto c) { lanes = decltype(l)::value, vectors = decltype(c)::value; });
+  auto f = [&](auto l, auto c) { lanes = decltype(l)::value, vectors = decltype(c)::value; };
+  if (bytes_of(type) == 2) by_width<8>(nv, f);
+  else by_width<4>(nv, f);
 }
 int vectors_of(int n, int type) { const int e = 16 / bytes_of(type); return (n + e - 1) / e; }
 
@@ -351,7 +387,7 @@ int vectors_of(int n, int type) { const int e = 16 / bytes_of(type); return (n +
 // with three, 194 with four, which take a second round.
 int vjp_blocks(long long rows, int n, int type) {
   int lanes, vectors;
-  group_of(vectors_of(n, type), lanes, vectors);
+  group_of(vectors_of(n, type), type, lanes, vectors);
   const int groups = vjp_block(lanes) / lanes;
   const long long need = (rows + groups - 1) / groups, most = (vectors == 1 && lanes <= 512 ? 3 : 2) * CUS;
   return (int)(need < most ? need : most);
@@ -365,7 +401,7 @@ int norm(hipStream_t st, long long rows, int n, int type, const void* x, long lo
     kernel<<<(unsigned)(need < most ? need : most), block, 0, st>>>(rows, n, (const T*)x, xs, (const W*)w, (const W*)b,
                                                                     eps, (T*)y, stats);
   };
-  if (!by_width(vectors_of(n, type), [&](auto l, auto c) {
+  if (!by_width<Vec<T>::E>(vectors_of(n, type), [&](auto l, auto c) {
         constexpr int L = decltype(l)::value, C = decltype(c)::value, BLOCK = L > 256 ? L : 256;
         launch(k_norm<T, W, L, C>, BLOCK, BLOCK / L);
       }))
@@ -382,7 +418,7 @@ int norm_vjp(hipStream_t st, long long rows, int n, int type, const void* x, lon
     auto launch = [&](auto kernel, int block) {
       kernel<<<blocks, block, 0, st>>>(rows, n, (const T*)x, xs, (const T*)dy, dys, (const W*)w, stats, (T*)dx, part);
     };
-    if (!by_width(vectors_of(n, type), [&](auto l, auto c) {
+    if (!by_width<Vec<T>::E>(vectors_of(n, type), [&](auto l, auto c) {
           launch(k_norm_vjp<T, W, decltype(l)::value, decltype(c)::value>, vjp_block(decltype(l)::value));
         }))
       launch(k_norm_vjp_wide<T, W>, WIDE);
