@@ -34,8 +34,8 @@ struct Attend {
   const void *q, *k, *v;
   long long q_t, q_h, k_t, k_h, v_t, v_h;  // elements from token to token, and from head to head
   int heads, kv_heads, group, dim, seqs, tq, tk;
-  int by_sequence;  // the order of the tiles, see below
-  int key_waves;  // 32 keys each: a tile of the keys' gradients (1, 2 or 4)
+  int by_sequence;  // bit `list`: its order, see below
+  int key_waves;  // 32 keys each: a tile of the keys' gradients (1 or 4)
   int parts_q, parts_k;  // workgroups (of a role) among which a query tile's keys, a key tile's rows are split
   const int *starts_q, *starts_k;
   float scale;
@@ -52,12 +52,12 @@ struct Attend {
 
 // The order: two lists of tiles, (sequence, tile of it): the query tiles (QROWS rows of a key/value head's queries, row =
 // token * group + head of the group) and the key tiles (32 * key_waves keys). A list is heaviest first, by the tiles of
-// the other side that each one reads: over all tiles where sequences are long; over sequences, each one's tiles one after
-// another, where they are not (by_sequence). Workgroups go to the XCDs in turn, and each XCD has an L2 cache of its own:
-// in the second case WINDOW neighbours of the list go to one XCD, so that a sequence's tiles find what they share in one
-// cache; in the first a list's neighbours are tiles of different sequences and heads anyway.
+// the other side that each one reads: over all tiles, or over sequences, each one's tiles one after another (by_sequence).
+// Workgroups go to the XCDs in turn, and each XCD has an L2 cache of its own: in the second case WINDOW neighbours of the
+// list go to one XCD, so that a sequence's tiles find what they share in one cache; in the first a list's neighbours are
+// tiles of different sequences and heads anyway.
 constexpr int WINDOW = 64, XCDS = 8;
-constexpr int LONG = 2048;  // tokens a sequence, in the mean: from there on single tiles are ordered
+constexpr int LONG = 1792;  // tokens a sequence, in the mean: above it single tiles are ordered
 constexpr int ORDER_HEAD = 16;  // ints before the lists: their lengths
 __host__ __device__ inline long long order_queries(int seqs, int tq, int group) {
   return (long long)tq * group / QROWS + seqs + 1;

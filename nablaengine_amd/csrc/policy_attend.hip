@@ -30,10 +30,10 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
     __syncthreads();
   }
   int ls = 1;
-  if (!by_sequence)
+  if (by_sequence < 3)
     while (ls < 1024 && ls * 2 * (long long)(seqs + 1) <= 1024) ls *= 2;
   const int lane = threadIdx.x % ls, first_seq = threadIdx.x / ls, stride = 1024 / ls;
-  const int bits[2] = {7, key_waves == 1 ? 5 : key_waves == 2 ? 6 : 7};  // of a tile's rows
+  const int bits[2] = {7, key_waves == 1 ? 5 : 7};  // of a tile's rows
   static_assert(QROWS == 128, "");
   const long long caps[2] = {order_queries(seqs, tq, group), order_keys(seqs, tk, key_waves)};
   int* const lists[2] = {order + ORDER_HEAD, order + ORDER_HEAD + 2 * caps[0]};
@@ -66,8 +66,8 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
           }
           return bucket_of(cost);
         };
-        if (by_sequence) {  // its heaviest tile: the last row sees every key, the first key almost every row
-          f(which, s, 0, tiles, bucket_of(which ? (mq < mk ? mq : mk) * group : mk));
+        if (by_sequence >> which & 1) {  // its heaviest tile: the last row sees every key, the first key almost every row
+          f(which, s, 0, lane == 0 ? tiles : 0, bucket_of(which ? (mq < mk ? mq : mk) * group : mk));
         } else {
           for (int t = lane; __any(t < tiles); t += ls) f(which, s, t, t < tiles ? 1 : 0, bucket(t));
         }
@@ -143,7 +143,7 @@ __device__ __forceinline__ bool place(const Attend& a, int which, int at, Place&
 __device__ __forceinline__ bool place_of_block(const Attend& a, int which, int parts, Place& p) {
   const int b = blockIdx.x;
   int at;
-  if (a.by_sequence) {
+  if (a.by_sequence >> which & 1) {
     const int all = uniform(a.order[which]) * a.kv_heads * parts, base = b / (WINDOW * XCDS) * (WINDOW * XCDS);
     const int left = all - base, mine = left < WINDOW * XCDS ? (left + XCDS - 1) / XCDS : WINDOW, r = b - base;
     if (left <= 0 || r / XCDS >= mine) return false;
@@ -604,7 +604,7 @@ template <typename T, int DP, int KW, int WAVES, int ROLE, bool PARTS>
 __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, WAVES>& lds) {
   constexpr int RT = DkvTiles<T, DP, WAVES>::RT;
   constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 64 * WAVES / CH, SPLIT = WAVES / KW;
-  constexpr int AHEAD = DP == 64 ? 2 : KW == 4 && !PARTS ? 1 : 0;  // of a subtile's two column operands, those read during the exponentials
+  constexpr int AHEAD = DP == 64 ? 2 : !PARTS ? 1 : 0;  // of a subtile's two column operands, those read during the exponentials
   constexpr int SUB = RT / 32, N = RT / STEP;
   auto& tiles = lds.tiles;
   auto &lses = lds.lses, &deltas = lds.deltas;
@@ -830,12 +830,23 @@ __global__ __launch_bounds__(256) void k_attend_dkv_join(Attend a) {
 
 // ---- launches -------------------------------------------------------------------------------------------------------
 
-// Keys a tile of the keys' gradients: 128; where sequences are short (most of a workgroup's waves would have no keys) 32,
-// a wave each, for heads up to 64, and 64 for larger ones.
-int key_waves(int dim, int seqs, int tk) {
-  if (dim <= 64) return tk <= 64LL * seqs ? 1 : 4;
-  return tk <= 96LL * seqs ? 2 : 4;
+// Keys a tile of the keys' gradients: 128; 32, a wave each, where sequences are short and heads up to 64, since most of a
+// workgroup's waves would have no keys there. Backward of 65536 tokens of 8 heads on 2, lengths 1 to twice the mean, alone
+// and together: mean 16 113 and 157 us, 32 105 and 125, 64 115 and 123, 96 120 and 146 (all of 96: 107 and 111; all of 128:
+// 121 and 114). Heads of 128 gain nothing from tiles of 64 keys (mean 32 445 us for 434, 64 413 for 363).
+int key_waves(int dim, int seqs, int tk) { return dim <= 64 && tk <= 96LL * seqs ? 1 : 4; }
+
+// The lists in the order of the sequences: bit 0 the query tiles, bit 1 the key tiles. 131072 tokens of 8 heads on 2, by
+// sequence and singly: heads of 64, mean length 100, forward 97 and 102 us, dq 136 and 141, dkv 183 and 135; 700, 194 and 206,
+// 265 and 272, 389 and 353; 1500, 297 and 308, 388 and 405, 654 and 574; heads of 128, 700, 358 and 394, 470 and 498, 929
+// and 1038; 1500, 544 and 618, 711 and 768, 1540 and 1617. 65536 tokens, mean 2048, heads of 64: forward 220 and 196, all of
+// the backward 800 and 605; of 128, 401 and 372, 1559 and 1470. A wave alone has no neighbours: the shorter listing.
+int by_sequence(int dim, int seqs, int tq, int tk) {
+  const bool queries = (tq > tk ? tq : tk) <= (long long)LONG * seqs;
+  const bool keys = key_waves(dim, seqs, tk) == 1 || (dim > 64 && queries);
+  return (queries ? 1 : 0) | (keys ? 2 : 0);
 }
+
 // Few tiles leave compute units idle while each walks over all keys (rows) alone. Their loops are then split among as many
 // workgroups as fill the GPU, but with LEAST tiles a part for a sequence of twice the mean length.
 constexpr int FILL = 512;
@@ -906,8 +917,6 @@ int attend_vjp(hipStream_t st, const Attend& a) {
     k_attend_dkv<T, DP, 4, DP / 16, false><<<blocks_of(a, tiles, ROLES), THREADS, 0, st>>>(a);
   } else if constexpr (DP == 64) {
     k_attend_dkv<T, 64, 1, 1, false><<<(unsigned)((tiles * a.kv_heads + 3) / 4), 256, 0, st>>>(a);
-  } else {
-    k_attend_dkv<T, 128, 2, 8, false><<<blocks_of(a, tiles, 2), 512, 0, st>>>(a);
   }
   return (int)hipGetLastError();
 }
@@ -953,7 +962,7 @@ int dk_attention(hipStream_t st, int type, int heads, int kv_heads, int dim, int
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
   a.key_waves = pol::key_waves(dim, seqs, tk);
-  a.by_sequence = (tq > tk ? tq : tk) <= (long long)pol::LONG * seqs;
+  a.by_sequence = pol::by_sequence(dim, seqs, tq, tk);
   a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group), a.scratch = (float*)scratch;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.out = out, a.lse = lse, a.order = (const int*)work;
   return pol::launch_attend(st, type, a);
@@ -974,7 +983,7 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
   a.key_waves = pol::key_waves(dim, seqs, tk);
-  a.by_sequence = (tq > tk ? tq : tk) <= (long long)pol::LONG * seqs;
+  a.by_sequence = pol::by_sequence(dim, seqs, tq, tk);
   a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group), a.scratch = (float*)scratch;
   a.parts_k = pol::key_parts(kv_heads, dim, seqs, tq, tk, a.group);
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.order = (const int*)work;

@@ -168,6 +168,7 @@ __global__ __launch_bounds__(256) void k_step(Step a) {
     }
   }
   if constexpr (W == 1) {  // the wave's own LDS: what it wrote it reads
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     __builtin_amdgcn_wave_barrier();
     for (int i = l; i < GC * LPR * 8; i += 64) {
       const int g = i / (LPR * 8), d = i % (LPR * 8);
@@ -258,12 +259,14 @@ size_t step_work_bytes(int worlds, int heads, int kv_heads, int dim, int capacit
   return n == 1 ? 0 : sizeof(float) * (size_t)n * worlds * heads * (dim + 2);
 }
 
-// Where there are units for every wave the GPU holds, a wave takes one alone: nothing is joined over LDS, and short
-// histories do not leave three waves of four idle.
-constexpr int ALONE = 4096;
+// Where there are many units, a wave takes one alone: nothing is joined over LDS, and short histories do not leave three
+// waves of four idle. Histories of 256, 8 heads on 2 of 64, alone and by four waves: 1024 units 21.4 and 20.1 us, 2048 28.5
+// and 34.0, 4096 53.0 and 62.6, 8192 107 and 131; of 511, 1024 units 36.8 and 30.1. Stretches are long: 2048 of 1024 keys and
+// heads of 128 take 215 us alone, 180 by four.
+constexpr int ALONE = 2048;
 template <typename T, int LPR, int GC>
 void step_units(hipStream_t st, const Step& a) {
-  if (a.units >= ALONE) k_step<T, LPR, GC, 1><<<(a.units + 3) / 4, 256, 0, st>>>(a);
+  if (a.stretches == 1 && a.units >= ALONE) k_step<T, LPR, GC, 1><<<(a.units + 3) / 4, 256, 0, st>>>(a);
   else k_step<T, LPR, GC, 4><<<a.units, 256, 0, st>>>(a);
 }
 template <typename T, int LPR>
