@@ -5,6 +5,14 @@
 //
 // A workgroup of four waves takes 128 rows of one key/value head's queries, row = token * group + head, so that the
 // heads of a group share each key and value tile and short sequences still fill the rows; a wave takes 32 rows.
+//
+// What bounds it. A pair of a query and a key costs the forward 4 dim operations in products and one exponential with some ten
+// vector instructions beside it, the backward 10 dim (14 with the scores that two kernels compute for themselves) and two
+// exponentials. At heads of 64 the vector instructions take longer than the products: 256 episodes of up to 1000 tokens, 8
+// heads on 2, forward 250 us (550 TFLOP/s), dq 350, dkv 445 (610 with what they compute again). At heads of 128 the products
+// lead: 2 sequences of 8192 and 2800 tokens, 16 heads on 4, forward 340 us (900 TFLOP/s; a large library product of 16
+// bits reaches 1200), dq 430, dkv 955. Short sequences are bound by their bytes and by the latency of few tiles each:
+// 4096 segments of up to 32 tokens, 8 heads on 2, forward 56 us (4.0 TB/s), dq 81, dkv 60.
 #include "../../include/nablaengine_policy.h"
 #include "policy_attend.h"
 
@@ -15,7 +23,9 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // ---- the order ------------------------------------------------------------------------------------------------------
 
 // One workgroup lists the tiles by a counting sort (a tile's place among equals is free, results do not depend on the
-// order). seqs + 1 sequences, LS lanes on each.
+// order). seqs + 1 sequences, LS lanes on each. Sequence lengths are on the GPU only: without the lists each workgroup would
+// have to search the offsets for its tile, and the heaviest tiles would not start first (2 sequences of 8192 and 2800
+// tokens: 350 us forward for 470). 4 us for a few sequences, 15 for 4096; the backward takes the forward's lists.
 __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk, int group, int key_waves, int by_sequence,
                                                        const int* starts_q, const int* starts_k,
                                                        int* __restrict__ order) {
@@ -224,6 +234,12 @@ struct Sight {
 
 // ---- forward --------------------------------------------------------------------------------------------------------
 
+// One pass over the keys with the running maximum and sum of the softmax, both in float32; the next tile of keys and values
+// is on its way to LDS while the products of this one run, and one barrier a tile orders both. Two workgroups a CU (four at
+// heads of 64) cover each other's waits; holding a tile's operands in registers one phase ahead cost a workgroup of them
+// (258 us to 283, heads of 64). The probabilities are rounded to 16 bits for the second product, as the values are; the sum
+// they are divided by is that of the unrounded ones, which the backward needs.
+
 // What a tile's parts hand to the join, in the order of the registers: each lane's N sums, and for N + 2 a row's maximum and
 // its sum of probabilities.
 template <int N>
@@ -294,7 +310,8 @@ __device__ __forceinline__ void finish_rows(const Attend& a, const Place& p, con
       o.add(pr, Row<DP>((const T*)a.v + (p.k0 + j) * a.v_t + p.kv * a.v_h, dim));
       top = top1;
     }
-    o.store((T*)a.out + (one.token * a.heads + one.head) * dim, d0, d0 + 32 * N < dim ? d0 + 32 * N : dim, total == 0.0f ? 0.0f : 1.0f / total);
+    o.store((T*)a.out + (one.token * a.heads + one.head) * dim, d0, d0 + 32 * N < dim ? d0 + 32 * N : dim,
+            total == 0.0f ? 0.0f : 1.0f / total);
   }
 }
 
@@ -408,6 +425,10 @@ __global__ __launch_bounds__(256) void k_attend_join(Attend a) {
 
 // ---- backward: the queries' gradient --------------------------------------------------------------------------------
 
+// The forward's walk with the stored log-sum: P and dP a tile from two products over the same keys, dS rounded to 16 bits for
+// the third. Both gradients from one kernel would need atomics on dq, whose order changes results from run to run, or a
+// buffer of float32 a key tile: dq has a kernel of its own, at two products of seven computed again.
+
 template <typename T, int DP, int N>
 __device__ __forceinline__ void finish_dq(const Attend& a, const Place& p, const Rows& r, int d0, const F16x* acc, float lse,
                                           float delta) {
@@ -415,7 +436,8 @@ __device__ __forceinline__ void finish_dq(const Attend& a, const Place& p, const
   const float c = a.scale * LOG2E;
   const long long token = p.q0 + r.pos;
   const unsigned bad = bad_columns(r.valid && not_finite<N>(acc) != 0.0f);
-  store_rows<N>(r.valid && !(bad >> n & 1) ? (T*)a.dq + (token * a.heads + r.head) * dim : nullptr, d0, dim, h, acc, a.scale);
+  store_rows<N>(r.valid && !(bad >> n & 1) ? (T*)a.dq + (token * a.heads + r.head) * dim : nullptr, d0, dim, h, acc,
+                a.scale);
   for (unsigned left = bad; left; left &= left - 1) {
     const int i = __builtin_ctz(left);
     const Sight one(a, p, r, i);
@@ -538,6 +560,7 @@ __global__ __launch_bounds__(256) void k_attend_dq_join(Attend a) {
 
 // ---- backward: the keys' and values' gradients ----------------------------------------------------------------------
 
+// Gradients of shared heads add up in the same sums, since the rows of a key/value head's whole group pass by.
 // A wave keeps 32 keys and their values as B operands and walks over the rows that see them; rows lie in LDS, RT at a
 // time. S = Q K^T here, so that a lane holds 16 rows of ONE key and P, dS are the B operands of dV^T = dO^T P and dK^T =
 // Q^T dS. KW of the waves differ in their keys, the others take every SPLIT-th subtile of 32 rows of the same keys, and
@@ -550,15 +573,18 @@ struct DkvTiles {
   alignas(16) int places_of[2][RT];  // a row's token from its tile's first
 };
 // Heads of 128: dk and dv together take 128 registers a lane, with the keys and values more than two waves a SIMD have.
-// One workgroup takes dk and another dv (a fourth more products, the scores twice): 1150 us at 2 x (8192 and 2800) tokens
-// of 16 heads against 1480 us with both in one and part of the operands in LDS or scratch. Eight waves share a tile of
-// 128 rows there: with four, the tiles that all rows read are one round's length each.
+// One workgroup takes dk and another dv (a fourth more products, the scores twice): 1150 us at sequences of 8192 and 2800
+// tokens of 16 heads on 4 against 1480 us with both in one and part of the operands in LDS or scratch, and 1230 us with one
+// wave a SIMD. Eight waves share a tile of 128 rows, 995 us: twice the products a byte read. Their waves run their products
+// at a higher priority than another's exponentials, 955 us; at heads of 64, where those are the longer part, that gains
+// nothing (forward 249 us to 260).
 enum Role { BOTH, KEYS, VALUES };
 struct RowTiles {  // the rows that see a key tile, in tiles of RT rows or a little less
   int used, first, tiles;
   __device__ __forceinline__ RowTiles(const Attend& a, const Place& p, int kw, int rt) {
     used = a.group <= rt ? rt / a.group * a.group : rt;
-    const int rows = p.nq * a.group, from = p.tile * 32 * kw - (p.nk - p.nq);  // the first token that sees the tile's first key
+    const int rows = p.nq * a.group;
+    const int from = p.tile * 32 * kw - (p.nk - p.nq);  // the first token that sees the tile's first key
     first = (from > 0 ? from : 0) * a.group;
     tiles = rows > first ? (rows - 1 - first) / used + 1 : 0;
   }
@@ -604,7 +630,8 @@ template <typename T, int DP, int KW, int WAVES, int ROLE, bool PARTS>
 __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, WAVES>& lds) {
   constexpr int RT = DkvTiles<T, DP, WAVES>::RT;
   constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 64 * WAVES / CH, SPLIT = WAVES / KW;
-  constexpr int AHEAD = DP == 64 ? 2 : !PARTS ? 1 : 0;  // of a subtile's two column operands, those read during the exponentials
+  // of a subtile's two column operands, those read during the exponentials (heads of 128 in parts: none, no register is left)
+  constexpr int AHEAD = DP == 64 ? 2 : !PARTS ? 1 : 0;
   constexpr int SUB = RT / 32, N = RT / STEP;
   auto& tiles = lds.tiles;
   auto &lses = lds.lses, &deltas = lds.deltas;
@@ -712,7 +739,7 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
           if (ROLE != VALUES) gr[x] = read_rows<DP>(gt, 32 * i, y + x, n, h);
         }
         phase();
-        if (WAVES == 8) __builtin_amdgcn_s_setprio(1);  // products first: 965 us for 993 without
+        if (WAVES == 8) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           s = mfma(qr[x], k[y + x], s);
@@ -848,10 +875,12 @@ int by_sequence(int dim, int seqs, int tq, int tk) {
 }
 
 // Few tiles leave compute units idle while each walks over all keys (rows) alone. Their loops are then split among as many
-// workgroups as fill the GPU, but with LEAST tiles a part for a sequence of twice the mean length.
+// workgroups as fill the GPU twice, but with LEAST tiles a part, and not where a sequence of twice the mean length has less
+// than four parts: the join takes 4 us. Whole and split, us: 64 queries of 16 heads on 4 of 128 over 100000 keys, forward 2530
+// and 123; one sequence of 4096, 1 head of 64, forward 71 and 26, with its backward 246 and 91; 8 of 1000, 8 on 2, 169 and
+// 111; one of 3000, 16 on 4 of 128, 460 and 358. Below the limit, one sequence of 500, 4 on 2: 81 and 98.
 constexpr int FILL = 512;
 int parts_of(long long blocks, long long others, int tile, int seqs) {
-  if (blocks > FILL / 2) return 1;
   const long long most = 2 * others / ((long long)(seqs > 0 ? seqs : 1) * LEAST * tile), fill = FILL / (blocks > 0 ? blocks : 1);
   return most < 4 || fill < 2 ? 1 : (int)(fill < most ? fill : most);
 }
@@ -860,7 +889,8 @@ int query_parts(int kv_heads, int seqs, int tq, int tk, int group) {
 }
 int key_parts(int kv_heads, int dim, int seqs, int tq, int tk, int group) {
   const int kw = key_waves(dim, seqs, tk);
-  return kw < 4 ? 1 : parts_of(order_keys(seqs, tk, kw) * kv_heads * (dim <= 64 ? 1 : 2), (long long)tq * group, dim <= 64 ? 64 : 128, seqs);
+  return kw < 4 ? 1 : parts_of(order_keys(seqs, tk, kw) * kv_heads * (dim <= 64 ? 1 : 2), (long long)tq * group,
+                               dim <= 64 ? 64 : 128, seqs);
 }
 size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group) {
   return sizeof(int) * (ORDER_HEAD + 2 * (size_t)(order_queries(seqs, tq, group) +

@@ -8,6 +8,11 @@
 // float32 sums and DPP adds over the LPR lanes, and each group of LPR lanes keeps its own running maximum, sum and
 // output in float32 over the keys it reads. The groups are joined at the end in registers and LDS, and stretches (long
 // histories of few worlds) by a second kernel in a fixed order.
+//
+// Measured: 4096 worlds with up to 256 tokens, 8 heads on 2 of 64, 0.39 GB in 96 us (4.1 TB/s, of the 3.9 that a sum over one
+// large tensor and the 5.2 that a copy reach); 4 worlds with up to 131072 tokens, 16 heads on 4 of 128, 0.9 GB in 176 us (5.1
+// TB/s) and 5 us for the join; one world with 257 tokens 5.4 us, bound by its launch and one read after another. A turn
+// reads the next one's keys and values ahead, two a lane: with four a wave less fits (104 us for 100).
 #include "../../include/nablaengine_policy.h"
 #include "policy_device.h"
 
