@@ -248,14 +248,19 @@ __global__ __launch_bounds__(1024) void k_step_join(Step a) {
   }
 }
 
-// Stretches: enough workgroups for the 256 CUs where worlds and heads alone are too few, none under 512 keys (joining
-// takes a second launch: 3.4 us beside 4.7 us at 257 keys).
+// Stretches. Many worlds or long histories: enough workgroups for the 256 CUs twice over, none under 512 keys. Few: up to a
+// workgroup a CU of stretches down to 128 keys, where there are four of them at least, since the join takes 4 us. 8 heads
+// on 2 of 64, stretches of 512 and of 128: one world of 1000 tokens 13.6 and 9.2 us, of 8000 13.9 and 10.3, 16 worlds of 1000
+// 13.7 and 9.6; but one of 257 8.1 and 8.8, 64 of 500 10.9 and 11.9, 256 of 333 14 and 28, one of 131072 22.6 and 32.7.
 int step_heads_a_group(int group) { return group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8; }
 int step_stretches(int worlds, int kv_heads, int group, int capacity) {
   const int gc = step_heads_a_group(group);
   const long long blocks = (long long)worlds * kv_heads * ((group + gc - 1) / gc);
-  const long long want = (2048 + blocks - 1) / blocks, most = (capacity + 511) / 512;
-  const long long n = want < most ? want : most;
+  auto of = [&](int fill, int least) {
+    const long long want = (fill + blocks - 1) / blocks, most = (capacity + least - 1) / least;
+    return want < most ? want : most;
+  };
+  const long long many = of(2048, 512), few = of(256, 128), n = few >= 4 && few > many ? few : many;
   return (int)(n < 1 ? 1 : n < MOST_STRETCHES ? n : MOST_STRETCHES);
 }
 size_t step_work_bytes(int worlds, int heads, int kv_heads, int dim, int capacity) {
