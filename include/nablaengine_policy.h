@@ -4,7 +4,7 @@
  * and returns 0 or a hipError_t (hipErrorInvalidValue before any launch for arguments it does not take). Element types
  * are 0 float32, 1 bfloat16, 2 float16; strides count elements; pointers need the element type's alignment only.
  * Everything is summed in float32 or float64 and rounded once to the output's type; no atomics touch a result, which
- * is bitwise the same on every run. */
+ * is bitwise the same on every run. No output overlaps an input or another output, but where an entry says so. */
 #ifndef NABLAENGINE_POLICY_H
 #define NABLAENGINE_POLICY_H
 #include <hip/hip_runtime_api.h>
