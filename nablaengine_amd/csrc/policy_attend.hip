@@ -11,8 +11,8 @@
 // exponentials. At heads of 64 the vector instructions take longer than the products: 256 episodes of up to 1000 tokens, 8
 // heads on 2, forward 250 us (550 TFLOP/s), dq 350, dkv 445 (610 with what they compute again). At heads of 128 the products
 // lead: 2 sequences of 8192 and 2800 tokens, 16 heads on 4, forward 340 us (900 TFLOP/s; a large library product of 16
-// bits reaches 1200), dq 430, dkv 955. Short sequences are bound by their bytes and by the latency of few tiles each:
-// 4096 segments of up to 32 tokens, 8 heads on 2, forward 56 us (4.0 TB/s), dq 81, dkv 60.
+// bits reaches 1200), dq 430, dkv 955. Short sequences are bound by their bytes: 4096
+// segments of up to 32 tokens, 8 heads on 2, forward 56 us (4.0 TB/s), dq 81 (3.8), dkv 60 (4.4).
 #include "../../include/nablaengine_policy.h"
 #include "policy_attend.h"
 
