@@ -410,6 +410,26 @@ def test_attention_few_sequences_what_the_mask_hides(dim, bad):
     check(("out", "dq"))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_long_sequences(dim):
+    """Sequences long enough that their tiles are listed one by one, and enough of them that none is split."""
+    print("attention long", dim, flush=True)
+    lq, lk = [2500, 1900], [2500, 2100]
+    q = rand((sum(lq), 16, dim), BF16, 1)
+    k, v = rand((sum(lk), 8, dim), BF16, 2), rand((sum(lk), 8, dim), BF16, 3)
+    check_attention(q, k, v, lq, lk)
+
+
+def test_attention_one_long_among_short():
+    """The mean length chooses the key tiles and the order: one sequence far above it, by either rule."""
+    for dtype, dim, heads in ((BF16, 64, 8), (F16, 40, 2), (BF16, 128, 4)):
+        print("attention one long", dtype, dim, heads, flush=True)
+        lq, lk = [3, 0, 1] * 20 + [700] + [2] * 30, [3, 2, 1] * 20 + [900] + [40] * 30
+        q = rand((sum(lq), heads, dim), dtype, 1)
+        k, v = rand((sum(lk), 2, dim), dtype, 2), rand((sum(lk), 2, dim), dtype, 3)
+        check_attention(q, k, v, lq, lk)
+
+
 def test_attention_strides():
     """Slices of one projection at odd offsets, heads before tokens, a cotangent with its own strides."""
     lq = [40, 0, 77]
@@ -648,6 +668,23 @@ def test_step_capacities(worlds, capacity):
     lengths = [[capacity, capacity // 2 + 1, 0, 1][w % 4] for w in range(worlds)]
     k, v = rand((worlds, capacity, 2, 64), BF16, 2), rand((worlds, capacity, 2, 64), BF16, 3)
     check_step(rand((worlds, 4, 64), BF16, 1), k, v, lengths, scale=0.2)
+
+
+@pytest.mark.parametrize("heads,kv,dim,capacity", [(1, 1, 64, 50), (4, 2, 64, 130), (6, 2, 40, 33), (8, 1, 128, 20), (24, 2, 8, 9)])
+def test_step_many_worlds(heads, kv, dim, capacity):
+    """Enough worlds that a wave takes each alone."""
+    print("step many", heads, kv, dim, capacity, flush=True)
+    W = 2049
+    q, k, v = (rand((W, *s, dim), BF16, i) for i, s in enumerate(((heads,), (capacity, kv), (capacity, kv))))
+    lengths = torch.tensor([(37 * w) % (capacity + 1) for w in range(W)], dtype=torch.int32, device="cuda")
+    out = policy.attention_step(q, k, v, lengths)
+    K, V = (x.double().repeat_interleave(heads // kv, 2).permute(0, 2, 1, 3) for x in (k, v))
+    s = (K * q.double()[:, :, None]).sum(3) / math.sqrt(dim)
+    seen = (torch.arange(capacity, device="cuda") < lengths[:, None])[:, None].expand_as(s)
+    some = lengths[:, None, None] > 0
+    p = torch.softmax(s.masked_fill(~seen & some, -math.inf), 2) * (seen & some)
+    want, size = (p[..., None] * V).sum(2), (p[..., None] * V.abs()).sum(2)
+    within("out", out, want, U[BF16] * want.abs() + EXP * size + TINY[BF16])
 
 
 def test_step_reads_only_the_history():
