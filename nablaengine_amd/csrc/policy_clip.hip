@@ -14,9 +14,10 @@
 // which saves a launch in between.
 //
 // Measured: 302 million weights in 196 tensors (bfloat16 matrices, float32 vectors), 0.6 GB read, read again and written as
-// 1.2 GB of float32: 513 us, 160 for the squares (3.8 TB/s, what a sum over one large tensor reaches) and 345 for the second
-// pass (5.2 TB/s, a copy's rate). The gradients of a small network, 16 tensors of 256 x 256 and less: 4.3 and 4.7 us of two
-// launches and 16 us a call from Python. Units of 8192 or 16384 elements and four times the sums gained nothing.
+// 1.2 GB of float32: 513 us, 160 for the squares and 345 for the second pass, together 4.7 TB/s, what a copy of 4 GiB
+// reaches (the squares alone 3.8: the cache still writes back the last pass's outputs). More sums in flight, two and four
+// accumulators a thread gained nothing. The gradients of a small network, 16 tensors of 256 x 256 and less: 4.3 and 4.7 us of two
+// launches and 16 us a call from Python. Units of 8192 or 16384 elements gained nothing.
 #include "../../include/nablaengine_policy.h"
 #include "policy_device.h"
 
