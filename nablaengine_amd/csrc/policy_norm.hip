@@ -384,7 +384,7 @@ int vectors_of(int n, int type) { const int e = 16 / bytes_of(type); return (n +
 
 // The backward's workgroups: each row in flight at once at most, and what the CUs hold at once (of 8 waves: three with one
 // vector a lane, two with two; more would only write more partial rows). 524288 x 256 bfloat16: 174 us with two a CU, 151
-// with three, 194 with four, which take a second round.
+// with three, 194 with four, which are not all held at once.
 int vjp_blocks(long long rows, int n, int type) {
   int lanes, vectors;
   group_of(vectors_of(n, type), type, lanes, vectors);
