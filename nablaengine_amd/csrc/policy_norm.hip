@@ -97,12 +97,15 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void k_norm(long long rows, int 
   if (KEEP)
 #pragma unroll
     for (int c = 0; c < C; ++c) params(c, c);
-  for (long long row = (long long)blockIdx.x * GROUPS + group; row < rows; row += (long long)gridDim.x * GROUPS) {
+  // groups of several waves meet at barriers: the workgroup stays together, a group past the last row has none of it
+  for (long long row = (long long)blockIdx.x * GROUPS + group;; row += (long long)gridDim.x * GROUPS) {
+    if (L > 64 ? row - group >= rows : row >= rows) break;
+    const int m = row < rows ? n : 0;
     float f[C][E];
     float s = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      row_load<E>(x + row * xs, lane + c * L, n, 0.0f, f[c]);
+      row_load<E>(x + row * xs, lane + c * L, m, 0.0f, f[c]);
 #pragma unroll
       for (int e = 0; e < E; ++e) s += own<E>(lane + c * L, n, e) ? f[c][e] : 0.0f;
     }
@@ -117,13 +120,13 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void k_norm(long long rows, int 
         q += d * d;
       }
     const float r = 1.0f / sqrtf(group_sum<L>(q, red) / (float)n + eps);
-    if (stats && lane == 0) {
+    if (stats && lane == 0 && m) {
       stats[row] = mu;
       stats[rows + row] = r;
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      if ((lane + c * L) * E >= n) continue;
+      if ((lane + c * L) * E >= m) continue;
       const int at = KEEP ? c : 0;
       if (!KEEP) params(c, at);
 #pragma unroll
@@ -203,7 +206,7 @@ __global__ __launch_bounds__(vjp_block(L)) void k_norm_vjp(long long rows, int n
   if (KEEP)
 #pragma unroll
     for (int c = 0; c < C; ++c) row_load<E>(w, lane + c * L, n, 1.0f, wf[c]);
-  // groups of several waves meet at barriers: the workgroup stays together, a group past the last row has none of it
+  // as in the forward, groups of several waves stay together
   for (long long row = (long long)blockIdx.x * GROUPS + group;; row += (long long)gridDim.x * GROUPS) {
     if (L > 64 ? row - group >= rows : row >= rows) break;
     const int m = row < rows ? n : 0;

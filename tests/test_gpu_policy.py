@@ -124,6 +124,22 @@ def test_norm_strides_and_alignments():
         policy.layer_norm(rand((4, 6, 10)).transpose(0, 1))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows", [1, 2, 3, 16385, 16387, 40001])
+def test_norm_groups_of_two_waves(dtype, rows):
+    """16-bit rows of 513 to 1024 elements share a workgroup of two groups, which meet at barriers: odd numbers of rows, fewer
+    than the launch's groups and more, leave the last workgroup's second group without a row."""
+    for width in (520, 777, 1024):
+        print("norm two waves", dtype, rows, width, flush=True)
+        x = rand((rows, width), dtype, rows + width, 2.0) + 0.5
+        y, stats = policy._ops().layer_norm_forward(x, None, None, 1e-5, True)
+        want, xh, r, mean = norm64(x, None, None, 1e-5)
+        dxh = SUM * (r * x.double().abs().mean(-1, keepdim=True) + xh.abs() + 1)
+        within("y", y, want, U[dtype] * want.abs() + dxh + SUM * want.abs() + TINY[dtype])
+        within("mean", stats[0], mean[:, 0], SUM * x.double().abs().mean(-1))
+        within("deviation", stats[1], r[:, 0], 4 * SUM * r[:, 0])
+
+
 def test_norm_extremes():
     """Constant rows (variance 0), a large mean, large and small values, rows that hold inf or NaN and their neighbours."""
     x = torch.full((3, 100), 7.25, device="cuda")
