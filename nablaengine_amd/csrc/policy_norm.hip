@@ -22,12 +22,15 @@ namespace pol {
 // Rows that no register variant holds: each pass reads the row again (it stays in the L2 cache: at most a few MB).
 constexpr int WIDE = 1024;  // lanes of the largest groups, and of the wide rows'
 
+// the vectors of E that hold n elements, n up to 2^31 - 1
+__host__ __device__ __forceinline__ int vectors_in(int n, int e) { return n / e + (n % e != 0); }
+
 // A row of n elements in vectors of E. The last one ends with the row: where n is no multiple of E it holds elements of the
 // one before again, which both write, with the same values, and only the first counts in sums. A tail of single elements
 // cost the waves that hold it as much again as the row: 2^27 elements in rows of 99 bfloat16 211 us forward and 307
 // backward, now 107 and 182.
 template <int E>
-__device__ __forceinline__ int first_of(int v, int n) { return v * E + E <= n || n < E ? v * E : n - E; }
+__device__ __forceinline__ int first_of(int v, int n) { return v * E <= n - E || n < E ? v * E : n - E; }
 // whether element e of vector v counts
 template <int E>
 __device__ __forceinline__ bool own(int v, int n, int e) {
@@ -142,7 +145,7 @@ __global__ __launch_bounds__(WIDE) void k_norm_wide(long long rows, int n, const
                                                     T* __restrict__ y, float* __restrict__ stats) {
   constexpr int E = Vec<T>::E;
   __shared__ float red[WIDE / 64];
-  const int nv = (n + E - 1) / E;
+  const int nv = vectors_in(n, E);
   for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * xs;
     float f[E], s = 0.0f, q = 0.0f;
@@ -289,8 +292,9 @@ __global__ __launch_bounds__(WIDE) void k_norm_vjp_wide(long long rows, int n, c
                                                         T* __restrict__ dx, float* __restrict__ part) {
   constexpr int E = Vec<T>::E;
   __shared__ float red[WIDE / 64];
-  const int nv = (n + E - 1) / E;
+  const int nv = vectors_in(n, E);
   float* out = part ? part + (long long)blockIdx.x * 2 * n : nullptr;
+  float* out_b = part ? out + n : nullptr;  // 2 n may pass 2^31
   bool first = true;
   for (long long row = blockIdx.x; row < rows; row += gridDim.x, first = false) {
     const float mu = stats[row], r = stats[rows + row];
@@ -308,7 +312,7 @@ __global__ __launch_bounds__(WIDE) void k_norm_vjp_wide(long long rows, int n, c
         const int col = first_of<E>(v, n) + e;
         if (out) {
           out[col] = (first ? 0.0f : out[col]) + g[e] * f[e];
-          out[n + col] = (first ? 0.0f : out[n + col]) + g[e];
+          out_b[col] = (first ? 0.0f : out_b[col]) + g[e];
         }
         ts += g[e] * wf[e];
         tq += g[e] * wf[e] * f[e];
@@ -330,26 +334,30 @@ __global__ __launch_bounds__(WIDE) void k_norm_vjp_wide(long long rows, int n, c
   }
 }
 
-// dw, db from the partial rows: 64 columns a workgroup, 16 waves each adding every 16th row, then the waves' sums
+// dw, db from the partial rows: 64 columns a workgroup at a time, 16 waves each adding every 16th row, then the waves' sums
+constexpr int MOST_BLOCKS = 1 << 21;  // a launch's work-items stay below 2^32
 template <typename W>
 __global__ __launch_bounds__(1024) void k_norm_params(int blocks, int n, const float* __restrict__ part,
                                                       W* __restrict__ dw, W* __restrict__ db) {
   __shared__ float add[16][64];
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const long long col = (long long)blockIdx.x * 64 + lane;  // of the 2 n columns
-  float s = 0.0f;
-  if (col < 2LL * n) {
+  for (long long first = (long long)blockIdx.x * 64; first < 2LL * n; first += (long long)gridDim.x * 64) {
+    const long long col = first + lane;  // of the 2 n columns
+    float s = 0.0f;
+    if (col < 2LL * n) {
 #pragma unroll 8
-    for (int i = wave; i < blocks; i += 16) s += part[(long long)i * 2 * n + col];
-  }
-  add[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0 && col < 2LL * n) {
-    s = 0.0f;
+      for (int i = wave; i < blocks; i += 16) s += part[(long long)i * 2 * n + col];
+    }
+    add[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && col < 2LL * n) {
+      s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s += add[i][lane];
-    W* out = col < n ? dw : db;
-    if (out) out[col < n ? col : col - n] = (W)s;
+      for (int i = 0; i < 16; ++i) s += add[i][lane];
+      W* out = col < n ? dw : db;
+      if (out) out[col < n ? col : col - n] = (W)s;
+    }
+    __syncthreads();
   }
 }
 
@@ -383,7 +391,7 @@ void group_of(int nv, int type, int& lanes, int& vectors) {
   if (bytes_of(type) == 2) by_width<8>(nv, f);
   else by_width<4>(nv, f);
 }
-int vectors_of(int n, int type) { const int e = 16 / bytes_of(type); return (n + e - 1) / e; }
+int vectors_of(int n, int type) { return vectors_in(n, 16 / bytes_of(type)); }
 
 // The backward's workgroups: each row in flight at once at most, and what the CUs hold at once (of 8 waves: three with one
 // vector a lane, two with two; more would only write more partial rows). 524288 x 256 bfloat16: 174 us with two a CU, 151
@@ -428,8 +436,11 @@ int norm_vjp(hipStream_t st, long long rows, int n, int type, const void* x, lon
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
   }
-  if (dw || db)  // no rows: no partial rows, and zeros
-    k_norm_params<W><<<(2LL * n + 63) / 64, 1024, 0, st>>>(rows > 0 ? blocks : 0, n, part, (W*)dw, (W*)db);
+  if (dw || db) {  // no rows: no partial rows, and zeros
+    const long long need = (2LL * n + 63) / 64;
+    k_norm_params<W><<<(unsigned)(need < MOST_BLOCKS ? need : MOST_BLOCKS), 1024, 0, st>>>(rows > 0 ? blocks : 0, n, part,
+                                                                                           (W*)dw, (W*)db);
+  }
   return (int)hipGetLastError();
 }
 

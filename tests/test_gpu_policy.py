@@ -140,6 +140,42 @@ def test_norm_groups_of_two_waves(dtype, rows):
         within("deviation", stats[1], r[:, 0], 4 * SUM * r[:, 0])
 
 
+@pytest.mark.parametrize("width,rows", [(2 ** 31 - 1, 1), (2 ** 30 + 5, 1), (2 ** 27 + 3, 2)])
+def test_norm_widest_rows(width, rows):
+    """Rows up to the longest that is taken. Of alternating 1 and -1 with whole-number parameters and cotangents: each sum of
+    x, of its squares and of g is of whole numbers that float32 holds, the outputs but dx are exact after rounding to
+    bfloat16. The sum of g xh takes a thread 2^18 steps at most, each off by half a unit of what it has so far."""
+    print("norm widest", width, rows, flush=True)
+    one = torch.ones((rows, width), dtype=BF16, device="cuda")
+    x, dy, w, b = one.clone(), one.clone(), one[0].clone(), one[0].clone()
+    x[:, 1::2], dy[:, ::5], w[::3] = -1, 3, 2
+    b[:] = 8  # no sum near zero
+    b[::7] = 16
+    del one
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = policy.layer_norm(*leaves)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    x, w, b, y = (t.detach() for t in (x, w, b, y))
+    for i in range(0, width, 2 ** 28):
+        c = slice(i, min(i + 2 ** 28, width))
+        assert torch.equal(y[:, c], x[:, c] * w[c] + b[c]), c
+        assert torch.equal(dw[c], (dy[:, c] * x[:, c]).sum(0)) and torch.equal(db[c], dy[:, c].sum(0)), c
+    sums = [[0.0] * rows for _ in range(3)]
+    for i in range(0, width, 2 ** 28):
+        c = slice(i, min(i + 2 ** 28, width))
+        for r in range(rows):
+            g = dy[r, c].double() * w[c].double()
+            for s, t in zip(sums, (g, g * x[r, c].double(), g.abs())):
+                s[r] += t.sum().item() / width
+    for i in range(0, width, 2 ** 28):
+        c = slice(i, min(i + 2 ** 28, width))
+        for r in range(rows):
+            xh = x[r, c].double() / math.sqrt(1 + 1e-5)
+            g = dy[r, c].double() * w[c].double()
+            want = (g - sums[0][r] - xh * sums[1][r]) / math.sqrt(1 + 1e-5)
+            within("dx", dx[r, c], want, U[BF16] * want.abs() + 2.0 ** -6 * sums[2][r] + 1e-4)
+
+
 def test_norm_extremes():
     """Constant rows (variance 0), a large mean, large and small values, rows that hold inf or NaN and their neighbours."""
     x = torch.full((3, 100), 7.25, device="cuda")
