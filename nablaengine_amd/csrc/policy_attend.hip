@@ -30,8 +30,10 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
                                                        const int* starts_q, const int* starts_k,
                                                        int* __restrict__ order) {
   constexpr int BUCKETS = 1024;
-  __shared__ int count[2][BUCKETS];
-  __shared__ int wave_sum[2][16];
+  // Places are unsigned: offsets that fall make sequences overlap, whose tiles together can pass 2^32. A place past the list
+  // is not written. Places that wrap fill the list again, so that an entry may mix two of them: place() looks at it.
+  __shared__ unsigned count[2][BUCKETS];
+  __shared__ unsigned wave_sum[2][16];
   constexpr int STAGED = 8192;  // sequences whose offsets are read to LDS, all at once: the passes below wait for none
   __shared__ int staged[2][STAGED + 1];
   if (seqs <= STAGED) {
@@ -45,8 +47,8 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   const int lane = threadIdx.x % ls, first_seq = threadIdx.x / ls, stride = 1024 / ls;
   const int bits[2] = {7, key_waves == 1 ? 5 : 7};  // of a tile's rows
   static_assert(QROWS == 128, "");
-  const long long caps[2] = {order_queries(seqs, tq, group), order_keys(seqs, tk, key_waves)};
-  int* const lists[2] = {order + ORDER_HEAD, order + ORDER_HEAD + 2 * caps[0]};
+  const unsigned caps[2] = {(unsigned)order_queries(seqs, tq, group), (unsigned)order_keys(seqs, tk, key_waves)};
+  int* const lists[2] = {order + ORDER_HEAD, order + ORDER_HEAD + 2LL * caps[0]};
   auto bucket_of = [](int cost) {  // rows or keys of the other side, below 2^30
     const int tiles = cost > 0 ? (int)((unsigned)(cost + TILE - 1) / TILE) : 0;
     return BUCKETS - 1 - (tiles < BUCKETS ? tiles : BUCKETS - 1);
@@ -86,22 +88,22 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   };
   // adds n to a bucket's count and returns what it was; lanes that all add to one bucket (short sequences mostly cost the
   // same) add at once: one after another they took half of this kernel's time
-  auto add = [&](int which, int n, int b) {
+  auto add = [&](int which, int n, int b) -> unsigned {
     const unsigned long long some = __ballot(n > 0);
     if (!some) return 0;
     const int lead = uniform(__builtin_ctzll(some)), b0 = __builtin_amdgcn_readlane(b, lead);
-    if (!__all(n == 0 || b == b0)) return n ? atomicAdd(&count[which][b], n) : 0;
-    const int before = scan_wave(n), all = __builtin_amdgcn_readlane(before, 63);
-    int base = 0;
+    if (!__all(n == 0 || b == b0)) return n ? atomicAdd(&count[which][b], (unsigned)n) : 0;
+    const unsigned before = scan_wave((unsigned)n), all = __builtin_amdgcn_readlane(before, 63);
+    unsigned base = 0;
     if ((int)threadIdx.x % 64 == lead) base = atomicAdd(&count[which][b0], all);
-    return __builtin_amdgcn_readlane(base, lead) + before - n;
+    return __builtin_amdgcn_readlane(base, lead) + before - (unsigned)n;
   };
   count[0][threadIdx.x] = count[1][threadIdx.x] = 0;
   __syncthreads();
   each([&](int which, int, int, int n, int b) { add(which, n, b); });
   __syncthreads();
   // exclusive prefixes over the buckets
-  int mine[2], sum[2];
+  unsigned mine[2], sum[2];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     mine[which] = count[which][threadIdx.x];
@@ -111,21 +113,21 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   __syncthreads();
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    int before = 0, total = 0;
+    unsigned before = 0, total = 0;
     for (int w = 0; w < 16; ++w) {
       if (w < (int)threadIdx.x / 64) before += wave_sum[which][w];
       total += wave_sum[which][w];
     }
     count[which][threadIdx.x] = before + sum[which] - mine[which];
-    if (threadIdx.x == 0) order[which] = total < caps[which] ? total : (int)caps[which];
+    if (threadIdx.x == 0) order[which] = (int)(total < caps[which] ? total : caps[which]);
   }
   __syncthreads();
   each([&](int which, int s, int t, int n, int b) {
-    int at = add(which, n, b);
+    unsigned at = add(which, n, b);
     for (int i = 0; i < n; ++i, ++at)  // the heaviest of the sequence first
       if (at < caps[which]) {
-        lists[which][2 * at] = s;
-        lists[which][2 * at + 1] = t + (which ? i : n - 1 - i);
+        lists[which][2LL * at] = s;
+        lists[which][2LL * at + 1] = t + (which ? i : n - 1 - i);
       }
   });
 }
@@ -147,7 +149,7 @@ __device__ __forceinline__ bool place(const Attend& a, int which, int at, Place&
   sequence(a.starts_k, s, a.seqs, a.tk, p.k0, p.nk);
   p.q0 = uniform(p.q0), p.nq = uniform(p.nq), p.k0 = uniform(p.k0), p.nk = uniform(p.nk);
   if (s == a.seqs) (which ? p.nq : p.nk) = 0;
-  return true;
+  return which ? p.tile * 32 * a.key_waves < p.nk : p.tile * QROWS < p.nq * a.group;
 }
 // this workgroup's, of `parts` a tile and key/value head
 __device__ __forceinline__ bool place_of_block(const Attend& a, int which, int parts, Place& p) {

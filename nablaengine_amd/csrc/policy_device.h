@@ -74,8 +74,10 @@ __device__ __forceinline__ float sum_lanes(float x) {
 
 // the sum of x over this lane and those before it in the wave
 template <int CTRL, int ROWS>
-__device__ __forceinline__ int shifted(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
-__device__ __forceinline__ int scan_wave(int x) {
+__device__ __forceinline__ unsigned shifted(unsigned x) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ unsigned scan_wave(unsigned x) {
   x += shifted<0x111, 0xf>(x);  // within each sixteen: from 1, 2, 4 and 8 lanes before
   x += shifted<0x112, 0xf>(x);
   x += shifted<0x114, 0xf>(x);

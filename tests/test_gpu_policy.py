@@ -525,6 +525,22 @@ def test_attention_offsets_that_are_wrong_stay_in_bounds():
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("pairs,tq", [(3 << 19, 1 << 18), (1 << 20, 1 << 19)])
+def test_attention_offsets_whose_tiles_pass_32_bits(pairs, tq):
+    """Offsets that go back and forth over all queries: 3 and 4 times 2^30 tiles where the list holds 3 million. Without
+    keys every query's output is zero, whichever of the tiles are computed."""
+    print("offsets past 32 bits", pairs, tq, flush=True)
+    q, k = rand((tq, 1, 8), BF16, 1), rand((64, 1, 8), BF16, 2)
+    a = torch.zeros(2 * pairs + 1, dtype=torch.int32, device="cuda")
+    a[1::2] = tq
+    out, _, work = policy._ops().attention_forward(q, k, k, a, torch.zeros_like(a), 0.5, True)
+    torch.cuda.synchronize()
+    entries = work[16:16 + 2 * int(work[0])].view(-1, 2)
+    assert 0 <= int(work[0]) <= tq // 128 + 2 * pairs + 1 and 0 <= int(work[1]) <= 64 // 32 + 2 * pairs + 1
+    assert ((entries[:, 0] >= 0) & (entries[:, 0] <= 2 * pairs)).all()
+    assert ((entries[:, 1] >= 0) & (entries[:, 1] < tq // 128)).all() and not out[:128].any()
+
+
 def test_attention_sharp_and_equal_scores():
     """Scores far apart (one key takes all), all equal (the mean), and too large for float16's range when exponentiated."""
     lq = [200]
