@@ -27,7 +27,11 @@ __device__ __forceinline__ F16x mfma(V8<_Float16> a, V8<_Float16> b, F16x c) {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int QROWS = 128;  // query rows a workgroup: 32 a wave
-constexpr float SLACK = 8.0f;  // log2
+// log2: by how much the subtracted maximum may lag behind the true one, and what probabilities are lifted by before they are
+// rounded. float16 holds 2^-24 to 2^16: lifted by 2^11 those down to 2^-36 of the largest stay, so that the many small ones of
+// a long history are not lost beside a large one (up to 2^24 keys they then miss less than half a rounding of the result).
+template <typename T> struct Range { static constexpr float SLACK = 8.0f, LIFT = 0.0f; };
+template <> struct Range<_Float16> { static constexpr float SLACK = 4.0f, LIFT = 11.0f; };
 constexpr int TILE = 64;    // keys of an LDS tile of the forward and the queries' gradient
 
 struct Attend {

@@ -294,7 +294,7 @@ __device__ __forceinline__ void finish_rows(const Attend& a, const Place& p, con
   const float c = a.scale * LOG2E;
   const long long token = p.q0 + r.pos;
   if (a.lse && r.valid && h == 0 && d0 == 0)
-    a.lse[(long long)r.head * a.tq + token] = sum == 0.0f ? INFINITY : m * c + log2f(sum);
+    a.lse[(long long)r.head * a.tq + token] = sum == 0.0f ? INFINITY : m * c + (log2f(sum) - Range<T>::LIFT);
   const unsigned bad = bad_columns(r.valid && not_finite<N>(acc) != 0.0f);
   store_rows<N>(r.valid && !(bad >> n & 1) ? (T*)a.out + (token * a.heads + r.head) * dim : nullptr, d0, dim, h, acc,
                 sum == 0.0f ? 0.0f : 1.0f / sum);
@@ -367,8 +367,9 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
     for (int j = 0; j < 16; ++j) top = fmaxf(top, s[1][j]);
     top = max_halves(top);
     // The subtracted maximum may lag behind the true one by 2^SLACK: sums and products stay far inside float32 and the
-    // probabilities inside float16, and the quotient at the end is the same. The outputs are then hardly ever rescaled.
-    if (__any(top * c > m * c + SLACK)) {
+    // probabilities, at most 2^(SLACK + LIFT), inside float16; the quotient at the end is the same. The outputs are then
+    // hardly ever rescaled.
+    if (__any(top * c > m * c + Range<T>::SLACK)) {
       const float m1 = fmaxf(m, top), f = m == -INFINITY ? 0.0f : exp2_fast((m - m1) * c);
       sum *= f;
 #pragma unroll
@@ -377,7 +378,7 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
         for (int j = 0; j < 16; ++j) acc[d][j] *= f;
       m = m1;
     }
-    const float base = m == -INFINITY ? 0.0f : m * c;  // a row that has seen no key yet
+    const float base = (m == -INFINITY ? 0.0f : m * c) - Range<T>::LIFT;  // 0: a row that has seen no key yet
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll

@@ -559,6 +559,25 @@ def test_attention_sharp_and_equal_scores():
     within("equal", out[:, 0], want, U[F16] * want.abs() + (U[F16] + EXP) * mean + 1e-7)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lq,lk,heads", [([1], [100000], 1), ([7] * 40, [3000] * 40, 8), ([7] * 400, [500] * 400, 8)])
+def test_attention_many_small_beside_a_large_one(dim, lq, lk, heads):
+    """One key whose score is far above all others', whose probabilities are 2^-26 of its own: together they have a part in
+    the output (values of 0 there and about 1 at the others), in float16 too, whose smallest step is 2^-24."""
+    for dtype in (BF16, F16):
+        print("small beside large", dtype, dim, lq[0], lk[0], flush=True)
+        q = torch.zeros((sum(lq), heads, dim), dtype=dtype, device="cuda")
+        k = torch.zeros((sum(lk), 1, dim), dtype=dtype, device="cuda")
+        v = 1 + rand((sum(lk), 1, dim), dtype, 3, 0.1)
+        q[..., 0] = 1.0
+        first = starts(lk)[:-1].long()
+        k[first, :, 0], v[first] = 26.0, 0.0
+        out = policy.attention(q, k, v, starts(lq), starts(lk), scale=math.log(2))
+        want, bound = attend64(q, k, v, lq, lk, math.log(2))["out"]
+        within("out", out, want, bound)
+        assert want.abs().min() > 4 * bound.max()  # it is not the bound that hides them
+
+
 def test_attention_keeps_sequences_apart():
     """inf and NaN in one sequence reach no other sequence."""
     lq = [40, 40, 100]
