@@ -30,8 +30,9 @@ constexpr int QROWS = 128;  // query rows a workgroup: 32 a wave
 // log2: by how much the subtracted maximum may lag behind the true one, and what probabilities are lifted by before they are
 // rounded. float16 holds 2^-24 to 2^16: lifted by 2^11 those down to 2^-36 of the largest stay, so that the many small ones of
 // a long history are not lost beside a large one (up to 2^24 keys they then miss less than half a rounding of the result).
-template <typename T> struct Range { static constexpr float SLACK = 8.0f, LIFT = 0.0f; };
-template <> struct Range<_Float16> { static constexpr float SLACK = 4.0f, LIFT = 11.0f; };
+// The backward's probabilities are those of the whole row, 1 at most: they can be lifted further.
+template <typename T> struct Range { static constexpr float SLACK = 8.0f, LIFT = 0.0f, LIFT_BACK = 0.0f; };
+template <> struct Range<_Float16> { static constexpr float SLACK = 4.0f, LIFT = 11.0f, LIFT_BACK = 14.0f; };
 constexpr int TILE = 64;    // keys of an LDS tile of the forward and the queries' gradient
 
 struct Attend {
@@ -125,6 +126,50 @@ __device__ __forceinline__ V8<T> pack(const F16x& c, int s) {
   const F8 f = s ? __builtin_shufflevector(c, c, 8, 9, 10, 11, 12, 13, 14, 15) : __builtin_shufflevector(c, c, 0, 1, 2, 3, 4, 5, 6, 7);
   return __builtin_convertvector(f, V8<T>);
 }
+
+// Score gradients on their way to 16 bits. bfloat16 has the range of float32. float16 has not: over a long history, or where
+// the loss is a mean, they are far below its smallest step of 2^-24, and where the loss is scaled they pass its 2^16. Each
+// column (a query's, a key's) has a factor, a power of two: the first gradients that are not 0 are brought to 2^7, and later
+// ones that pass 2^15 lower the factor, and with it the sums so far. The sums are divided by it at the end.
+template <typename T> struct Lift {
+  template <int N>
+  __device__ __forceinline__ void scale(F16x&, F16x*) {}
+  template <int N>
+  __device__ __forceinline__ void unscale(F16x*, float) const {}
+};
+template <> struct Lift<_Float16> {
+  float f = 0.0f;  // 0: none yet
+  template <int N>
+  __device__ __forceinline__ void scale(F16x& ds, F16x* acc) {
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(ds[j]));
+    auto other = [&](float t) { return f == 0.0f ? t > 0.0f : t * f > 32768.0f; };
+    if (__any(other(top))) {
+      top = max_halves(top);
+      if (other(top)) {
+        const int e = 261 - (int)(__float_as_uint(top) >> 23);  // of 2^7 / top, between 2^-100 and 2^100
+        const float f1 = __uint_as_float((unsigned)(e < 27 ? 27 : e > 227 ? 227 : e) << 23), less = f == 0.0f ? 1.0f : f1 / f;
+#pragma unroll
+        for (int d = 0; d < N; ++d)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[d][j] *= less;
+        f = f1;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) ds[j] *= f;
+  }
+  // the sums of products with the scaled gradients, without the factor and times `more`
+  template <int N>
+  __device__ __forceinline__ void unscale(F16x* acc, float more) const {
+    const float g = f == 0.0f ? 1.0f : more / f;
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[d][j] *= g;
+  }
+};
 
 // Infinities and NaN under the mask. A masked probability is 0, but 0 times an infinity in a row that the mask hides is
 // NaN: such sums are not what the mask asks for. The kernels do not look for them; they look at their results, and compute

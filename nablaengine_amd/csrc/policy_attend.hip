@@ -506,6 +506,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
     delta = add_halves(delta);
   }
   F16x acc[DT] = {};
+  Lift<T> lift;
   for (int t = first; t < end; ++t) {
     const int key0 = t * TILE;
     const T *kt = ks[t & 1], *vt = vs[t & 1];
@@ -529,6 +530,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
       products(kt, vt, key0, i, s, dp);
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[j] *= dp[j] - delta;
+      lift.template scale<DT>(s, acc);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const V8<T> ds = pack<T>(s, x);
@@ -537,6 +539,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
       }
     }
   }
+  lift.template unscale<DT>(acc, 1.0f);
   if (r.valid && h == 0 && (!SPLIT || p.part == 0)) a.delta[(long long)r.head * a.tq + token] = delta;
   if (SPLIT && my.parts > 1) {
     RowsPart<DP>(a, (size_t)p.at * a.parts_q + p.part, uniform(threadIdx.x / 64)).put(0, acc, DT);
@@ -683,7 +686,7 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
     }
     if (tid < RT) {
       const bool there = tid < used && r0 + tid < rows;
-      lse = there ? a.lse[stat] : INFINITY;
+      lse = there ? a.lse[stat] - Range<T>::LIFT_BACK : INFINITY;
       if (ROLE != VALUES) delta = there ? a.delta[stat] : 0.0f;
     }
     if (group > RT) {
@@ -707,6 +710,7 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
   if (ROLE != VALUES)
     load_rows<DP>(valid ? (const T*)a.v + (long long)(p.k0 + key) * a.v_t + (long long)p.kv * a.v_h : nullptr, dim, h, v);
   F16x dk[DT] = {}, dv[DT] = {};
+  Lift<T> lift;
   if (tid < RT && group <= RT) places_of[0][tid] = places_of[1][tid] = tid / group;
   // tokens from a tile's first to those of a subtile's first row and, at most, its last: x / group for x < RT as a product
   const int inverse = 65535 / group + 1;
@@ -778,6 +782,7 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
             if (key > li[e]) s[4 * j + e] = dp[4 * j + e] = 0.0f;
         }
       }
+      if (ROLE != VALUES) lift.template scale<DT>(dp, dk);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const V8<T> pr = pack<T>(s, x), ds = pack<T>(dp, x);
@@ -790,6 +795,15 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
         if (WAVES == 8) __builtin_amdgcn_s_setprio(0);
       }
     }
+  }
+  if (Range<T>::LIFT_BACK != 0.0f) {
+    constexpr float back = 1.0f / (1 << (int)Range<T>::LIFT_BACK);
+    if (ROLE != VALUES) lift.template unscale<DT>(dk, back);
+    if (ROLE != KEYS)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) dv[d][j] *= back;
   }
   // the waves of the same keys: split 0 adds the others' sums, one after another
   if constexpr (SPLIT > 1) {

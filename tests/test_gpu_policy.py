@@ -578,6 +578,27 @@ def test_attention_many_small_beside_a_large_one(dim, lq, lk, heads):
         assert want.abs().min() > 4 * bound.max()  # it is not the bound that hides them
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(2, 1, 64), (4, 2, 128), (1, 1, 40)])
+@pytest.mark.parametrize("lq,lk", [([3000, 40, 1, 0, 700], [3000, 40, 1, 3, 700]), ([1], [20000]), ([30] * 100, [30] * 100),
+                                   ([150] * 150, [170] * 150)])
+@pytest.mark.parametrize("size", ["2^-18", "2^-10", "1", "2^12", "rising", "falling"])
+def test_attention_float16_gradients_of_any_size(size, lq, lk, heads, kv, dim):
+    """Cotangents from float16's smallest (a mean loss) to its largest (a scaled one), and of all sizes in one sequence: the
+    score gradients, a probability times them, are far outside float16's range. Queries and keys are small and the scale is
+    large where cotangents are small, so that the results are inside it."""
+    print("float16 gradients", size, lq[:3], heads, dim, flush=True)
+    q, k = rand((sum(lq), heads, dim), F16, 1, 0.02), rand((sum(lk), kv, dim), F16, 2, 0.02)
+    v, dout = rand((sum(lk), kv, dim), F16, 3), rand(q.shape, torch.float64, 4)
+    if size in ("rising", "falling"):
+        at = torch.cat([torch.arange(n, device="cuda") / max(n - 1, 1) for n in lq])
+        at = 1 - at if size == "falling" else at
+        dout = dout * torch.exp2(-16 + 26 * at)[:, None, None]
+    else:
+        dout = dout * 2.0 ** (0 if size == "1" else int(size[2:]))
+    scale = 64.0 if size in ("2^-18", "2^-10") else 1.0
+    check_attention(q, k, v, lq, lk, scale=scale, dout=dout.clamp(-6e4, 6e4).to(F16))
+
+
 def test_attention_keeps_sequences_apart():
     """inf and NaN in one sequence reach no other sequence."""
     lq = [40, 40, 100]
