@@ -286,7 +286,8 @@ __device__ __forceinline__ F16x add_parts(const Attend& a, size_t slot, int part
   return acc;
 }
 
-// what a wave's rows come to, from their outputs' sums, the maximum that these lack and the probabilities' sum
+// what a wave's rows come to, from their outputs' sums, the maximum that these lack and the probabilities' sum: zeros where
+// a row sees no key, NaN where every score it sees is -inf (0 / 0, as the softmax's definition has it)
 template <typename T, int DP, int N>
 __device__ __forceinline__ void finish_rows(const Attend& a, const Place& p, const Rows& r, int d0, const F16x* acc, float m,
                                             float sum) {
@@ -294,10 +295,10 @@ __device__ __forceinline__ void finish_rows(const Attend& a, const Place& p, con
   const float c = a.scale * LOG2E;
   const long long token = p.q0 + r.pos;
   if (a.lse && r.valid && h == 0 && d0 == 0)
-    a.lse[(long long)r.head * a.tq + token] = sum == 0.0f ? INFINITY : m * c + (log2f(sum) - Range<T>::LIFT);
+    a.lse[(long long)r.head * a.tq + token] = r.limit < 0 ? INFINITY : m * c + (log2f(sum) - Range<T>::LIFT);
   const unsigned bad = bad_columns(r.valid && not_finite<N>(acc) != 0.0f);
   store_rows<N>(r.valid && !(bad >> n & 1) ? (T*)a.out + (token * a.heads + r.head) * dim : nullptr, d0, dim, h, acc,
-                sum == 0.0f ? 0.0f : 1.0f / sum);
+                r.limit < 0 ? 0.0f : 1.0f / sum);
   for (unsigned left = bad; left; left &= left - 1) {
     const Sight one(a, p, r, __builtin_ctz(left));
     const Row<DP> qr((const T*)a.q + one.token * a.q_t + one.head * a.q_h, dim);
@@ -313,7 +314,7 @@ __device__ __forceinline__ void finish_rows(const Attend& a, const Place& p, con
       top = top1;
     }
     o.store((T*)a.out + (one.token * a.heads + one.head) * dim, d0, d0 + 32 * N < dim ? d0 + 32 * N : dim,
-            total == 0.0f ? 0.0f : 1.0f / total);
+            one.limit < 0 ? 0.0f : 1.0f / total);
   }
 }
 

@@ -1,6 +1,7 @@
 // Attention of one new query a world over that world's cached history: the control loop's form.
 //
-//   o = sum_j softmax_j(scale q . k_j) v_j over the world's first `length` cached tokens; zeros where there are none
+//   o = sum_j softmax_j(scale q . k_j) v_j over the world's first `length` cached tokens; zeros where there are none, NaN (0 / 0) where
+//       every score is -inf
 //
 // Memory bounds it: each cached key and value is read once, for all the query heads that share it. A workgroup takes
 // one world, one key/value head and one stretch of the history. A key's 16-byte chunks lie across LPR lanes, so that a
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(256) void k_step(Step a) {
   auto put = [&](int g, int d, float top, float total, float x) {
     const long long head = (long long)world * a.heads + kv * a.group + g0 + g;
     if (a.stretches == 1) {
-      ((T*)a.out)[head * a.dim + d] = (T)(total == 0.0f ? 0.0f : x / total);
+      ((T*)a.out)[head * a.dim + d] = (T)(length == 0 ? 0.0f : x / total);
     } else {
       float* to_part = a.part + ((long long)stretch * a.worlds * a.heads + head) * (a.dim + 2);
       to_part[d] = x;
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(1024) void k_step_join(Step a) {
     x = 0.0f;
 #pragma unroll
     for (int i = 0; i < JW; ++i) x += sums[i][d];
-    ((T*)a.out)[head * a.dim + d] = (T)(total == 0.0f ? 0.0f : x / total);
+    ((T*)a.out)[head * a.dim + d] = (T)(a.lengths[head / a.heads] <= 0 ? 0.0f : x / total);
   }
 }
 

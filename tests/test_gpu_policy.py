@@ -822,6 +822,34 @@ def test_step_is_attentions_last_row():
     assert (a - b).abs().max() < 4 * U[F16]
 
 
+def test_scores_that_are_all_minus_infinity():
+    """Softmax over scores that are all -inf is 0 / 0: NaN, from an infinite key or from a product past float32, in the rows
+    that see no other score and the keys they see; not zeros, which stand for rows without keys."""
+    for dtype, dim, low in ((BF16, 64, -math.inf), (BF16, 128, -3e30), (F16, 40, -math.inf)):
+        q, k, v = rand((240, 2, dim), dtype, 1), rand((240, 1, dim), dtype, 2), rand((240, 1, dim), dtype, 3)
+        lq = [100, 140]
+        clean = policy.attention(q, k, v, starts(lq))
+        q[:100, :, 0], q[:100, :, 1:] = 3e30 if dtype == BF16 else 1.0, 0.0
+        k[:30, :, 0], k[30:100, :, 0] = low, 0.0
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        out = policy.attention(*leaves, starts(lq))
+        dq, dk, dv = torch.autograd.grad(out, leaves, rand(q.shape, dtype, 4))
+        assert torch.isnan(out[:30]).all() and torch.isfinite(out[30:]).all() and torch.equal(out[100:], clean[100:])
+        assert torch.isnan(dv[0]).all() and torch.isnan(dq[:30, :, 0]).all()
+        assert all(torch.isfinite(g[100:]).all() for g in (dq, dk, dv))
+        rows = torch.arange(30, 100, device="cuda")
+        mean = v[30:100, 0].double().cumsum(0) / (rows - 29)[:, None]  # the seen keys' scores are 0, the first 30 have no part
+        size = v[30:100, 0].double().abs().cumsum(0) / (rows - 29)[:, None]
+        within("rows", out[30:100, 0], mean, U[dtype] * mean.abs() + (U[dtype] + EXP) * size + TINY[dtype])
+        for capacity in (30, 3000):  # whole, and in stretches
+            cache = torch.zeros((3, capacity, 1, dim), dtype=dtype, device="cuda")
+            cache[..., 0], cache[2, -1] = low, 0.0
+            values = torch.ones_like(cache)
+            n = torch.tensor([0, capacity, capacity], dtype=torch.int32, device="cuda")
+            got = policy.attention_step(q[:3], cache, values, n)
+            assert not got[0].any() and torch.isnan(got[1]).all() and torch.equal(got[2], torch.ones_like(got[2]))
+
+
 def test_step_past_32_bits():
     cap, worlds = 2 ** 22, 5
     k = torch.zeros((worlds, cap, 1, 128), dtype=BF16, device="cuda")
