@@ -357,23 +357,55 @@ Tensor attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const T
 // ---- autograd -------------------------------------------------------------------------------------------------------
 
 // The dispatcher's operators (a node calls them rather than the functions above, so that torch.compile sees them).
-template <typename F>
-const auto& op(const char* name) {
-  static const auto handle = c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
-  return handle;
-}
-const auto& norm_forward_op() { return op<decltype(layer_norm_forward)>("nablaengine::layer_norm_forward"); }
-const auto& norm_backward_op() { return op<decltype(layer_norm_backward)>("nablaengine::layer_norm_backward"); }
-const auto& attention_forward_op() { return op<decltype(attention_forward)>("nablaengine::attention_forward"); }
-const auto& attention_backward_op() { return op<decltype(attention_backward)>("nablaengine::attention_backward"); }
+#define OP(name)                                                                                                        \
+  const auto& name##_op() {                                                                                             \
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("nablaengine::" #name, "").typed<decltype(name)>(); \
+    return op;                                                                                                          \
+  }
+OP(layer_norm_forward) OP(layer_norm_backward) OP(grad_norm) OP(clip_grads_) OP(clip_grads_out)
+OP(attention_forward) OP(attention_backward) OP(attention_step)
+#undef OP
 
 bool wants(const Tensor& x) { return x.defined() && x.requires_grad(); }
 bool wants(const OptTensor& x) { return x && wants(*x); }
 
+// There are gradients of first order by reverse mode, and no others: a tangent that reaches an operator (forward mode), or a
+// gradient that is differentiated again, is an error, where below autograd it would be lost.
+bool dual(const Tensor& x) { return x.defined() && x._fw_grad(/*level=*/0).defined(); }
+bool dual(const OptTensor& x) { return x && dual(*x); }
+bool dual(at::TensorList xs) { return std::any_of(xs.begin(), xs.end(), [](const Tensor& x) { return dual(x); }); }
+template <typename... Xs>
+void no_tangents(const char* what, const Xs&... xs) {
+  TORCH_CHECK(!(dual(xs) || ...), POL, what, " has no forward-mode derivative");
+}
+// a gradient's operator as a node, for graphs of gradients (create_graph), that raises when it is run backward
+#define FIRST_ORDER(what)                                                          \
+  static variable_list backward(AutogradContext*, variable_list) {                 \
+    TORCH_CHECK(false, POL what "'s gradients cannot be differentiated again");    \
+  }
+struct LayerNormBackward : torch::autograd::Function<LayerNormBackward> {
+  static variable_list forward(AutogradContext*, const Tensor& dy, const Tensor& x, const OptTensor& weight,
+                               const OptTensor& bias, const Tensor& stats, bool want_x, bool want_weight, bool want_bias) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return layer_norm_backward_op().call(dy, x, weight, bias, stats, want_x, want_weight, want_bias);
+  }
+  FIRST_ORDER("layer_norm")
+};
+struct AttentionBackward : torch::autograd::Function<AttentionBackward> {
+  static variable_list forward(AutogradContext*, const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v,
+                               const Tensor& starts_q, const Tensor& starts_k, const Tensor& out, const Tensor& lse,
+                               const Tensor& work, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return attention_backward_op().call(dout, q, k, v, starts_q, starts_k, out, lse, work, scale);
+  }
+  FIRST_ORDER("attention")
+};
+#undef FIRST_ORDER
+
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto r = norm_forward_op().call(x, weight, bias, eps, true);
+    auto r = layer_norm_forward_op().call(x, weight, bias, eps, true);
     ctx->saved_data["want"] = std::vector<int64_t>{wants(x), wants(weight), wants(bias)};
     ctx->save_for_backward({x, weight ? *weight : Tensor(), bias ? *bias : Tensor(), r[1]});
     return r[0];
@@ -384,19 +416,26 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     if (!grad[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const Tensor dy = row_stride(grad[0]) < 0 ? grad[0].contiguous() : grad[0];
     auto param = [](const Tensor& p) { return p.defined() ? OptTensor(p) : OptTensor(); };
-    at::AutoDispatchBelowADInplaceOrView below;
-    auto r = norm_backward_op().call(dy, saved[0], param(saved[1]), param(saved[2]), saved[3], want[0], want[1], want[2]);
+    no_tangents("layer_norm's gradient", dy, saved[0], saved[1], saved[2]);
+    auto run = [&] {
+      if (at::GradMode::is_enabled())
+        return LayerNormBackward::apply(dy, saved[0], param(saved[1]), param(saved[2]), saved[3], !!want[0], !!want[1], !!want[2]);
+      at::AutoDispatchBelowADInplaceOrView below;
+      return layer_norm_backward_op().call(dy, saved[0], param(saved[1]), param(saved[2]), saved[3], want[0], want[1], want[2]);
+    };
+    const variable_list r = run();
     return {want[0] ? r[0] : Tensor(), want[1] ? r[1] : Tensor(), want[2] ? r[2] : Tensor(), Tensor()};
   }
 };
 Tensor layer_norm_autograd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+  no_tangents("layer_norm", x, weight, bias);
   if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias)))
     return LayerNorm::apply(x, weight, bias, eps);
   at::AutoDispatchBelowADInplaceOrView below;
-  return norm_forward_op().call(x, weight, bias, eps, false)[0];
+  return layer_norm_forward_op().call(x, weight, bias, eps, false)[0];
 }
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
-  return norm_forward_op().call(x, weight, bias, eps, false)[0];
+  return layer_norm_forward_op().call(x, weight, bias, eps, false)[0];
 }
 
 struct Attention : torch::autograd::Function<Attention> {
@@ -412,14 +451,21 @@ struct Attention : torch::autograd::Function<Attention> {
     const auto s = ctx->get_saved_variables();
     if (!grad[0].defined()) return variable_list(6);
     const Tensor dout = grad[0].numel() && grad[0].stride(2) != 1 ? grad[0].contiguous() : grad[0];
-    at::AutoDispatchBelowADInplaceOrView below;
-    auto r = attention_backward_op().call(dout, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7],
-                                          ctx->saved_data["scale"].toDouble());
+    no_tangents("attention's gradient", dout, s[0], s[1], s[2]);
+    const double scale = ctx->saved_data["scale"].toDouble();
+    auto run = [&] {
+      if (at::GradMode::is_enabled())
+        return AttentionBackward::apply(dout, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], scale);
+      at::AutoDispatchBelowADInplaceOrView below;
+      return attention_backward_op().call(dout, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], scale);
+    };
+    const variable_list r = run();
     return {r[0], r[1], r[2], Tensor(), Tensor(), Tensor()};
   }
 };
 Tensor attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& starts_q,
                           const Tensor& starts_k, double scale) {
+  no_tangents("attention", q, k, v);
   if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v)))
     return Attention::apply(q, k, v, starts_q, starts_k, scale);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -430,9 +476,43 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   return attention_forward_op().call(q, k, v, starts_q, starts_k, scale, false)[0];
 }
 
+Tensor grad_norm_autograd(at::TensorList grads) {
+  no_tangents("grad_norm", grads);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return grad_norm_op().call(grads);
+}
+Tensor clip_grads_autograd(at::TensorList grads, double max_norm) {
+  no_tangents("clip_grads_", grads);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return clip_grads__op().call(grads, max_norm);
+}
+Tensor clip_grads_out_autograd(at::TensorList grads, at::TensorList out, double max_norm) {
+  no_tangents("clip_grads_", grads, out);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return clip_grads_out_op().call(grads, out, max_norm);
+}
+Tensor attention_step_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, double scale) {
+  no_tangents("attention_step", q, k, v);
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(wants(q) || wants(k) || wants(v)), POL "attention_step has no gradient");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return attention_step_op().call(q, k, v, lengths, scale);
+}
+// the nodes' operators, where they are called above autograd: by name, or at a transform's inner level
+void inner_autograd(const c10::OperatorHandle& op, torch::jit::Stack* stack) {
+  const std::string& name = op.schema().name();
+  const size_t count = op.schema().arguments().size();
+  for (size_t i = stack->size() - count; i < stack->size(); ++i) {
+    if (!(*stack)[i].isTensor()) continue;
+    const Tensor& x = (*stack)[i].toTensor();
+    no_tangents(name.c_str(), x);
+    TORCH_CHECK(!at::GradMode::is_enabled() || !wants(x), POL, name, " has no gradient: call layer_norm or attention");
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  op.callBoxed(stack);
+}
+
 }  // namespace
 
-// addresses: those of ENTRIES, in that order
 // the entries' names, in the order in which dk_policy_torch_bind takes their addresses
 extern "C" const char* dk_policy_torch_entries() {
 #define X(name) #name " "
@@ -478,4 +558,10 @@ TORCH_LIBRARY_IMPL(nablaengine, CompositeExplicitAutograd, m) {
 TORCH_LIBRARY_IMPL(nablaengine, Autograd, m) {
   m.impl("layer_norm", layer_norm_autograd);
   m.impl("attention", attention_autograd);
+  m.impl("grad_norm", grad_norm_autograd);
+  m.impl("clip_grads_", clip_grads_autograd);
+  m.impl("clip_grads_out", clip_grads_out_autograd);
+  m.impl("attention_step", attention_step_autograd);
+  for (const char* name : {"layer_norm_forward", "layer_norm_backward", "attention_forward", "attention_backward"})
+    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&inner_autograd>());
 }

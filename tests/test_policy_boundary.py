@@ -103,3 +103,66 @@ def test_fake_shapes():
         assert out.shape == q.shape and lse.shape == (4, 7) and work.dtype == torch.int32
         assert [t.shape for t in ops.attention_backward(q, q, k, k, a, a, out, lse, work, 0.125)] == [q.shape, k.shape, k.shape]
         assert ops.attention_step(q, k[:7, None], k[:7, None], a, 0.125).shape == q.shape
+
+
+def _differentiable():
+    """(call, its first argument) of the operators with gradients, on what is made under a FakeTensorMode"""
+    x, w, b = torch.randn(4, 8), torch.randn(8), torch.randn(8)
+    q, k, a = torch.randn(5, 2, 8).bfloat16(), torch.randn(5, 1, 8).bfloat16(), torch.zeros(2, dtype=torch.int32)
+    return ((lambda x: policy.layer_norm(x, w, b), x), (lambda q: policy.attention(q, k, k, a), q))
+
+
+def test_forward_mode_raises():
+    """A tangent is never dropped: not by an operator without gradients, not by a tensor that does not require grad, not in
+    the backward."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.autograd import forward_ad
+    ops = policy._ops()
+    with FakeTensorMode():
+        x, n = torch.randn(4, 8), torch.zeros(5, dtype=torch.int32)
+        q, k = torch.randn(5, 2, 8).bfloat16(), torch.randn(5, 3, 1, 8).bfloat16()
+        others = ((lambda g: policy.grad_norm([g]), x), (lambda g: policy.clip_grads_([g], 1.0), x),
+                  (lambda g: policy.clip_grads_([g], 1.0, out=[x.clone()]), x), (lambda q: policy.attention_step(q, k, k, n), q),
+                  (lambda x: ops.layer_norm_forward(x, None, None, 1e-5, True)[0], x))
+        for call, at in (*_differentiable(), *others):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.func.jvp(call, (at,), (at.clone(),))
+            with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+                call(forward_ad.make_dual(at.clone(), at))
+        for call, at in _differentiable():
+            y = call(at.clone().requires_grad_())
+            with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+                y.backward(forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+def test_second_order_raises():
+    """A gradient that is differentiated again raises, also where the loss reaches the input on another path; without
+    create_graph it is a plain tensor, and under it one of inputs that need none."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    policy._ops()
+    with FakeTensorMode():
+        for call, at in _differentiable():
+            x = at.clone().requires_grad_()
+            g, = torch.autograd.grad(call(x).float().sum(), x, create_graph=True)
+            assert g.requires_grad
+            with pytest.raises(RuntimeError, match="differentiated again"):
+                (g.float().square().sum() + x.float().sum()).backward()
+            dy = at.clone().requires_grad_()
+            g, = torch.autograd.grad(call(x), x, dy, create_graph=True)
+            with pytest.raises(RuntimeError, match="differentiated again"):
+                torch.autograd.grad(g.float().sum(), dy)
+            assert not torch.autograd.grad(call(x).float().sum(), x)[0].requires_grad
+
+
+def test_the_nodes_operators_have_no_gradient():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = policy._ops()
+    with FakeTensorMode():
+        x = torch.randn(4, 8, requires_grad=True)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            ops.layer_norm_forward(x, None, None, 1e-5, True)
+        with torch.no_grad():
+            ops.layer_norm_forward(x, None, None, 1e-5, True)
+        q, k, n = torch.randn(5, 2, 8).bfloat16(), torch.randn(5, 3, 1, 8).bfloat16(), torch.zeros(5, dtype=torch.int32)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            ops.attention_step(q.requires_grad_(), k, k, n, 0.5)
