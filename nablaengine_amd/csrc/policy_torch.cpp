@@ -153,12 +153,13 @@ std::vector<Tensor> layer_norm_forward(const Tensor& x, const OptTensor& weight,
   return {y, s};
 }
 
-std::vector<Tensor> layer_norm_backward(const Tensor& dy, const Tensor& x, const OptTensor& weight, const OptTensor& bias,
+// dy: any strides (a cotangent is what torch makes it; the node, which may hold tensors of symbolic sizes, does not look)
+std::vector<Tensor> layer_norm_backward(const Tensor& grad, const Tensor& x, const OptTensor& weight, const OptTensor& bias,
                                         const Tensor& stats, bool want_x, bool want_weight, bool want_bias) {
   const Norm a = norm_checks(x, weight, bias);
-  check_as("dy", dy, x, x.scalar_type(), x.sizes());
+  check_as("dy", grad, x, x.scalar_type(), x.sizes());
+  const Tensor dy = row_stride(grad) < 0 ? grad.contiguous() : grad;
   const int64_t dy_stride = row_stride(dy);
-  CHECK_TYPE(dy_stride >= 0, "dy: expected evenly spaced rows of neighbouring elements, got ", described(dy));
   check_as("stats", stats, x, at::kFloat, {2, a.rows});
   const Tensor dx = at::empty(want_x ? x.sizes() : at::IntArrayRef{0}, x.options());
   const auto params = x.options().dtype(a.params);
@@ -306,15 +307,16 @@ std::vector<Tensor> attention_forward(const Tensor& q, const Tensor& k, const Te
   return {out, lse, work};
 }
 
-std::vector<Tensor> attention_backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v,
+// dout: any strides, as layer_norm_backward's
+std::vector<Tensor> attention_backward(const Tensor& grad, const Tensor& q, const Tensor& k, const Tensor& v,
                                        const Tensor& starts_q, const Tensor& starts_k, const Tensor& out,
                                        const Tensor& lse, const Tensor& work, double scale) {
   const Heads h = heads_checks(q, k, v, 3);
   const int seqs = sequences_checks(q, k, starts_q, starts_k, h);
   check_bound();
-  check_as("dout", dout, q, q.scalar_type(), q.sizes());
+  check_as("dout", grad, q, q.scalar_type(), q.sizes());
   check_as("out", out, q, q.scalar_type(), q.sizes());
-  CHECK_TYPE(dout.numel() == 0 || dout.stride(2) == 1, "dout: a head's elements must be neighbours, got ", described(dout));
+  const Tensor dout = grad.numel() && grad.stride(2) != 1 ? grad.contiguous() : grad;
   check_as("lse", lse, q, at::kFloat, {h.heads, q.size(0)});
   check_as("work", work, q, at::kInt, {order_words(h, seqs, q, k)});
   CHECK_TYPE(out.is_contiguous() && lse.is_contiguous() && work.is_contiguous(), "out, lse and work must be contiguous");
@@ -414,7 +416,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const auto saved = ctx->get_saved_variables();
     const auto want = ctx->saved_data["want"].toIntVector();
     if (!grad[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    const Tensor dy = row_stride(grad[0]) < 0 ? grad[0].contiguous() : grad[0];
+    const Tensor& dy = grad[0];
     auto param = [](const Tensor& p) { return p.defined() ? OptTensor(p) : OptTensor(); };
     no_tangents("layer_norm's gradient", dy, saved[0], saved[1], saved[2]);
     auto run = [&] {
@@ -450,7 +452,7 @@ struct Attention : torch::autograd::Function<Attention> {
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     const auto s = ctx->get_saved_variables();
     if (!grad[0].defined()) return variable_list(6);
-    const Tensor dout = grad[0].numel() && grad[0].stride(2) != 1 ? grad[0].contiguous() : grad[0];
+    const Tensor& dout = grad[0];
     no_tangents("attention's gradient", dout, s[0], s[1], s[2]);
     const double scale = ctx->saved_data["scale"].toDouble();
     auto run = [&] {

@@ -95,9 +95,15 @@ def _fake_norm(grads, *_):
     return grads[0].new_empty((), dtype=torch.float32)
 
 
+def _order_words(group, dim, seqs, tq, tk):
+    """dk_attention_work_bytes / 4, written out so that sizes may be symbolic (the library's own takes numbers only): a
+    head of 16, and two words each of the query tiles of 128 rows and of the key tiles of 128 or 32 keys."""
+    keys = 32 if dim <= 64 and tk <= 96 * seqs else 128
+    return 16 + 2 * (tq * group // 128 + tk // keys + 2 * (seqs + 1))
+
+
 def _fake_attention_forward(q, k, v, starts_q, starts_k, scale, train):
-    words = int(torch_ffi._load().dll.dk_attention_work_bytes(q.shape[1], k.shape[1], q.shape[2], starts_q.shape[0] - 1,
-                                                              q.shape[0], k.shape[0])) // 4
+    words = _order_words(q.shape[1] // k.shape[1], q.shape[2], starts_q.shape[0] - 1, q.shape[0], k.shape[0])
     return [q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0] if train else 0), dtype=torch.float32),
             starts_q.new_empty((words,))]
 
@@ -119,7 +125,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=EPS):
     wider one's columns); weight, bias: float32 or x's type, or None. y is contiguous and has x's type; mean, variance
     and every sum are float32, and the gradients have their inputs' types."""
     e = float(eps)
-    if not (math.isfinite(e) and e >= 0.0):
+    if not 0.0 <= e < math.inf:
         raise _err(f"eps must be finite and >= 0, got {eps}", ValueError)
     return _ops().layer_norm(_tensor("x", x), weight, bias, e)
 
@@ -189,7 +195,7 @@ def _scale(scale, q):
     if scale is None:
         return 1.0 / math.sqrt(q.shape[2])
     s = float(scale)
-    if not (math.isfinite(s) and s > 0.0):
+    if not 0.0 < s < math.inf:
         raise _err(f"scale must be finite and > 0, got {scale}", ValueError)
     return s
 

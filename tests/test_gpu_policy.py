@@ -953,6 +953,26 @@ def test_operators_compiled():
     assert torch.equal(clip(one), policy.clip_grads_(two, 0.5) * 2) and all(torch.equal(p, q) for p, q in zip(one, two))
 
 
+def test_operators_compiled_over_sizes():
+    """One compiled function over several batches, cotangents in their own strides: eager's results for each."""
+    w, b = rand((64,), F32, 2), rand((64,), F32, 3)
+
+    def loss(x, w, b, heads, a):
+        y = policy.layer_norm(torch.sin(x), w, b)
+        o = policy.attention(heads[:, :2], heads[:, 2:4], heads[:, 4:], a)
+        return (y.t() @ y).sum() + (o.float().transpose(0, 2) * 3).cumsum(0).sum()
+
+    def run(f, rows, lq):
+        leaves = [t.detach().requires_grad_() for t in (rand((rows, 64), F32, 1), w, b, rand((sum(lq), 6, 64), BF16, 4))]
+        value = f(*leaves, starts(lq))
+        return [value.detach(), *torch.autograd.grad(value, leaves)]
+    torch._dynamo.reset()
+    compiled = torch.compile(loss, fullgraph=True, backend="aot_eager")
+    for rows, lq in ((300, [20, 0, 44, 11]), (301, [7, 300]), (4, [1]), (77, [500, 900, 2, 2, 2]), (5000, [33] * 40)):
+        for i, (e, c) in enumerate(zip(run(loss, rows, lq), run(compiled, rows, lq))):
+            assert torch.equal(e, c), (rows, i)
+
+
 def test_clipping_marks_what_it_writes():
     """A graph that saved a tensor which clipping then overwrites notices."""
     w = rand((8,), F32, 1).requires_grad_()

@@ -166,3 +166,57 @@ def test_the_nodes_operators_have_no_gradient():
         q, k, n = torch.randn(5, 2, 8).bfloat16(), torch.randn(5, 3, 1, 8).bfloat16(), torch.zeros(5, dtype=torch.int32)
         with pytest.raises(RuntimeError, match="no gradient"):
             ops.attention_step(q.requires_grad_(), k, k, n, 0.5)
+
+
+def _compiles(call, inputs, dynamic):
+    """How often torch.compile compiles call for the inputs, one list of arguments after another. Compilation needs no GPU; each
+    call then ends in the operators' TypeError."""
+    from torch._dynamo.backends.debugging import aot_eager
+    count = []
+
+    def backend(graph, example):
+        count.append(1)
+        return aot_eager(graph, example)
+    torch._dynamo.reset()
+    compiled = torch.compile(call, backend=backend, fullgraph=True, dynamic=dynamic)
+    for args in inputs:
+        with pytest.raises(TypeError, match="ROCm device"):
+            compiled(*args)
+    return len(count)
+
+
+@pytest.mark.parametrize("dynamic", [None, True])
+def test_compiled_once_for_all_sizes(dynamic):
+    """After the first size torch.compile takes sizes as symbols: the operators, their nodes and their fake implementations
+    read none of them as a number. Two graphs at most (numbers, then symbols; or symbols, and again with layer_norm's eps as
+    a number), and one more for attention's short sequences."""
+    leaf = lambda *shape, dtype=torch.float32: torch.randn(shape).to(dtype).requires_grad_()  # noqa: E731
+    half = torch.bfloat16
+    rows = [(leaf(n, 5, 8), leaf(8), leaf(8)) for n in (4, 6, 9, 11, 700)]
+    assert _compiles(lambda x, w, b: policy.layer_norm(torch.sin(x), w, b).sum(), rows, dynamic) <= 2
+    packed = [(leaf(n, 4, 64, dtype=half), leaf(n + 1, 2, 64, dtype=half), torch.zeros(3, dtype=torch.int32))
+              for n in (4, 60, 900, 7, 11, 3000, 5000)]
+    assert _compiles(lambda q, k, a: policy.attention(q * 2, k, k, a).float().sum(), packed, dynamic) <= 3
+    worlds = [(torch.randn(n, 4, 64).bfloat16(), torch.randn(n, 9, 2, 64).bfloat16(), torch.zeros(n, dtype=torch.int32))
+              for n in (4, 60, 900, 7)]
+    assert _compiles(lambda q, k, n: policy.attention_step(q * 2, k, k, n), worlds, dynamic) <= 2
+    assert _compiles(lambda g: policy.clip_grads_([g], 0.5), [(torch.randn(n, 3),) for n in (4, 60, 900)], dynamic) <= 2
+
+
+def test_options_that_change_under_compile():
+    x, h = torch.randn(4, 8, requires_grad=True), torch.randn(4, 2, 8).bfloat16()
+    a = torch.zeros(2, dtype=torch.int32)
+    for dynamic in (None, True):
+        for call, at in ((lambda x, o: policy.layer_norm(torch.sin(x), eps=o).sum(), x),
+                         (lambda h, o: policy.attention(h * 2, h, h, a, scale=o), h), (lambda g, o: policy.clip_grads_([g], o), h)):
+            _compiles(call, [(at, o) for o in (0.1, 0.25, 0.5)], dynamic)
+
+
+def test_fake_order_is_the_librarys():
+    dll = torch_ffi.load_library()
+    for heads, kv in ((1, 1), (8, 2), (6, 2), (70, 1)):
+        for dim in (8, 64, 72, 128):
+            for seqs, tq, tk in ((0, 0, 0), (0, 5, 9), (1, 1, 1), (1, 300, 5000), (3, 96, 288), (3, 96, 289), (4096, 70001, 130000),
+                                 (1 << 20, 1 << 24, 1 << 27)):
+                want = dll.dk_attention_work_bytes(heads, kv, dim, seqs, tq, tk)
+                assert 4 * policy._order_words(heads // kv, dim, seqs, tq, tk) == want, (heads, kv, dim, seqs, tq, tk)
