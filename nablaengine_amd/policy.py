@@ -71,11 +71,14 @@ def _bind():
             raise _err(f"{TORCH_LIB} is missing: build it with `python -m nablaengine_amd.build`", RuntimeError)
         if not hasattr(torch.ops.nablaengine, "attention_step"):
             _define()
-        dll = torch_ffi._load().dll
+        native = torch_ffi._load()
         lib = ctypes.CDLL(TORCH_LIB)
         lib.dk_policy_torch_entries.restype, lib.dk_policy_torch_bind.restype = ctypes.c_char_p, None
         names = lib.dk_policy_torch_entries().decode().split()
-        entries = (ctypes.c_void_p * len(names))(*(ctypes.cast(getattr(dll, n), ctypes.c_void_p).value for n in names))
+        missing = [n for n in names if not hasattr(native.dll, n)]
+        if missing:
+            raise _err(f"{native.path} has no {missing[0]}: a build from before the policy operators", RuntimeError)
+        entries = (ctypes.c_void_p * len(names))(*(ctypes.cast(getattr(native.dll, n), ctypes.c_void_p).value for n in names))
         lib.dk_policy_torch_bind(entries)
         _bound.append(lib)
 

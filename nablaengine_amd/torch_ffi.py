@@ -105,7 +105,9 @@ _PROTOTYPES = {
     "dk_torch_diag_bwd": "i:ppi" + "p" * 6,
     "dk_prof_read": "i:pi",
     "dk_prof_read_adj": "i:pi",
-    # the policy operators (policy.py)
+}
+# the policy operators (policy.py): a library built before them runs the step all the same
+_POLICY_PROTOTYPES = {
     "dk_layer_norm": "i:pqiipqippfpp",
     "dk_layer_norm_vjp": "i:pqiipqpqi" + "p" * 6,
     "dk_layer_norm_work_bytes": "q:qii",
@@ -118,6 +120,7 @@ _PROTOTYPES = {
     "dk_attention_step": "i:piiiiii" + "pqq" + "pqqq" * 2 + "pfpp",
     "dk_attention_step_work_bytes": "q:iiiii",
 }
+_PROTOTYPES.update(_POLICY_PROTOTYPES)
 _CTYPE = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float, "q": ctypes.c_longlong, "-": None}
 
 
@@ -129,6 +132,8 @@ class _Native:
         self.path = path
         self.dll = ctypes.CDLL(path)
         for name, proto in _PROTOTYPES.items():
+            if name in _POLICY_PROTOTYPES and not hasattr(self.dll, name):
+                continue
             result, args = proto.split(":")
             entry = getattr(self.dll, name)
             entry.restype = _CTYPE[result]

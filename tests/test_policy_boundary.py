@@ -4,6 +4,8 @@ implementations give the library's output shapes and types."""
 import ctypes
 import os
 import re
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -220,3 +222,18 @@ def test_fake_order_is_the_librarys():
                                  (1 << 20, 1 << 24, 1 << 27)):
                 want = dll.dk_attention_work_bytes(heads, kv, dim, seqs, tq, tk)
                 assert 4 * policy._order_words(heads // kv, dim, seqs, tq, tk) == want, (heads, kv, dim, seqs, tq, tk)
+
+
+def test_a_library_without_the_policy_entries(tmp_path):
+    """A library built before these operators still runs the step; the operators raise RuntimeError."""
+    step = [n for n in torch_ffi._PROTOTYPES if n not in _prototypes()]
+    (tmp_path / "old.c").write_text("".join(f"void {n}(void) {{}}\n" for n in step))
+    lib = tmp_path / "old.so"
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", lib, tmp_path / "old.c"], check=True)
+    code = ("import pytest, torch\n"
+            "from nablaengine_amd import policy, torch_ffi\n"
+            "assert torch_ffi.load_library().dk_fwd_forward and torch_ffi.rec_words() == 0\n"
+            "for call in (lambda: policy.layer_norm(torch.zeros(2, 3)), lambda: policy.grad_norm([torch.zeros(3)])):\n"
+            "    with pytest.raises(RuntimeError, match='before the policy operators'):\n"
+            "        call()\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT, env={**os.environ, "DK_TORCH_ARTIFACT": str(lib)})
