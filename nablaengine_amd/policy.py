@@ -16,7 +16,8 @@ Conventions are torch_ffi's: tensors lie on one ROCm device and are never cast, 
 device is a TypeError, a bad option a ValueError, a failed library call a RuntimeError; there is no CPU path. Calls only
 launch kernels on the device's current stream and take memory from torch's caching allocator: nothing synchronizes, so
 they may be captured in a HIP graph, and each is an operator of the ``nablaengine`` namespace with a fake
-implementation, which torch.compile keeps as one node. A tensor made on another stream than the call's is the caller's
+implementation, which torch.compile keeps as one node (torch_ffi.init() first, as for the step: a trace cannot load the
+library). A tensor made on another stream than the call's is the caller's
 to synchronize and to keep alive (Tensor.record_stream), as with torch's own operators. Results are bitwise the same on
 every run. Gradients are first order only.
 """
@@ -234,5 +235,15 @@ def attention_step(q, k, v, lengths, *, scale=None):
     return _ops().attention_step(q, _tensor("k", k), _tensor("v", v), _tensor("lengths", lengths), _scale(scale, q))
 
 
+def _bind_loaded():
+    try:
+        _bind()
+    except Exception:  # a library without the operators: their first call says so, and the step needs none of them
+        pass
+
+
 if os.path.exists(TORCH_LIB):
-    _define()  # at import: defining operators inside a torch.compile trace is not traceable
+    _define()  # at import: defining operators inside a torch.compile trace is not traceable, nor is binding them
+    torch_ffi._on_load.append(_bind_loaded)
+    if torch_ffi._native is not None:
+        _bind_loaded()

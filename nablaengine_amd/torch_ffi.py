@@ -152,6 +152,7 @@ class _Native:
 
 _lock = threading.RLock()
 _native: Optional[_Native] = None
+_on_load = []  # called once the library is loaded: policy.py's operators take their entries then
 _counters = {}  # device index -> int64 (len(DIAG),) tensor; a device is ready once it has one
 _settings = {"count": True, "warn": os.environ.get("DK_OVERFLOW_WARN", "0") not in ("", "0")}
 
@@ -179,6 +180,8 @@ def _load(artifact=None):
             if not os.path.exists(path):
                 raise _err(f"{path} is missing: build it with `python -m nablaengine_amd.build`", RuntimeError)
             _native = _Native(path)
+            for ready in _on_load:
+                ready()
         elif artifact is not None and os.path.realpath(library_path(artifact)) != os.path.realpath(_native.path):
             raise _err(f"{_native.path} is loaded already: one library per process", RuntimeError)
         return _native

@@ -237,3 +237,16 @@ def test_a_library_without_the_policy_entries(tmp_path):
             "    with pytest.raises(RuntimeError, match='before the policy operators'):\n"
             "        call()\n")
     subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT, env={**os.environ, "DK_TORCH_ARTIFACT": str(lib)})
+
+
+@pytest.mark.parametrize("order", ["policy, torch_ffi\ntorch_ffi.load_library()", "torch_ffi\ntorch_ffi.load_library()\n"
+                                   "from nablaengine_amd import policy"])
+def test_ready_with_the_library(order):
+    """The operators are ready once the library is loaded, before or after their module: the first call may be a compiled
+    one, or one by the operator's name."""
+    code = (f"import pytest, torch\nfrom nablaengine_amd import {order}\n"
+            "f = torch.compile(lambda x: policy.layer_norm(x) * 2, fullgraph=True, backend='aot_eager')\n"
+            "with pytest.raises(TypeError, match='ROCm device'):\n"
+            "    f(torch.zeros(2, 3))\n"
+            "assert policy._bound\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT)
