@@ -37,7 +37,8 @@ long long dk_clip_work_bytes(int count);
 /* Causal attention over packed sequences. q (tq, heads, dim), k, v (tk, kv_heads, dim) in type 1 or 2, rows of dim
  * elements contiguous, q_t / q_h (...) elements from token to token and from head to head; heads a multiple of
  * kv_heads, query head i reading key/value head i / (heads / kv_heads); dim a multiple of 8, at most 128; tq * (heads /
- * kv_heads) and tk below 2^30. starts_q, starts_k: seqs + 1 int32 on the device, 0 first: sequence s has the tokens
+ * kv_heads) and tk below 2^30, and (tq * (heads / kv_heads) / 128 + seqs) * kv_heads and (tk / 32 + seqs) * kv_heads a little
+ * below 2^22 (a launch's work-items). starts_q, starts_k: seqs + 1 int32 on the device, 0 first: sequence s has the tokens
  * starts[s] .. starts[s + 1] - 1. Query i of a sequence of nq queries and nk keys sees its keys 0 .. i + nk - nq; one
  * that sees none gives zeros, as do tokens past the last sequence. out (tq, heads, dim) contiguous; lse (heads, tq)
  * float32 for the backward, or NULL; work: dk_attention_work_bytes bytes, which the backward reads again; scratch:

@@ -10,6 +10,7 @@
 // the row-major LDS tile with ds_read_b64_tr_b16, which gives each lane four consecutive rows of its column.
 #pragma once
 #include "policy_device.h"
+#include "policy_sizes.h"
 
 namespace pol {
 
@@ -26,7 +27,6 @@ __device__ __forceinline__ F16x mfma(V8<_Float16> a, V8<_Float16> b, F16x c) {
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int QROWS = 128;  // query rows a workgroup: 32 a wave
 // log2: by how much the subtracted maximum may lag behind the true one, and what probabilities are lifted by before they are
 // rounded. float16 holds 2^-24 to 2^16: lifted by 2^11 those down to 2^-36 of the largest stay, so that the many small ones of
 // a long history are not lost beside a large one (up to 2^24 keys they then miss less than half a rounding of the result).
@@ -60,16 +60,10 @@ struct Attend {
 // the other side that each one reads: over all tiles, or over sequences, each one's tiles one after another (by_sequence).
 // Workgroups go to the XCDs in turn, and each XCD has an L2 cache of its own: in the second case WINDOW neighbours of the
 // list go to one XCD, so that a sequence's tiles find what they share in one cache; in the first a list's neighbours are
-// tiles of different sequences and heads anyway.
+// tiles of different sequences and heads anyway. order_queries() and order_keys() are the lists' lengths at most.
 constexpr int WINDOW = 64, XCDS = 8;
 constexpr int LONG = 1792;  // tokens a sequence, in the mean: above it single tiles are ordered
 constexpr int ORDER_HEAD = 16;  // ints before the lists: their lengths
-__host__ __device__ inline long long order_queries(int seqs, int tq, int group) {
-  return (long long)tq * group / QROWS + seqs + 1;
-}
-__host__ __device__ inline long long order_keys(int seqs, int tk, int key_waves) {
-  return (long long)tk / (32 * key_waves) + seqs + 1;
-}
 
 // A tile's loop over `tiles` tiles of the other side, split among `parts` workgroups (at least LEAST each): this one's.
 constexpr int LEAST = 4;

@@ -985,13 +985,9 @@ int launch_attend_vjp(hipStream_t st, int type, const Attend& a) {
 }  // namespace pol
 
 namespace {
-// whether the kernels and their grids hold these sizes
 bool attention_takes(int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk) {
-  if ((type != pol::BF16 && type != pol::F16) || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 8 || dim > 128 ||
-      dim % 8 || seqs < 0 || tq < 0 || tk < 0 || tk >= 1 << 30 || (long long)tq * (heads / kv_heads) >= 1 << 30)
-    return false;
-  const long long most = (1LL << 22) - 1024;  // workgroups of 256 or 512 work-items a launch
-  return pol::order_queries(seqs, tq, heads / kv_heads) * kv_heads <= most && pol::order_keys(seqs, tk, 1) * kv_heads <= most;
+  return (type == pol::BF16 || type == pol::F16) && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && dim >= 8 &&
+         dim <= 128 && dim % 8 == 0 && pol::attention_sizes(heads, kv_heads, seqs, tq, tk);
 }
 }  // namespace
 

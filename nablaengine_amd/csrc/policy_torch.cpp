@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "../../include/nablaengine_policy.h"
+#include "policy_sizes.h"
 
 namespace {
 
@@ -270,9 +271,9 @@ int sequences_checks(const Tensor& q, const Tensor& k, const Tensor& starts_q, c
                    x.numel() == starts_q.numel(),
                name, ": expected contiguous int32 offsets, one more than sequences in both, got ", described(x));
   }
-  const int64_t seqs = starts_q.numel() - 1, rows = q.size(0) * (h.heads / h.kv);
-  CHECK_VALUE(rows < 1 << 30 && k.size(0) < 1 << 30 &&
-                  (std::max(rows, k.size(0)) / 128 + seqs + 1) * h.kv < 1 << 24,
+  const int64_t seqs = starts_q.numel() - 1, most = 1 << 30;
+  CHECK_VALUE(q.size(0) < most && k.size(0) < most && seqs < most &&
+                  pol::attention_sizes(h.heads, h.kv, (int)seqs, (int)q.size(0), (int)k.size(0)),
               q.size(0), " queries of ", h.heads, " heads and ", k.size(0), " keys of ", h.kv, " in ", seqs,
               " sequences exceed one launch");
   return (int)seqs;

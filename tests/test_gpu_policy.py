@@ -744,6 +744,24 @@ def test_attention_refusals():
             policy.attention(q, k, v, a, scale=scale)
 
 
+def test_attention_sizes_past_one_launch():
+    """ValueError, before anything is allocated, for each of the limits (strides of 0: the tensors are small)."""
+    def of(tq, tk, kv, seqs, heads=None):
+        q, k = (torch.zeros((1, 1, 8), dtype=BF16, device="cuda").expand(n, h, 8) for n, h in ((tq, heads or kv), (tk, kv)))
+        a = torch.zeros(seqs + 1, dtype=torch.int32, device="cuda")
+        before = torch.cuda.memory_allocated()
+        with pytest.raises(ValueError, match="exceed one launch"):
+            policy.attention(q, k, k, a)
+        assert torch.cuda.memory_allocated() == before
+    of(8, 2 ** 27, 1, 1)
+    of(8, 2 ** 24, 8, 1)
+    of(8, 8, 1, 2 ** 22)
+    of(2 ** 29, 8, 1, 1)
+    of(2 ** 28, 8, 1, 1, heads=4)
+    of(8, 2 ** 30, 1, 1)
+    of(2 ** 32 + 5, 8, 1, 1)
+
+
 # ---- one new token --------------------------------------------------------------------------------------------------
 
 def check_step(q, k, v, lengths, scale=None):
