@@ -49,6 +49,9 @@ def build_torch(verbose=False):
         os.unlink(tmp)
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError(f"g++ failed ({r.returncode})")
+    mask = os.umask(0)  # the temporary file is its owner's alone, and g++ keeps that
+    os.umask(mask)
+    os.chmod(tmp, 0o777 & ~mask)
     os.replace(tmp, TORCH_LIB)
     return TORCH_LIB
 

@@ -250,3 +250,9 @@ def test_ready_with_the_library(order):
             "    f(torch.zeros(2, 3))\n"
             "assert policy._bound\n")
     subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT)
+
+
+def test_both_libraries_are_readable_alike():
+    """What one user builds another may load: the torch side has the kernels' library's permissions."""
+    mode = lambda path: os.stat(path).st_mode & 0o555  # noqa: E731
+    assert mode(policy.TORCH_LIB) == mode(torch_ffi.LIB_PATH)
