@@ -991,6 +991,20 @@ def test_operators_compiled_over_sizes():
             assert torch.equal(e, c), (rows, i)
 
 
+def test_gradients_in_a_graph_of_gradients():
+    """Under create_graph the gradients are those without it, and differentiating them again raises."""
+    x, w, b, dy = rand((40, 99), F32, 1), rand((99,), F32, 2), rand((99,), F32, 3), rand((40, 99), F32, 4)
+    q, k, v = (rand((90, n, 64), BF16, n) for n in (4, 2, 2))
+    a, dout = starts([20, 70]), rand((90, 4, 64), BF16, 9)
+    for call, at, cot in ((policy.layer_norm, (x, w, b), dy), (lambda *t: policy.attention(*t, a), (q, k, v), dout)):
+        leaves = [t.detach().requires_grad_() for t in at]
+        want = torch.autograd.grad(call(*leaves), leaves, cot)
+        got = torch.autograd.grad(call(*leaves), leaves, cot, create_graph=True)
+        assert all(torch.equal(p, r) and r.requires_grad and not p.requires_grad for p, r in zip(want, got))
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            sum(g.float().square().sum() for g in got).backward()
+
+
 def test_clipping_marks_what_it_writes():
     """A graph that saved a tensor which clipping then overwrites notices."""
     w = rand((8,), F32, 1).requires_grad_()
