@@ -1,0 +1,35 @@
+/* C ABI of the operators of policies with a longer memory in libnablaengine_g1.so (no counterpart in the reference): a gated
+ * linear recurrence. The conventions are nablaengine_policy.h's. */
+#ifndef NABLAENGINE_MEMORY_H
+#define NABLAENGINE_MEMORY_H
+#include <hip/hip_runtime_api.h>
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* The recurrence h_t = a_t h_{t-1} + (1 - a_t) x_t, a = 1 / (1 + exp(-gate)), of each channel over packed sequences. x, gate:
+ * (tokens, channels), x_t and gate_t elements from token to token; starts: seqs + 1 int32 on the device, 0 first: sequence s has
+ * the tokens starts[s] .. starts[s + 1] - 1, not falling (offsets outside the tokens are moved inside them). initial: (seqs,
+ * channels) float32, the states before the first tokens, or NULL for zeros. h (tokens, channels) contiguous, zeros behind the
+ * last sequence; last (seqs, channels) float32, the states after the last tokens (of a sequence without tokens: its initial one).
+ * carry: dk_recurrence_carry_bytes bytes, which the backward reads again; work: dk_recurrence_work_bytes bytes (vjp 0); both
+ * NULL when 0. channels >= 1; a launch's work-items bound (tokens / 128) (channels / 64) by a little below 2^23. */
+int dk_recurrence(hipStream_t st, int type, int tokens, int channels, int seqs, const void* x, long long x_t, const void* gate,
+                  long long gate_t, const int* starts, const float* initial, void* h, float* last, float* carry, void* work);
+/* Its VJP, from the forward's arguments and carry: dh (type, dh_t elements from token to token) and dlast (seqs, channels)
+ * float32, each NULL for zeros -> dx, dgate (tokens, channels) contiguous, dinitial (seqs, channels) float32, each NULL where not
+ * wanted. work: dk_recurrence_work_bytes bytes (vjp 1). */
+int dk_recurrence_vjp(hipStream_t st, int type, int tokens, int channels, int seqs, const void* x, long long x_t,
+                      const void* gate, long long gate_t, const int* starts, const float* initial, const float* carry,
+                      const void* dh, long long dh_t, const float* dlast, void* dx, void* dgate, float* dinitial, void* work);
+long long dk_recurrence_carry_bytes(int tokens, int channels);
+long long dk_recurrence_work_bytes(int tokens, int channels, int vjp);
+/* One token of every world: next = a state + (1 - a) x, float32, and h, its value in `type`; x, gate, state: (worlds, channels),
+ * x_w, gate_w, state_w elements from world to world; h, next contiguous. next may be state where that is contiguous. */
+int dk_recurrence_step(hipStream_t st, int type, long long worlds, int channels, const void* x, long long x_w, const void* gate,
+                       long long gate_w, const float* state, long long state_w, void* h, float* next);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

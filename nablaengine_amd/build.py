@@ -1,5 +1,5 @@
 """Build the HIP library libnablaengine_g1.so in-tree for gfx950 (hipcc; one shared library, the C ABI of
-include/nablaengine_g1.h and nablaengine_policy.h), and beside it the policy operators' torch side (g++).
+include/nablaengine_g1.h, nablaengine_policy.h and nablaengine_memory.h), and beside it the policy operators' torch side (g++).
 `python -m nablaengine_amd.build`."""
 import concurrent.futures
 import os
@@ -11,9 +11,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libnablaengine_g1.so")
 PROF_LIB = os.path.join(HERE, "libnablaengine_g1_prof.so")
-TORCH_LIB, TORCH_SOURCE = os.path.join(HERE, "libnablaengine_policy_torch.so"), "policy_torch.cpp"
+TORCH_LIB, TORCH_SOURCES = os.path.join(HERE, "libnablaengine_policy_torch.so"), ["policy_torch.cpp", "policy_memory_torch.cpp"]
 SOURCES = ["g1_forward.hip", "g1_adjoint.hip", "g1_order.hip", "g1_kinematics.hip", "g1_diag.hip", "g1_capi.hip",
-           "policy_norm.hip", "policy_clip.hip", "policy_attend.hip", "policy_step.hip"]
+           "policy_norm.hip", "policy_clip.hip", "policy_attend.hip", "policy_step.hip",
+           "policy_scan.hip"]
 ARCH = os.environ.get("NABLA_OFFLOAD_ARCH", "gfx950")
 # packed FP32 instructions off (-packed-fp32-ops): the kernels are written for scalar FP32. Warnings that mark
 # undefined behaviour the optimizer exploits (a non-void function falling off its end becomes unreachable code, and a
@@ -38,17 +39,23 @@ def build_torch(verbose=False):
     from torch.utils.cpp_extension import include_paths
     fd, tmp = tempfile.mkstemp(prefix="libnablaengine_policy_torch.", suffix=".so.tmp", dir=HERE)
     os.close(fd)
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-Wall", "-Wno-sign-compare"]
-    cmd += [f"-I{p}" for p in include_paths()] + ["-I/opt/rocm/include", "-o", tmp, os.path.join(CSRC, TORCH_SOURCE)]
-    cmd += [f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}", "-lc10", "-ltorch_cpu", "-lc10_hip", "-lamdhip64"]
-    if verbose:
-        print(" ".join(cmd))
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
+    flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-Wall", "-Wno-sign-compare"]
+    flags += [f"-I{p}" for p in include_paths()] + ["-I/opt/rocm/include"]
+    with tempfile.TemporaryDirectory() as objects, concurrent.futures.ThreadPoolExecutor(2) as pool:
+        def run(cmd):
+            if verbose:
+                print(" ".join(cmd))
+            return subprocess.run(cmd, capture_output=True, text=True)
+        objs = [os.path.join(objects, source + ".o") for source in TORCH_SOURCES]
+        runs = list(pool.map(lambda o, s: run(["g++", *flags, "-c", "-o", o, os.path.join(CSRC, s)]), objs, TORCH_SOURCES))
+        if all(r.returncode == 0 for r in runs):
+            runs.append(run(["g++", "-shared", "-o", tmp, *objs, f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}",
+                             "-lc10", "-ltorch_cpu", "-lc10_hip", "-L/opt/rocm/lib", "-lamdhip64"]))
+    if any(r.returncode for r in runs):
         os.unlink(tmp)
-        sys.stderr.write(r.stdout + r.stderr)
-        raise RuntimeError(f"g++ failed ({r.returncode})")
+        sys.stderr.write("".join(r.stdout + r.stderr for r in runs if r.returncode))
+        raise RuntimeError(f"g++ failed ({[r.returncode for r in runs]})")
     mask = os.umask(0)  # the temporary file is its owner's alone, and g++ keeps that
     os.umask(mask)
     os.chmod(tmp, 0o777 & ~mask)

@@ -1,4 +1,4 @@
-// The attention's sizes, for its kernels and for the checks of whoever calls them (no device code).
+// The attention's and the recurrence's sizes, for their kernels and for the checks of whoever calls them (no device code).
 #pragma once
 
 namespace pol {
@@ -15,6 +15,14 @@ constexpr bool attention_sizes(int heads, int kv_heads, int seqs, int tq, int tk
   const long long most = (1LL << 22) - 1024;  // workgroups of 256 or 512 work-items a launch
   return seqs >= 0 && tq >= 0 && tk >= 0 && tk < 1 << 30 && (long long)tq * group < 1 << 30 &&
          order_queries(seqs, tq, group) * kv_heads <= most && order_keys(seqs, tk, 1) * kv_heads <= most;
+}
+
+constexpr int SCAN_TOKENS = 16, SCAN_CHUNK = 128;  // the recurrence's tokens a wave and a workgroup
+
+// whether the recurrence's indices and grids hold these sizes: workgroups of 512 work-items, one a chunk and 64 channels at least
+constexpr bool scan_sizes(int tokens, int channels, int seqs) {
+  return tokens >= 0 && tokens < 0x7fffffff - 2 * SCAN_CHUNK && channels >= 1 && channels < 1 << 30 && seqs >= 0 &&
+         seqs < 1 << 30 && ((long long)tokens / SCAN_CHUNK + 1) * ((long long)channels / 64 + 1) <= (1LL << 23) - 1024;
 }
 
 }  // namespace pol

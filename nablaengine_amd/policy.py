@@ -48,12 +48,16 @@ def _tensor(name, x):
 # ---- the operators (csrc/policy_torch.cpp defines them, with their autograd nodes) ------------------------------------
 
 _bound = []  # the operators' library, once it has the kernels' entries
+_later = []  # those of the operators from recurrence on that the kernels' library does not have
 
 
-def _ops():
-    """torch.ops.nablaengine with this module's operators, bound to the kernels' library (torch_ffi's, one a process)."""
+def _ops(later=False):
+    """torch.ops.nablaengine with this module's operators, bound to the kernels' library (torch_ffi's, one a process);
+    later: for one of the operators from recurrence on."""
     if not _bound:
         _bind()
+    if later and _later:
+        raise _err(f"{torch_ffi._load().path} has no {_later[0]}: a build from before this operator", RuntimeError)
     return torch.ops.nablaengine
 
 
@@ -74,14 +78,21 @@ def _bind():
             _define()
         native = torch_ffi._load()
         lib = ctypes.CDLL(TORCH_LIB)
-        lib.dk_policy_torch_entries.restype, lib.dk_policy_torch_bind.restype = ctypes.c_char_p, None
-        names = lib.dk_policy_torch_entries().decode().split()
-        missing = [n for n in names if not hasattr(native.dll, n)]
+        missing = _hand_over(native, lib.dk_policy_torch_entries, lib.dk_policy_torch_bind)
         if missing:
             raise _err(f"{native.path} has no {missing[0]}: a build from before the policy operators", RuntimeError)
-        entries = (ctypes.c_void_p * len(names))(*(ctypes.cast(getattr(native.dll, n), ctypes.c_void_p).value for n in names))
-        lib.dk_policy_torch_bind(entries)
+        _later[:] = _hand_over(native, lib.dk_memory_torch_entries, lib.dk_memory_torch_bind)
         _bound.append(lib)
+
+
+def _hand_over(native, entries, bind):
+    """Give the operators the addresses of their entries, or return those that the kernels' library does not have."""
+    entries.restype, bind.restype = ctypes.c_char_p, None
+    names = entries().decode().split()
+    missing = [n for n in names if not hasattr(native.dll, n)]
+    if not missing:
+        bind((ctypes.c_void_p * len(names))(*(ctypes.cast(getattr(native.dll, n), ctypes.c_void_p).value for n in names)))
+    return missing
 
 
 def _fake_layer_norm_forward(x, weight, bias, eps, stats):
@@ -112,12 +123,34 @@ def _fake_attention_forward(q, k, v, starts_q, starts_k, scale, train):
             starts_q.new_empty((words,))]
 
 
+def _fake_recurrence(x, gate, starts, initial):
+    return x.new_empty(x.shape), x.new_empty((starts.shape[0] - 1, x.shape[1]), dtype=torch.float32)
+
+
+def _carry_words(tokens, channels):
+    """dk_recurrence_carry_bytes / 4, of symbolic sizes too: a row for each chunk of 128 tokens."""
+    return (tokens + 127) // 128 * channels
+
+
+def _fake_recurrence_forward(x, gate, starts, initial):
+    return [*_fake_recurrence(x, gate, starts, initial), x.new_empty((_carry_words(*x.shape),), dtype=torch.float32)]
+
+
+def _fake_recurrence_backward(dh, dlast, x, gate, starts, initial, carry, want_x, want_gate, want_initial):
+    seqs = starts.shape[0] - 1
+    return [x.new_empty(x.shape if want else (0,)) for want in (want_x, want_gate)] + [
+        x.new_empty((seqs, x.shape[1]) if want_initial else (0,), dtype=torch.float32)]
+
+
 _FAKES = {"layer_norm": lambda x, *_: x.new_empty(x.shape), "layer_norm_forward": _fake_layer_norm_forward,
           "layer_norm_backward": _fake_layer_norm_backward, "grad_norm": _fake_norm, "clip_grads_": _fake_norm,
           "clip_grads_out": _fake_norm, "attention": lambda q, *_: q.new_empty(q.shape),
           "attention_forward": _fake_attention_forward,
           "attention_backward": lambda dout, q, k, v, *_: [q.new_empty(x.shape) for x in (q, k, v)],
-          "attention_step": lambda q, *_: q.new_empty(q.shape)}
+          "attention_step": lambda q, *_: q.new_empty(q.shape),
+          "recurrence": _fake_recurrence, "recurrence_forward": _fake_recurrence_forward,
+          "recurrence_backward": _fake_recurrence_backward,
+          "recurrence_step": lambda x, gate, state: (x.new_empty(x.shape), state.new_empty(x.shape))}
 
 
 # ---- layer norm -----------------------------------------------------------------------------------------------------
@@ -234,6 +267,34 @@ def attention_step(q, k, v, lengths, *, scale=None):
     if _wants_grad(q, k, v):
         raise _err("attention_step has no gradient: use attention (one query a sequence), or torch.no_grad()", RuntimeError)
     return _ops().attention_step(q, _tensor("k", k), _tensor("v", v), _tensor("lengths", lengths), _scale(scale, q))
+
+
+# ---- recurrence -----------------------------------------------------------------------------------------------------
+
+def recurrence(x, gate, starts, initial=None):
+    """A gated linear recurrence over packed sequences (episodes of different lengths, one after another): h_t = a_t h_{t-1} +
+    (1 - a_t) x_t with a = sigmoid(gate), a channel at a time, differentiable in x, gate and initial. Returns h and each
+    sequence's state after its last token, to be carried on.
+
+    x, gate: (tokens, channels), float32, bfloat16 or float16, each token's elements neighbours, tokens any distance apart
+    (slices of one projection's output; a gate of one row for all, expanded). starts: int32 offsets on the device, 0 first, not
+    falling, sequence s being tokens starts[s] .. starts[s + 1] - 1. initial: (sequences, channels) float32, the states before
+    the first tokens, or None for zeros. h has x's type and is zero behind the last sequence (padding, whose gradients are zero
+    too); the last states are float32, those of sequences without tokens their initial ones.
+
+    The gate is given before its sigmoid, since 16 bits do not tell long memories apart after it: 1 - a keeps its own last
+    places for every a. States and all sums are float32 and each output is rounded once. Infinities and NaN stay in their
+    channel and sequence."""
+    return _ops(True).recurrence(_tensor("x", x), _tensor("gate", gate), _tensor("starts", starts), initial)
+
+
+def recurrence_step(x, gate, state):
+    """One token of every world: (h, next state) with next = a state + (1 - a) x, a = sigmoid(gate), float32 as state is, and h
+    its value in x's type; without gradients. x, gate, state: (worlds, channels), rows any distance apart. The control loop's
+    form of recurrence."""
+    if _wants_grad(x, gate, state):
+        raise _err("recurrence_step has no gradient: use recurrence (one token a sequence), or torch.no_grad()", RuntimeError)
+    return _ops(True).recurrence_step(_tensor("x", x), _tensor("gate", gate), _tensor("state", state))
 
 
 def _bind_loaded():

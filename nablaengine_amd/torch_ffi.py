@@ -120,7 +120,16 @@ _POLICY_PROTOTYPES = {
     "dk_attention_step": "i:piiiiii" + "pqq" + "pqqq" * 2 + "pfpp",
     "dk_attention_step_work_bytes": "q:iiiii",
 }
-_PROTOTYPES.update(_POLICY_PROTOTYPES)
+# those of policies with a longer memory, in the same way
+_MEMORY_PROTOTYPES = {
+    "dk_recurrence": "i:piiii" + "pq" * 2 + "pppppp",
+    "dk_recurrence_vjp": "i:piiii" + "pq" * 2 + "ppp" + "pq" + "ppppp",
+    "dk_recurrence_carry_bytes": "q:ii",
+    "dk_recurrence_work_bytes": "q:iii",
+    "dk_recurrence_step": "i:piqi" + "pq" * 3 + "pp",
+}
+_OPTIONAL = {**_POLICY_PROTOTYPES, **_MEMORY_PROTOTYPES}
+_PROTOTYPES.update(_OPTIONAL)
 _CTYPE = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float, "q": ctypes.c_longlong, "-": None}
 
 
@@ -132,7 +141,7 @@ class _Native:
         self.path = path
         self.dll = ctypes.CDLL(path)
         for name, proto in _PROTOTYPES.items():
-            if name in _POLICY_PROTOTYPES and not hasattr(self.dll, name):
+            if name in _OPTIONAL and not hasattr(self.dll, name):
                 continue
             result, args = proto.split(":")
             entry = getattr(self.dll, name)

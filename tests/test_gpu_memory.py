@@ -1,0 +1,375 @@
+"""The operators of policies with a longer memory on a GPU against their definitions in float64, at the sizes, strides and
+masks where they can go wrong. Tolerances follow from the operators' roundings: U[type] is half a unit in the last place
+relative to the value (2^-24, 2^-8, 2^-11), and an output is rounded once; SUM = 64 2^-24 stands for float32 sums as in the
+other policy operators' tests; what else an operator rounds is derived beside its check."""
+import math
+
+import pytest
+import torch
+
+from nablaengine_amd import policy
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+U = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}
+SUM = 64 * 2.0 ** -24
+TINY = {F32: 1e-37, BF16: 1e-37, F16: 2.0 ** -24}  # a value rounded to the type's smallest steps
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.fail("no GPU visible")
+
+
+def rand(shape, dtype=F32, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda", dtype=torch.float64) * scale).to(dtype)
+
+
+def within(name, got, want, bound):
+    got, want, bound = got.double().cpu(), want.double().cpu(), bound.double().cpu()
+    assert got.shape == want.shape, name
+    assert torch.isfinite(got).all(), f"{name}: not finite"
+    over = (got - want).abs() - bound
+    assert (over <= 0).all(), f"{name}: {int((over > 0).sum())} values off, the worst {over.max().item():.3g} over its bound"
+
+
+def starts(lengths):
+    return torch.tensor([0] + list(lengths), dtype=torch.int64).cumsum(0).to(torch.int32).cuda()
+
+
+# ---- recurrence -----------------------------------------------------------------------------------------------------
+
+# What a gate's sigmoid is off by, relative to it: the exponential's argument is rounded, |gate| 2^-24 of the result (|gate| < 16
+# here: 2^-20), the exponential, the sum, the reciprocal and the product by 2^-23, 2^-24, 2^-23 and 2^-24; twice that leaves room for
+# the rounding of each step's product and sum.
+GATE = 2.0 ** -19
+
+
+def recur64(x, f, lengths, initial, dh=None, dlast=None):
+    """The definition step by step in float64 on the CPU, with each output's bound: magnitudes (m: the same sums of absolute
+    values) and errors (e) run along, each step's product off by GATE of its magnitude."""
+    dtype, (n, c) = x.dtype, x.shape
+    x, f = x.detach().double().cpu(), f.detach().double().cpu()
+    keep, take = torch.sigmoid(f), torch.sigmoid(-f)
+    r = {"h": torch.zeros(n, c), "last": torch.zeros(len(lengths), c)}
+    if dh is not None:
+        r.update(dx=torch.zeros(n, c), dgate=torch.zeros(n, c), dinitial=torch.zeros(len(lengths), c))
+        dh, dlast = dh.double().cpu(), dlast.double().cpu()
+    r = {k: [v.double(), v.double()] for k, v in r.items()}
+    u, tiny = U[dtype], TINY[dtype]
+
+    def put(name, at, value, error, rounding=u, least=tiny):
+        r[name][0][at], r[name][1][at] = value, error + rounding * value.abs() + least
+    t = 0
+    for s, length in enumerate(lengths):
+        h = torch.zeros(c, dtype=torch.float64) if initial is None else initial[s].detach().double().cpu()
+        m, e, before = h.abs(), torch.zeros(c, dtype=torch.float64), []
+        for i in range(t, t + length):
+            before.append((h, m, e))
+            h = keep[i] * h + take[i] * x[i]
+            e = keep[i] * (e + GATE * m) + GATE * take[i] * x[i].abs()
+            m = keep[i] * m + take[i] * x[i].abs()
+            put("h", i, h, e)
+        put("last", s, h, e, U[F32], TINY[F32])
+        if dh is not None:
+            g = dlast[s].clone()
+            m, e = g.abs(), torch.zeros(c, dtype=torch.float64)
+            for i in range(t + length - 1, t - 1, -1):
+                g, m = g + dh[i], m + dh[i].abs()
+                e = e + U[F32] * m
+                h0, m0, e0 = before[i - t]
+                put("dx", i, take[i] * g, take[i] * (e + GATE * m))
+                d = keep[i] * take[i]
+                put("dgate", i, g * (h0 - x[i]) * d, d * ((e + 3 * GATE * m) * (m0 + x[i].abs()) + m * e0))
+                g, m, e = keep[i] * g, keep[i] * m, keep[i] * (e + GATE * m)
+            put("dinitial", s, g, e, U[F32], TINY[F32])
+        t += length
+    return {k: tuple(v) for k, v in r.items()}
+
+
+def check_recurrence(x, f, lengths, initial=None, a=None):
+    a = starts(lengths) if a is None else a
+    leaves = [t.detach().requires_grad_() for t in (x, f)] + ([initial.detach().requires_grad_()] if initial is not None else [])
+    h, last = policy.recurrence(leaves[0], leaves[1], a, leaves[2] if initial is not None else None)
+    dh, dlast = rand(x.shape, x.dtype, 91), rand((len(lengths), x.shape[1]), F32, 92)
+    grads = torch.autograd.grad((h, last), leaves, (dh, dlast))
+    with torch.no_grad():
+        again = policy.recurrence(x, f, a, initial)
+    assert torch.equal(h, again[0]) and torch.equal(last, again[1])
+    want = recur64(x, f, lengths, initial, dh, dlast)
+    got = dict(zip(("h", "last", "dx", "dgate", "dinitial"), (h, last, *grads)))
+    for name, t in got.items():
+        within(name, t.detach(), *want[name])
+    return got
+
+
+def gated(n, c, dtype, seed=1, mean=1.5):
+    return rand((n, c), dtype, seed), (rand((n, c), F32, seed + 1, 2.0) + mean).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("channels", [1, 2, 3, 7, 63, 64, 65, 127, 128, 129, 130, 257])
+def test_recurrence_channels(dtype, channels):
+    print("recurrence", dtype, channels, flush=True)
+    lengths = [1, 33, 0, 70, 200, 5]
+    x, f = gated(sum(lengths), channels, dtype, channels)
+    check_recurrence(x, f, lengths, rand((len(lengths), channels), F32, 3))
+    check_recurrence(x, f, lengths)
+
+
+@pytest.mark.parametrize("lengths", [[1], [0], [], [15], [16], [17], [127], [128], [129], [1, 127], [127, 1, 128], [128, 128], [16] * 20,
+                                     [300], [1] * 300, [0, 5, 0, 0, 7, 0], [0] * 40, [1000], [200, 0, 1, 900, 31, 32, 33], [5000]])
+def test_recurrence_lengths(lengths):
+    """One token to many chunks, sequences that end and start on the edges of stretches and chunks, several in one stretch,
+    and those without tokens."""
+    print("recurrence lengths", lengths[:6], len(lengths), flush=True)
+    for dtype, c, mean in ((F32, 70, 1.5), (BF16, 130, 4.0)):
+        x, f = gated(sum(lengths), c, dtype, len(lengths), mean)
+        check_recurrence(x, f, lengths, rand((len(lengths), c), F32, 3))
+
+
+def test_recurrence_long_memory_over_many_chunks():
+    """More chunks than runs of the kernel that carries states over them, and gates whose states last for thousands of
+    steps."""
+    print("recurrence many chunks", flush=True)
+    for lengths in ([20000], [9000, 3, 12000]):
+        x, f = gated(sum(lengths), 5, F32, 1, 9.0)
+        check_recurrence(x, f, lengths, rand((len(lengths), 5), F32, 3))
+
+
+@pytest.mark.parametrize("seqs", [511, 512, 513, 3000, 300000])
+def test_recurrence_many_sequences(seqs):
+    """More sequences than a workgroup reads offsets of at once, and than two such reads find; half of them without tokens.
+    Sequences of one token: h = a initial + (1 - a) x."""
+    print("recurrence many sequences", seqs, flush=True)
+    g = torch.Generator().manual_seed(seqs)
+    lengths = torch.randint(0, 2, (seqs,), generator=g)
+    lengths[:200] = 0  # many that start at one token
+    n, c = int(lengths.sum()), 3
+    x, f = gated(n, c, F32, 1)
+    initial = rand((seqs, c), F32, 3)
+    leaves = [t.detach().requires_grad_() for t in (x, f, initial)]
+    h, last = policy.recurrence(*leaves[:2], starts(lengths.tolist()), leaves[2])
+    dh, dlast = rand((n, c), F32, 5), rand((seqs, c), F32, 6)
+    dx, df, di = torch.autograd.grad((h, last), leaves, (dh, dlast))
+    some = (lengths == 1).cuda()
+    xd, fd, s0 = x.double(), f.double(), initial.double()[some]
+    keep, take = torch.sigmoid(fd), torch.sigmoid(-fd)
+    want = keep * s0 + take * xd
+    size = keep * s0.abs() + take * xd.abs()
+    within("h", h.detach(), want, 2 * GATE * size)
+    assert torch.equal(last[some], h) and torch.equal(last[~some], initial[~some]) and torch.equal(di[~some], dlast[~some])
+    g0 = dh.double() + dlast.double()[some]
+    gs = dh.double().abs() + dlast.double()[some].abs()
+    within("dx", dx, take * g0, 2 * GATE * take * gs)
+    within("dinitial", di[some], keep * g0, 2 * GATE * keep * gs)
+    within("dgate", df, g0 * (s0 - xd) * keep * take, 6 * GATE * keep * take * gs * (s0.abs() + xd.abs()))
+
+
+def test_recurrence_strides():
+    """Slices of one projection at odd offsets, rows of a wider buffer, one gate row for all tokens, cotangents in other
+    strides, an initial state that needs no gradient."""
+    lengths = [40, 0, 150]
+    for dtype in (F32, BF16, F16):
+        wide = rand((190, 131), dtype, 6)
+        for off in (0, 1, 3, 8):
+            check_recurrence(wide[:, off:off + 50], wide[:, off + 51:off + 101] + 0, lengths, rand((3, 50), F32, 4))
+            check_recurrence(wide[:, off:off + 50], wide[:, off + 51:off + 101], lengths)
+    x, row = rand((190, 33), BF16, 1), rand((33,), BF16, 2).requires_grad_()
+    h, _ = policy.recurrence(x, row.expand(190, 33), starts(lengths))
+    dh = rand((190, 33), BF16, 3)
+    each = rand((33,), BF16, 2).expand(190, 33).contiguous().requires_grad_()
+    h2, _ = policy.recurrence(x, each, starts(lengths))
+    assert torch.equal(h, h2)
+    one, = torch.autograd.grad(h, row, dh)
+    many, = torch.autograd.grad(h2, each, dh)
+    assert torch.equal(one, many.sum(0))
+    xs = rand((190, 33), F32, 1).requires_grad_()
+    turned = rand((33, 190), F32, 4).t()
+    a, = torch.autograd.grad(policy.recurrence(xs, xs, starts(lengths))[0], xs, turned)
+    b, = torch.autograd.grad(policy.recurrence(xs, xs, starts(lengths))[0], xs, turned.contiguous())
+    assert torch.equal(a, b)
+
+
+def test_recurrence_partial_gradients():
+    """Any of the inputs with a gradient and any of the outputs with a cotangent alone."""
+    lengths, c = [70, 0, 200], 20
+    x, f = gated(270, c, F32, 1)
+    initial = rand((3, c), F32, 3)
+    dh, dlast = rand((270, c), F32, 4), rand((3, c), F32, 5)
+    leaves = [t.detach().requires_grad_() for t in (x, f, initial)]
+    h, last = policy.recurrence(leaves[0], leaves[1], starts(lengths), leaves[2])
+    for outs, cots, d, l in (((h,), (dh,), dh, 0 * dlast), ((last,), (dlast,), 0 * dh, dlast)):
+        got = torch.autograd.grad(outs, leaves, cots, retain_graph=True)
+        want = recur64(x, f, lengths, initial, d, l)
+        for name, t in zip(("dx", "dgate", "dinitial"), got):
+            within(name, t, *want[name])
+    full = torch.autograd.grad((h, last), leaves, (dh, dlast))
+    for i in range(3):
+        some = [t.detach().requires_grad_(i == j) for j, t in enumerate((x, f, initial))]
+        out = policy.recurrence(some[0], some[1], starts(lengths), some[2])
+        assert torch.equal(torch.autograd.grad(out, some[i], (dh, dlast))[0], full[i])
+
+
+def test_recurrence_padding():
+    """Tokens behind the last sequence give zeros and take none, whatever they hold; the last sequence's state is whole."""
+    for lengths, more in (([40, 100], 1), ([40, 100], 300), ([], 20), ([0, 0], 150), ([128], 128), ([120], 8)):
+        n, c = sum(lengths), 33
+        x, f = gated(n + more, c, BF16, 1)
+        x[n:], f[n:] = math.nan, math.inf
+        initial = rand((len(lengths), c), F32, 3)
+        leaves = [t.detach().requires_grad_() for t in (x, f, initial)]
+        h, last = policy.recurrence(leaves[0], leaves[1], starts(lengths), leaves[2])
+        dh, dlast = rand(x.shape, BF16, 4), rand(initial.shape, F32, 5)
+        dh[n:] = math.nan
+        dx, df, di = torch.autograd.grad((h, last), leaves, (dh, dlast))
+        assert not h[n:].any() and not dx[n:].any() and not df[n:].any()
+        want = recur64(x[:n], f[:n], lengths, initial, dh[:n], dlast)
+        for name, t in (("h", h[:n]), ("last", last), ("dx", dx[:n]), ("dgate", df[:n]), ("dinitial", di)):
+            within(name, t.detach(), *want[name])
+
+
+def test_recurrence_keeps_sequences_and_channels_apart():
+    """What is not finite stays in its channel, and in its sequence from its token on (gradients: up to it)."""
+    lengths, c = [40, 300, 5, 150], 66
+    x, f = gated(495, c, F32, 1)
+    initial, dh = rand((4, c), F32, 3), rand((495, c), F32, 4)
+
+    def run(x, f, initial, dh):
+        leaves = [t.detach().clone().requires_grad_() for t in (x, f, initial)]
+        h, last = policy.recurrence(leaves[0], leaves[1], starts(lengths), leaves[2])
+        return [h.detach(), last.detach(), *torch.autograd.grad(h, leaves, dh)]
+    clean = run(x, f, initial, dh)
+    for bad in (math.nan, math.inf):
+        x2, i2, d2 = x.clone(), initial.clone(), dh.clone()
+        x2[200, 3], i2[1, 4], d2[200, 5] = bad, bad, bad
+        got = run(x2, f, i2, d2)
+        others = [i for i in range(c) if i not in (3, 4, 5)]
+        for a, b in zip(clean, got):
+            assert torch.equal(a[:, others], b[:, others])
+        for i in (0, 2, 3):  # by token
+            for t in (slice(0, 40), slice(340, 495)):
+                assert torch.equal(clean[i][t], got[i][t]), i
+        assert torch.equal(clean[0][:200], got[0][:200][:, :]) or not torch.isfinite(got[0][40:200, 4]).any()
+        assert torch.equal(clean[0][40:200, 3], got[0][40:200, 3]) and not torch.isfinite(got[0][200:340, 3]).any()
+        assert not torch.isfinite(got[1][1, [3, 4]]).any() and torch.equal(clean[1][[0, 2, 3]], got[1][[0, 2, 3]])
+        assert torch.equal(clean[2][201:340, 5], got[2][201:340, 5]) and not torch.isfinite(got[2][40:201, 5]).any()
+        assert torch.equal(clean[4][[0, 2, 3]], got[4][[0, 2, 3]])
+
+
+def test_recurrence_gates_at_their_ends():
+    """Gates that keep all or take all: exactly 1 and 0; and far ones, whose small side keeps its own places."""
+    x = rand((300, 8), F32, 1)
+    f = torch.full((300, 8), math.inf, device="cuda")
+    h, last = policy.recurrence(x, f, starts([300]), rand((1, 8), F32, 2))
+    assert torch.equal(last, rand((1, 8), F32, 2)) and torch.equal(h, last.expand(300, 8))
+    h, last = policy.recurrence(x, -f, starts([300]), rand((1, 8), F32, 2))
+    assert torch.equal(h, x) and torch.equal(last, x[-1:])
+    for dtype in (F32, BF16, F16):
+        for far in (30.0, 60.0, 85.0):
+            one, zero = torch.ones((1, 8), dtype=dtype, device="cuda"), torch.zeros((1, 8), dtype=dtype, device="cuda")
+            g = torch.full((1, 8), far, dtype=dtype, device="cuda")
+            small = torch.sigmoid(-g.double())
+            off = (1 if dtype == F32 else far / 4) * GATE  # 16 bits: the argument's rounding, |gate| 2^-24
+            within("take", policy.recurrence(one, g, starts([1]))[1], small, off * small)
+            within("keep", policy.recurrence(zero, -g, starts([1]), torch.ones((1, 8), device="cuda"))[1], small, off * small)
+
+
+def test_recurrence_offsets_that_are_wrong_stay_in_bounds():
+    x, f = gated(500, 40, BF16, 1)
+    for bad in ([0, 2 ** 31 - 1, 3], [0, -5, -(2 ** 31)], [7, 300, 100, 500], [0, 600, 400, 200], [500, 500]):
+        a = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        leaves = [t.detach().requires_grad_() for t in (x, f, rand((len(bad) - 1, 40), F32, 2))]
+        out = policy.recurrence(leaves[0], leaves[1], a, leaves[2])
+        torch.autograd.grad(out, leaves, (x, leaves[2].detach()))
+    torch.cuda.synchronize()
+
+
+def test_recurrence_gradient_is_the_slope():
+    """The gradients against central differences of the definition in float64, along random directions."""
+    lengths, c = [20, 150], 30
+    x, f = gated(170, c, F32, 1)
+    initial, dh, dlast = rand((2, c), F32, 3), rand((170, c), F32, 4), rand((2, c), F32, 5)
+    leaves = [t.clone().requires_grad_() for t in (x, f, initial)]
+    grads = torch.autograd.grad(policy.recurrence(leaves[0], leaves[1], starts(lengths), leaves[2]), leaves, (dh, dlast))
+    dirs = [rand(t.shape, torch.float64, 6 + i) for i, t in enumerate((x, f, initial))]
+    step = 1e-6
+
+    def value(s):
+        xs, fs, h0 = (t.double() + s * step * d for t, d in zip((x, f, initial), dirs))
+        keep, total, t = torch.sigmoid(fs), 0.0, 0
+        for i, n in enumerate(lengths):
+            h = h0[i]
+            for j in range(t, t + n):
+                h = keep[j] * h + (1 - keep[j]) * xs[j]
+                total = total + (h * dh[j].double()).sum()
+            total, t = total + (h * dlast[i].double()).sum(), t + n
+        return total
+    slope = (value(1) - value(-1)) / (2 * step)
+    got = sum((g.double() * d).sum() for g, d in zip(grads, dirs))
+    size = sum((g.double() * d).abs().sum() for g, d in zip(grads, dirs))
+    assert abs(slope - got) <= 1e-6 * size, (slope.item(), got.item())
+
+
+def test_recurrence_past_32_bits():
+    """Tokens 2^20 elements apart: offsets past 2^31 elements."""
+    big = torch.zeros((2200, 2 ** 20), dtype=BF16, device="cuda")
+    x, f = gated(2200, 130, BF16, 1)
+    big[:, 1:131], big[:, 140:270] = x, f
+
+    def run(x, f):
+        leaves = [t.detach().requires_grad_() for t in (x, f)]
+        h, last = policy.recurrence(*leaves, starts([1000, 1200]))
+        return [h, last, *torch.autograd.grad((h, last), leaves, (gated(2200, 130, BF16, 5)[0], last.detach()))]
+    assert all(torch.equal(a, b) for a, b in zip(run(x, f), run(big[:, 1:131], big[:, 140:270])))
+
+
+def test_recurrence_refusals():
+    x, f, a, s = rand((10, 6), BF16, 1), rand((10, 6), BF16, 2), starts([4, 6]), rand((2, 6), F32, 3)
+    for args in ((x.double(), f.double(), a), (x, f.float(), a), (x, f[:9], a), (x.t(), f.t(), a), (x, f, a.long()), (x, f, a[None]),
+                 (x, f, a[:0]), (x, f, a[::2]), (x, f, a.cpu()), (x.cpu(), f.cpu(), a.cpu()), (x, f, a, s.to(BF16)), (x, f, a, s[:1]),
+                 (x, f, a, rand((6, 2), F32).t()), (x[0], f[0], a), (x[:, :0], f[:, :0], a), (x, f, a, s.cpu()), (x, None, a)):
+        with pytest.raises(TypeError):
+            policy.recurrence(*args)
+    with pytest.raises(ValueError):
+        policy.recurrence(x[:1, :1].expand(2 ** 28, 1000), x[:1, :1].expand(2 ** 28, 1000), a)
+
+
+# ---- one token a world ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("worlds,channels", [(0, 5), (1, 1), (3, 3), (1, 256), (7, 4), (5, 9), (300, 99), (1000, 130), (20000, 64),
+                                             (3, 100001)])
+def test_recurrence_step(dtype, worlds, channels):
+    print("recurrence step", dtype, worlds, channels, flush=True)
+    x, f = gated(worlds, channels, dtype, 1)
+    s = rand((worlds, channels), F32, 3)
+    h, new = policy.recurrence_step(x, f, s)
+    keep, take = torch.sigmoid(f.double()), torch.sigmoid(-f.double())
+    want, size = keep * s.double() + take * x.double(), keep * s.double().abs() + take * x.double().abs()
+    within("state", new, want, 2 * GATE * size)
+    assert h.dtype == dtype and torch.equal(h, new.to(dtype))
+
+
+def test_recurrence_step_is_the_recurrence():
+    """Strided rows, and one token a sequence of the packed form, bit for bit."""
+    for dtype in (F32, BF16, F16):
+        wide, s = rand((50, 210), dtype, 1), rand((50, 104), F32, 2)[:, 3:102]
+        x, f = wide[:, 1:100], wide[:, 105:204]
+        h, new = policy.recurrence_step(x, f, s)
+        h2, last = policy.recurrence(x, f, starts([1] * 50), s.contiguous())
+        assert torch.equal(h, h2) and torch.equal(new, last)
+
+
+def test_recurrence_step_refusals():
+    x, f, s = rand((10, 6), BF16, 1), rand((10, 6), BF16, 2), rand((10, 6), F32, 3)
+    for args in ((x, f, s.to(BF16)), (x, f.float(), s), (x, f, s[:9]), (x.cpu(), f.cpu(), s.cpu()), (x, f, s.cpu()), (x.t(), f.t(), s.t()),
+                 (x.double(), f.double(), s), (x[0], f[0], s[0])):
+        with pytest.raises(TypeError):
+            policy.recurrence_step(*args)
+    with pytest.raises(RuntimeError):
+        policy.recurrence_step(x, f, s.requires_grad_())
+    with torch.no_grad():
+        policy.recurrence_step(x, f, s)
