@@ -1,5 +1,5 @@
 /* C ABI of the operators of policies with a longer memory in libnablaengine_g1.so (no counterpart in the reference): a gated
- * linear recurrence. The conventions are nablaengine_policy.h's. */
+ * linear recurrence, and the gated residual between two blocks' norms. The conventions are nablaengine_policy.h's. */
 #ifndef NABLAENGINE_MEMORY_H
 #define NABLAENGINE_MEMORY_H
 #include <hip/hip_runtime_api.h>
@@ -28,6 +28,22 @@ long long dk_recurrence_work_bytes(int tokens, int channels, int vjp);
  * x_w, gate_w, state_w elements from world to world; h, next contiguous. next may be state where that is contiguous. */
 int dk_recurrence_step(hipStream_t st, int type, long long worlds, int channels, const void* x, long long x_w, const void* gate,
                        long long gate_w, const float* state, long long state_w, void* h, float* next);
+
+/* The gated residual of `rows` rows of n elements: y = x + scale sg rms(u) w, z = rms(y) next_w (of the y that is not rounded),
+ * rms(v) = v / sqrt(mean v^2 + eps), sg = 1 / (1 + exp(-gate)). Rows of x, u, gate (NULL: sg = 1) x_row, u_row, gate_row
+ * elements apart, y and z contiguous; w, next_w, scale: n elements of type w_type (0, or the type of x), each NULL for ones.
+ * stats: (2, rows) float32, both norms' factors for the backward, or NULL. */
+int dk_gated_residual(hipStream_t st, long long rows, int n, int type, const void* x, long long x_row, const void* u,
+                      long long u_row, const void* gate, long long gate_row, int w_type, const void* w, const void* next_w,
+                      const void* scale, float eps, void* y, void* z, float* stats);
+/* Its VJP from the same inputs and the stats: rows of dy and dz (each NULL: zeros) dy_row and dz_row apart -> dx, du, dgate (rows
+ * contiguous), dw, dnext_w, dscale (type w_type), each NULL where not wanted. work: dk_gated_residual_work_bytes bytes, NULL
+ * allowed without dw, dnext_w and dscale. No rows give zero dw, dnext_w, dscale. */
+int dk_gated_residual_vjp(hipStream_t st, long long rows, int n, int type, const void* x, long long x_row, const void* u,
+                          long long u_row, const void* gate, long long gate_row, int w_type, const void* w, const void* next_w,
+                          const void* scale, const float* stats, const void* dy, long long dy_row, const void* dz,
+                          long long dz_row, void* dx, void* du, void* dgate, void* dw, void* dnext_w, void* dscale, void* work);
+long long dk_gated_residual_work_bytes(long long rows, int n, int type);
 
 #ifdef __cplusplus
 }

@@ -8,7 +8,8 @@
 namespace {
 
 #define ENTRIES(X)                                                                                                    \
-  X(dk_recurrence) X(dk_recurrence_vjp) X(dk_recurrence_carry_bytes) X(dk_recurrence_work_bytes) X(dk_recurrence_step)
+  X(dk_recurrence) X(dk_recurrence_vjp) X(dk_recurrence_carry_bytes) X(dk_recurrence_work_bytes) X(dk_recurrence_step) \
+  X(dk_gated_residual) X(dk_gated_residual_vjp) X(dk_gated_residual_work_bytes)
 struct Entries {
 #define X(name) decltype(&::name) name;
   ENTRIES(X)
@@ -109,9 +110,89 @@ std::tuple<Tensor, Tensor> recurrence_step(const Tensor& x, const Tensor& gate, 
   return {h, next};
 }
 
+// ---- gated residual -------------------------------------------------------------------------------------------------
+
+struct Rows {
+  int64_t n, rows, x, u, gate;  // elements from row to row
+  int type, param_type;
+  at::ScalarType params;
+};
+Rows residual_checks(const Tensor& x, const Tensor& u, const OptTensor& weight, const OptTensor& next_weight, const OptTensor& gate,
+                     const OptTensor& scale) {
+  check_device("x", x, x);
+  Rows r = {};
+  r.type = type_of(x);
+  CHECK_TYPE(r.type >= 0 && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < 1LL << 31,
+             "x: expected float32, bfloat16 or float16 with a last dimension of 1 to 2^31 - 1 elements, got ", described(x));
+  check_as("u", u, x, x.scalar_type(), x.sizes());
+  if (in(gate)) check_as("gate", *gate, x, x.scalar_type(), x.sizes());
+  r.n = x.size(-1), r.rows = x.numel() / r.n, r.params = at::kFloat;
+  const Tensor* first = nullptr;
+  for (const auto& [name, p] : {std::pair<const char*, const OptTensor&>{"weight", weight}, {"next_weight", next_weight}, {"scale", scale}}) {
+    if (!in(p)) continue;
+    check_device(name, *p, x);
+    CHECK_TYPE((p->scalar_type() == at::kFloat || p->scalar_type() == x.scalar_type()) && p->dim() == 1 && p->size(0) == r.n &&
+                   p->is_contiguous(),
+               name, ": expected ", r.n, " contiguous elements of float32 or ", x.scalar_type(), ", got ", described(*p));
+    CHECK_TYPE(!first || first->scalar_type() == p->scalar_type(), "weight, next_weight and scale must have one type");
+    first = &*p, r.params = p->scalar_type(), r.param_type = type_of(*p);
+  }
+  r.x = row_stride(x), r.u = row_stride(u), r.gate = in(gate) ? row_stride(*gate) : 0;
+  CHECK_TYPE(r.x >= 0 && r.u >= 0 && r.gate >= 0, "x, u and gate: expected evenly spaced rows of neighbouring elements, got ",
+             described(x), ", ", described(u), in(gate) ? ", " + described(*gate) : "");
+  return r;
+}
+
+std::vector<Tensor> gated_residual_forward(const Tensor& x, const Tensor& u, const OptTensor& weight, const OptTensor& next_weight,
+                                           const OptTensor& gate, const OptTensor& scale, double eps, bool stats) {
+  const Rows a = residual_checks(x, u, weight, next_weight, gate, scale);
+  const Tensor y = at::empty(x.sizes(), x.options()), z = at::empty(x.sizes(), x.options());
+  const Tensor s = at::empty({2, stats ? a.rows : 0}, x.options().dtype(at::kFloat));
+  call("the gated residual launch", x, [&](hipStream_t st) {
+    return lib.dk_gated_residual(st, a.rows, (int)a.n, a.type, x.data_ptr(), a.x, u.data_ptr(), a.u, in(gate), a.gate, a.param_type,
+                                 in(weight), in(next_weight), in(scale), (float)eps, y.data_ptr(), z.data_ptr(),
+                                 stats ? s.data_ptr<float>() : nullptr);
+  });
+  return {y, z, s};
+}
+
+// want: a bit for each of x, u, weight, next_weight, gate, scale
+std::vector<Tensor> gated_residual_backward(const OptTensor& dy, const OptTensor& dz, const Tensor& x, const Tensor& u,
+                                            const OptTensor& weight, const OptTensor& next_weight, const OptTensor& gate,
+                                            const OptTensor& scale, const Tensor& stats, int64_t want) {
+  const Rows a = residual_checks(x, u, weight, next_weight, gate, scale);
+  Tensor cots[2];
+  int64_t strides[2] = {};
+  for (const auto& [i, name, g] : {std::tuple<int, const char*, const OptTensor&>{0, "dy", dy}, {1, "dz", dz}}) {
+    if (!g || !g->defined()) continue;
+    check_as(name, *g, x, x.scalar_type(), x.sizes());
+    cots[i] = row_stride(*g) < 0 ? g->contiguous() : *g;
+    strides[i] = row_stride(cots[i]);
+  }
+  check_as("stats", stats, x, at::kFloat, {2, a.rows});
+  CHECK_TYPE(stats.is_contiguous(), "stats must be contiguous");
+  const auto params = x.options().dtype(a.params);
+  std::vector<Tensor> r;
+  void* to[6];
+  for (int i = 0; i < 6; ++i) {
+    const bool row = i == 0 || i == 1 || i == 4, wanted = want >> i & 1;
+    r.push_back(row ? at::empty(wanted ? x.sizes() : at::IntArrayRef{0}, x.options()) : at::empty({wanted ? a.n : 0}, params));
+    to[i] = wanted ? r.back().data_ptr() : nullptr;
+  }
+  Tensor work;
+  if (bound && (to[2] || to[3] || to[5])) work = work_of(x, lib.dk_gated_residual_work_bytes(a.rows, (int)a.n, a.type));
+  call("the gated residual VJP launch", x, [&](hipStream_t st) {
+    return lib.dk_gated_residual_vjp(st, a.rows, (int)a.n, a.type, x.data_ptr(), a.x, u.data_ptr(), a.u, in(gate), a.gate,
+                                     a.param_type, in(weight), in(next_weight), in(scale), stats.data_ptr<float>(),
+                                     out_of<void>(cots[0]), strides[0], out_of<void>(cots[1]), strides[1], to[0], to[1], to[4], to[2],
+                                     to[3], to[5], work.defined() ? work.data_ptr() : nullptr);
+  });
+  return r;
+}
+
 // ---- autograd -------------------------------------------------------------------------------------------------------
 
-OP(recurrence_forward) OP(recurrence_backward) OP(recurrence_step)
+OP(recurrence_forward) OP(recurrence_backward) OP(recurrence_step) OP(gated_residual_forward) OP(gated_residual_backward)
 
 OptTensor given(const Tensor& x) { return x.defined() ? OptTensor(x) : OptTensor(); }
 bool wants_any(at::TensorList xs) { return std::any_of(xs.begin(), xs.end(), [](const Tensor& x) { return wants(x); }); }
@@ -172,6 +253,66 @@ std::tuple<Tensor, Tensor> recurrence_step_autograd(const Tensor& x, const Tenso
   return recurrence_step_op().call(x, gate, state);
 }
 
+struct GatedResidualBackward : torch::autograd::Function<GatedResidualBackward> {
+  static variable_list forward(AutogradContext*, const OptTensor& dy, const OptTensor& dz, const Tensor& x, const Tensor& u,
+                               const OptTensor& weight, const OptTensor& next_weight, const OptTensor& gate, const OptTensor& scale,
+                               const Tensor& stats, int64_t want) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return gated_residual_backward_op().call(dy, dz, x, u, weight, next_weight, gate, scale, stats, want);
+  }
+  FIRST_ORDER("gated_residual")
+};
+struct GatedResidual : torch::autograd::Function<GatedResidual> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& u, const OptTensor& weight,
+                               const OptTensor& next_weight, const OptTensor& gate, const OptTensor& scale, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto r = gated_residual_forward_op().call(x, u, weight, next_weight, gate, scale, eps, true);
+    ctx->set_materialize_grads(false);
+    int64_t want = 0, bit = 1;
+    for (bool w : {wants(x), wants(u), wants(weight), wants(next_weight), wants(gate), wants(scale)}) want |= w ? bit : 0, bit *= 2;
+    ctx->saved_data["want"] = want;
+    auto tensor = [](const OptTensor& p) { return p ? *p : Tensor(); };
+    ctx->save_for_backward({x, u, tensor(weight), tensor(next_weight), tensor(gate), tensor(scale), r[2]});
+    return {r[0], r[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    const auto s = ctx->get_saved_variables();
+    const int64_t want = ctx->saved_data["want"].toInt();
+    if (!grad[0].defined() && !grad[1].defined()) return variable_list(7);
+    no_tangents("gated_residual's gradient", grad[0], grad[1], s[0], s[1], s[2], s[3], s[4], s[5]);
+    auto run = [&] {
+      const OptTensor dy = given(grad[0]), dz = given(grad[1]);
+      if (at::GradMode::is_enabled())
+        return GatedResidualBackward::apply(dy, dz, s[0], s[1], given(s[2]), given(s[3]), given(s[4]), given(s[5]), s[6], want);
+      at::AutoDispatchBelowADInplaceOrView below;
+      return gated_residual_backward_op().call(dy, dz, s[0], s[1], given(s[2]), given(s[3]), given(s[4]), given(s[5]), s[6], want);
+    };
+    variable_list r = run();
+    for (int i = 0; i < 6; ++i)
+      if (!(want >> i & 1)) r[i] = Tensor();
+    r.push_back(Tensor());
+    return r;
+  }
+};
+std::tuple<Tensor, Tensor> gated_residual_autograd(const Tensor& x, const Tensor& u, const OptTensor& weight,
+                                                   const OptTensor& next_weight, const OptTensor& gate, const OptTensor& scale,
+                                                   double eps) {
+  no_tangents("gated_residual", x, u, weight, next_weight, gate, scale);
+  if (at::GradMode::is_enabled() &&
+      (wants(x) || wants(u) || wants(weight) || wants(next_weight) || wants(gate) || wants(scale))) {
+    const variable_list r = GatedResidual::apply(x, u, weight, next_weight, gate, scale, eps);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto r = gated_residual_forward_op().call(x, u, weight, next_weight, gate, scale, eps, false);
+  return {r[0], r[1]};
+}
+std::tuple<Tensor, Tensor> gated_residual(const Tensor& x, const Tensor& u, const OptTensor& weight, const OptTensor& next_weight,
+                                          const OptTensor& gate, const OptTensor& scale, double eps) {
+  const auto r = gated_residual_forward_op().call(x, u, weight, next_weight, gate, scale, eps, false);
+  return {r[0], r[1]};
+}
+
 }  // namespace
 
 // the entries' names, in the order in which dk_memory_torch_bind takes their addresses
@@ -194,16 +335,26 @@ TORCH_LIBRARY_FRAGMENT(nablaengine, m) {
   m.def("recurrence_backward(Tensor? dh, Tensor? dlast, Tensor x, Tensor gate, Tensor starts, Tensor? initial, Tensor carry, "
         "bool want_x, bool want_gate, bool want_initial) -> Tensor[]");
   m.def("recurrence_step(Tensor x, Tensor gate, Tensor state) -> (Tensor, Tensor)");
+  m.def("gated_residual(Tensor x, Tensor u, Tensor? weight, Tensor? next_weight, Tensor? gate, Tensor? scale, float eps) "
+        "-> (Tensor, Tensor)");
+  m.def("gated_residual_forward(Tensor x, Tensor u, Tensor? weight, Tensor? next_weight, Tensor? gate, Tensor? scale, float eps, "
+        "bool stats) -> Tensor[]");
+  m.def("gated_residual_backward(Tensor? dy, Tensor? dz, Tensor x, Tensor u, Tensor? weight, Tensor? next_weight, Tensor? gate, "
+        "Tensor? scale, Tensor stats, int want) -> Tensor[]");
 }
 TORCH_LIBRARY_IMPL(nablaengine, CompositeExplicitAutograd, m) {
   m.impl("recurrence", recurrence);
   m.impl("recurrence_forward", recurrence_forward);
   m.impl("recurrence_backward", recurrence_backward);
   m.impl("recurrence_step", recurrence_step);
+  m.impl("gated_residual", gated_residual);
+  m.impl("gated_residual_forward", gated_residual_forward);
+  m.impl("gated_residual_backward", gated_residual_backward);
 }
 TORCH_LIBRARY_IMPL(nablaengine, Autograd, m) {
   m.impl("recurrence", recurrence_autograd);
   m.impl("recurrence_step", recurrence_step_autograd);
-  for (const char* name : {"recurrence_forward", "recurrence_backward"})
+  m.impl("gated_residual", gated_residual_autograd);
+  for (const char* name : {"recurrence_forward", "recurrence_backward", "gated_residual_forward", "gated_residual_backward"})
     m.impl(name, torch::CppFunction::makeFromBoxedFunction<&inner_autograd>());
 }

@@ -38,24 +38,6 @@ struct Scan {
   float *dinitial, *back;  // back (chunks, channels): what the next chunk's first token hands to a chunk's last
 };
 
-constexpr float LOG2E_SCAN = 1.4426950408889634f;
-// a = 1 / (1 + exp(-f)) and 1 - a, each to its own last places
-template <typename T>
-__device__ __forceinline__ void gates(float f, float& keep, float& take) {
-  float e;
-  if constexpr (sizeof(T) == 4) {  // with the product's rounding, which is felt by far gates
-    const float z = -fminf(fabsf(f), 200.0f), t = z * LOG2E_SCAN;
-    e = __builtin_amdgcn_exp2f(t);
-    e = fmaf(e, fmaf(z, LOG2E_SCAN, -t) * 0.6931472f, e);
-    if (f != f) e = f;
-  } else {
-    e = __builtin_amdgcn_exp2f(-fabsf(f) * LOG2E_SCAN);
-  }
-  const float r = __builtin_amdgcn_rcpf(1.0f + e), small = e * r;
-  keep = f >= 0.0f ? r : small;
-  take = f >= 0.0f ? small : r;
-}
-
 // V neighbouring elements
 template <typename T, int V> struct Few { T v[V]; };
 template <typename T, int V>

@@ -142,6 +142,13 @@ def _fake_recurrence_backward(dh, dlast, x, gate, starts, initial, carry, want_x
         x.new_empty((seqs, x.shape[1]) if want_initial else (0,), dtype=torch.float32)]
 
 
+def _fake_gated_residual_backward(dy, dz, x, u, weight, next_weight, gate, scale, stats, want):
+    n, ptype = x.shape[-1], next((p.dtype for p in (weight, next_weight, scale) if p is not None), torch.float32)
+    row = lambda bit: x.new_empty(x.shape if want >> bit & 1 else (0,))  # noqa: E731
+    param = lambda bit: x.new_empty((n if want >> bit & 1 else 0,), dtype=ptype)  # noqa: E731
+    return [row(0), row(1), param(2), param(3), row(4), param(5)]
+
+
 _FAKES = {"layer_norm": lambda x, *_: x.new_empty(x.shape), "layer_norm_forward": _fake_layer_norm_forward,
           "layer_norm_backward": _fake_layer_norm_backward, "grad_norm": _fake_norm, "clip_grads_": _fake_norm,
           "clip_grads_out": _fake_norm, "attention": lambda q, *_: q.new_empty(q.shape),
@@ -150,6 +157,10 @@ _FAKES = {"layer_norm": lambda x, *_: x.new_empty(x.shape), "layer_norm_forward"
           "attention_step": lambda q, *_: q.new_empty(q.shape),
           "recurrence": _fake_recurrence, "recurrence_forward": _fake_recurrence_forward,
           "recurrence_backward": _fake_recurrence_backward,
+          "gated_residual": lambda x, *_: (x.new_empty(x.shape), x.new_empty(x.shape)),
+          "gated_residual_forward": lambda x, u, w, w2, gate, scale, eps, stats: [
+              x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty((2, x.numel() // x.shape[-1] if stats else 0), dtype=torch.float32)],
+          "gated_residual_backward": _fake_gated_residual_backward,
           "recurrence_step": lambda x, gate, state: (x.new_empty(x.shape), state.new_empty(x.shape))}
 
 
@@ -295,6 +306,23 @@ def recurrence_step(x, gate, state):
     if _wants_grad(x, gate, state):
         raise _err("recurrence_step has no gradient: use recurrence (one token a sequence), or torch.no_grad()", RuntimeError)
     return _ops(True).recurrence_step(_tensor("x", x), _tensor("gate", gate), _tensor("state", state))
+
+
+# ---- gated residual -------------------------------------------------------------------------------------------------
+
+def gated_residual(x, u, weight=None, next_weight=None, *, gate=None, scale=None, eps=EPS):
+    """What lies between two blocks of a policy: (y, z) with y = x + scale sigmoid(gate) rms(u) weight, the residual stream x
+    with a block's output u normed, gated and scaled onto it, and z = rms(y) next_weight, the next block's input (or the head's,
+    behind the last block); rms(v) = v / sqrt(mean v^2 + eps) over the last dimension. Differentiable in all but eps.
+
+    x, u, gate: float32, bfloat16 or float16, one type and shape, rows evenly spaced (as layer_norm's x); weight, next_weight,
+    scale: vectors of float32 or x's type, one type. Without a gate it is open (1), without scale and weights they are ones. y
+    and z are contiguous and have x's type. All is computed in float32: z comes of the y that is not rounded yet, and so do the
+    gradients."""
+    e = float(eps)
+    if not 0.0 <= e < math.inf:
+        raise _err(f"eps must be finite and >= 0, got {eps}", ValueError)
+    return _ops(True).gated_residual(_tensor("x", x), _tensor("u", u), weight, next_weight, gate, scale, e)
 
 
 def _bind_loaded():

@@ -127,6 +127,9 @@ _MEMORY_PROTOTYPES = {
     "dk_recurrence_carry_bytes": "q:ii",
     "dk_recurrence_work_bytes": "q:iii",
     "dk_recurrence_step": "i:piqi" + "pq" * 3 + "pp",
+    "dk_gated_residual": "i:pqii" + "pq" * 3 + "ipppfppp",
+    "dk_gated_residual_vjp": "i:pqii" + "pq" * 3 + "ipppp" + "pq" * 2 + "ppppppp",
+    "dk_gated_residual_work_bytes": "q:qii",
 }
 _OPTIONAL = {**_POLICY_PROTOTYPES, **_MEMORY_PROTOTYPES}
 _PROTOTYPES.update(_OPTIONAL)

@@ -373,3 +373,196 @@ def test_recurrence_step_refusals():
         policy.recurrence_step(x, f, s.requires_grad_())
     with torch.no_grad():
         policy.recurrence_step(x, f, s)
+
+
+# ---- gated residual -------------------------------------------------------------------------------------------------
+
+def residual64(x, u, w, w2, gate, scale, eps, dy, dz):
+    """The definition and its gradients in float64, and each output's bound. Written out a step at a time: a value's error is
+    its inputs' errors through the formula's derivatives, and SUM of its terms' magnitudes for each float32 sum or product; the
+    norms' factors are off by SUM of themselves, since all their squares are positive; a gate by GATE."""
+    type_, n = x.dtype, x.shape[-1]
+    one = torch.ones(n, dtype=torch.float64, device=x.device)
+    wt, w2t, st = (p.dtype if p is not None else F32 for p in (w, w2, scale))
+    w, w2, s = (p.double() if p is not None else one for p in (w, w2, scale))
+    x, u, dy, dz = (t.double() for t in (x, u, dy, dz))
+    sg = torch.sigmoid(gate.double()) if gate is not None else torch.ones_like(x)
+    shut = torch.sigmoid(-gate.double()) if gate is not None else torch.zeros_like(x)
+    mean = lambda v: v.mean(-1, keepdim=True)  # noqa: E731
+    r = 1 / (mean(u * u) + eps).sqrt()
+    uh = u * r
+    f = s * sg * uh * w
+    y = x + f
+    ey = 2 * SUM * f.abs() + SUM * y.abs()  # the branch's factors, SUM each, and the sum
+    r2 = 1 / (mean(y * y) + eps).sqrt()
+    er2 = r2 * (SUM + r2 * r2 * mean(y.abs() * ey))
+    yh = y * r2
+    eyh = ey * r2 + y.abs() * er2 + SUM * yh.abs()
+    out = {"y": (y, ey), "z": (yh * w2, (eyh + SUM * yh.abs()) * w2.abs())}
+    gz = dz * w2
+    q = mean(gz * yh)
+    eq = mean(gz.abs() * eyh) + SUM * mean(gz.abs() * yh.abs())
+    e = dy + r2 * (gz - yh * q)
+    ee = er2 * (gz - yh * q).abs() + r2 * (eyh * q.abs() + yh.abs() * eq) + SUM * (dy.abs() + r2 * (gz.abs() + yh.abs() * q.abs()))
+    out["dx"] = (e, ee)
+    es, ees = e * s, ee * s.abs()
+    out["dgate"] = (es * uh * w * sg * shut, (ees + 2 * SUM * es.abs()) * (uh * w).abs() * sg * shut)
+    c, ec = es * sg * w, (ees + 2 * SUM * es.abs()) * sg * w.abs()
+    p = mean(c * uh)
+    ep = mean(ec * uh.abs()) + 2 * SUM * mean((c * uh).abs())
+    out["du"] = (r * (c - uh * p), r * (ec + uh.abs() * ep + 2 * SUM * (uh * p).abs() + 2 * SUM * (c - uh * p).abs()))
+    rows = lambda v: v.reshape(-1, n).sum(0)  # noqa: E731
+    m, em = rows(e * sg * uh), rows((ee + 3 * SUM * e.abs()) * sg * uh.abs())
+    out["dweight"], out["dscale"] = (s * m, s.abs() * em), (w * m, w.abs() * em)
+    out["dnext_weight"] = (rows(dz * yh), rows(dz.abs() * eyh + SUM * (dz * yh).abs()))
+    types = {"dweight": wt, "dnext_weight": w2t, "dscale": st}
+    return {k: (v, b + U[types.get(k, type_)] * v.abs() + TINY[types.get(k, type_)]) for k, (v, b) in out.items()}
+
+
+def check_residual(x, u, w=None, w2=None, gate=None, scale=None, eps=1e-5, dy=None, dz=None):
+    given = {"x": x, "u": u, "weight": w, "next_weight": w2, "gate": gate, "scale": scale}
+    leaves = {k: t.detach().requires_grad_() for k, t in given.items() if t is not None}
+    opt = lambda k: leaves.get(k)  # noqa: E731
+    y, z = policy.gated_residual(leaves["x"], leaves["u"], opt("weight"), opt("next_weight"), gate=opt("gate"), scale=opt("scale"), eps=eps)
+    dy = rand(x.shape, x.dtype, 71) if dy is None else dy
+    dz = rand(x.shape, x.dtype, 72) if dz is None else dz
+    grads = torch.autograd.grad((y, z), list(leaves.values()), (dy, dz))
+    with torch.no_grad():
+        again = policy.gated_residual(x, u, w, w2, gate=gate, scale=scale, eps=eps)
+    assert torch.equal(y, again[0]) and torch.equal(z, again[1])
+    want = residual64(x, u, w, w2, gate, scale, eps, dy, dz)
+    got = {"y": y.detach(), "z": z.detach(), **{f"d{k}": g for k, g in zip(leaves, grads)}}
+    for name, t in got.items():
+        within(name, t, *want[name])
+    return got
+
+
+def residual_inputs(rows, width, dtype, ptype=F32):
+    x, u, g = (rand((rows, width), dtype, i, 1.5) for i in (1, 2, 3))
+    return x, u, *((rand((width,), F32, 4 + i, 0.3) + 1).to(ptype) for i in range(2)), g, (rand((width,), F32, 6, 0.2) + 0.4).to(ptype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("width", [1, 2, 7, 8, 9, 31, 32, 33, 63, 64, 65, 99, 127, 129, 255, 257, 511, 512, 513, 1023, 1025, 2047,
+                                   2049, 4095, 4097, 8191, 8193, 16385])
+def test_residual_widths(dtype, width):
+    """Every group size and both sides of each change between them, the wide rows' kernels among them."""
+    print("residual", dtype, width, flush=True)
+    check_residual(*residual_inputs(37 if width < 4096 else 5, width, dtype))
+
+
+@pytest.mark.parametrize("rows,width", [(1, 99), (2, 512), (5000, 99), (9000, 16), (20000, 64), (2100, 256), (1100, 1000), (600, 2050)])
+def test_residual_rows(rows, width):
+    """From one row to more than the backward's workgroups take at once."""
+    print("residual rows", rows, width, flush=True)
+    for dtype in (F32, BF16):
+        check_residual(*residual_inputs(rows, width, dtype))
+
+
+@pytest.mark.parametrize("which", range(16))
+def test_residual_without(which):
+    """Any of the weights, the gate and the scale missing; parameters in half precision."""
+    x, u, *rest = residual_inputs(65, 77, BF16, BF16 if which % 2 else F32)
+    check_residual(x, u, *[t if which >> i & 1 else None for i, t in enumerate(rest)])
+
+
+def test_residual_strides_and_alignments():
+    for dtype in (F32, BF16, F16):
+        x, u, w, w2, g, s = residual_inputs(50, 131, dtype)
+        for off in (0, 1, 3, 8):
+            check_residual(x[:, off:off + 99], u[:, 5:104], w[:99], w2[1:100], g[:, off + 2:off + 101], s[3:102],
+                           dy=rand((50, 104), dtype, 7)[:, 5:], dz=rand((99, 50), dtype, 8).t())
+    x, u, w, w2, g, s = residual_inputs(24, 40, F32)
+    check_residual(*(t.view(2, 3, 4, 40) if t.dim() == 2 else t for t in (x, u, w, w2, g, s)))
+    check_residual(x, u[:1].expand(24, 40), w, w2, g[:1].expand(24, 40), s)
+    with pytest.raises(TypeError):
+        policy.gated_residual(x.t(), u.t())
+
+
+def test_residual_partial_gradients():
+    """Either output's cotangent alone, and any one input's gradient alone."""
+    x, u, w, w2, g, s = residual_inputs(300, 90, F32)
+    dy, dz = rand(x.shape, F32, 8), rand(x.shape, F32, 9)
+    names = ("x", "u", "weight", "next_weight", "gate", "scale")
+
+    def run(which):
+        t = [v.detach().requires_grad_(which in (None, i)) for i, v in enumerate((x, u, w, w2, g, s))]
+        return t, policy.gated_residual(*t[:4], gate=t[4], scale=t[5])
+    t, out = run(None)
+    for i, cots in ((0, (dy, 0 * dz)), (1, (0 * dy, dz))):
+        # next_weight has no part in y
+        some = [v for j, v in enumerate(t) if i == 1 or j != 3]
+        grads = torch.autograd.grad(out[i], some, cots[i], retain_graph=True)
+        want = residual64(x, u, w, w2, g, s, 1e-5, *cots)
+        for name, v in zip([n for j, n in enumerate(names) if i == 1 or j != 3], grads):
+            within(f"d{name}", v, *want[f"d{name}"])
+    full = torch.autograd.grad(out, t, (dy, dz))
+    for i in range(6):
+        t, out = run(i)
+        assert torch.equal(torch.autograd.grad(out, t[i], (dy, dz))[0], full[i]), names[i]
+
+
+def test_residual_empty_rows():
+    t = [v.requires_grad_() for v in residual_inputs(0, 9, F32)]
+    y, z = policy.gated_residual(*t[:4], gate=t[4], scale=t[5])
+    grads = torch.autograd.grad((y, z), t, (torch.empty_like(y), torch.empty_like(z)))
+    assert y.shape == z.shape == (0, 9) and not any(g.any() for g in grads) and [g.shape for g in grads] == [v.shape for v in t]
+
+
+def test_residual_extremes():
+    """Rows of zeros, large and small values, closed and open gates, and what is not finite in a row of its own."""
+    x, u, w, w2, g, s = residual_inputs(16, 333, F32)
+    y, z = policy.gated_residual(torch.zeros_like(x), torch.zeros_like(u), w, w2, gate=g, scale=s)
+    assert not y.any() and not z.any()
+    for scale in (1e-12, 1e12):
+        check_residual(scale * x, u, w, w2, g, scale * s, eps=0.0)
+        check_residual(x, scale * u, w, w2, g, s, eps=0.0)
+    full, none = torch.full_like(g, math.inf), torch.full_like(g, -math.inf)
+    assert all(torch.equal(a, b) for a, b in zip(policy.gated_residual(x, u, w, w2, gate=full, scale=s),
+                                                 policy.gated_residual(x, u, w, w2, scale=s)))
+    y, z = policy.gated_residual(x, u, w, w2, gate=none, scale=s)
+    assert torch.equal(y, x)
+    check_residual(x, u, w, w2, 40 * g, s)
+    leaves = [t.detach().clone().requires_grad_() for t in (x, u, g)]
+    clean = policy.gated_residual(leaves[0], leaves[1], w, w2, gate=leaves[2], scale=s)
+    cg = torch.autograd.grad(clean, leaves, (x, u))
+    with torch.no_grad():
+        leaves[0][1, 3], leaves[1][3, 332], leaves[2][5, 0] = math.inf, math.nan, math.nan
+    bad = policy.gated_residual(leaves[0], leaves[1], w, w2, gate=leaves[2], scale=s)
+    bg = torch.autograd.grad(bad, leaves, (x, u))
+    good = [i for i in range(16) if i not in (1, 3, 5)]
+    assert all(torch.equal(a[good], b[good]) for a, b in zip((*clean, *cg), (*bad, *bg)))
+    assert torch.isnan(bad[1][[3, 5]]).all() and not torch.isfinite(bad[0][1, 3])
+
+
+def test_residual_gradient_is_the_slope():
+    x, u, w, w2, g, s = residual_inputs(33, 50, F32)
+    dy, dz = rand(x.shape, F32, 8), rand(x.shape, F32, 9)
+    at = (x, u, w, w2, g, s)
+    t = [v.clone().requires_grad_() for v in at]
+    grads = torch.autograd.grad(policy.gated_residual(*t[:4], gate=t[4], scale=t[5]), t, (dy, dz))
+    dirs = [rand(v.shape, torch.float64, 10 + i) for i, v in enumerate(at)]
+    h = 1e-6
+
+    def value(sign):
+        x, u, w, w2, g, s = (v.double() + sign * h * d for v, d in zip(at, dirs))
+        rms = lambda v: v / (v.square().mean(-1, keepdim=True) + 1e-5).sqrt()  # noqa: E731
+        y = x + s * torch.sigmoid(g) * rms(u) * w
+        return (y * dy.double()).sum() + (rms(y) * w2 * dz.double()).sum()
+    slope = (value(1) - value(-1)) / (2 * h)
+    got = sum((a.double() * d).sum() for a, d in zip(grads, dirs))
+    size = sum((a.double() * d).abs().sum() for a, d in zip(grads, dirs))
+    assert abs(slope - got) <= 1e-6 * size, (slope.item(), got.item())
+
+
+def test_residual_refusals():
+    x, u, w, w2, g, s = residual_inputs(10, 6, BF16)
+    for args, kw in (((x, u.float()), {}), ((x, u[:9]), {}), ((x, u, w[:5]), {}), ((x, u, w, w2.to(BF16)), {}), ((x, u, w.half()), {}),
+                     ((x, u), dict(gate=g.float())), ((x, u), dict(gate=g[:, :5])), ((x, u), dict(scale=s[None])),
+                     ((x.cpu(), u.cpu()), {}), ((x, u.cpu()), {}), ((x, u, w.cpu()), {}), ((x.double(), u.double()), {}), ((x, None), {}),
+                     ((x[0, 0], u[0, 0]), {}), ((x[:, :0], u[:, :0]), {}), ((x, u), dict(gate=g.t().contiguous().t()))):
+        with pytest.raises(TypeError):
+            policy.gated_residual(*args, **kw)
+    for eps in (-1.0, math.nan, math.inf):
+        with pytest.raises(ValueError):
+            policy.gated_residual(x, u, eps=eps)
