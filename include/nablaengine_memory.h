@@ -1,5 +1,5 @@
 /* C ABI of the operators of policies with a longer memory in libnablaengine_g1.so (no counterpart in the reference): a gated
- * linear recurrence, and the gated residual between two blocks' norms. The conventions are nablaengine_policy.h's. */
+ * linear recurrence, the gated residual between two blocks' norms, and single-token attention over paged histories. The conventions are nablaengine_policy.h's. */
 #ifndef NABLAENGINE_MEMORY_H
 #define NABLAENGINE_MEMORY_H
 #include <hip/hip_runtime_api.h>
@@ -44,6 +44,27 @@ int dk_gated_residual_vjp(hipStream_t st, long long rows, int n, int type, const
                           const void* scale, const float* stats, const void* dy, long long dy_row, const void* dz,
                           long long dz_row, void* dx, void* du, void* dgate, void* dw, void* dnext_w, void* dscale, void* work);
 long long dk_gated_residual_work_bytes(long long rows, int n, int type);
+
+/* Attention of one query a world over its history in pages: q (worlds, heads, dim); k, v: pools of `count` pages (count, page,
+ * kv_heads, dim) with elements from page to page (_p), token to token (_t) and head to head (_h), page a power of two; pages:
+ * (worlds, most) int32 on the device, rows pages_w apart: token j of world w is token j % page of page pages[w][j / page];
+ * lengths: worlds int32 on the device, the world's tokens, its newest one's query being q (below 0 is 0, above most * page that).
+ * window > 0: the query sees the window last tokens and the sinks first ones (0: all); what it does not see is not read, nor are
+ * the entries of its pages. out (worlds, heads, dim) contiguous, zeros for a world without tokens, NaN for one that has a page
+ * in sight whose number is none of the pool's. most * page < 2^30, worlds * heads < 2^24. work: dk_attention_paged_work_bytes
+ * bytes, or NULL when 0. */
+int dk_attention_paged(hipStream_t st, int type, int worlds, int heads, int kv_heads, int dim, int count, int page, int most,
+                       const void* q, long long q_w, long long q_h, const void* k, long long k_p, long long k_t, long long k_h,
+                       const void* v, long long v_p, long long v_t, long long v_h, const int* pages, long long pages_w,
+                       const int* lengths, int window, int sinks, float scale, void* out, void* work);
+long long dk_attention_paged_work_bytes(int worlds, int heads, int kv_heads, int dim, int page, int most, int window, int sinks);
+/* New keys and values into the pages: k, v (tokens, kv_heads, dim), packed by starts (worlds + 1 int32 on the device, 0 first, not
+ * falling), or one a world where starts is NULL (tokens = worlds). The i-th of world w becomes its token lengths[w] + i. One
+ * that has no place, below 0, past `most` pages or on a page that is not in the pool, is dropped. */
+int dk_cache_append(hipStream_t st, int type, int worlds, int tokens, int kv_heads, int dim, int count, int page, int most,
+                    const void* k, long long k_t, long long k_h, const void* v, long long v_t, long long v_h, const int* starts,
+                    void* k_pages, long long kp_p, long long kp_t, long long kp_h, void* v_pages, long long vp_p, long long vp_t,
+                    long long vp_h, const int* pages, long long pages_w, const int* lengths);
 
 #ifdef __cplusplus
 }

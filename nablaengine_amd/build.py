@@ -14,7 +14,7 @@ PROF_LIB = os.path.join(HERE, "libnablaengine_g1_prof.so")
 TORCH_LIB, TORCH_SOURCES = os.path.join(HERE, "libnablaengine_policy_torch.so"), ["policy_torch.cpp", "policy_memory_torch.cpp"]
 SOURCES = ["g1_forward.hip", "g1_adjoint.hip", "g1_order.hip", "g1_kinematics.hip", "g1_diag.hip", "g1_capi.hip",
            "policy_norm.hip", "policy_clip.hip", "policy_attend.hip", "policy_step.hip",
-           "policy_scan.hip", "policy_residual.hip"]
+           "policy_scan.hip", "policy_residual.hip", "policy_paged.hip"]
 ARCH = os.environ.get("NABLA_OFFLOAD_ARCH", "gfx950")
 # packed FP32 instructions off (-packed-fp32-ops): the kernels are written for scalar FP32. Warnings that mark
 # undefined behaviour the optimizer exploits (a non-void function falling off its end becomes unreachable code, and a

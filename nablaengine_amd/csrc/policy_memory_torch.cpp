@@ -9,7 +9,8 @@ namespace {
 
 #define ENTRIES(X)                                                                                                    \
   X(dk_recurrence) X(dk_recurrence_vjp) X(dk_recurrence_carry_bytes) X(dk_recurrence_work_bytes) X(dk_recurrence_step) \
-  X(dk_gated_residual) X(dk_gated_residual_vjp) X(dk_gated_residual_work_bytes)
+  X(dk_gated_residual) X(dk_gated_residual_vjp) X(dk_gated_residual_work_bytes)             \
+  X(dk_attention_paged) X(dk_attention_paged_work_bytes) X(dk_cache_append)
 struct Entries {
 #define X(name) decltype(&::name) name;
   ENTRIES(X)
@@ -190,9 +191,81 @@ std::vector<Tensor> gated_residual_backward(const OptTensor& dy, const OptTensor
   return r;
 }
 
+// ---- paged histories ------------------------------------------------------------------------------------------------
+
+struct Pool { int count, page, most; };
+// a pool of pages (count, page, kv_heads, dim), and the worlds' tables and lengths
+Pool pool_checks(const Tensor& k_pages, const Tensor& pages, const Tensor& lengths, int64_t worlds) {
+  const int64_t count = k_pages.size(0), page = k_pages.size(1);
+  CHECK_VALUE(page >= 1 && !(page & (page - 1)), "a page holds a power of two of tokens, not ", page);
+  check_device("pages", pages, k_pages);
+  CHECK_TYPE(pages.scalar_type() == at::kInt && pages.dim() == 2 && pages.size(0) == worlds &&
+                 (pages.numel() == 0 || pages.size(1) == 1 || pages.stride(1) == 1),
+             "pages: expected int32 page numbers of ", worlds, " worlds, each world's neighbours, got ", described(pages));
+  check_as("lengths", lengths, k_pages, at::kInt, {worlds});
+  CHECK_TYPE(lengths.is_contiguous(), "lengths must be contiguous, got ", described(lengths));
+  const int64_t most = 1 << 30;
+  CHECK_VALUE(count < most && page < most && pages.size(1) < most && pages.size(1) * page < most, count, " pages of ", page,
+              " tokens, ", pages.size(1), " a world, exceed one launch");
+  return {(int)count, (int)page, (int)pages.size(1)};
+}
+
+Tensor attention_paged(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& pages, const Tensor& lengths,
+                       double scale, int64_t window, int64_t sinks) {
+  const Heads h = heads_checks(q, k_pages, v_pages, 4);
+  const int64_t worlds = q.size(0);
+  const Pool p = pool_checks(k_pages, pages, lengths, worlds);
+  CHECK_VALUE(worlds * h.heads < 1 << 24, worlds, " worlds of ", h.heads, " heads exceed one launch");
+  CHECK_VALUE(window >= 0 && sinks >= 0, "window and sinks must not be negative, got ", window, " and ", sinks);
+  const int w = (int)std::min<int64_t>(window, 1 << 30), s = (int)std::min<int64_t>(sinks, 1 << 30);
+  check_bound();
+  const Tensor out = at::empty(q.sizes(), q.options());
+  const long long bytes = lib.dk_attention_paged_work_bytes((int)worlds, h.heads, h.kv, h.dim, p.page, p.most, w, s);
+  const Tensor work = bytes ? work_of(q, bytes) : Tensor();
+  const Tensor &k = k_pages, &v = v_pages;
+  call("the paged attention launch", q, [&](hipStream_t st) {
+    return lib.dk_attention_paged(st, h.type, (int)worlds, h.heads, h.kv, h.dim, p.count, p.page, p.most, q.data_ptr(), q.stride(0),
+                                  q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(), v.stride(0),
+                                  v.stride(1), v.stride(2), pages.data_ptr<int>(), pages.stride(0), lengths.data_ptr<int>(), w, s,
+                                  (float)scale, out.data_ptr(), bytes ? work.data_ptr() : nullptr);
+  });
+  return out;
+}
+
+void cache_append_(const Tensor& k_pages, const Tensor& v_pages, const Tensor& k, const Tensor& v, const Tensor& pages,
+                   const Tensor& lengths, const OptTensor& starts) {
+  const Heads h = heads_checks(k, k_pages, v_pages, 4);
+  CHECK_TYPE(h.heads == h.kv, "k has ", h.heads, " heads, the pages ", h.kv);
+  check_as("v", v, k, k.scalar_type(), k.sizes());
+  CHECK_TYPE(v.numel() == 0 || v.stride(2) == 1, "v: a head's elements must be neighbours, got ", described(v));
+  for (const auto& [name, x] : {std::pair<const char*, const Tensor&>{"k_pages", k_pages}, {"v_pages", v_pages}})
+    for (int64_t i = 0; i < 4; ++i)
+      CHECK_TYPE(x.size(i) <= 1 || x.stride(i) != 0, name, " is written: expected no expanded tensor, got ", described(x));
+  const int64_t tokens = k.size(0), worlds = lengths.dim() == 1 ? lengths.size(0) : -1;
+  CHECK_TYPE(worlds >= 0, "lengths: expected one dimension, got ", described(lengths));
+  const Pool p = pool_checks(k_pages, pages, lengths, worlds);
+  if (in(starts)) {
+    check_as("starts", *starts, k, at::kInt, {worlds + 1});
+    CHECK_TYPE(starts->is_contiguous(), "starts must be contiguous, got ", described(*starts));
+  } else {
+    CHECK_TYPE(tokens == worlds, "without starts there is one token a world: ", tokens, " tokens, ", worlds, " worlds");
+  }
+  CHECK_VALUE(tokens < 1 << 30 && worlds < 1 << 24 && worlds * h.kv * (h.dim / 8) < 1LL << 30, tokens, " tokens of ", worlds,
+              " worlds exceed one launch");
+  call("the cache append launch", k, [&](hipStream_t st) {
+    return lib.dk_cache_append(st, h.type, (int)worlds, (int)tokens, h.kv, h.dim, p.count, p.page, p.most, k.data_ptr(), k.stride(0),
+                               k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), (const int*)in(starts), k_pages.data_ptr(),
+                               k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), v_pages.data_ptr(), v_pages.stride(0),
+                               v_pages.stride(1), v_pages.stride(2), pages.data_ptr<int>(), pages.stride(0), lengths.data_ptr<int>());
+  });
+  for (const Tensor& y : {k_pages, v_pages})  // a graph that saved one of them notices
+    if (!y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
+}
+
 // ---- autograd -------------------------------------------------------------------------------------------------------
 
 OP(recurrence_forward) OP(recurrence_backward) OP(recurrence_step) OP(gated_residual_forward) OP(gated_residual_backward)
+OP(attention_paged) OP(cache_append_)
 
 OptTensor given(const Tensor& x) { return x.defined() ? OptTensor(x) : OptTensor(); }
 bool wants_any(at::TensorList xs) { return std::any_of(xs.begin(), xs.end(), [](const Tensor& x) { return wants(x); }); }
@@ -313,6 +386,21 @@ std::tuple<Tensor, Tensor> gated_residual(const Tensor& x, const Tensor& u, cons
   return {r[0], r[1]};
 }
 
+Tensor attention_paged_autograd(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& pages,
+                                const Tensor& lengths, double scale, int64_t window, int64_t sinks) {
+  no_tangents("attention_paged", q, k_pages, v_pages);
+  TORCH_CHECK(!at::GradMode::is_enabled() || !wants_any({q, k_pages, v_pages}), POL "attention_paged has no gradient");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return attention_paged_op().call(q, k_pages, v_pages, pages, lengths, scale, window, sinks);
+}
+void cache_append_autograd(const Tensor& k_pages, const Tensor& v_pages, const Tensor& k, const Tensor& v, const Tensor& pages,
+                           const Tensor& lengths, const OptTensor& starts) {
+  no_tangents("cache_append_", k_pages, v_pages, k, v);
+  TORCH_CHECK(!at::GradMode::is_enabled() || !wants_any({k_pages, v_pages, k, v}), POL "cache_append_ has no gradient");
+  at::AutoDispatchBelowADInplaceOrView below;
+  cache_append__op().call(k_pages, v_pages, k, v, pages, lengths, starts);
+}
+
 }  // namespace
 
 // the entries' names, in the order in which dk_memory_torch_bind takes their addresses
@@ -341,8 +429,14 @@ TORCH_LIBRARY_FRAGMENT(nablaengine, m) {
         "bool stats) -> Tensor[]");
   m.def("gated_residual_backward(Tensor? dy, Tensor? dz, Tensor x, Tensor u, Tensor? weight, Tensor? next_weight, Tensor? gate, "
         "Tensor? scale, Tensor stats, int want) -> Tensor[]");
+  m.def("attention_paged(Tensor q, Tensor k_pages, Tensor v_pages, Tensor pages, Tensor lengths, float scale, int window, "
+        "int sinks) -> Tensor");
+  m.def("cache_append_(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor k, Tensor v, Tensor pages, Tensor lengths, Tensor? starts) "
+        "-> ()");
 }
 TORCH_LIBRARY_IMPL(nablaengine, CompositeExplicitAutograd, m) {
+  m.impl("attention_paged", attention_paged);
+  m.impl("cache_append_", cache_append_);
   m.impl("recurrence", recurrence);
   m.impl("recurrence_forward", recurrence_forward);
   m.impl("recurrence_backward", recurrence_backward);
@@ -355,6 +449,8 @@ TORCH_LIBRARY_IMPL(nablaengine, Autograd, m) {
   m.impl("recurrence", recurrence_autograd);
   m.impl("recurrence_step", recurrence_step_autograd);
   m.impl("gated_residual", gated_residual_autograd);
+  m.impl("attention_paged", attention_paged_autograd);
+  m.impl("cache_append_", cache_append_autograd);
   for (const char* name : {"recurrence_forward", "recurrence_backward", "gated_residual_forward", "gated_residual_backward"})
     m.impl(name, torch::CppFunction::makeFromBoxedFunction<&inner_autograd>());
 }

@@ -156,25 +156,6 @@ Tensor clip_grads_out(at::TensorList grads, at::TensorList out, double max_norm)
 
 // ---- attention ------------------------------------------------------------------------------------------------------
 
-struct Heads { int type, heads, kv, dim; };
-// q (.., heads, dim), k and v of `dims` dimensions ending in (kv_heads, dim)
-Heads heads_checks(const Tensor& q, const Tensor& k, const Tensor& v, int64_t dims) {
-  check_device("q", q, q);
-  CHECK_TYPE((q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) && q.dim() == 3,
-             "q: expected bfloat16 or float16 of 3 dimensions, got ", described(q));
-  check_device("k", k, q);
-  CHECK_TYPE(k.scalar_type() == q.scalar_type() && k.dim() == dims, "k: expected ", q.scalar_type(), " of ", dims,
-             " dimensions, got ", described(k));
-  check_as("v", v, q, q.scalar_type(), k.sizes());
-  const int64_t heads = q.size(1), dim = q.size(2), kv = k.size(-2);
-  CHECK_TYPE(k.size(-1) == dim && dim % 8 == 0 && dim >= 8 && dim <= 128,
-             "q and k need heads of one size, a multiple of 8 up to 128, got ", dim, " and ", k.size(-1));
-  CHECK_TYPE(kv >= 1 && heads >= 1 && heads % kv == 0 && heads < 1 << 20, "q's heads must be a multiple of k's, got ",
-             heads, " and ", kv);
-  for (const auto& [name, x] : {std::pair<const char*, const Tensor&>{"q", q}, {"k", k}, {"v", v}})
-    CHECK_TYPE(x.numel() == 0 || x.stride(-1) == 1, name, ": a head's elements must be neighbours, got ", described(x));
-  return {type_of(q), (int)heads, (int)kv, (int)dim};
-}
 int sequences_checks(const Tensor& q, const Tensor& k, const Tensor& starts_q, const Tensor& starts_k, const Heads& h) {
   for (const auto& [name, x] : {std::pair<const char*, const Tensor&>{"starts_q", starts_q}, {"starts_k", starts_k}}) {
     check_device(name, x, q);

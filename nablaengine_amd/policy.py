@@ -23,6 +23,7 @@ by reverse mode: forward mode, the backward of a gradient and torch.func's deriv
 """
 import ctypes
 import math
+import operator
 import os
 
 import torch
@@ -161,6 +162,7 @@ _FAKES = {"layer_norm": lambda x, *_: x.new_empty(x.shape), "layer_norm_forward"
           "gated_residual_forward": lambda x, u, w, w2, gate, scale, eps, stats: [
               x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty((2, x.numel() // x.shape[-1] if stats else 0), dtype=torch.float32)],
           "gated_residual_backward": _fake_gated_residual_backward,
+          "attention_paged": lambda q, *_: q.new_empty(q.shape), "cache_append_": lambda *_: None,
           "recurrence_step": lambda x, gate, state: (x.new_empty(x.shape), state.new_empty(x.shape))}
 
 
@@ -323,6 +325,48 @@ def gated_residual(x, u, weight=None, next_weight=None, *, gate=None, scale=None
     if not 0.0 <= e < math.inf:
         raise _err(f"eps must be finite and >= 0, got {eps}", ValueError)
     return _ops(True).gated_residual(_tensor("x", x), _tensor("u", u), weight, next_weight, gate, scale, e)
+
+
+# ---- paged histories ------------------------------------------------------------------------------------------------
+
+def _sight(window, sinks):
+    """window (0: none) and sinks as numbers."""
+    w, s = 0 if window is None else operator.index(window), operator.index(sinks)
+    if w < (0 if window is None else 1) or s < 0:
+        raise _err(f"window must be None or at least 1 and sinks at least 0, got {window} and {sinks}", ValueError)
+    return w, s
+
+
+def cache_append_(k_pages, v_pages, k, v, pages, lengths, starts=None):
+    """Write new keys and values into the pages: one token a world, k and v (worlds, kv_heads, dim), or with starts (int32
+    offsets on the device, one more than worlds) any number of each, packed (tokens, kv_heads, dim). The i-th of world w becomes
+    its token lengths[w] + i, lengths being those without the new ones; adding them to lengths is the caller's.
+
+    k_pages, v_pages: (pool, page, kv_heads, dim), bfloat16 or float16, page a power of two; pages: (worlds, most) int32 on the
+    device, the numbers of each world's pages in order. A page that is written belongs to one world alone. A token that has no
+    place, past the `most` pages or on a page whose number is none of the pool's (-1, say), is dropped. No gradients."""
+    for name, x in (("k_pages", k_pages), ("v_pages", v_pages), ("k", k), ("v", v), ("pages", pages), ("lengths", lengths)):
+        _tensor(name, x)
+    if _wants_grad(k_pages, v_pages, k, v):
+        raise _err("cache_append_ has no gradient: call it under torch.no_grad()", RuntimeError)
+    _ops(True).cache_append_(k_pages, v_pages, k, v, pages, lengths, starts)
+
+
+def attention_paged(q, k_pages, v_pages, pages, lengths, *, scale=None, window=None, sinks=0):
+    """The control loop's attention over histories in pages: each world's one new query over its lengths[w] tokens, its newest
+    one among them, without gradients. With a window the query sees the `window` last tokens and the `sinks` first ones, as
+    attention's with the same window; pages that hold neither are not read and may serve others (their entries in `pages` may
+    hold anything).
+
+    q: (worlds, heads, dim); k_pages, v_pages, pages: as cache_append_'s; lengths: (worlds,) int32 on the device, moved into 0 ..
+    most * page; heads, dim, strides and scale as attention's. A world without tokens gives zeros, one with a page in sight
+    whose number is none of the pool's NaN. Worlds may share pages."""
+    s = _scale(scale, q)
+    for name, x in (("k_pages", k_pages), ("v_pages", v_pages), ("pages", pages), ("lengths", lengths)):
+        _tensor(name, x)
+    if _wants_grad(q, k_pages, v_pages):
+        raise _err("attention_paged has no gradient: use attention (one query a sequence), or torch.no_grad()", RuntimeError)
+    return _ops(True).attention_paged(q, k_pages, v_pages, pages, lengths, s, *_sight(window, sinks))
 
 
 def _bind_loaded():

@@ -130,6 +130,9 @@ _MEMORY_PROTOTYPES = {
     "dk_gated_residual": "i:pqii" + "pq" * 3 + "ipppfppp",
     "dk_gated_residual_vjp": "i:pqii" + "pq" * 3 + "ipppp" + "pq" * 2 + "ppppppp",
     "dk_gated_residual_work_bytes": "q:qii",
+    "dk_attention_paged": "i:p" + "i" * 8 + "pqq" + "pqqq" * 2 + "pqpiifpp",
+    "dk_attention_paged_work_bytes": "q:iiiiiiii",
+    "dk_cache_append": "i:p" + "i" * 8 + "pqq" * 2 + "p" + "pqqq" * 2 + "pqp",
 }
 _OPTIONAL = {**_POLICY_PROTOTYPES, **_MEMORY_PROTOTYPES}
 _PROTOTYPES.update(_OPTIONAL)

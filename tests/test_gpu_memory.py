@@ -566,3 +566,284 @@ def test_residual_refusals():
     for eps in (-1.0, math.nan, math.inf):
         with pytest.raises(ValueError):
             policy.gated_residual(x, u, eps=eps)
+
+
+# ---- paged histories ------------------------------------------------------------------------------------------------
+
+EXP = 2.0 ** -12  # what float32 scores (|s| < 20 here, sums of at most 128 products) put on a probability
+
+
+def visible(n, window, sinks):
+    keys = torch.arange(n, device="cuda")
+    return keys if window is None else keys[(keys >= n - window) | (keys < sinks)]
+
+
+def paged_tables(lengths, page, most, spare=3, seed=0):
+    """Each world's pages, drawn from a pool that holds a few more; entries past a world's last page name no page."""
+    need = [-(-n // page) for n in lengths]
+    order = torch.randperm(sum(need) + spare, generator=torch.Generator().manual_seed(seed)).tolist()
+    table = torch.full((len(lengths), most), -1, dtype=torch.int32)
+    for w, k in enumerate(need):
+        table[w, :k] = torch.tensor(order[:k], dtype=torch.int32)
+        order = order[k:]
+    return table.cuda(), sum(need) + spare
+
+
+def paged64(q, k, v, table, lengths, page, window, sinks, scale):
+    out, bound = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    G, u = q.shape[1] // k.shape[2], U[q.dtype]
+    for w, n in enumerate(lengths):
+        keys = visible(n, window, sinks)
+        if not len(keys):
+            continue
+        at, off = table[w].long()[keys // page], keys % page
+        for h in range(q.shape[1]):
+            K, V = k[at, off, h // G].double(), v[at, off, h // G].double()
+            p = torch.softmax(K @ q[w, h].double() * scale, 0)
+            out[w, h] = p @ V
+            bound[w, h] = u * out[w, h].abs() + (2 * EXP + SUM) * (p @ V.abs()) + TINY[q.dtype]
+    return out, bound
+
+
+def check_paged(lengths, page, heads, kv, dim, dtype, window=None, sinks=0, scale=None, most=None):
+    most = max([-(-n // page) for n in lengths] + [1]) if most is None else most
+    table, count = paged_tables(lengths, page, most)
+    q, k, v = rand((len(lengths), heads, dim), dtype, 1), rand((count, page, kv, dim), dtype, 2), rand((count, page, kv, dim), dtype, 3)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    got = policy.attention_paged(q, k, v, table, n, scale=scale, window=window, sinks=sinks)
+    within("out", got, *paged64(q, k, v, table, lengths, page, window, sinks, 1 / math.sqrt(dim) if scale is None else scale))
+    return q, k, v, table, n, got
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv,dim", [(1, 1, 64), (8, 2, 64), (6, 2, 128), (5, 5, 40), (8, 1, 8), (3, 1, 72), (7, 1, 120), (24, 2, 64),
+                                          (70, 1, 128)])
+def test_paged_heads(dtype, heads, kv, dim):
+    print("paged", dtype, heads, kv, dim, flush=True)
+    for window, sinks in ((None, 0), (20, 3)):
+        check_paged([1, 0, 33, 16, 200, 17], 16, heads, kv, dim, dtype, window, sinks)
+
+
+@pytest.mark.parametrize("page", [1, 2, 8, 16, 64, 256])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (None, 5), (1, 0), (1, 1), (16, 0), (16, 16), (17, 4), (100, 200), (1000, 0)])
+def test_paged_windows(page, window, sinks):
+    """Windows and sinks that begin and end inside pages, meet, and reach past the history."""
+    print("paged window", page, window, sinks, flush=True)
+    check_paged([0, 1, 2, 15, 16, 17, 18, 31, 33, 47, 64, 100, 116, 117, 300], page, 4, 2, 64, BF16, window, sinks)
+
+
+@pytest.mark.parametrize("worlds,length,window,sinks", [(1, 5000, None, 0), (1, 70000, None, 0), (3, 9000, 4000, 100), (1, 600, 300, 4),
+                                                        (40, 700, None, 0), (2100, 40, None, 0), (2100, 90, 30, 2), (1100, 64, None, 0)])
+def test_paged_many_and_long(worlds, length, window, sinks):
+    """Few worlds with long histories, whose stretches are joined, and many worlds, a wave each."""
+    print("paged many", worlds, length, flush=True)
+    g = torch.Generator().manual_seed(worlds)
+    lengths = torch.randint(0, length + 1, (worlds,), generator=g).tolist()
+    lengths[0] = length
+    check_paged(lengths, 16, 4, 2, 64, BF16, window, sinks)
+
+
+def test_paged_is_the_dense_form():
+    """Pages in order are a cache: the same tokens give the dense form's results, bit for bit where no window hides any."""
+    lengths, page, most = [0, 1, 100, 512, 333], 32, 16
+    q, cache = rand((5, 8, 64), BF16, 1), rand((2, 5, 512, 2, 64), BF16, 2)
+    table = torch.arange(5 * most, dtype=torch.int32, device="cuda").view(5, most)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    got = policy.attention_paged(q, cache[0].view(-1, page, 2, 64), cache[1].view(-1, page, 2, 64), table, n)
+    assert torch.equal(got, policy.attention_step(q, cache[0], cache[1], n))
+
+
+def test_paged_reads_only_what_is_in_sight():
+    """Tokens past the length and outside the window hold NaN, their pages' entries any number; lengths outside the table are
+    moved inside it."""
+    page, lengths, window, sinks = 8, [100, 37, 64, 9, 0], 20, 5
+    q, k, v, table, n, want = check_paged(lengths, page, 4, 2, 64, BF16, window, sinks, most=13)
+    k2, v2, t2 = torch.full_like(k, math.nan), torch.full_like(v, math.nan), torch.full_like(table, -7)
+    for w, length in enumerate(lengths):
+        keys = visible(length, window, sinks)
+        at, off = table[w].long()[keys // page], keys % page
+        k2[at, off], v2[at, off] = k[at, off], v[at, off]
+        t2[w, keys // page] = table[w, keys // page]
+    t2[4] = 2 ** 31 - 1
+    assert torch.equal(policy.attention_paged(q, k2, v2, t2, n, window=window, sinks=sinks), want)
+    full = torch.arange(13, dtype=torch.int32, device="cuda").expand(5, 13)
+    far = torch.tensor([2 ** 31 - 1, 104, -1, -(2 ** 31), 0], dtype=torch.int32, device="cuda")
+    near = torch.tensor([104, 104, 0, 0, 0], dtype=torch.int32, device="cuda")
+    a, b = (policy.attention_paged(q, k, v, full, x, window=window, sinks=sinks) for x in (far, near))
+    assert torch.equal(a, b) and not a[2:].any()
+
+
+def test_paged_pages_that_are_not_there():
+    """A world that needs one gives NaN in all its heads, its neighbours are as they were."""
+    for lengths in ([100, 37, 64], [3000, 2900, 2000]):  # whole, and in stretches
+        q, k, v, table, n, want = check_paged(lengths, 16, 4, 2, 64, BF16)
+        for bad in (-1, k.shape[0], 2 ** 31 - 1, -(2 ** 31)):
+            t2 = table.clone()
+            t2[1, 1] = bad
+            got = policy.attention_paged(q, k, v, t2, n)
+            assert torch.isnan(got[1]).all() and torch.equal(got[[0, 2]], want[[0, 2]])
+    none = policy.attention_paged(q, k[:0], v[:0], table, n)
+    assert torch.isnan(none).all()
+    assert not policy.attention_paged(q, k, v, table[:, :0], n).any()  # no entries: no tokens
+
+
+def test_paged_strides():
+    """Pools that are halves of one, heads before tokens, tables and queries that are slices; worlds that share pages."""
+    lengths = [40, 0, 77]
+    q, k, v, table, n, want = check_paged(lengths, 16, 4, 2, 64, F16)
+    both = torch.stack([k, v], 1)
+    wide = torch.full((3, 40), -1, dtype=torch.int32, device="cuda")
+    wide[:, 7:7 + table.shape[1]] = table
+    qs = rand((3, 9, 70), F16, 9)
+    qs[:, 3:7, 5:69] = q
+    assert torch.equal(policy.attention_paged(qs[:, 3:7, 5:69], both[:, 0], both[:, 1], wide[:, 7:7 + table.shape[1]], n), want)
+    kt, vt = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (k, v))
+    assert torch.equal(policy.attention_paged(q, kt, vt, table, n), want)
+    shared = policy.attention_paged(q, k, v, table[2:].expand(3, -1), n[2:].expand(3).contiguous())
+    assert torch.equal(shared[2], want[2])
+
+
+def test_paged_scores_that_are_not_finite():
+    """Every score -inf: NaN, as the dense form; an infinite value reaches its own column."""
+    q = torch.ones((1, 1, 8), dtype=BF16, device="cuda")
+    k, v = torch.full((2, 16, 1, 8), -math.inf, dtype=BF16, device="cuda"), rand((2, 16, 1, 8), BF16, 2)
+    table, n = torch.tensor([[1, 0]], dtype=torch.int32, device="cuda"), torch.tensor([20], dtype=torch.int32, device="cuda")
+    assert torch.isnan(policy.attention_paged(q, k, v, table, n)).all()
+    k[0, 3] = 1
+    assert torch.equal(policy.attention_paged(q, k, v, table, n)[0, 0], v[0, 3, 0])
+    v[0, 3, 0, 5] = math.inf
+    assert torch.isinf(policy.attention_paged(q, k, v, table, n)[0, 0, 5])
+
+
+def test_paged_past_32_bits():
+    """Pages 2^20 elements apart: offsets past 2^31 elements."""
+    big = torch.zeros((2200, 2 ** 20), dtype=BF16, device="cuda")
+    q, k, v = rand((2, 4, 64), BF16, 1), rand((2200, 4, 2, 64), BF16, 2), rand((2200, 4, 2, 64), BF16, 3)
+    kb, vb = (big[:, 512 * i:512 * i + 512].view(2200, 4, 2, 64) for i in (1, 2))
+    table = torch.randperm(2200, generator=torch.Generator().manual_seed(1)).to(torch.int32).cuda().view(2, 1100)
+    n, zero = torch.tensor([4400, 4001], dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    packed = [x[table.long()].flatten(1, 2) for x in (k, v)]
+    new = [torch.cat([x[0, :4400], x[1, :4001]]) for x in packed]
+    policy.cache_append_(kb, vb, *new, table, zero, starts([4400, 4001]))
+    k2, v2 = torch.zeros_like(k), torch.zeros_like(v)
+    policy.cache_append_(k2, v2, *new, table, zero, starts([4400, 4001]))
+    assert torch.equal(kb, k2) and torch.equal(vb, v2) and k2.any()
+    assert torch.equal(policy.attention_paged(q, kb, vb, table, n), policy.attention_paged(q, k, v, table, n))
+
+
+def append_by_hand(kp, vp, k, v, table, lengths, counts):
+    t, page = 0, kp.shape[1]
+    for w, (n, c) in enumerate(zip(lengths, counts)):
+        for i in range(c):
+            at = n + i
+            if 0 <= at < table.shape[1] * page and 0 <= int(table[w, at // page]) < len(kp):
+                kp[int(table[w, at // page]), at % page], vp[int(table[w, at // page]), at % page] = k[t], v[t]
+            t += 1
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("kv,dim,page", [(1, 8, 1), (2, 64, 16), (3, 40, 8), (5, 128, 32)])
+def test_append(dtype, kv, dim, page):
+    """One token a world, and packed ones: none, one and many a world, over pages' edges, without a place or a page."""
+    print("append", dtype, kv, dim, page, flush=True)
+    lengths, most = [0, 1, 15, 16, 31, 64, -3, 100, 2 ** 31 - 1], -(-110 // page)
+    table = torch.randperm(most * 9 + 4, generator=torch.Generator().manual_seed(1))[:most * 9].view(9, most).to(torch.int32).cuda()
+    table[3, 0:2], table[4, -1] = -1, most * 9 + 4
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for counts in ([1] * 9, [0, 3, 40, 2, 0, 50, 7, 30, 4]):
+        t = sum(counts)
+        kp, vp = rand((most * 9 + 4, page, kv, dim), dtype, 2), rand((most * 9 + 4, page, kv, dim), dtype, 3)
+        both = rand((t + 2, 2 * kv + 1, dim + 3), dtype, 4)
+        k, v = both[:t, :kv, 1:dim + 1], both[:t, kv:2 * kv, 2:dim + 2]  # slices at odd offsets
+        want = kp.clone(), vp.clone()
+        append_by_hand(*want, k, v, table.cpu(), lengths, counts)
+        policy.cache_append_(kp, vp, k, v, table, n, None if counts == [1] * 9 else starts(counts))
+        assert torch.equal(kp, want[0]) and torch.equal(vp, want[1])
+
+
+def test_append_of_nothing_and_of_much():
+    kp, vp = rand((700, 16, 2, 64), BF16, 1), rand((700, 16, 2, 64), BF16, 2)
+    keep = kp.clone()
+    none = torch.zeros((0, 2, 64), dtype=BF16, device="cuda")
+    table, zero = torch.arange(700, dtype=torch.int32, device="cuda")[None], torch.zeros(1, dtype=torch.int32, device="cuda")
+    policy.cache_append_(kp, vp, none, none, table[:0], zero[:0])
+    policy.cache_append_(kp, vp, none, none, table, zero, starts([0]))
+    assert torch.equal(kp, keep)
+    k, v = rand((11000, 2, 64), BF16, 3), rand((11000, 2, 64), BF16, 4)
+    policy.cache_append_(kp, vp, k, v, table, zero + 9, starts([11000]))
+    assert torch.equal(kp.flatten(0, 1)[9:11009], k) and torch.equal(vp.flatten(0, 1)[9:11009], v)
+    assert torch.equal(kp.flatten(0, 1)[:9], keep.flatten(0, 1)[:9])
+    bad = torch.tensor([5, -9, 2 ** 31 - 1], dtype=torch.int32, device="cuda")  # offsets that are wrong stay in bounds
+    policy.cache_append_(kp, vp, k[:40], v[:40], table.expand(2, 700), zero.expand(2).contiguous(), bad)
+    torch.cuda.synchronize()
+
+
+def test_append_and_attend_step_by_step():
+    """A control loop's calls: each step's token appended, lengths counted on, and what the query sees, with pages that leave
+    the window given to the next tokens; against the packed form over the whole history with the same window."""
+    worlds, steps, page, window, sinks = 3, 70, 4, 13, 2
+    kv, heads, dim = 2, 4, 64
+    k, v, q = (rand((steps, worlds, n, dim), BF16, n + i) for i, n in enumerate((kv, kv, heads)))
+    # pages of the sinks, and five in turn: the window's 13 tokens touch at most five pages
+    kp, vp = torch.full((worlds * 6, page, kv, dim), math.nan, dtype=BF16, device="cuda"), rand((worlds * 6, page, kv, dim), BF16, 9)
+    vp[:] = math.nan
+    table = torch.full((worlds, -(-steps // page)), -1, dtype=torch.int32, device="cuda")
+    lengths = torch.zeros(worlds, dtype=torch.int32, device="cuda")
+    kd, vd, qd = (x.double() for x in (k, v, q))
+    for t in range(steps):
+        if t % page == 0:
+            for w in range(worlds):
+                table[w, t // page] = w * 6 + (0 if t == 0 else 1 + t // page % 5)
+        policy.cache_append_(kp, vp, k[t], v[t], table, lengths)
+        lengths += 1
+        got = policy.attention_paged(q[t], kp, vp, table, lengths, window=window, sinks=sinks)
+        keys = visible(t + 1, window, sinks)
+        for w in range(worlds):
+            for h in range(heads):
+                p = torch.softmax(kd[keys, w, h // 2] @ qd[t, w, h] / 8, 0)
+                V = vd[keys, w, h // 2]
+                within(f"step {t}", got[w, h], p @ V, U[BF16] * (p @ V).abs() + (2 * EXP + SUM) * (p @ V.abs()))
+
+
+def test_paged_refusals():
+    q, kp, vp = rand((3, 4, 64), BF16, 1), rand((9, 16, 2, 64), BF16, 2), rand((9, 16, 2, 64), BF16, 3)
+    t, n = torch.zeros((3, 5), dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    k, v = rand((3, 2, 64), BF16, 4), rand((3, 2, 64), BF16, 5)
+    for args in ((q.float(), kp.float(), vp.float(), t, n), (q, kp.half(), vp.half(), t, n), (q, kp, vp[:8], t, n), (q, kp, vp, t.long(), n),
+                 (q, kp, vp, t[:2], n), (q, kp, vp, t, n[:2]), (q, kp, vp, t, n.long()), (q[:2], kp, vp, t, n), (q[:, :3], kp, vp, t, n),
+                 (q, kp[..., :32], vp[..., :32], t, n), (q, kp[0], vp[0], t, n), (q.cpu(), kp.cpu(), vp.cpu(), t.cpu(), n.cpu()),
+                 (q, kp, vp, t.cpu(), n), (q, kp, vp, t.t().contiguous().t(), n), (q, kp, None, t, n), (q, kp, vp, t[0], n)):
+        with pytest.raises(TypeError):
+            policy.attention_paged(*args)
+    for kw in (dict(window=0), dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=math.nan)):
+        with pytest.raises(ValueError):
+            policy.attention_paged(q, kp, vp, t, n, **kw)
+    with pytest.raises(TypeError):
+        policy.attention_paged(q, kp, vp, t, n, window=1.5)
+    with pytest.raises(ValueError):
+        policy.attention_paged(q, kp[:, :12], vp[:, :12], t, n)
+    with pytest.raises(ValueError):
+        policy.attention_paged(q, kp, vp, torch.zeros((3, 2 ** 26), dtype=torch.int32, device="cuda"), n)
+    with pytest.raises(RuntimeError):
+        policy.attention_paged(q.clone().requires_grad_(), kp, vp, t, n)
+    for args in ((kp, vp, k.half(), v.half(), t, n), (kp, vp, k[:, :1], v[:, :1], t, n), (kp, vp, k, v[:2], t, n), (kp, vp, k, v, t[:2], n),
+                 (kp, vp, k[:2], v[:2], t, n), (kp, vp, k, v, t, n.long()), (kp, vp, k, v, t, n, n), (kp, vp, k, v, t, n, starts([1, 1, 1]).long()),
+                 (kp[:1].expand(9, 16, 2, 64), vp, k, v, t, n), (kp, vp, k, v, t, n[0]), (kp, vp, k.cpu(), v.cpu(), t, n),
+                 (kp, vp, k, rand((3, 64, 2), BF16).transpose(1, 2), t, n), (kp, None, k, v, t, n)):
+        with pytest.raises(TypeError):
+            policy.cache_append_(*args)
+    with pytest.raises(ValueError):
+        policy.cache_append_(kp[:, :12], vp[:, :12], k, v, t, n)
+    with pytest.raises(RuntimeError):
+        policy.cache_append_(kp, vp, k.clone().requires_grad_(), v, t, n)
+
+
+def test_appending_marks_what_it_writes():
+    """A graph that saved a pool which appending then overwrites notices."""
+    w = rand((4, 16, 1, 8), BF16, 1).requires_grad_()
+    kp, vp = rand((4, 16, 1, 8), BF16, 2), rand((4, 16, 1, 8), BF16, 3)
+    y = (w * kp).float().sum()
+    one = torch.ones((1, 1, 8), dtype=BF16, device="cuda")
+    policy.cache_append_(kp, vp, one, one, torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
