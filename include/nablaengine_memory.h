@@ -1,5 +1,6 @@
 /* C ABI of the operators of policies with a longer memory in libnablaengine_g1.so (no counterpart in the reference): a gated
- * linear recurrence, the gated residual between two blocks' norms, and single-token attention over paged histories. The conventions are nablaengine_policy.h's. */
+ * linear recurrence, the gated residual between two blocks' norms, single-token attention over paged
+ * histories, and attention over packed sequences with a window. The conventions are nablaengine_policy.h's. */
 #ifndef NABLAENGINE_MEMORY_H
 #define NABLAENGINE_MEMORY_H
 #include <hip/hip_runtime_api.h>
@@ -65,6 +66,21 @@ int dk_cache_append(hipStream_t st, int type, int worlds, int tokens, int kv_hea
                     const void* k, long long k_t, long long k_h, const void* v, long long v_t, long long v_h, const int* starts,
                     void* k_pages, long long kp_p, long long kp_t, long long kp_h, void* v_pages, long long vp_p, long long vp_t,
                     long long vp_h, const int* pages, long long pages_w, const int* lengths);
+
+/* dk_attention and its VJP with a window: of the keys that the causal mask leaves a query, it sees the `window` last ones and the
+ * `sinks` first ones of its sequence (window 0, or as long as tk: all). rest: (tq, heads, dim) in the outputs' type, contiguous:
+ * what their rounding took off, which the backward adds where it is given one; worth its bytes for windows of few keys, whose
+ * outputs' rounding is felt in the gradients. NULL: none. work: dk_attention_work_bytes bytes. */
+int dk_attention_window(hipStream_t st, int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk, const void* q,
+                        long long q_t, long long q_h, const void* k, long long k_t, long long k_h, const void* v, long long v_t,
+                        long long v_h, const int* starts_q, const int* starts_k, float scale, int window, int sinks, void* out,
+                        void* rest, float* lse, void* work, void* scratch);
+int dk_attention_window_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk, const void* q,
+                            long long q_t, long long q_h, const void* k, long long k_t, long long k_h, const void* v, long long v_t,
+                            long long v_h, const int* starts_q, const int* starts_k, float scale, int window, int sinks,
+                            const void* out, const void* rest, const float* lse, const void* work, const void* dout,
+                            long long do_t, long long do_h, float* delta, void* dq, void* dk, void* dv, void* scratch);
+long long dk_attention_window_scratch_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk, int window, int sinks, int vjp);
 
 #ifdef __cplusplus
 }

@@ -53,7 +53,13 @@ struct Attend {
   long long do_t, do_h;
   float* delta;  // (heads, tq): the row's dout . out
   void *dq, *dk, *dv;
+  // a window (WIN kernels): key j of a row whose last key is i is seen if j > i - window or j < sinks
+  int window, sinks;
+  void* rest;  // (tq, heads, dim): what the outputs' rounding took off, for delta; NULL: not kept
 };
+
+// whether the window hides key j from a row whose last key is i
+__device__ __forceinline__ bool window_hides(const Attend& a, int j, int i) { return j <= i - a.window && j >= a.sinks; }
 
 // The order: two lists of tiles, (sequence, tile of it): the query tiles (QROWS rows of a key/value head's queries, row =
 // token * group + head of the group) and the key tiles (32 * key_waves keys). A list is heaviest first, by the tiles of
@@ -278,6 +284,28 @@ __device__ __forceinline__ void store_rows(T* p, int d0, int dim, int h, const F
         T4 o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = (T)(acc[t][4 * j + e] * f);
+        __builtin_memcpy(p + d, &o, 8);
+      }
+    }
+}
+
+// what store_rows' rounding takes off, rounded in its turn
+template <int N, typename T>
+__device__ __forceinline__ void store_rests(T* p, int d0, int dim, int h, const F16x* acc, float f) {
+  if (!p) return;
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = d0 + 32 * t + 8 * j + 4 * h;
+      if (d < dim) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = acc[t][4 * j + e] * f;
+          o[e] = f == 0.0f ? (T)0.0f : (T)(x - (float)(T)x);
+        }
         __builtin_memcpy(p + d, &o, 8);
       }
     }

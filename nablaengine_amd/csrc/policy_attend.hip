@@ -1,6 +1,7 @@
 // Causal attention over packed sequences with shared key/value heads: forward and backward.
 //
-//   S = scale Q K^T, key j <= i + (keys - queries), P = softmax(S), O = P V
+//   S = scale Q K^T, key j <= i' = i + (keys - queries), P = softmax(S), O = P V
+//   with a window (WIN): only keys j > i' - window, and the first `sinks` ones
 //   dV = P^T dO,  dP = dO V^T,  dS = P (dP - delta), delta = dO . O a row,  dQ = scale dS K,  dK = scale dS^T Q
 //
 // A workgroup of four waves takes 128 rows of one key/value head's queries, row = token * group + head, so that the
@@ -14,6 +15,7 @@
 // with what they compute again). At heads of 128 the products lead: 2 sequences of 8192 and 2752 tokens, 16 heads on 4,
 // forward 340 us (900 TFLOP/s; a large library product of 16 bits reaches 1200), dq 440, dkv 955. Short sequences are bound
 // by their bytes: 4096 segments of up to 32 tokens, 8 heads on 2, forward 56 us (4.0 TB/s), dq 81 (3.8), dkv 60 (4.4).
+#include "../../include/nablaengine_memory.h"
 #include "../../include/nablaengine_policy.h"
 #include "policy_attend.h"
 
@@ -28,7 +30,7 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // have to search the offsets for its tile, and the heaviest tiles would not start first (2 sequences of 8192 and 2800
 // tokens: 350 us forward for 470). 4 us for a few sequences, 15 for 4096; the backward takes the forward's lists.
 __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk, int group, int key_waves, int by_sequence,
-                                                       const int* starts_q, const int* starts_k,
+                                                       int window, int sinks, const int* starts_q, const int* starts_k,
                                                        int* __restrict__ order) {
   constexpr int BUCKETS = 1024;
   // Places are unsigned: offsets that fall make sequences overlap, whose tiles together can pass 2^32. A place past the list
@@ -50,6 +52,7 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   static_assert(QROWS == 128, "");
   const unsigned caps[2] = {(unsigned)order_queries(seqs, tq, group), (unsigned)order_keys(seqs, tk, key_waves)};
   int* const lists[2] = {order + ORDER_HEAD, order + ORDER_HEAD + 2LL * caps[0]};
+  auto near = [&](long long cost, long long most) { return (int)(window && most < cost ? most : cost); };
   auto bucket_of = [](int cost) {  // rows or keys of the other side, below 2^30
     const int tiles = cost > 0 ? (int)((unsigned)(cost + TILE - 1) / TILE) : 0;
     return BUCKETS - 1 - (tiles < BUCKETS ? tiles : BUCKETS - 1);
@@ -73,9 +76,10 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
             const int from = (t << bits[1]) - (mk - mq);
             cost = mq - (from > 0 ? from : 0);
             cost = (cost > 0 ? cost : 0) * group;
+            if (t << bits[1] >= sinks) cost = near(cost, ((long long)window + (1 << bits[1])) * group);
           } else {  // the keys that the tile's last row sees
             const int last = ((t + 1) * QROWS < rows ? (t + 1) * QROWS : rows) - 1;
-            cost = last / group + mk - mq + 1;
+            cost = near(last / group + mk - mq + 1, (long long)window + sinks + QROWS / group);
           }
           return bucket_of(cost);
         };
@@ -174,15 +178,56 @@ unsigned blocks_of(const Attend& a, long long most, int parts) {
   return (unsigned)((most * a.kv_heads * parts + XCDS - 1) / XCDS * XCDS);
 }
 
+// The rows' side: a wave's 32 query rows of a workgroup's 128
+template <bool WIN>
+struct Rows {
+  int pos, head, limit, all_see, any_sees, tiles;
+  bool valid;
+  int sunk, skipped;  // WIN: the tiles that hold sinks, and those behind them that no row sees; `tiles` counts without these
+  __device__ __forceinline__ Rows(const Attend& a, const Place& p, int w) {
+    const int rows = p.nq * a.group, off = p.nk - p.nq;
+    const int row0 = p.tile * QROWS + 32 * w, row = row0 + threadIdx.x % 32;
+    valid = row < rows;
+    pos = row / a.group;
+    head = p.kv * a.group + row % a.group;
+    limit = valid ? pos + off : -1;  // the row's last key (below 0: none)
+    // of the wave's rows: the last key that all see, and the last that any sees; the workgroup's tiles of keys
+    all_see = row0 < rows ? row0 / a.group + off : -1;
+    any_sees = row0 < rows ? (row0 + 31 < rows ? row0 + 31 : rows - 1) / a.group + off : -1;
+    const int end = p.tile * QROWS + QROWS < rows ? p.tile * QROWS + QROWS : rows, last = (end - 1) / a.group + off;
+    tiles = last < 0 ? 0 : last / TILE + 1;
+    if (WIN) {
+      const int from = p.tile * QROWS / a.group + off - a.window + 1, near = from > 0 ? from / TILE : 0;
+      sunk = a.sinks > tiles * TILE ? tiles : (a.sinks + TILE - 1) / TILE;
+      skipped = near > sunk ? (near < tiles ? near : tiles) - sunk : 0;
+      tiles -= skipped;
+    }
+  }
+  __device__ __forceinline__ int tile_of(int turn) const { return WIN && turn >= sunk ? turn + skipped : turn; }
+  // whether any of the wave's rows sees one of the 32 keys from key0 on (key0 <= any_sees), and whether some row does not see all
+  __device__ __forceinline__ bool sees(const Attend& a, int key0) const {
+    return !WIN || key0 + 31 > all_see - a.window || key0 < a.sinks;
+  }
+  __device__ __forceinline__ bool masks(const Attend& a, int key0) const {
+    return key0 + 31 > all_see || (WIN && key0 <= any_sees - a.window && key0 + 31 >= a.sinks);
+  }
+  __device__ __forceinline__ bool hides(const Attend& a, int key) const {  // from this lane's row
+    return key > limit || (WIN && window_hides(a, key, limit));
+  }
+};
+
 // The keys' side of the forward and of the queries' gradient: tiles of TILE keys and their values, one tile ahead.
-template <int DP, typename T>
+template <int DP, typename T, bool WIN>
 struct Keys {
   static constexpr int CH = DP / 8, STEP = 256 / CH, N = TILE / STEP;  // chunks a row; rows a turn of the workgroup
   const T *k, *v;  // this thread's chunk of the tile's first rows
   long long k_t, v_t;
   int row, at, left;  // this thread's row; its wave's place in LDS; keys from the tile's first on
   bool in_row;
-  __device__ __forceinline__ Keys(const Attend& a, const Place& p, int first) {  // from tile `first` on
+  int before, jump;  // WIN: tiles before the hidden ones, and how many these are
+  __device__ __forceinline__ Keys(const Attend& a, const Place& p, const Rows<WIN>& r, int turn) {  // from that turn's tile on
+    const int first = r.tile_of(turn);
+    before = WIN ? r.sunk - turn : 0, jump = WIN ? r.skipped * TILE : 0;
     row = threadIdx.x / CH;
     const int c = threadIdx.x % CH ^ swizzle<DP>(row);  // LDS is filled in order: the swizzle is the source's
     in_row = 8 * c < a.dim;
@@ -202,25 +247,7 @@ struct Keys {
     k += TILE * k_t;
     v += TILE * v_t;
     left -= TILE;
-  }
-};
-
-// The rows' side: a wave's 32 query rows of a workgroup's 128
-struct Rows {
-  int pos, head, limit, all_see, any_sees, tiles;
-  bool valid;
-  __device__ __forceinline__ Rows(const Attend& a, const Place& p, int w) {
-    const int rows = p.nq * a.group, off = p.nk - p.nq;
-    const int row0 = p.tile * QROWS + 32 * w, row = row0 + threadIdx.x % 32;
-    valid = row < rows;
-    pos = row / a.group;
-    head = p.kv * a.group + row % a.group;
-    limit = valid ? pos + off : -1;  // the row's last key (below 0: none)
-    // of the wave's rows: the last key that all see, and the last that any sees; the workgroup's tiles of keys
-    all_see = row0 < rows ? row0 / a.group + off : -1;
-    any_sees = row0 < rows ? (row0 + 31 < rows ? row0 + 31 : rows - 1) / a.group + off : -1;
-    const int end = p.tile * QROWS + QROWS < rows ? p.tile * QROWS + QROWS : rows, last = (end - 1) / a.group + off;
-    tiles = last < 0 ? 0 : last / TILE + 1;
+    if (WIN && --before == 0) k += jump * k_t, v += jump * v_t, left -= jump;
   }
 };
 
@@ -228,7 +255,8 @@ struct Rows {
 struct Sight {
   long long token, head;
   int limit;
-  __device__ __forceinline__ Sight(const Attend& a, const Place& p, const Rows& r, int n) {
+  template <bool WIN>
+  __device__ __forceinline__ Sight(const Attend& a, const Place& p, const Rows<WIN>& r, int n) {
     token = p.q0 + __builtin_amdgcn_readlane(r.pos, n);
     head = __builtin_amdgcn_readlane(r.head, n);
     limit = __builtin_amdgcn_readlane(r.limit, n);
@@ -290,8 +318,8 @@ __device__ __forceinline__ F16x add_parts(const Attend& a, size_t slot, int part
 
 // what a wave's rows come to, from their outputs' sums, the maximum that these lack and the probabilities' sum: zeros where
 // a row sees no key, NaN where every score it sees is -inf (0 / 0, as the softmax's definition has it)
-template <typename T, int DP, int N>
-__device__ __forceinline__ void finish_rows(const Attend& a, const Place& p, const Rows& r, int d0, const F16x* acc, float m,
+template <typename T, int DP, int N, bool WIN>
+__device__ __forceinline__ void finish_rows(const Attend& a, const Place& p, const Rows<WIN>& r, int d0, const F16x* acc, float m,
                                             float sum) {
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
   const float c = a.scale * LOG2E;
@@ -301,12 +329,19 @@ __device__ __forceinline__ void finish_rows(const Attend& a, const Place& p, con
   const unsigned bad = bad_columns(r.valid && not_finite<N>(acc) != 0.0f);
   store_rows<N>(r.valid && !(bad >> n & 1) ? (T*)a.out + (token * a.heads + r.head) * dim : nullptr, d0, dim, h, acc,
                 r.limit < 0 ? 0.0f : 1.0f / sum);
+  if (WIN && a.rest)
+    store_rests<N>(r.valid ? (T*)a.rest + (token * a.heads + r.head) * dim : nullptr, d0, dim, h, acc,
+                   r.limit < 0 || (bad >> n & 1) ? 0.0f : 1.0f / sum);
   for (unsigned left = bad; left; left &= left - 1) {
     const Sight one(a, p, r, __builtin_ctz(left));
     const Row<DP> qr((const T*)a.q + one.token * a.q_t + one.head * a.q_h, dim);
     Row<DP> o = {};
     float top = -INFINITY, total = 0.0f;
     for (int j = 0; j <= one.limit && total == total; ++j) {
+      if (WIN && window_hides(a, j, one.limit)) {
+        j = one.limit - a.window;
+        continue;
+      }
       const float x = qr.dot(Row<DP>((const T*)a.k + (p.k0 + j) * a.k_t + p.kv * a.k_h, dim)) * c, top1 = fmaxf(top, x);
       const float base1 = top1 == -INFINITY ? 0.0f : top1, f = exp2_fast(top - base1), pr = exp2_fast(x - base1);
       total = total * f + pr;
@@ -320,7 +355,7 @@ __device__ __forceinline__ void finish_rows(const Attend& a, const Place& p, con
   }
 }
 
-template <typename T, int DP, bool SPLIT>
+template <typename T, int DP, bool SPLIT, bool WIN>
 __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
   constexpr int KS = DP / 16, DT = DP / 32;
   __shared__ __align__(16) T ks[2][TILE * DP];
@@ -328,11 +363,11 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
   Place p;
   if (!place_of_block(a, 0, SPLIT ? a.parts_q : 1, p)) return;
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
-  const Rows r(a, p, uniform(threadIdx.x / 64));
+  const Rows<WIN> r(a, p, uniform(threadIdx.x / 64));
   const Slice my(r.tiles, SPLIT ? a.parts_q : 1, SPLIT ? p.part : 0);
   const int first = SPLIT ? my.first : 0, end = SPLIT ? my.end : r.tiles;
   if (SPLIT && p.part >= my.parts) return;
-  Keys<DP, T> keys(a, p, first);
+  Keys<DP, T, WIN> keys(a, p, r, first);
   if (first < end) keys.next(ks[first & 1], vs[first & 1]);
   V8<T> q[KS];
   load_rows<DP>(r.valid ? (const T*)a.q + (long long)(p.q0 + r.pos) * a.q_t + (long long)r.head * a.q_h : nullptr, dim, h,
@@ -341,27 +376,28 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
   float m = -INFINITY, sum = 0.0f;
   const float c = a.scale * LOG2E;
   for (int t = first; t < end; ++t) {
-    const int key0 = t * TILE;
+    const int key0 = r.tile_of(t) * TILE;
     const T *kt = ks[t & 1], *vt = vs[t & 1];
     loads_done();
     __syncthreads();  // this tile is there for all, and all are done with the one before
     if (t + 1 < end) keys.next(ks[(t + 1) & 1], vs[(t + 1) & 1]);
     if (key0 > r.any_sees) continue;
-    const bool second = key0 + 32 <= r.any_sees;
+    const bool first_half = r.sees(a, key0), second = key0 + 32 <= r.any_sees && r.sees(a, key0 + 32);
+    if (WIN && !first_half && !second) continue;
     F16x s[2] = {};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (i == 1 && !second) {
+      if (i == 1 ? !second : WIN && !first_half) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[1][j] = -INFINITY;
-        break;
+        for (int j = 0; j < 16; ++j) s[i][j] = -INFINITY;
+        continue;
       }
 #pragma unroll
       for (int x = 0; x < KS; ++x) s[i] = mfma(read_rows<DP>(kt, 32 * i, x, n, h), q[x], s[i]);
-      if (key0 + 32 * i + 31 > r.all_see)
+      if (r.masks(a, key0 + 32 * i))
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (key0 + 32 * i + j % 4 + 8 * (j / 4) + 4 * h > r.limit) s[i][j] = -INFINITY;
+          if (r.hides(a, key0 + 32 * i + j % 4 + 8 * (j / 4) + 4 * h)) s[i][j] = -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
@@ -392,6 +428,7 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       if (x == 2 && !second) break;
+      if (WIN && x < 2 && !first_half) continue;
       const V8<T> pr = pack<T>(s[x / 2], x % 2);
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[d] = mfma(read_columns<DP>(vt, 16 * x, d, l), pr, acc[d]);
@@ -404,16 +441,16 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
     mine.at[64 * 16 * DT] = m, mine.at[64 * (16 * DT + 1)] = sum;
     return;
   }
-  finish_rows<T, DP, DT>(a, p, r, 0, acc, m, sum);
+  finish_rows<T, DP, DT, WIN>(a, p, r, 0, acc, m, sum);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool WIN>
 __global__ __launch_bounds__(256) void k_attend_join(Attend a) {
   constexpr int DT = DP / 32, N = DP / 2 + 2;
   const int wave = blockIdx.y / DT, block = blockIdx.y % DT;
   Place p;
   if (!place_of_block(a, 0, 1, p)) return;
-  const Rows r(a, p, wave);
+  const Rows<WIN> r(a, p, wave);
   const int parts = Slice(r.tiles, a.parts_q, 0).parts;
   if (parts == 1) return;
   const size_t slot = (size_t)p.at * a.parts_q;
@@ -426,7 +463,7 @@ __global__ __launch_bounds__(256) void k_attend_join(Attend a) {
 #pragma unroll 8
   for (int i = 0; i < parts; ++i) sum += exp2_fast((stat(i, 0) - base) * c) * stat(i, 1);
   const F16x acc = add_parts<N>(a, slot, parts, wave, block, [&](int i) { return exp2_fast((stat(i, 0) - base) * c); });
-  if (threadIdx.x < 64) finish_rows<T, DP, 1>(a, p, r, 32 * block, &acc, m, sum);
+  if (threadIdx.x < 64) finish_rows<T, DP, 1, WIN>(a, p, r, 32 * block, &acc, m, sum);
 }
 
 // ---- backward: the queries' gradient --------------------------------------------------------------------------------
@@ -435,8 +472,8 @@ __global__ __launch_bounds__(256) void k_attend_join(Attend a) {
 // the third. Both gradients from one kernel would need atomics on dq, whose order changes results from run to run, or a
 // buffer of float32 a key tile: dq has a kernel of its own, at two products of seven computed again.
 
-template <typename T, int DP, int N>
-__device__ __forceinline__ void finish_dq(const Attend& a, const Place& p, const Rows& r, int d0, const F16x* acc, float lse,
+template <typename T, int DP, int N, bool WIN>
+__device__ __forceinline__ void finish_dq(const Attend& a, const Place& p, const Rows<WIN>& r, int d0, const F16x* acc, float lse,
                                           float delta) {
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
   const float c = a.scale * LOG2E;
@@ -452,6 +489,10 @@ __device__ __forceinline__ void finish_dq(const Attend& a, const Place& p, const
     const float lse1 = __shfl(lse, i), delta1 = __shfl(delta, i);
     Row<DP> o = {};
     for (int j = 0; j <= one.limit && !o.all_nan(dim); ++j) {
+      if (WIN && window_hides(a, j, one.limit)) {
+        j = one.limit - a.window;
+        continue;
+      }
       const Row<DP> kr((const T*)a.k + (p.k0 + j) * a.k_t + p.kv * a.k_h, dim);
       const float dp = gr.dot(Row<DP>((const T*)a.v + (p.k0 + j) * a.v_t + p.kv * a.v_h, dim));
       o.add(exp2_fast(qr.dot(kr) * c - lse1) * (dp - delta1), kr);
@@ -460,7 +501,7 @@ __device__ __forceinline__ void finish_dq(const Attend& a, const Place& p, const
   }
 }
 
-template <typename T, int DP, bool SPLIT>
+template <typename T, int DP, bool SPLIT, bool WIN>
 __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
   constexpr int KS = DP / 16, DT = DP / 32;
   __shared__ __align__(16) T ks[2][TILE * DP];
@@ -468,11 +509,11 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
   Place p;
   if (!place_of_block(a, 0, SPLIT ? a.parts_q : 1, p)) return;
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim;
-  const Rows r(a, p, uniform(threadIdx.x / 64));
+  const Rows<WIN> r(a, p, uniform(threadIdx.x / 64));
   const Slice my(r.tiles, SPLIT ? a.parts_q : 1, SPLIT ? p.part : 0);
   const int first = SPLIT ? my.first : 0, end = SPLIT ? my.end : r.tiles;
   if (SPLIT && p.part >= my.parts) return;
-  Keys<DP, T> keys(a, p, first);
+  Keys<DP, T, WIN> keys(a, p, r, first);
   if (first < end) keys.next(ks[first & 1], vs[first & 1]);
   const long long token = p.q0 + r.pos;
   V8<T> q[KS], g[KS];
@@ -488,10 +529,10 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
       s = mfma(read_rows<DP>(kt, 32 * i, x, n, h), q[x], s);
       dp = mfma(read_rows<DP>(vt, 32 * i, x, n, h), g[x], dp);
     }
-    if (key0 + 32 * i + 31 > r.all_see)
+    if (r.masks(a, key0 + 32 * i))
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        if (key0 + 32 * i + j % 4 + 8 * (j / 4) + 4 * h > r.limit) s[j] = -INFINITY, dp[j] = 0.0f;
+        if (r.hides(a, key0 + 32 * i + j % 4 + 8 * (j / 4) + 4 * h)) s[j] = -INFINITY, dp[j] = 0.0f;
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[j] = exp2_fast(fmaf(s[j], c, -lse));
   };
@@ -506,12 +547,19 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta += (float)o[s][e] * (float)g[s][e];
+    if (WIN && a.rest) {  // a narrow window: few keys share every row
+      load_rows<DP>(r.valid ? (const T*)a.rest + (token * a.heads + r.head) * dim : nullptr, dim, h, o);
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta += (float)o[s][e] * (float)g[s][e];
+    }
     delta = add_halves(delta);
   }
   F16x acc[DT] = {};
   Lift<T> lift;
   for (int t = first; t < end; ++t) {
-    const int key0 = t * TILE;
+    const int key0 = r.tile_of(t) * TILE;
     const T *kt = ks[t & 1], *vt = vs[t & 1];
     loads_done();
     __syncthreads();
@@ -529,6 +577,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (key0 + 32 * i > r.any_sees) break;
+      if (WIN && !r.sees(a, key0 + 32 * i)) continue;
       F16x s, dp;
       products(kt, vt, key0, i, s, dp);
 #pragma unroll
@@ -548,23 +597,23 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
     RowsPart<DP>(a, (size_t)p.at * a.parts_q + p.part, uniform(threadIdx.x / 64)).put(0, acc, DT);
     return;
   }
-  finish_dq<T, DP, DT>(a, p, r, 0, acc, lse, delta);
+  finish_dq<T, DP, DT, WIN>(a, p, r, 0, acc, lse, delta);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool WIN>
 __global__ __launch_bounds__(256) void k_attend_dq_join(Attend a) {
   constexpr int DT = DP / 32;
   const int wave = blockIdx.y / DT, block = blockIdx.y % DT;
   Place p;
   if (!place_of_block(a, 0, 1, p)) return;
-  const Rows r(a, p, wave);
+  const Rows<WIN> r(a, p, wave);
   const int parts = Slice(r.tiles, a.parts_q, 0).parts;
   if (parts == 1) return;
   const F16x acc =
       add_parts<DP / 2 + 2>(a, (size_t)p.at * a.parts_q, parts, wave, block, [](int) { return 1.0f; });
   const long long at = (long long)r.head * a.tq + p.q0 + r.pos;
   if (threadIdx.x < 64)
-    finish_dq<T, DP, 1>(a, p, r, 32 * block, &acc, r.valid ? a.lse[at] : INFINITY, r.valid ? a.delta[at] : 0.0f);
+    finish_dq<T, DP, 1, WIN>(a, p, r, 32 * block, &acc, r.valid ? a.lse[at] : INFINITY, r.valid ? a.delta[at] : 0.0f);
 }
 
 // ---- backward: the keys' and values' gradients ----------------------------------------------------------------------
@@ -589,11 +638,18 @@ struct DkvTiles {
 // nothing (forward 249 us to 260). The wait for the next tile's load stands between the first products and the column
 // operands here; the eight waves fill a CU's LDS, so that no other workgroup covers it.
 enum Role { BOTH, KEYS, VALUES };
+template <bool WIN>
 struct RowTiles {  // the rows that see a key tile, in tiles of RT rows or a little less
   int used, first, tiles;
+  int rows;  // their end
   __device__ __forceinline__ RowTiles(const Attend& a, const Place& p, int kw, int rt) {
     used = a.group <= rt ? rt / a.group * a.group : rt;
-    const int rows = p.nq * a.group;
+    rows = p.nq * a.group;
+    if (WIN && p.tile * 32 * kw >= a.sinks) {  // no sinks: the first token behind the last key's window
+      const int keys = (p.tile + 1) * 32 * kw < p.nk ? (p.tile + 1) * 32 * kw : p.nk;
+      const long long end = (long long)keys - 1 + a.window - (p.nk - p.nq);
+      rows = end < p.nq ? (end > 0 ? (int)end : 0) * a.group : rows;
+    }
     const int from = p.tile * 32 * kw - (p.nk - p.nq);  // the first token that sees the tile's first key
     first = (from > 0 ? from : 0) * a.group;
     tiles = rows > first ? (rows - 1 - first) / used + 1 : 0;
@@ -604,7 +660,7 @@ constexpr int KEY_PART = 64;
 __device__ __forceinline__ size_t key_slot(const Attend& a, const Place& p, int role) {
   return ((size_t)p.at * (role == BOTH ? 1 : 2) + (role == VALUES)) * a.parts_k;
 }
-template <typename T, int DP, int N, int ROLE>
+template <typename T, int DP, int N, int ROLE, bool WIN>
 __device__ __forceinline__ void finish_dkv(const Attend& a, const Place& p, int key0, int d0, const F16x* dk, const F16x* dv) {
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim, group = a.group;
   const int rows = p.nq * group, off = p.nk - p.nq, key = key0 + n;
@@ -623,6 +679,7 @@ __device__ __forceinline__ void finish_dkv(const Attend& a, const Place& p, int 
     Row<DP> ok = {}, ov = {};
     for (int r = (one - off > 0 ? one - off : 0) * group;
          r < rows && !((ROLE == VALUES || ok.all_nan(dim)) && (ROLE == KEYS || ov.all_nan(dim))); ++r) {
+      if (WIN && window_hides(a, one, r / group + off)) continue;
       const long long token = p.q0 + r / group, head = p.kv * group + r % group;
       const Row<DP> qr((const T*)a.q + token * a.q_t + head * a.q_h, dim);
       const Row<DP> gr((const T*)a.dout + token * a.do_t + head * a.do_h, dim);
@@ -636,7 +693,7 @@ __device__ __forceinline__ void finish_dkv(const Attend& a, const Place& p, int 
     if (ROLE != KEYS) ov.store((T*)a.dv + to, d0, d1, 1.0f);
   }
 }
-template <typename T, int DP, int KW, int WAVES, int ROLE, bool PARTS>
+template <typename T, int DP, int KW, int WAVES, int ROLE, bool PARTS, bool WIN>
 __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, WAVES>& lds) {
   constexpr int RT = DkvTiles<T, DP, WAVES>::RT;
   constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 64 * WAVES / CH, SPLIT = WAVES / KW;
@@ -657,15 +714,15 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
     }
   };
   const int kw = w % KW, split = w / KW;
-  const int rows = p.nq * group, off = p.nk - p.nq;
+  const int off = p.nk - p.nq;
   const int key0 = p.tile * 32 * KW + 32 * kw, key = key0 + n;
   const bool valid = key < p.nk;
   const float c = a.scale * LOG2E;
 
   // Row tiles start at whole tokens (but for groups above RT, whose rows' places are computed anew for each tile), so
   // that a thread's rows keep their distance from the tile's first token: RT or a little less rows are used of each.
-  const RowTiles all(a, p, KW, RT);
-  const int used = all.used, first = all.first, back = used / group;  // back: tokens of a tile
+  const RowTiles<WIN> all(a, p, KW, RT);
+  const int rows = all.rows, used = all.used, first = all.first, back = used / group;  // back: tokens of a tile
   auto chunk = [&](int i) { return tid % CH ^ swizzle<DP>(tid / CH + i * STEP); };
   const T *qp[N], *gp[N];  // this thread's rows of the next tile to load, and its row's place in lse and delta
   long long stat = 0;
@@ -740,6 +797,7 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
       const int low = token + (group <= RT ? tokens(32 * i) : 0) + off;
       const int most = token + (group <= RT ? tokens(32 * i + 31 < used ? 32 * i + 31 : used - 1) : 1) + off;
       if (32 * i >= used || r0 + 32 * i >= rows || most < key0) continue;
+      if (WIN && low - a.window >= key0 + 31 && key0 >= a.sinks) continue;
       F16x s = {}, dp = {};
 #pragma unroll
       for (int y = 0; y < KS; y += 4) {
@@ -767,7 +825,7 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
           if (ROLE != VALUES) qc[x][d] = read_columns<DP>(qt, 32 * i + 16 * x, d, l);
         }
       phase();
-      const bool masked = low < key0 + 31;
+      const bool masked = low < key0 + 31 || (WIN && key0 <= most - a.window && key0 + 31 >= a.sinks);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int at = 32 * i + 8 * j + 4 * h;
@@ -783,7 +841,7 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
           const I4 li = *(const I4*)(places_of[turn] + at) + (token + off);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (key > li[e]) s[4 * j + e] = dp[4 * j + e] = 0.0f;
+            if (key > li[e] || (WIN && window_hides(a, key, li[e]))) s[4 * j + e] = dp[4 * j + e] = 0.0f;
         }
       }
       if (ROLE != VALUES) lift.template scale<DT>(dp, dk);
@@ -840,40 +898,40 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
     if (ROLE != KEYS) mine.put(ROLE == BOTH ? DT : 0, dv, DT);
     return;
   }
-  finish_dkv<T, DP, DT, ROLE>(a, p, key0, 0, dk, dv);
+  finish_dkv<T, DP, DT, ROLE, WIN>(a, p, key0, 0, dk, dv);
 }
 
-template <typename T, int DP, int KW, int WAVES, bool PARTS>
+template <typename T, int DP, int KW, int WAVES, bool PARTS, bool WIN>
 __global__ __launch_bounds__(WAVES == 8 ? 512 : 256) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_dkv(Attend a) {
   __shared__ DkvTiles<T, DP, WAVES> lds[WAVES == 1 ? 4 : 1];
   const int parts = PARTS ? a.parts_k : 1;
   Place p;
   if constexpr (WAVES == 1) {  // each wave a tile of its own
     const int w = uniform(threadIdx.x / 64);
-    if (place(a, 1, blockIdx.x * 4 + w, p)) dkv_tile<T, DP, KW, WAVES, BOTH, false>(a, p, lds[w]);
+    if (place(a, 1, blockIdx.x * 4 + w, p)) dkv_tile<T, DP, KW, WAVES, BOTH, false, WIN>(a, p, lds[w]);
   } else if constexpr (DP == 64) {
-    if (place_of_block(a, 1, parts, p)) dkv_tile<T, DP, KW, WAVES, BOTH, PARTS>(a, p, lds[0]);
+    if (place_of_block(a, 1, parts, p)) dkv_tile<T, DP, KW, WAVES, BOTH, PARTS, WIN>(a, p, lds[0]);
   } else {
     if (!place_of_block(a, 1, 2 * parts, p)) return;
-    if (p.part >= parts) dkv_tile<T, DP, KW, WAVES, VALUES, PARTS>(a, p, lds[0]);
-    else dkv_tile<T, DP, KW, WAVES, KEYS, PARTS>(a, p, lds[0]);
+    if (p.part >= parts) dkv_tile<T, DP, KW, WAVES, VALUES, PARTS, WIN>(a, p, lds[0]);
+    else dkv_tile<T, DP, KW, WAVES, KEYS, PARTS, WIN>(a, p, lds[0]);
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool WIN>
 __global__ __launch_bounds__(256) void k_attend_dkv_join(Attend a) {
   constexpr int DT = DP / 32;
   const int role = blockIdx.y / (4 * DT) ? VALUES : KEYS, wave = blockIdx.y / DT % 4, block = blockIdx.y % DT;
   Place p;
   if (!place_of_block(a, 1, 1, p)) return;
-  const int parts = Slice(RowTiles(a, p, 4, DkvTiles<T, DP, DP / 16>::RT).tiles, a.parts_k, 0).parts;
+  const int parts = Slice(RowTiles<WIN>(a, p, 4, DkvTiles<T, DP, DP / 16>::RT).tiles, a.parts_k, 0).parts;
   if (parts == 1) return;
   const F16x acc = add_parts<KEY_PART>(a, key_slot(a, p, DP == 64 ? BOTH : role), parts, wave,
                                        (DP == 64 && role == VALUES ? DT : 0) + block, [](int) { return 1.0f; });
   if (threadIdx.x >= 64) return;
   const int key0 = p.tile * 128 + wave * 32;
-  if (role == KEYS) finish_dkv<T, DP, 1, KEYS>(a, p, key0, 32 * block, &acc, nullptr);
-  else finish_dkv<T, DP, 1, VALUES>(a, p, key0, 32 * block, nullptr, &acc);
+  if (role == KEYS) finish_dkv<T, DP, 1, KEYS, WIN>(a, p, key0, 32 * block, &acc, nullptr);
+  else finish_dkv<T, DP, 1, VALUES, WIN>(a, p, key0, 32 * block, nullptr, &acc);
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------
@@ -905,84 +963,92 @@ int parts_of(long long blocks, long long others, int tile, int seqs) {
   const long long most = 2 * others / ((long long)(seqs > 0 ? seqs : 1) * LEAST * tile), fill = FILL / (blocks > 0 ? blocks : 1);
   return most < 4 || fill < 2 ? 1 : (int)(fill < most ? fill : most);
 }
-int query_parts(int kv_heads, int seqs, int tq, int tk, int group) {
-  return parts_of(order_queries(seqs, tq, group) * kv_heads, tk, TILE, seqs);
+// The other side's tokens, of which a window leaves each row (key) no more than itself.
+long long others_of(int tokens, int seqs, int window, int more) {
+  const long long most = ((long long)window + more) * (seqs > 0 ? seqs : 1);
+  return window && most < tokens ? most : tokens;
 }
-int key_parts(int kv_heads, int dim, int seqs, int tq, int tk, int group) {
+int query_parts(int kv_heads, int seqs, int tq, int tk, int group, int window, int sinks) {
+  return parts_of(order_queries(seqs, tq, group) * kv_heads, others_of(tk, seqs, window, sinks), TILE, seqs);
+}
+int key_parts(int kv_heads, int dim, int seqs, int tq, int tk, int group, int window) {
   const int kw = key_waves(dim, seqs, tk);
-  return kw < 4 ? 1 : parts_of(order_keys(seqs, tk, kw) * kv_heads * (dim <= 64 ? 1 : 2), (long long)tq * group,
+  return kw < 4 ? 1 : parts_of(order_keys(seqs, tk, kw) * kv_heads * (dim <= 64 ? 1 : 2), others_of(tq, seqs, window, 128) * group,
                                dim <= 64 ? 64 : 128, seqs);
 }
 size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group) {
   return sizeof(int) * (ORDER_HEAD + 2 * (size_t)(order_queries(seqs, tq, group) +
                                                   order_keys(seqs, tk, key_waves(dim, seqs, tk))));
 }
-size_t attend_scratch_bytes(int kv_heads, int dim, int seqs, int tq, int tk, int group, bool vjp) {
-  const size_t pq = query_parts(kv_heads, seqs, tq, tk, group), pk = vjp ? key_parts(kv_heads, dim, seqs, tq, tk, group) : 1;
+size_t attend_scratch_bytes(int kv_heads, int dim, int seqs, int tq, int tk, int group, int window, int sinks, bool vjp) {
+  const size_t pq = query_parts(kv_heads, seqs, tq, tk, group, window, sinks);
+  const size_t pk = vjp ? key_parts(kv_heads, dim, seqs, tq, tk, group, window) : 1;
   const size_t q = pq == 1 ? 0 : pq * order_queries(seqs, tq, group) * kv_heads * (dim <= 64 ? RowsPart<64>::SIZE : RowsPart<128>::SIZE);
   const size_t k = pk == 1 ? 0 : pk * order_keys(seqs, tk, 4) * kv_heads * (dim <= 64 ? 1 : 2) * Part<KEY_PART>::SIZE;
   return sizeof(float) * (q > k ? q : k);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool WIN>
 int attend(hipStream_t st, const Attend& a) {
   const long long tiles = order_queries(a.seqs, a.tq, a.group);
   if (a.parts_q == 1) {
-    k_attend<T, DP, false><<<blocks_of(a, tiles, 1), 256, 0, st>>>(a);
+    k_attend<T, DP, false, WIN><<<blocks_of(a, tiles, 1), 256, 0, st>>>(a);
   } else {
-    k_attend<T, DP, true><<<blocks_of(a, tiles, a.parts_q), 256, 0, st>>>(a);
+    k_attend<T, DP, true, WIN><<<blocks_of(a, tiles, a.parts_q), 256, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    k_attend_join<T, DP><<<dim3(blocks_of(a, tiles, 1), 4 * (DP / 32)), 256, 0, st>>>(a);
+    k_attend_join<T, DP, WIN><<<dim3(blocks_of(a, tiles, 1), 4 * (DP / 32)), 256, 0, st>>>(a);
   }
   return (int)hipGetLastError();
 }
-template <typename T, int DP>
+template <typename T, int DP, bool WIN>
 int attend_dq(hipStream_t st, const Attend& a) {
   const long long tiles = order_queries(a.seqs, a.tq, a.group);
   if (a.parts_q == 1) {
-    k_attend_dq<T, DP, false><<<blocks_of(a, tiles, 1), 256, 0, st>>>(a);
+    k_attend_dq<T, DP, false, WIN><<<blocks_of(a, tiles, 1), 256, 0, st>>>(a);
   } else {
-    k_attend_dq<T, DP, true><<<blocks_of(a, tiles, a.parts_q), 256, 0, st>>>(a);
+    k_attend_dq<T, DP, true, WIN><<<blocks_of(a, tiles, a.parts_q), 256, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    k_attend_dq_join<T, DP><<<dim3(blocks_of(a, tiles, 1), 4 * (DP / 32)), 256, 0, st>>>(a);
+    k_attend_dq_join<T, DP, WIN><<<dim3(blocks_of(a, tiles, 1), 4 * (DP / 32)), 256, 0, st>>>(a);
   }
   return (int)hipGetLastError();
 }
-template <typename T, int DP>
+template <typename T, int DP, bool WIN>
 int attend_vjp(hipStream_t st, const Attend& a) {
   if (a.tq) {
-    const int e = attend_dq<T, DP>(st, a);
+    const int e = attend_dq<T, DP, WIN>(st, a);
     if (e) return e;
   }
   if (!a.tk) return 0;
   const long long tiles = order_keys(a.seqs, a.tk, a.key_waves);
   constexpr int ROLES = DP == 64 ? 1 : 2, THREADS = DP == 64 ? 256 : 512;
   if (a.parts_k > 1) {
-    k_attend_dkv<T, DP, 4, DP / 16, true><<<blocks_of(a, tiles, ROLES * a.parts_k), THREADS, 0, st>>>(a);
+    k_attend_dkv<T, DP, 4, DP / 16, true, WIN><<<blocks_of(a, tiles, ROLES * a.parts_k), THREADS, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    k_attend_dkv_join<T, DP><<<dim3(blocks_of(a, tiles, 1), 8 * (DP / 32)), 256, 0, st>>>(a);
+    k_attend_dkv_join<T, DP, WIN><<<dim3(blocks_of(a, tiles, 1), 8 * (DP / 32)), 256, 0, st>>>(a);
   } else if (a.key_waves == 4) {
-    k_attend_dkv<T, DP, 4, DP / 16, false><<<blocks_of(a, tiles, ROLES), THREADS, 0, st>>>(a);
+    k_attend_dkv<T, DP, 4, DP / 16, false, WIN><<<blocks_of(a, tiles, ROLES), THREADS, 0, st>>>(a);
   } else if constexpr (DP == 64) {
-    k_attend_dkv<T, 64, 1, 1, false><<<(unsigned)((tiles * a.kv_heads + 3) / 4), 256, 0, st>>>(a);
+    k_attend_dkv<T, 64, 1, 1, false, WIN><<<(unsigned)((tiles * a.kv_heads + 3) / 4), 256, 0, st>>>(a);
   }
   return (int)hipGetLastError();
 }
 
+template <bool WIN>
 int launch_attend(hipStream_t st, int type, const Attend& a) {
-  k_attend_order<<<1, 1024, 0, st>>>(a.seqs, a.tq, a.tk, a.group, a.key_waves, a.by_sequence, a.starts_q, a.starts_k,
-                                  (int*)a.order);
+  k_attend_order<<<1, 1024, 0, st>>>(a.seqs, a.tq, a.tk, a.group, a.key_waves, a.by_sequence, WIN ? a.window : 0, WIN ? a.sinks : 0,
+                                  a.starts_q, a.starts_k, (int*)a.order);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.tq) return (int)e;
-  if (type == BF16) return a.dim <= 64 ? attend<__bf16, 64>(st, a) : attend<__bf16, 128>(st, a);
-  return a.dim <= 64 ? attend<_Float16, 64>(st, a) : attend<_Float16, 128>(st, a);
+  if (type == BF16) return a.dim <= 64 ? attend<__bf16, 64, WIN>(st, a) : attend<__bf16, 128, WIN>(st, a);
+  return a.dim <= 64 ? attend<_Float16, 64, WIN>(st, a) : attend<_Float16, 128, WIN>(st, a);
 }
+template <bool WIN>
 int launch_attend_vjp(hipStream_t st, int type, const Attend& a) {
-  if (type == BF16) return a.dim <= 64 ? attend_vjp<__bf16, 64>(st, a) : attend_vjp<__bf16, 128>(st, a);
-  return a.dim <= 64 ? attend_vjp<_Float16, 64>(st, a) : attend_vjp<_Float16, 128>(st, a);
+  if (type == BF16) return a.dim <= 64 ? attend_vjp<__bf16, 64, WIN>(st, a) : attend_vjp<__bf16, 128, WIN>(st, a);
+  return a.dim <= 64 ? attend_vjp<_Float16, 64, WIN>(st, a) : attend_vjp<_Float16, 128, WIN>(st, a);
 }
 
 }  // namespace pol
@@ -994,25 +1060,70 @@ bool attention_takes(int type, int heads, int kv_heads, int dim, int seqs, int t
 }
 }  // namespace
 
+// A window as long as the keys hides nothing: the kernels without one. Else its length, with the sinks within the keys.
+namespace {
+int window_of(int window, int tk) { return window < tk ? window : 0; }
+int sinks_of(int sinks, int tk) { return sinks < tk ? sinks : tk; }
+}  // namespace
+
 extern "C" {
 
-int dk_attention(hipStream_t st, int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk, const void* q,
-                 long long q_t, long long q_h, const void* k, long long k_t, long long k_h, const void* v,
-                 long long v_t, long long v_h, const int* starts_q, const int* starts_k, float scale, void* out,
-                 float* lse, void* work, void* scratch) {
-  if (!attention_takes(type, heads, kv_heads, dim, seqs, tq, tk) || !(scale > 0.0f) || !starts_q || !starts_k || !work ||
-      (tq && (!q || !out)) || (tk && (!k || !v)) ||
-      (!scratch && dk_attention_scratch_bytes(heads, kv_heads, dim, seqs, tq, tk, 0)))
+int dk_attention_window(hipStream_t st, int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk, const void* q,
+                        long long q_t, long long q_h, const void* k, long long k_t, long long k_h, const void* v, long long v_t,
+                        long long v_h, const int* starts_q, const int* starts_k, float scale, int window, int sinks, void* out,
+                        void* rest, float* lse, void* work, void* scratch) {
+  if (!attention_takes(type, heads, kv_heads, dim, seqs, tq, tk) || !(scale > 0.0f) || window < 0 || sinks < 0 || !starts_q ||
+      !starts_k || !work || (tq && (!q || !out)) || (tk && (!k || !v)) ||
+      (!scratch && dk_attention_window_scratch_bytes(heads, kv_heads, dim, seqs, tq, tk, window, sinks, 0)))
     return (int)hipErrorInvalidValue;
   pol::Attend a = {};
+  a.window = window_of(window, tk), a.sinks = sinks_of(sinks, tk), a.rest = rest;
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
   a.key_waves = pol::key_waves(dim, seqs, tk);
   a.by_sequence = pol::by_sequence(dim, seqs, tq, tk);
-  a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group), a.scratch = (float*)scratch;
+  a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group, a.window, a.sinks), a.scratch = (float*)scratch;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.out = out, a.lse = lse, a.order = (const int*)work;
-  return pol::launch_attend(st, type, a);
+  return a.window ? pol::launch_attend<true>(st, type, a) : pol::launch_attend<false>(st, type, a);
+}
+
+int dk_attention_window_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk, const void* q,
+                            long long q_t, long long q_h, const void* k, long long k_t, long long k_h, const void* v, long long v_t,
+                            long long v_h, const int* starts_q, const int* starts_k, float scale, int window, int sinks,
+                            const void* out, const void* rest, const float* lse, const void* work, const void* dout,
+                            long long do_t, long long do_h, float* delta, void* dq, void* dk, void* dv, void* scratch) {
+  if (!attention_takes(type, heads, kv_heads, dim, seqs, tq, tk) || !(scale > 0.0f) || window < 0 || sinks < 0 || !starts_q ||
+      !starts_k || !work || (tq && (!q || !out || !lse || !dout || !delta || !dq)) || (tk && (!k || !v || !dk || !dv)) ||
+      (!scratch && dk_attention_window_scratch_bytes(heads, kv_heads, dim, seqs, tq, tk, window, sinks, 1)))
+    return (int)hipErrorInvalidValue;
+  pol::Attend a = {};
+  a.window = window_of(window, tk), a.sinks = sinks_of(sinks, tk), a.rest = const_cast<void*>(rest);
+  a.q = q, a.k = k, a.v = v;
+  a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
+  a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
+  a.key_waves = pol::key_waves(dim, seqs, tk);
+  a.by_sequence = pol::by_sequence(dim, seqs, tq, tk);
+  a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group, a.window, a.sinks), a.scratch = (float*)scratch;
+  a.parts_k = pol::key_parts(kv_heads, dim, seqs, tq, tk, a.group, a.window);
+  a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.order = (const int*)work;
+  a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse);
+  a.dout = dout, a.do_t = do_t, a.do_h = do_h, a.delta = delta, a.dq = dq, a.dk = dk, a.dv = dv;
+  return a.window ? pol::launch_attend_vjp<true>(st, type, a) : pol::launch_attend_vjp<false>(st, type, a);
+}
+
+long long dk_attention_window_scratch_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk, int window, int sinks, int vjp) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads || seqs < 0 || tq < 0 || tk < 0 || window < 0 || sinks < 0) return 0;
+  return (long long)pol::attend_scratch_bytes(kv_heads, dim, seqs, tq, tk, heads / kv_heads, window_of(window, tk),
+                                              sinks_of(sinks, tk), vjp != 0);
+}
+
+int dk_attention(hipStream_t st, int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk, const void* q,
+                 long long q_t, long long q_h, const void* k, long long k_t, long long k_h, const void* v,
+                 long long v_t, long long v_h, const int* starts_q, const int* starts_k, float scale, void* out,
+                 float* lse, void* work, void* scratch) {
+  return dk_attention_window(st, type, heads, kv_heads, dim, seqs, tq, tk, q, q_t, q_h, k, k_t, k_h, v, v_t, v_h, starts_q, starts_k,
+                             scale, 0, 0, out, nullptr, lse, work, scratch);
 }
 
 int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk,
@@ -1021,22 +1132,8 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
                      float scale, const void* out, const float* lse, const void* work, const void* dout,
                      long long do_t, long long do_h, float* delta, void* dq, void* dk, void* dv,
                      void* scratch) {
-  if (!attention_takes(type, heads, kv_heads, dim, seqs, tq, tk) || !(scale > 0.0f) || !starts_q || !starts_k || !work ||
-      (tq && (!q || !out || !lse || !dout || !delta || !dq)) || (tk && (!k || !v || !dk || !dv)) ||
-      (!scratch && dk_attention_scratch_bytes(heads, kv_heads, dim, seqs, tq, tk, 1)))
-    return (int)hipErrorInvalidValue;
-  pol::Attend a = {};
-  a.q = q, a.k = k, a.v = v;
-  a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
-  a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
-  a.key_waves = pol::key_waves(dim, seqs, tk);
-  a.by_sequence = pol::by_sequence(dim, seqs, tq, tk);
-  a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group), a.scratch = (float*)scratch;
-  a.parts_k = pol::key_parts(kv_heads, dim, seqs, tq, tk, a.group);
-  a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.order = (const int*)work;
-  a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse);
-  a.dout = dout, a.do_t = do_t, a.do_h = do_h, a.delta = delta, a.dq = dq, a.dk = dk, a.dv = dv;
-  return pol::launch_attend_vjp(st, type, a);
+  return dk_attention_window_vjp(st, type, heads, kv_heads, dim, seqs, tq, tk, q, q_t, q_h, k, k_t, k_h, v, v_t, v_h, starts_q,
+                                 starts_k, scale, 0, 0, out, nullptr, lse, work, dout, do_t, do_h, delta, dq, dk, dv, scratch);
 }
 
 long long dk_attention_work_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk) {
@@ -1045,8 +1142,7 @@ long long dk_attention_work_bytes(int heads, int kv_heads, int dim, int seqs, in
 }
 
 long long dk_attention_scratch_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk, int vjp) {
-  if (heads < 1 || kv_heads < 1 || heads % kv_heads || seqs < 0 || tq < 0 || tk < 0) return 0;
-  return (long long)pol::attend_scratch_bytes(kv_heads, dim, seqs, tq, tk, heads / kv_heads, vjp != 0);
+  return dk_attention_window_scratch_bytes(heads, kv_heads, dim, seqs, tq, tk, 0, 0, vjp);
 }
 
 }  // extern "C"

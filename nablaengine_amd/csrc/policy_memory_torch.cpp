@@ -3,14 +3,15 @@
 #include "policy_torch.h"
 
 #include "../../include/nablaengine_memory.h"
-#include "policy_sizes.h"
+#include "../../include/nablaengine_policy.h"
 
 namespace {
 
 #define ENTRIES(X)                                                                                                    \
   X(dk_recurrence) X(dk_recurrence_vjp) X(dk_recurrence_carry_bytes) X(dk_recurrence_work_bytes) X(dk_recurrence_step) \
   X(dk_gated_residual) X(dk_gated_residual_vjp) X(dk_gated_residual_work_bytes)             \
-  X(dk_attention_paged) X(dk_attention_paged_work_bytes) X(dk_cache_append)
+  X(dk_attention_paged) X(dk_attention_paged_work_bytes) X(dk_cache_append)                             \
+  X(dk_attention_window) X(dk_attention_window_vjp) X(dk_attention_window_scratch_bytes) X(dk_attention_work_bytes)
 struct Entries {
 #define X(name) decltype(&::name) name;
   ENTRIES(X)
@@ -262,10 +263,78 @@ void cache_append_(const Tensor& k_pages, const Tensor& v_pages, const Tensor& k
     if (!y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
 }
 
+// ---- attention with a window ----------------------------------------------------------------------------------------
+
+struct Sight { int window, sinks; };
+Sight sight_checks(int64_t window, int64_t sinks) {
+  CHECK_VALUE(window >= 1 && sinks >= 0, "window must be at least 1 and sinks at least 0, got ", window, " and ", sinks);
+  return {(int)std::min<int64_t>(window, 1 << 30), (int)std::min<int64_t>(sinks, 1 << 30)};
+}
+Tensor window_scratch(const Heads& h, int seqs, const Tensor& q, const Tensor& k, const Sight& s, int vjp) {
+  const long long bytes = lib.dk_attention_window_scratch_bytes(h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0), s.window,
+                                                                s.sinks, vjp);
+  return bytes ? work_of(q, bytes) : Tensor();
+}
+long long order_words(const Heads& h, int seqs, const Tensor& q, const Tensor& k) {
+  return lib.dk_attention_work_bytes(h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0)) / 4;
+}
+
+// out, lse, work and rest (what the output's rounding took off, for narrow windows)
+std::vector<Tensor> attention_window_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& starts_q,
+                                             const Tensor& starts_k, double scale, int64_t window, int64_t sinks, bool train) {
+  const Heads h = heads_checks(q, k, v, 3);
+  const int seqs = sequences_checks(q, k, starts_q, starts_k, h);
+  const Sight s = sight_checks(window, sinks);
+  check_bound();
+  const Tensor out = at::empty(q.sizes(), q.options());
+  const Tensor lse = at::empty({h.heads, train ? q.size(0) : 0}, q.options().dtype(at::kFloat));
+  const Tensor work = at::empty({order_words(h, seqs, q, k)}, q.options().dtype(at::kInt));
+  const Tensor rest = at::empty(train && window + sinks <= pol::NARROW ? q.sizes() : at::IntArrayRef{0}, q.options());
+  const Tensor scratch = window_scratch(h, seqs, q, k, s, 0);
+  call("the windowed attention launch", q, [&](hipStream_t st) {
+    return lib.dk_attention_window(st, h.type, h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0), q.data_ptr(), q.stride(0),
+                                   q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                   starts_q.data_ptr<int>(), starts_k.data_ptr<int>(), (float)scale, s.window, s.sinks, out.data_ptr(),
+                                   rest.numel() ? rest.data_ptr() : nullptr, train ? lse.data_ptr<float>() : nullptr, work.data_ptr(),
+                                   out_of<void>(scratch));
+  });
+  return {out, lse, work, rest};
+}
+
+// dout: any strides
+std::vector<Tensor> attention_window_backward(const Tensor& grad, const Tensor& q, const Tensor& k, const Tensor& v,
+                                              const Tensor& starts_q, const Tensor& starts_k, const Tensor& out, const Tensor& lse,
+                                              const Tensor& work, const Tensor& rest, double scale, int64_t window, int64_t sinks) {
+  const Heads h = heads_checks(q, k, v, 3);
+  const int seqs = sequences_checks(q, k, starts_q, starts_k, h);
+  const Sight s = sight_checks(window, sinks);
+  check_bound();
+  check_as("dout", grad, q, q.scalar_type(), q.sizes());
+  check_as("out", out, q, q.scalar_type(), q.sizes());
+  if (rest.numel()) check_as("rest", rest, q, q.scalar_type(), q.sizes());
+  const Tensor dout = grad.numel() && grad.stride(2) != 1 ? grad.contiguous() : grad;
+  check_as("lse", lse, q, at::kFloat, {h.heads, q.size(0)});
+  check_as("work", work, q, at::kInt, {order_words(h, seqs, q, k)});
+  CHECK_TYPE(out.is_contiguous() && lse.is_contiguous() && work.is_contiguous() && rest.is_contiguous(),
+             "out, lse, work and rest must be contiguous");
+  const Tensor delta = at::empty(lse.sizes(), lse.options());
+  const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), q.options()), dv = at::empty(k.sizes(), q.options());
+  const Tensor scratch = window_scratch(h, seqs, q, k, s, 1);
+  call("the windowed attention VJP launch", q, [&](hipStream_t st) {
+    return lib.dk_attention_window_vjp(
+        st, h.type, h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
+        k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), starts_q.data_ptr<int>(), starts_k.data_ptr<int>(),
+        (float)scale, s.window, s.sinks, out.data_ptr(), rest.numel() ? rest.data_ptr() : nullptr, lse.data_ptr<float>(),
+        work.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
+        dv.data_ptr(), out_of<void>(scratch));
+  });
+  return {dq, dk, dv};
+}
+
 // ---- autograd -------------------------------------------------------------------------------------------------------
 
 OP(recurrence_forward) OP(recurrence_backward) OP(recurrence_step) OP(gated_residual_forward) OP(gated_residual_backward)
-OP(attention_paged) OP(cache_append_)
+OP(attention_paged) OP(cache_append_) OP(attention_window_forward) OP(attention_window_backward)
 
 OptTensor given(const Tensor& x) { return x.defined() ? OptTensor(x) : OptTensor(); }
 bool wants_any(at::TensorList xs) { return std::any_of(xs.begin(), xs.end(), [](const Tensor& x) { return wants(x); }); }
@@ -401,6 +470,56 @@ void cache_append_autograd(const Tensor& k_pages, const Tensor& v_pages, const T
   cache_append__op().call(k_pages, v_pages, k, v, pages, lengths, starts);
 }
 
+struct WindowBackward : torch::autograd::Function<WindowBackward> {
+  static variable_list forward(AutogradContext*, const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v,
+                               const Tensor& starts_q, const Tensor& starts_k, const Tensor& out, const Tensor& lse,
+                               const Tensor& work, const Tensor& rest, double scale, int64_t window, int64_t sinks) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return attention_window_backward_op().call(dout, q, k, v, starts_q, starts_k, out, lse, work, rest, scale, window, sinks);
+  }
+  FIRST_ORDER("attention")
+};
+struct Window : torch::autograd::Function<Window> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& starts_q,
+                        const Tensor& starts_k, double scale, int64_t window, int64_t sinks) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto r = attention_window_forward_op().call(q, k, v, starts_q, starts_k, scale, window, sinks, true);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->save_for_backward({q, k, v, starts_q, starts_k, r[0], r[1], r[2], r[3]});
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    const auto s = ctx->get_saved_variables();
+    if (!grad[0].defined()) return variable_list(8);
+    const Tensor& dout = grad[0];
+    no_tangents("attention's gradient", dout, s[0], s[1], s[2]);
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const int64_t window = ctx->saved_data["window"].toInt(), sinks = ctx->saved_data["sinks"].toInt();
+    auto run = [&] {
+      if (at::GradMode::is_enabled())
+        return WindowBackward::apply(dout, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], scale, window, sinks);
+      at::AutoDispatchBelowADInplaceOrView below;
+      return attention_window_backward_op().call(dout, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], scale, window, sinks);
+    };
+    const variable_list r = run();
+    return {r[0], r[1], r[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor attention_window_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& starts_q, const Tensor& starts_k,
+                                 double scale, int64_t window, int64_t sinks) {
+  no_tangents("attention", q, k, v);
+  if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v)))
+    return Window::apply(q, k, v, starts_q, starts_k, scale, window, sinks);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return attention_window_forward_op().call(q, k, v, starts_q, starts_k, scale, window, sinks, false)[0];
+}
+Tensor attention_window(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& starts_q, const Tensor& starts_k,
+                        double scale, int64_t window, int64_t sinks) {
+  return attention_window_forward_op().call(q, k, v, starts_q, starts_k, scale, window, sinks, false)[0];
+}
+
 }  // namespace
 
 // the entries' names, in the order in which dk_memory_torch_bind takes their addresses
@@ -433,8 +552,17 @@ TORCH_LIBRARY_FRAGMENT(nablaengine, m) {
         "int sinks) -> Tensor");
   m.def("cache_append_(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor k, Tensor v, Tensor pages, Tensor lengths, Tensor? starts) "
         "-> ()");
+  m.def("attention_window(Tensor q, Tensor k, Tensor v, Tensor starts_q, Tensor starts_k, float scale, int window, int sinks) "
+        "-> Tensor");
+  m.def("attention_window_forward(Tensor q, Tensor k, Tensor v, Tensor starts_q, Tensor starts_k, float scale, int window, "
+        "int sinks, bool train) -> Tensor[]");
+  m.def("attention_window_backward(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor starts_q, Tensor starts_k, Tensor out, "
+        "Tensor lse, Tensor work, Tensor rest, float scale, int window, int sinks) -> Tensor[]");
 }
 TORCH_LIBRARY_IMPL(nablaengine, CompositeExplicitAutograd, m) {
+  m.impl("attention_window", attention_window);
+  m.impl("attention_window_forward", attention_window_forward);
+  m.impl("attention_window_backward", attention_window_backward);
   m.impl("attention_paged", attention_paged);
   m.impl("cache_append_", cache_append_);
   m.impl("recurrence", recurrence);
@@ -450,7 +578,9 @@ TORCH_LIBRARY_IMPL(nablaengine, Autograd, m) {
   m.impl("recurrence_step", recurrence_step_autograd);
   m.impl("gated_residual", gated_residual_autograd);
   m.impl("attention_paged", attention_paged_autograd);
+  m.impl("attention_window", attention_window_autograd);
   m.impl("cache_append_", cache_append_autograd);
-  for (const char* name : {"recurrence_forward", "recurrence_backward", "gated_residual_forward", "gated_residual_backward"})
+  for (const char* name : {"recurrence_forward", "recurrence_backward", "gated_residual_forward", "gated_residual_backward",
+                           "attention_window_forward", "attention_window_backward"})
     m.impl(name, torch::CppFunction::makeFromBoxedFunction<&inner_autograd>());
 }

@@ -17,6 +17,10 @@ constexpr bool attention_sizes(int heads, int kv_heads, int seqs, int tq, int tk
          order_queries(seqs, tq, group) * kv_heads <= most && order_keys(seqs, tk, 1) * kv_heads <= most;
 }
 
+// Windows of so few keys (sinks among them) that the rounding of the outputs is felt in the gradients: what it took off is kept
+// for the backward, as for rows of no more keys without a window.
+constexpr int NARROW = 64;
+
 constexpr int SCAN_TOKENS = 16, SCAN_CHUNK = 128;  // the recurrence's tokens a wave and a workgroup
 
 // whether the recurrence's indices and grids hold these sizes: workgroups of 512 work-items, one a chunk and 64 channels at least

@@ -156,20 +156,6 @@ Tensor clip_grads_out(at::TensorList grads, at::TensorList out, double max_norm)
 
 // ---- attention ------------------------------------------------------------------------------------------------------
 
-int sequences_checks(const Tensor& q, const Tensor& k, const Tensor& starts_q, const Tensor& starts_k, const Heads& h) {
-  for (const auto& [name, x] : {std::pair<const char*, const Tensor&>{"starts_q", starts_q}, {"starts_k", starts_k}}) {
-    check_device(name, x, q);
-    CHECK_TYPE(x.scalar_type() == at::kInt && x.dim() == 1 && x.is_contiguous() && x.numel() >= 1 &&
-                   x.numel() == starts_q.numel(),
-               name, ": expected contiguous int32 offsets, one more than sequences in both, got ", described(x));
-  }
-  const int64_t seqs = starts_q.numel() - 1, most = 1 << 30;
-  CHECK_VALUE(q.size(0) < most && k.size(0) < most && seqs < most &&
-                  pol::attention_sizes(h.heads, h.kv, (int)seqs, (int)q.size(0), (int)k.size(0)),
-              q.size(0), " queries of ", h.heads, " heads and ", k.size(0), " keys of ", h.kv, " in ", seqs,
-              " sequences exceed one launch");
-  return (int)seqs;
-}
 long long order_words(const Heads& h, int seqs, const Tensor& q, const Tensor& k) {
   return lib.dk_attention_work_bytes(h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0)) / 4;
 }

@@ -124,6 +124,11 @@ def _fake_attention_forward(q, k, v, starts_q, starts_k, scale, train):
             starts_q.new_empty((words,))]
 
 
+def _fake_attention_window_forward(q, k, v, starts_q, starts_k, scale, window, sinks, train):
+    rest = q.new_empty(q.shape if train and window + sinks <= 64 else (0,))
+    return _fake_attention_forward(q, k, v, starts_q, starts_k, scale, train) + [rest]
+
+
 def _fake_recurrence(x, gate, starts, initial):
     return x.new_empty(x.shape), x.new_empty((starts.shape[0] - 1, x.shape[1]), dtype=torch.float32)
 
@@ -162,6 +167,8 @@ _FAKES = {"layer_norm": lambda x, *_: x.new_empty(x.shape), "layer_norm_forward"
           "gated_residual_forward": lambda x, u, w, w2, gate, scale, eps, stats: [
               x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty((2, x.numel() // x.shape[-1] if stats else 0), dtype=torch.float32)],
           "gated_residual_backward": _fake_gated_residual_backward,
+          "attention_window": lambda q, *_: q.new_empty(q.shape), "attention_window_forward": _fake_attention_window_forward,
+          "attention_window_backward": lambda dout, q, k, v, *_: [q.new_empty(x.shape) for x in (q, k, v)],
           "attention_paged": lambda q, *_: q.new_empty(q.shape), "cache_append_": lambda *_: None,
           "recurrence_step": lambda x, gate, state: (x.new_empty(x.shape), state.new_empty(x.shape))}
 
@@ -250,7 +257,15 @@ def _scale(scale, q):
     return s
 
 
-def attention(q, k, v, starts_q, starts_k=None, *, scale=None):
+def _sight(window, sinks):
+    """window (0: none) and sinks as numbers."""
+    w, s = 0 if window is None else operator.index(window), operator.index(sinks)
+    if w < (0 if window is None else 1) or s < 0:
+        raise _err(f"window must be None or at least 1 and sinks at least 0, got {window} and {sinks}", ValueError)
+    return w, s
+
+
+def attention(q, k, v, starts_q, starts_k=None, *, scale=None, window=None, sinks=0):
     """Causal attention over packed sequences (episodes of different lengths, one after another), differentiable in q, k
     and v: out = softmax(scale q k^T) v within each sequence, in q's type.
 
@@ -262,11 +277,17 @@ def attention(q, k, v, starts_q, starts_k=None, *, scale=None):
     (nq = 1: one new query over a history). A query that sees no key gives zeros, and so do tokens past the last
     sequence (padding), whose gradients are zero too. scale (> 0) defaults to 1 / sqrt(dim).
 
+    window: of those keys a query sees the `window` last ones only, and the `sinks` first ones of its sequence; the time goes by
+    the keys in sight then. A window that no sequence is longer than hides nothing; without one, sinks have no part.
+
     Scores, softmax statistics and all sums are float32; probabilities and score gradients are rounded to q's type for
     the matrix instructions, as the inputs are (float16: brought inside its range first). A query whose every score is -inf
     gives NaN."""
     starts_k = starts_q if starts_k is None else starts_k
-    s = _scale(scale, q)
+    s, (w, first) = _scale(scale, q), _sight(window, sinks)
+    if w:
+        return _ops(True).attention_window(q, _tensor("k", k), _tensor("v", v), _tensor("starts_q", starts_q),
+                                           _tensor("starts_k", starts_k), s, w, first)
     return _ops().attention(q, _tensor("k", k), _tensor("v", v), _tensor("starts_q", starts_q),
                             _tensor("starts_k", starts_k), s)
 
@@ -328,14 +349,6 @@ def gated_residual(x, u, weight=None, next_weight=None, *, gate=None, scale=None
 
 
 # ---- paged histories ------------------------------------------------------------------------------------------------
-
-def _sight(window, sinks):
-    """window (0: none) and sinks as numbers."""
-    w, s = 0 if window is None else operator.index(window), operator.index(sinks)
-    if w < (0 if window is None else 1) or s < 0:
-        raise _err(f"window must be None or at least 1 and sinks at least 0, got {window} and {sinks}", ValueError)
-    return w, s
-
 
 def cache_append_(k_pages, v_pages, k, v, pages, lengths, starts=None):
     """Write new keys and values into the pages: one token a world, k and v (worlds, kv_heads, dim), or with starts (int32

@@ -847,3 +847,272 @@ def test_appending_marks_what_it_writes():
     policy.cache_append_(kp, vp, one, one, torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+# ---- attention with a window ----------------------------------------------------------------------------------------
+
+def window64(q, k, v, lq, lk, scale, window, sinks, dout):
+    """The definition in float64, and the bounds of each output's error: {name: (value, bound)}. Probabilities and score
+    gradients are rounded to the inputs' type (U) and come of float32 scores (EXP), as attention's without a window. Narrow windows
+    (64 keys with the sinks) take delta = dout . out from the output and what its rounding took off, others from the rounded
+    output, but for rows whose keys all lie in a sequence's first 64."""
+    u, tiny = U[q.dtype], TINY[q.dtype]
+    q, k, v, dout = (x.double() for x in (q, k, v, dout))
+    G = q.shape[1] // k.shape[1]
+    r = {n: (torch.zeros_like(x), torch.zeros_like(x)) for n, x in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
+    aq = ak = 0
+    for nq, nk in zip(lq, lk):
+        sq, sk = slice(aq, aq + nq), slice(ak, ak + nk)
+        aq, ak = aq + nq, ak + nk
+        place, key = torch.arange(nq, device=q.device)[:, None] + nk - nq, torch.arange(nk, device=q.device)
+        mask = (key <= place) & ((key > place - window) | (key < sinks))
+        for h in range(q.shape[1]):
+            Q, K, V, d = q[sq, h], k[sk, h // G], v[sk, h // G], dout[sq, h]
+            some = mask.any(1, keepdim=True)
+            s = (Q @ K.t() * scale).masked_fill(~mask, -math.inf)
+            p = torch.where(some, torch.softmax(torch.where(some, s, 0.0), 1), 0.0) * mask
+            o = p @ V
+            ob = (u + 2 * EXP) * (p @ V.abs())
+            r["out"][0][sq, h], r["out"][1][sq, h] = o, u * o.abs() + ob + tiny
+            r["dv"][0][sk, h // G] += p.t() @ d
+            r["dv"][1][sk, h // G] += (u + 2 * EXP) * (p.t() @ d.abs())
+            ds = p * (d @ V.t() - (d * o).sum(1, keepdim=True))
+            left = u * u if window + sinks <= 64 else u  # of the output, after what was kept of its rounding
+            doff = (d.abs() * (left * o.abs() + ob)).sum(1, keepdim=True) + 2 * SUM * (d.abs() @ V.abs().t())
+            dsb = (u + 2 * EXP) * ds.abs() + p * doff
+            r["dq"][0][sq, h], r["dq"][1][sq, h] = ds @ K * scale, dsb @ K.abs() * scale
+            r["dk"][0][sk, h // G] += ds.t() @ Q * scale
+            r["dk"][1][sk, h // G] += dsb.t() @ Q.abs() * scale
+    return {n: (x, b + u * x.abs() + tiny if n != "out" else b) for n, (x, b) in r.items()}
+
+
+def run_window(q, k, v, lq, lk, window, sinks, dout, scale=None):
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = policy.attention(*leaves, starts(lq), starts(lk), scale=scale, window=window, sinks=sinks)
+    return dict(zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, dout))))
+
+
+def check_window(q, k, v, lq, lk, window, sinks=0, scale=None):
+    dout = rand(q.shape, q.dtype, 99)
+    got = run_window(q, k, v, lq, lk, window, sinks, dout, scale)
+    with torch.no_grad():
+        assert torch.equal(got["out"], policy.attention(q, k, v, starts(lq), starts(lk), scale=scale, window=window, sinks=sinks))
+    want = window64(q, k, v, lq, lk, 1 / math.sqrt(q.shape[2]) if scale is None else scale, window, sinks, dout)
+    for name, t in got.items():
+        within(name, t, *want[name])
+    return got
+
+
+def heads_of(lq, lk, heads, kv, dim, dtype=BF16):
+    return rand((sum(lq), heads, dim), dtype, 1), rand((sum(lk), kv, dim), dtype, 2), rand((sum(lk), kv, dim), dtype, 3)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv,dim", [(1, 1, 64), (4, 2, 64), (6, 2, 128), (5, 5, 40), (8, 1, 8), (3, 1, 72), (70, 1, 64), (130, 1, 128)])
+def test_window_heads(dtype, heads, kv, dim):
+    print("window", dtype, heads, kv, dim, flush=True)
+    lq = [1, 33, 70, 0, 300, 5]
+    for window, sinks in ((20, 3), (100, 0)):
+        check_window(*heads_of(lq, lq, heads, kv, dim, dtype), lq, lq, window, sinks)
+
+
+@pytest.mark.parametrize("window", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200, 500, 699, 700, 5000])
+@pytest.mark.parametrize("sinks", [0, 1, 4, 32, 64, 65, 130, 1000])
+def test_windows(window, sinks):
+    """Windows and sinks that end inside tiles and on their edges, meet, leave hidden tiles between them or none, and reach
+    past a sequence; long sequences, one with earlier keys, and many short ones (a wave alone takes their keys' gradients)."""
+    print("window", window, sinks, flush=True)
+    lq, lk = [700, 3, 260], [700, 3, 500]
+    check_window(*heads_of(lq, lk, 4, 2, 64), lq, lk, window, sinks)
+    short, past = [40, 0, 17, 90, 1] * 8, [60, 3, 17, 90, 100] * 8
+    check_window(*heads_of(short, past, 4, 2, 64, F16), short, past, window, sinks)
+
+
+@pytest.mark.parametrize("lq,lk", [([1], [1]), ([1], [300]), ([0], [5]), ([5], [0]), ([300], [1]), ([70, 3], [20, 200]), ([64], [65]),
+                                   ([129, 1], [127, 640]), ([1] * 90, [7] * 90), ([2, 0, 0, 4], [0, 9, 0, 4]), ([513], [520])])
+def test_window_lengths(lq, lk):
+    print("window lengths", lq[:4], lk[:4], flush=True)
+    for dim, heads in ((64, 2), (128, 6)):
+        for window, sinks in ((5, 2), (40, 0), (1, 0)):
+            check_window(*heads_of(lq, lk, heads, 2, dim), lq, lk, window, sinks)
+
+
+@pytest.mark.parametrize("dtype,dim,heads", [(BF16, 64, 2), (F16, 128, 6), (BF16, 40, 8)])
+@pytest.mark.parametrize("lq,lk", [([1], [4000]), ([5, 60], [1800, 2100]), ([1500], [1500]), ([1300, 700], [257, 1900]), ([129], [5000]),
+                                   ([4000], [4000])])
+def test_window_few_sequences(dtype, dim, heads, lq, lk):
+    """Few tiles, long sequences: a tile's keys (rows) are split among workgroups."""
+    print("window few", dtype, dim, heads, lq, lk, flush=True)
+    for window, sinks in ((1200, 70), (100, 4)):
+        check_window(*heads_of(lq, lk, heads, 2, dim, dtype), lq, lk, window, sinks)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_window_long_sequences(dim):
+    """Sequences long enough that their tiles are listed one by one, and enough of them that none is split."""
+    print("window long", dim, flush=True)
+    lq, lk = [2500, 1900], [2500, 2100]
+    check_window(*heads_of(lq, lk, 16, 8, dim), lq, lk, 300, 20)
+
+
+def test_window_as_long_as_the_keys_hides_nothing():
+    lq, lk = [300, 7, 512], [310, 7, 600]
+    q, k, v = heads_of(lq, lk, 4, 2, 64)
+    dout = rand(q.shape, BF16, 9)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = policy.attention(*leaves, starts(lq), starts(lk))
+    want = (out, *torch.autograd.grad(out, leaves, dout))
+    for window, sinks in ((sum(lk), 0), (2 ** 40, 2 ** 40), (None, 5)):
+        got = run_window(q, k, v, lq, lk, window, sinks, dout)
+        assert all(torch.equal(a, b) for a, b in zip(want, got.values()))
+
+
+def test_window_rounds_as_finely_as_few_keys_need():
+    """A window of one key: the output is the value and the scores have no part, so their gradients are exactly 0."""
+    lq = [300, 40]
+    for dtype in (BF16, F16):
+        q, k, v = heads_of(lq, lq, 4, 2, 64, dtype)
+        dout = rand(q.shape, dtype, 9)
+        got = run_window(q, k, v, lq, lq, 1, 0, dout)
+        assert torch.equal(got["out"], v.repeat_interleave(2, 1))
+        # P = 1, dP and delta the same sum in two orders
+        bound = (dout.double().abs() * got["out"].double().abs()).sum(2, keepdim=True) * (2 * SUM + U[dtype] ** 2)
+        within("dq", got["dq"], torch.zeros_like(got["dq"]), bound * k.repeat_interleave(2, 1).double().abs())
+
+
+def test_window_padding():
+    lq, lk, more = [40, 0, 130], [60, 10, 130], 70
+    q, k, v = heads_of(lq + [more], lk + [more], 4, 2, 64)
+    q[sum(lq):], k[sum(lk):], v[sum(lk):] = math.nan, math.inf, math.nan
+    dout = rand(q.shape, BF16, 99)
+    dout[sum(lq):] = math.nan
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = policy.attention(*leaves, starts(lq), starts(lk), window=30, sinks=2)
+    grads = torch.autograd.grad(out, leaves, dout)
+    nq, nk = sum(lq), sum(lk)
+    want = window64(q[:nq], k[:nk], v[:nk], lq, lk, 0.125, 30, 2, dout[:nq])
+    for name, t, n in (("out", out.detach(), nq), ("dq", grads[0], nq), ("dk", grads[1], nk), ("dv", grads[2], nk)):
+        within(name, t[:n], *want[name])
+        assert not t[n:].any(), name
+
+
+@pytest.mark.parametrize("dtype,dim,heads,n", [(BF16, 64, 2, 400), (F16, 64, 6, 400), (BF16, 128, 4, 400), (F16, 40, 2, 90), (BF16, 64, 2, 2500)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_window_what_it_hides(dtype, dim, heads, n, bad):
+    """A key, value, query or cotangent that is not finite reaches the rows and keys that see it, and no others: not those
+    behind the window, nor, for a row, the keys before it; a bad sink reaches every later row."""
+    print("window hidden", dtype, dim, heads, n, bad, flush=True)
+    lq, lk, window, sinks, at = [n, 30], [n, 30], 40, 3, 41
+    q, k, v = heads_of(lq, lk, heads, 2, dim, dtype)
+    dout = rand(q.shape, dtype, 99)
+    want = window64(q, k, v, lq, lk, 1 / math.sqrt(dim), window, sinks, dout)
+
+    def same(got, name, rows, cols=slice(None)):
+        w, b = want[name]
+        within(f"{name} {rows}", got[name][rows, :, cols], w[rows, :, cols], b[rows, :, cols])
+    unseen = [i for i in range(n + 30) if not at <= i < at + window]
+    v2 = v.clone()
+    v2[at, :, 7] = bad
+    got = run_window(q, k, v2, lq, lk, window, sinks, dout)
+    for name in ("out", "dq"):
+        same(got, name, unseen)
+    seen7 = got["out"][at:at + window, :, 7]
+    assert torch.isnan(seen7).all() if math.isnan(bad) else (seen7 == bad).all()
+    same(got, "dv", slice(None))
+    same(got, "dk", [i for i in range(n + 30) if i >= at + window + window or i >= n])
+    k2 = k.clone()
+    k2[at] = bad
+    got = run_window(q, k2, v, lq, lk, window, sinks, dout)
+    for name in ("out", "dq"):
+        same(got, name, unseen)
+    for name in ("dk", "dv"):
+        same(got, name, [i for i in range(n + 30) if i >= at + window or i >= n])
+    row = 60  # sees keys 21 .. 60 and the sinks
+    others = [i for i in range(n + 30) if not (row - window < i <= row or i < sinks)]
+    for which in ("q", "dout"):
+        q2, d2 = q.clone(), dout.clone()
+        (q2 if which == "q" else d2)[row] = bad
+        got = run_window(q2, k, v, lq, lk, window, sinks, d2)
+        for name in ("out", "dq"):
+            same(got, name, [i for i in range(n + 30) if i != row])
+        for name in ("dk", "dv"):
+            same(got, name, others)
+    v3 = v.clone()
+    v3[1, :, 5] = bad
+    got = run_window(q, k, v3, lq, lk, window, sinks, dout)
+    same(got, "out", [0]), same(got, "out", slice(n, None)), same(got, "out", slice(1, n), slice(0, 5))
+    assert not torch.isfinite(got["out"][1:n, :, 5]).any()
+
+
+def test_window_offsets_that_are_wrong_stay_in_bounds():
+    q, k, v = heads_of([500], [500], 4, 2, 64)
+    for bad in ([0, 2 ** 31 - 1, 3], [0, -5, -(2 ** 31)], [7, 300, 100, 500], [0, 600, 400, 200]):
+        a = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        torch.autograd.grad(policy.attention(*leaves, a, window=50, sinks=5), leaves, q)
+    torch.cuda.synchronize()
+
+
+def test_window_gradient_is_the_slope():
+    lq, lk, window, sinks = [20, 95], [33, 95], 30, 3
+    q, k, v = heads_of(lq, lk, 4, 2, 64, F16)
+    dout = rand(q.shape, F16, 4)
+    got = run_window(q, k, v, lq, lk, window, sinks, dout)
+    want = window64(q, k, v, lq, lk, 0.125, window, sinks, dout)
+    for i, name in enumerate(("dq", "dk", "dv")):
+        xs = [x.double() for x in (q, k, v)]
+        d = rand(xs[i].shape, torch.float64, 7)
+
+        def value(s):
+            ys = list(xs)
+            ys[i] = ys[i] + s * d
+            total, aq, ak = 0.0, 0, 0
+            for nq, nk in zip(lq, lk):
+                place, key = torch.arange(nq, device="cuda")[:, None] + nk - nq, torch.arange(nk, device="cuda")
+                mask = (key <= place) & ((key > place - window) | (key < sinks))
+                for h in range(4):
+                    p = torch.softmax((ys[0][aq:aq + nq, h] @ ys[1][ak:ak + nk, h // 2].t() * 0.125).masked_fill(~mask, -math.inf), 1)
+                    total = total + ((p @ ys[2][ak:ak + nk, h // 2]) * dout[aq:aq + nq, h].double()).sum()
+                aq, ak = aq + nq, ak + nk
+            return total
+        slope = (value(1e-5) - value(-1e-5)) / 2e-5
+        along = (got[name].double() * d).sum()
+        assert abs(slope - along) <= (want[name][1] * d.abs()).sum() + 1e-6 * abs(slope), name
+
+
+def test_window_past_32_bits():
+    """Tokens 2^20 elements apart: offsets past 2^31 elements."""
+    big = torch.zeros((2200, 2 ** 20), dtype=BF16, device="cuda")
+    q, k, v = (rand((2200, 1, 64), BF16, n) for n in (1, 2, 3))
+    views = []
+    for i, x in enumerate((q, k, v)):
+        view = big[:, 64 * i:64 * i + 64].unflatten(1, (1, 64))
+        view.copy_(x)
+        views.append(view)
+    run = lambda *xs: run_window(*xs, [1000, 1200], [1000, 1200], 200, 4, q).values()  # noqa: E731
+    assert all(torch.equal(a, b) for a, b in zip(run(q, k, v), run(*views)))
+
+
+def test_window_is_what_the_paged_form_sees():
+    """The last query of each sequence against the control loop's form over the same history in pages."""
+    lengths, window, sinks = [1, 17, 40, 300], 16, 3
+    q, k, v = heads_of([1] * 4, lengths, 4, 2, 64)
+    a = policy.attention(q, k, v, starts([1] * 4), starts(lengths), window=window, sinks=sinks)
+    table, count = paged_tables(lengths, 8, 40)
+    kp, vp = (torch.zeros((count, 8, 2, 64), dtype=BF16, device="cuda") for _ in range(2))
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    policy.cache_append_(kp, vp, k, v, table, torch.zeros_like(n), starts(lengths))
+    b = policy.attention_paged(q, kp, vp, table, n, window=window, sinks=sinks)
+    within("paged", b, a, 2 * U[BF16] * a.double().abs() + (U[BF16] + 4 * EXP + 2 * SUM) * v.double().abs().amax())
+
+
+def test_window_refusals():
+    q, k, v = heads_of([10], [10], 4, 2, 64)
+    for kw in (dict(window=0), dict(window=-3), dict(window=5, sinks=-1), dict(sinks=-1)):
+        with pytest.raises(ValueError):
+            policy.attention(q, k, v, starts([10]), **kw)
+    for kw in (dict(window=2.5), dict(window="3"), dict(window=3, sinks=1.0)):
+        with pytest.raises(TypeError):
+            policy.attention(q, k, v, starts([10]), **kw)
+    with pytest.raises(TypeError):
+        policy.attention(q.float(), k.float(), v.float(), starts([10]), window=3)
