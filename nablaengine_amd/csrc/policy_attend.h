@@ -56,6 +56,9 @@ struct Attend {
   // a window (WIN kernels): key j of a row whose last key is i is seen if j > i - window or j < sinks
   int window, sinks;
   void* rest;  // (tq, heads, dim): what the outputs' rounding took off, for delta; NULL: not kept
+  // the sinks' gradients from rows whose window has passed them: parts of far_tokens tokens, 0: with the others
+  int far_tokens, far_least, far_chunks;
+  float* far;
 };
 
 // whether the window hides key j from a row whose last key is i

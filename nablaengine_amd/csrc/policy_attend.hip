@@ -630,6 +630,7 @@ struct DkvTiles {
   alignas(16) float lses[2][RT], deltas[2][RT];
   alignas(16) int places_of[2][RT];  // a row's token from its tile's first
 };
+constexpr size_t far_slot(int dp) { return 2 * 32 * (size_t)dp; }  // floats of 32 keys' dk and dv
 // Heads of 128: dk and dv together take 128 registers a lane, with the keys and values more than two waves a SIMD have.
 // One workgroup takes dk and another dv (a fourth more products, the scores twice): 1150 us at sequences of 8192 and 2800
 // tokens of 16 heads on 4 against 1480 us with both in one and part of the operands in LDS or scratch, and 1230 us with one
@@ -638,14 +639,46 @@ struct DkvTiles {
 // nothing (forward 249 us to 260). The wait for the next tile's load stands between the first products and the column
 // operands here; the eight waves fill a CU's LDS, so that no other workgroup covers it.
 enum Role { BOTH, KEYS, VALUES };
-template <bool WIN>
+// A window's sinks are seen by all rows of their sequence, other keys by those of one window: their tiles would take many times as
+// long, most of their waves idle, and end last (two sequences of 8192 and 2752 tokens, window 1000, 16 sinks: 1121 us). The rows
+// behind the window of a sequence's first key are taken from those tiles and walked over by workgroups of their own, a part of
+// far_tokens tokens each for 32 sinks, all of whose waves share the rows; their sums in float32 go to slots that the key tile's
+// workgroup adds before it rounds. A part's slot follows from where its sequence lies: a sequence of n queries from q0 and m keys
+// from k0 on has at most one part more than multiples of far_tokens in (q0, q0 + n], and as it has m >= far_least keys there is a
+// multiple of that in (k0, k0 + m].
+struct Far {
+  int parts, base, from;  // its parts (0: none), the first one's slot, their first token
+  __device__ __forceinline__ Far(const Attend& a, const Place& p) {
+    const int off = p.nk - p.nq, behind = a.window > off ? a.window - off : 0;
+    const bool some = a.far_tokens && p.nk >= a.far_least && p.nq > behind;
+    from = behind;
+    parts = some ? (p.nq - behind - 1) / a.far_tokens + 1 : 0;
+    base = some ? p.q0 / a.far_tokens + p.k0 / a.far_least : 0;
+  }
+  template <int DP>
+  __device__ __forceinline__ float* slot(const Attend& a, const Place& p, int part, int chunk) const {
+    return a.far + (((size_t)(base + part) * a.far_chunks + chunk) * a.kv_heads + p.kv) * far_slot(DP);
+  }
+};
+// the sinks that a key tile's own walk reaches behind their window
+__device__ __forceinline__ int near_sinks(const Attend& a, const Place& p) { return Far(a, p).parts ? 0 : a.sinks; }
+
+enum Mode { ALL, WINDOWED, FAR };  // which of the rows a key tile walks over
+template <int MODE>
 struct RowTiles {  // the rows that see a key tile, in tiles of RT rows or a little less
   int used, first, tiles;
   int rows;  // their end
   __device__ __forceinline__ RowTiles(const Attend& a, const Place& p, int kw, int rt) {
     used = a.group <= rt ? rt / a.group * a.group : rt;
     rows = p.nq * a.group;
-    if (WIN && p.tile * 32 * kw >= a.sinks) {  // no sinks: the first token behind the last key's window
+    if (MODE == FAR) {
+      const long long from = Far(a, p).from + (long long)p.part * a.far_tokens, end = from + a.far_tokens;
+      first = (int)from * a.group;
+      if (end < p.nq) rows = (int)end * a.group;
+      tiles = rows > first ? (rows - 1 - first) / used + 1 : 0;
+      return;
+    }
+    if (MODE == WINDOWED && p.tile * 32 * kw >= near_sinks(a, p)) {  // no sinks: the first token behind the last key's window
       const int keys = (p.tile + 1) * 32 * kw < p.nk ? (p.tile + 1) * 32 * kw : p.nk;
       const long long end = (long long)keys - 1 + a.window - (p.nk - p.nq);
       rows = end < p.nq ? (end > 0 ? (int)end : 0) * a.group : rows;
@@ -661,8 +694,24 @@ __device__ __forceinline__ size_t key_slot(const Attend& a, const Place& p, int 
   return ((size_t)p.at * (role == BOTH ? 1 : 2) + (role == VALUES)) * a.parts_k;
 }
 template <typename T, int DP, int N, int ROLE, bool WIN>
-__device__ __forceinline__ void finish_dkv(const Attend& a, const Place& p, int key0, int d0, const F16x* dk, const F16x* dv) {
+__device__ __forceinline__ void finish_dkv(const Attend& a, const Place& p, int key0, int d0, F16x* dk, F16x* dv) {
   const int l = threadIdx.x % 64, n = l % 32, h = l / 32, dim = a.dim, group = a.group;
+  if (WIN && key0 < a.sinks && key0 < p.nk) {
+    const Far far(a, p);
+#pragma unroll 2
+    for (int i = 0; i < far.parts; ++i) {
+      const float* from = far.slot<DP>(a, p, i, key0 / 32) + l;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        if (ROLE == (which ? KEYS : VALUES)) continue;
+        F16x* acc = which ? dv : dk;
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[t][j] += from[64 * (16 * (which * (DP / 32) + d0 / 32 + t) + j)];
+      }
+    }
+  }
   const int rows = p.nq * group, off = p.nk - p.nq, key = key0 + n;
   const bool valid = key < p.nk;
   const float c = a.scale * LOG2E;
@@ -693,7 +742,7 @@ __device__ __forceinline__ void finish_dkv(const Attend& a, const Place& p, int 
     if (ROLE != KEYS) ov.store((T*)a.dv + to, d0, d1, 1.0f);
   }
 }
-template <typename T, int DP, int KW, int WAVES, int ROLE, bool PARTS, bool WIN>
+template <typename T, int DP, int KW, int WAVES, int ROLE, bool PARTS, int MODE>
 __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, WAVES>& lds) {
   constexpr int RT = DkvTiles<T, DP, WAVES>::RT;
   constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 64 * WAVES / CH, SPLIT = WAVES / KW;
@@ -721,7 +770,8 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
 
   // Row tiles start at whole tokens (but for groups above RT, whose rows' places are computed anew for each tile), so
   // that a thread's rows keep their distance from the tile's first token: RT or a little less rows are used of each.
-  const RowTiles<WIN> all(a, p, KW, RT);
+  const RowTiles<MODE> all(a, p, KW, RT);
+  const int sinks = MODE == WINDOWED ? near_sinks(a, p) : a.sinks;
   const int rows = all.rows, used = all.used, first = all.first, back = used / group;  // back: tokens of a tile
   auto chunk = [&](int i) { return tid % CH ^ swizzle<DP>(tid / CH + i * STEP); };
   const T *qp[N], *gp[N];  // this thread's rows of the next tile to load, and its row's place in lse and delta
@@ -797,7 +847,8 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
       const int low = token + (group <= RT ? tokens(32 * i) : 0) + off;
       const int most = token + (group <= RT ? tokens(32 * i + 31 < used ? 32 * i + 31 : used - 1) : 1) + off;
       if (32 * i >= used || r0 + 32 * i >= rows || most < key0) continue;
-      if (WIN && low - a.window >= key0 + 31 && key0 >= a.sinks) continue;
+      if (MODE == WINDOWED && low - a.window >= key0 + 31 && key0 >= sinks) continue;
+      if (MODE == FAR && most - a.window < key0) continue;
       F16x s = {}, dp = {};
 #pragma unroll
       for (int y = 0; y < KS; y += 4) {
@@ -825,7 +876,8 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
           if (ROLE != VALUES) qc[x][d] = read_columns<DP>(qt, 32 * i + 16 * x, d, l);
         }
       phase();
-      const bool masked = low < key0 + 31 || (WIN && key0 <= most - a.window && key0 + 31 >= a.sinks);
+      const bool masked = MODE == FAR ? low - a.window < key0 + 31 || key0 + 31 >= sinks
+                                      : low < key0 + 31 || (MODE == WINDOWED && key0 <= most - a.window && key0 + 31 >= sinks);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int at = 32 * i + 8 * j + 4 * h;
@@ -841,7 +893,9 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
           const I4 li = *(const I4*)(places_of[turn] + at) + (token + off);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (key > li[e] || (WIN && window_hides(a, key, li[e]))) s[4 * j + e] = dp[4 * j + e] = 0.0f;
+            if (MODE == FAR ? key > li[e] - a.window || key >= sinks
+                            : key > li[e] || (MODE == WINDOWED && key <= li[e] - a.window && key >= sinks))
+              s[4 * j + e] = dp[4 * j + e] = 0.0f;
         }
       }
       if (ROLE != VALUES) lift.template scale<DT>(dp, dk);
@@ -892,13 +946,24 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
       }
     if (split) return;
   }
+  if (MODE == FAR) {
+    float* to = Far(a, p).slot<DP>(a, p, p.part, p.tile) + l;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (ROLE != VALUES) to[64 * (16 * d + j)] = dk[d][j];
+        if (ROLE != KEYS) to[64 * (16 * (DT + d) + j)] = dv[d][j];
+      }
+    return;
+  }
   if (PARTS && my.parts > 1) {
     const Part<KEY_PART> mine(a, key_slot(a, p, ROLE) + p.part % a.parts_k, w);
     if (ROLE != VALUES) mine.put(0, dk, DT);
     if (ROLE != KEYS) mine.put(ROLE == BOTH ? DT : 0, dv, DT);
     return;
   }
-  finish_dkv<T, DP, DT, ROLE, WIN>(a, p, key0, 0, dk, dv);
+  finish_dkv<T, DP, DT, ROLE, MODE == WINDOWED>(a, p, key0, 0, dk, dv);
 }
 
 template <typename T, int DP, int KW, int WAVES, bool PARTS, bool WIN>
@@ -908,13 +973,52 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256) __attribute__((amdgpu_waves
   Place p;
   if constexpr (WAVES == 1) {  // each wave a tile of its own
     const int w = uniform(threadIdx.x / 64);
-    if (place(a, 1, blockIdx.x * 4 + w, p)) dkv_tile<T, DP, KW, WAVES, BOTH, false, WIN>(a, p, lds[w]);
+    if (place(a, 1, blockIdx.x * 4 + w, p)) dkv_tile<T, DP, KW, WAVES, BOTH, false, WIN ? WINDOWED : ALL>(a, p, lds[w]);
   } else if constexpr (DP == 64) {
-    if (place_of_block(a, 1, parts, p)) dkv_tile<T, DP, KW, WAVES, BOTH, PARTS, WIN>(a, p, lds[0]);
+    if (place_of_block(a, 1, parts, p)) dkv_tile<T, DP, KW, WAVES, BOTH, PARTS, WIN ? WINDOWED : ALL>(a, p, lds[0]);
   } else {
     if (!place_of_block(a, 1, 2 * parts, p)) return;
-    if (p.part >= parts) dkv_tile<T, DP, KW, WAVES, VALUES, PARTS, WIN>(a, p, lds[0]);
-    else dkv_tile<T, DP, KW, WAVES, KEYS, PARTS, WIN>(a, p, lds[0]);
+    if (p.part >= parts) dkv_tile<T, DP, KW, WAVES, VALUES, PARTS, WIN ? WINDOWED : ALL>(a, p, lds[0]);
+    else dkv_tile<T, DP, KW, WAVES, KEYS, PARTS, WIN ? WINDOWED : ALL>(a, p, lds[0]);
+  }
+}
+
+// the far rows' parts; WAVES waves, as many as a row tile has subtiles
+template <typename T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_far(Attend a) {
+  __shared__ DkvTiles<T, DP, WAVES> lds;
+  constexpr int ROLES = DP == 64 ? 1 : 2;
+  int b = blockIdx.x;
+  const int role = b % ROLES;
+  b /= ROLES;
+  Place p;
+  p.kv = b % a.kv_heads;
+  b /= a.kv_heads;
+  p.tile = b % a.far_chunks;
+  const int slot = b / a.far_chunks, l = threadIdx.x % 64;
+  auto in = [](int x, int most) { return x < 0 ? 0 : x > most ? most : x; };
+  auto base = [&](int s) {
+    return s == 0 ? 0 : in(a.starts_q[s], a.tq) / a.far_tokens + in(a.starts_k[s], a.tk) / a.far_least;
+  };
+  int s = 0;  // the last sequence whose slots begin at or before this one: 64 at once, one of s .. s + n - 1
+  for (int n = a.seqs; n > 1;) {
+    const int step = (n - 1) / 64 + 1, at = l * step;
+    const int c = __popcll(__ballot(at < n && base(s + (at < n ? at : 0)) <= slot)), skip = c > 0 ? (c - 1) * step : 0;
+    s += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  s = uniform(s);
+  sequence(a.starts_q, s, a.seqs, a.tq, p.q0, p.nq);
+  sequence(a.starts_k, s, a.seqs, a.tk, p.k0, p.nk);
+  p.q0 = uniform(p.q0), p.nq = uniform(p.nq), p.k0 = uniform(p.k0), p.nk = uniform(p.nk);
+  const Far far(a, p);
+  p.part = slot - far.base;
+  if (p.part < 0 || p.part >= far.parts || p.tile * 32 >= p.nk) return;
+  if constexpr (DP == 64) {
+    dkv_tile<T, DP, 1, WAVES, BOTH, false, FAR>(a, p, lds);
+  } else {
+    if (role) dkv_tile<T, DP, 1, WAVES, VALUES, false, FAR>(a, p, lds);
+    else dkv_tile<T, DP, 1, WAVES, KEYS, false, FAR>(a, p, lds);
   }
 }
 
@@ -924,9 +1028,9 @@ __global__ __launch_bounds__(256) void k_attend_dkv_join(Attend a) {
   const int role = blockIdx.y / (4 * DT) ? VALUES : KEYS, wave = blockIdx.y / DT % 4, block = blockIdx.y % DT;
   Place p;
   if (!place_of_block(a, 1, 1, p)) return;
-  const int parts = Slice(RowTiles<WIN>(a, p, 4, DkvTiles<T, DP, DP / 16>::RT).tiles, a.parts_k, 0).parts;
+  const int parts = Slice(RowTiles<WIN ? WINDOWED : ALL>(a, p, 4, DkvTiles<T, DP, DP / 16>::RT).tiles, a.parts_k, 0).parts;
   if (parts == 1) return;
-  const F16x acc = add_parts<KEY_PART>(a, key_slot(a, p, DP == 64 ? BOTH : role), parts, wave,
+  F16x acc = add_parts<KEY_PART>(a, key_slot(a, p, DP == 64 ? BOTH : role), parts, wave,
                                        (DP == 64 && role == VALUES ? DT : 0) + block, [](int) { return 1.0f; });
   if (threadIdx.x >= 64) return;
   const int key0 = p.tile * 128 + wave * 32;
@@ -980,12 +1084,29 @@ size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group) {
   return sizeof(int) * (ORDER_HEAD + 2 * (size_t)(order_queries(seqs, tq, group) +
                                                   order_keys(seqs, tk, key_waves(dim, seqs, tk))));
 }
+// Where the sinks' far rows are walked over apart: where there are sinks, at most four tiles of 32, and a sequence may be longer
+// than a window and half a part; not where their slots would take more than 1 GB.
+constexpr int FAR_TOKENS = 512;
+struct FarPlan { int tokens, least, chunks; long long slots; };
+FarPlan far_plan(int kv_heads, int dim, int tq, int tk, int window, int sinks) {
+  FarPlan r = {0, window + 1 > 64 ? window + 1 : 64, (sinks + 31) / 32, 0};
+  if (window < 1 || sinks < 1 || sinks > 128 || tk <= window + FAR_TOKENS / 2) return r;
+  r.slots = (long long)tq / FAR_TOKENS + tk / r.least + 1;
+  if (r.slots * r.chunks * kv_heads * far_slot(dim <= 64 ? 64 : 128) <= 1LL << 28) r.tokens = FAR_TOKENS;
+  return r;
+}
+size_t attend_parts_floats(int kv_heads, int dim, int seqs, int tq, int tk, int group, int window, int sinks, bool vjp);
 size_t attend_scratch_bytes(int kv_heads, int dim, int seqs, int tq, int tk, int group, int window, int sinks, bool vjp) {
+  const FarPlan far = far_plan(kv_heads, dim, tq, tk, window, sinks);
+  const size_t parts = attend_parts_floats(kv_heads, dim, seqs, tq, tk, group, window, sinks, vjp);
+  return sizeof(float) * (parts + (vjp && far.tokens ? (size_t)far.slots * far.chunks * kv_heads * far_slot(dim <= 64 ? 64 : 128) : 0));
+}
+size_t attend_parts_floats(int kv_heads, int dim, int seqs, int tq, int tk, int group, int window, int sinks, bool vjp) {
   const size_t pq = query_parts(kv_heads, seqs, tq, tk, group, window, sinks);
   const size_t pk = vjp ? key_parts(kv_heads, dim, seqs, tq, tk, group, window) : 1;
   const size_t q = pq == 1 ? 0 : pq * order_queries(seqs, tq, group) * kv_heads * (dim <= 64 ? RowsPart<64>::SIZE : RowsPart<128>::SIZE);
   const size_t k = pk == 1 ? 0 : pk * order_keys(seqs, tk, 4) * kv_heads * (dim <= 64 ? 1 : 2) * Part<KEY_PART>::SIZE;
-  return sizeof(float) * (q > k ? q : k);
+  return q > k ? q : k;
 }
 
 template <typename T, int DP, bool WIN>
@@ -1021,6 +1142,13 @@ int attend_vjp(hipStream_t st, const Attend& a) {
     if (e) return e;
   }
   if (!a.tk) return 0;
+  if (WIN && a.far_tokens) {
+    constexpr int WAVES = DP / 32;
+    const FarPlan far = far_plan(a.kv_heads, a.dim, a.tq, a.tk, a.window, a.sinks);
+    k_attend_far<T, DP, WAVES><<<(unsigned)(far.slots * far.chunks * a.kv_heads * (DP == 64 ? 1 : 2)), 64 * WAVES, 0, st>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
   const long long tiles = order_keys(a.seqs, a.tk, a.key_waves);
   constexpr int ROLES = DP == 64 ? 1 : 2, THREADS = DP == 64 ? 256 : 512;
   if (a.parts_k > 1) {
@@ -1038,7 +1166,7 @@ int attend_vjp(hipStream_t st, const Attend& a) {
 
 template <bool WIN>
 int launch_attend(hipStream_t st, int type, const Attend& a) {
-  k_attend_order<<<1, 1024, 0, st>>>(a.seqs, a.tq, a.tk, a.group, a.key_waves, a.by_sequence, WIN ? a.window : 0, WIN ? a.sinks : 0,
+  k_attend_order<<<1, 1024, 0, st>>>(a.seqs, a.tq, a.tk, a.group, a.key_waves, a.by_sequence, WIN ? a.window : 0, WIN && !a.far_tokens ? a.sinks : 0,
                                   a.starts_q, a.starts_k, (int*)a.order);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.tq) return (int)e;
@@ -1078,6 +1206,7 @@ int dk_attention_window(hipStream_t st, int type, int heads, int kv_heads, int d
     return (int)hipErrorInvalidValue;
   pol::Attend a = {};
   a.window = window_of(window, tk), a.sinks = sinks_of(sinks, tk), a.rest = rest;
+  a.far_tokens = pol::far_plan(kv_heads, dim, tq, tk, a.window, a.sinks).tokens;
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
@@ -1099,6 +1228,9 @@ int dk_attention_window_vjp(hipStream_t st, int type, int heads, int kv_heads, i
     return (int)hipErrorInvalidValue;
   pol::Attend a = {};
   a.window = window_of(window, tk), a.sinks = sinks_of(sinks, tk), a.rest = const_cast<void*>(rest);
+  const pol::FarPlan far = pol::far_plan(kv_heads, dim, tq, tk, a.window, a.sinks);
+  a.far_tokens = far.tokens, a.far_least = far.least, a.far_chunks = far.chunks;
+  if (scratch) a.far = (float*)scratch + pol::attend_parts_floats(kv_heads, dim, seqs, tq, tk, heads / kv_heads, a.window, a.sinks, true);
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
