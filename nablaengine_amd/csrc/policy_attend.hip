@@ -48,7 +48,7 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   if (by_sequence < 3)
     while (ls < 1024 && ls * 2 * (long long)(seqs + 1) <= 1024) ls *= 2;
   const int lane = threadIdx.x % ls, first_seq = threadIdx.x / ls, stride = 1024 / ls;
-  const int bits[2] = {7, key_waves == 1 ? 5 : 7};  // of a tile's rows
+  const int bits[2] = {7, key_waves == 1 ? 5 : key_waves == 2 ? 6 : 7};  // of a tile's rows
   static_assert(QROWS == 128, "");
   const unsigned caps[2] = {(unsigned)order_queries(seqs, tq, group), (unsigned)order_keys(seqs, tk, key_waves)};
   int* const lists[2] = {order + ORDER_HEAD, order + ORDER_HEAD + 2LL * caps[0]};
@@ -183,7 +183,9 @@ template <bool WIN>
 struct Rows {
   int pos, head, limit, all_see, any_sees, tiles;
   bool valid;
-  int sunk, skipped;  // WIN: the tiles that hold sinks, and those behind them that no row sees; `tiles` counts without these
+  // WIN: the workgroup's keys are the `front` sinks before its first row's window and all from that window on, `skip` keys
+  // further: their places are counted without the keys between, so that a few sinks fill no tile of their own
+  int front, skip;
   __device__ __forceinline__ Rows(const Attend& a, const Place& p, int w) {
     const int rows = p.nq * a.group, off = p.nk - p.nq;
     const int row0 = p.tile * QROWS + 32 * w, row = row0 + threadIdx.x % 32;
@@ -195,23 +197,25 @@ struct Rows {
     all_see = row0 < rows ? row0 / a.group + off : -1;
     any_sees = row0 < rows ? (row0 + 31 < rows ? row0 + 31 : rows - 1) / a.group + off : -1;
     const int end = p.tile * QROWS + QROWS < rows ? p.tile * QROWS + QROWS : rows, last = (end - 1) / a.group + off;
-    tiles = last < 0 ? 0 : last / TILE + 1;
+    front = skip = 0;
     if (WIN) {
-      const int from = p.tile * QROWS / a.group + off - a.window + 1, near = from > 0 ? from / TILE : 0;
-      sunk = a.sinks > tiles * TILE ? tiles : (a.sinks + TILE - 1) / TILE;
-      skipped = near > sunk ? (near < tiles ? near : tiles) - sunk : 0;
-      tiles -= skipped;
+      const int from = p.tile * QROWS / a.group + off - a.window + 1;
+      skip = from > a.sinks ? from - a.sinks : 0;
+      front = skip ? a.sinks : 0;
     }
+    tiles = last < 0 ? 0 : (last - skip) / TILE + 1;
   }
-  __device__ __forceinline__ int tile_of(int turn) const { return WIN && turn >= sunk ? turn + skipped : turn; }
-  // whether any of the wave's rows sees one of the 32 keys from key0 on (key0 <= any_sees), and whether some row does not see all
-  __device__ __forceinline__ bool sees(const Attend& a, int key0) const {
-    return !WIN || key0 + 31 > all_see - a.window || key0 < a.sinks;
+  __device__ __forceinline__ int last_place() const { return any_sees - skip; }
+  // whether any of the wave's rows sees one of the 32 keys from a place on (up to last_place()), and whether some row does not see all
+  __device__ __forceinline__ bool sees(const Attend& a, int place) const {
+    return !WIN || place < front || place + skip + 31 > all_see - a.window || place + skip < a.sinks;
   }
-  __device__ __forceinline__ bool masks(const Attend& a, int key0) const {
-    return key0 + 31 > all_see || (WIN && key0 <= any_sees - a.window && key0 + 31 >= a.sinks);
+  __device__ __forceinline__ bool masks(const Attend& a, int place) const {
+    if (WIN && place < front) return place + 31 >= front;
+    return place + skip + 31 > all_see || (WIN && place + skip <= any_sees - a.window && place + skip + 31 >= a.sinks);
   }
-  __device__ __forceinline__ bool hides(const Attend& a, int key) const {  // from this lane's row
+  __device__ __forceinline__ bool hides(const Attend& a, int place) const {  // from this lane's row
+    const int key = WIN && place >= front ? place + skip : place;
     return key > limit || (WIN && window_hides(a, key, limit));
   }
 };
@@ -224,30 +228,39 @@ struct Keys {
   long long k_t, v_t;
   int row, at, left;  // this thread's row; its wave's place in LDS; keys from the tile's first on
   bool in_row;
-  int before, jump;  // WIN: tiles before the hidden ones, and how many these are
-  __device__ __forceinline__ Keys(const Attend& a, const Place& p, const Rows<WIN>& r, int turn) {  // from that turn's tile on
-    const int first = r.tile_of(turn);
-    before = WIN ? r.sunk - turn : 0, jump = WIN ? r.skipped * TILE : 0;
+  int sunk, skip;  // WIN: sinks from the tile's first key on, and how much further the others lie
+  __device__ __forceinline__ Keys(const Attend& a, const Place& p, const Rows<WIN>& r, int first) {  // from tile `first` on
     row = threadIdx.x / CH;
     const int c = threadIdx.x % CH ^ swizzle<DP>(row);  // LDS is filled in order: the swizzle is the source's
     in_row = 8 * c < a.dim;
     k_t = a.k_t, v_t = a.v_t;
-    k = (const T*)a.k + (long long)(p.k0 + first * TILE) * k_t + (long long)p.kv * a.k_h + row * k_t + 8 * c;
-    v = (const T*)a.v + (long long)(p.k0 + first * TILE) * v_t + (long long)p.kv * a.v_h + row * v_t + 8 * c;
+    skip = WIN ? r.skip : 0, sunk = WIN ? r.front - first * TILE : 0;
+    k = (const T*)a.k + (long long)(p.k0 + skip + first * TILE) * k_t + (long long)p.kv * a.k_h + row * k_t + 8 * c;
+    v = (const T*)a.v + (long long)(p.k0 + skip + first * TILE) * v_t + (long long)p.kv * a.v_h + row * v_t + 8 * c;
     at = threadIdx.x / 64 * 64 * 8;
-    left = p.nk - first * TILE;
+    left = p.nk - skip - first * TILE;
   }
   __device__ __forceinline__ void next(T* ks, T* vs) {
+    if (WIN && sunk > 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const bool valid = in_row && row + i * STEP < left;
-      to_lds(k + i * STEP * k_t, valid, ks + i * 2048 + at);
-      to_lds(v + i * STEP * v_t, valid, vs + i * 2048 + at);
+      for (int i = 0; i < N; ++i) {
+        const bool valid = in_row && row + i * STEP < left;
+        const long long back = row + i * STEP < sunk ? skip : 0;
+        to_lds(k + (i * STEP - back) * k_t, valid, ks + i * 2048 + at);
+        to_lds(v + (i * STEP - back) * v_t, valid, vs + i * 2048 + at);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool valid = in_row && row + i * STEP < left;
+        to_lds(k + i * STEP * k_t, valid, ks + i * 2048 + at);
+        to_lds(v + i * STEP * v_t, valid, vs + i * 2048 + at);
+      }
     }
     k += TILE * k_t;
     v += TILE * v_t;
     left -= TILE;
-    if (WIN && --before == 0) k += jump * k_t, v += jump * v_t, left -= jump;
+    sunk -= TILE;
   }
 };
 
@@ -376,13 +389,13 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
   float m = -INFINITY, sum = 0.0f;
   const float c = a.scale * LOG2E;
   for (int t = first; t < end; ++t) {
-    const int key0 = r.tile_of(t) * TILE;
+    const int key0 = t * TILE;
     const T *kt = ks[t & 1], *vt = vs[t & 1];
     loads_done();
     __syncthreads();  // this tile is there for all, and all are done with the one before
     if (t + 1 < end) keys.next(ks[(t + 1) & 1], vs[(t + 1) & 1]);
-    if (key0 > r.any_sees) continue;
-    const bool first_half = r.sees(a, key0), second = key0 + 32 <= r.any_sees && r.sees(a, key0 + 32);
+    if (key0 > r.last_place()) continue;
+    const bool first_half = r.sees(a, key0), second = key0 + 32 <= r.last_place() && r.sees(a, key0 + 32);
     if (WIN && !first_half && !second) continue;
     F16x s[2] = {};
 #pragma unroll
@@ -537,9 +550,9 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
     for (int j = 0; j < 16; ++j) s[j] = exp2_fast(fmaf(s[j], c, -lse));
   };
   // delta = dout . out from the stored output, whose rounding is felt where few keys share a row: rows whose keys all
-  // lie in the first tile take it from that tile's products instead, sum P dP in float32, below
+  // lie in their first tile take it from that tile's products instead, sum P dP in float32, below
   float delta = 0.0f;
-  const bool few = r.any_sees < TILE;
+  const bool few = r.last_place() < TILE;
   if (!few) {
     V8<T> o[KS];
     load_rows<DP>(r.valid ? (const T*)a.out + (token * a.heads + r.head) * dim : nullptr, dim, h, o);
@@ -559,14 +572,14 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
   F16x acc[DT] = {};
   Lift<T> lift;
   for (int t = first; t < end; ++t) {
-    const int key0 = r.tile_of(t) * TILE;
+    const int key0 = t * TILE;
     const T *kt = ks[t & 1], *vt = vs[t & 1];
     loads_done();
     __syncthreads();
     if (t + 1 < end) keys.next(ks[(t + 1) & 1], vs[(t + 1) & 1]);
     if (t == 0 && few) {
 #pragma unroll 1
-      for (int i = 0; 32 * i <= r.any_sees; ++i) {
+      for (int i = 0; 32 * i <= r.last_place(); ++i) {
         F16x s, dp;
         products(kt, vt, 0, i, s, dp);
 #pragma unroll
@@ -576,7 +589,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (key0 + 32 * i > r.any_sees) break;
+      if (key0 + 32 * i > r.last_place()) break;
       if (WIN && !r.sees(a, key0 + 32 * i)) continue;
       F16x s, dp;
       products(kt, vt, key0, i, s, dp);
@@ -1040,11 +1053,14 @@ __global__ __launch_bounds__(256) void k_attend_dkv_join(Attend a) {
 
 // ---- launches -------------------------------------------------------------------------------------------------------
 
+constexpr int NARROW_TILES = 1 << 30;
 // Keys a tile of the keys' gradients: 128; 32, a wave each, where sequences are short and heads up to 64, since most of a
 // workgroup's waves would have no keys there. Backward of 65536 tokens of 8 heads on 2, lengths 1 to twice the mean, alone
 // and together: mean 16 113 and 157 us, 32 105 and 125, 64 115 and 123, 96 120 and 146 (all of 96: 107 and 111; all of 128:
 // 121 and 114). Heads of 128 gain nothing from tiles of 64 keys (mean 32 445 us for 434, 64 413 for 363).
-int key_waves(int dim, int seqs, int tk) { return dim <= 64 && tk <= 96LL * seqs ? 1 : 4; }
+int key_waves(int dim, int seqs, int tk, int window) {
+  return dim > 64 ? 4 : tk <= 96LL * seqs ? 1 : window && window <= NARROW_TILES ? 2 : 4;
+}
 
 // The lists in the order of the sequences: bit 0 the query tiles, bit 1 the key tiles. 131072 tokens of 8 heads on 2, by
 // sequence and singly: heads of 64, mean length 100, forward 97 and 102 us, dq 136 and 141, dkv 183 and 135; 700, 194 and 206,
@@ -1053,7 +1069,7 @@ int key_waves(int dim, int seqs, int tk) { return dim <= 64 && tk <= 96LL * seqs
 // the backward 800 and 605; of 128, 401 and 372, 1559 and 1470. A wave alone has no neighbours: the shorter listing.
 int by_sequence(int dim, int seqs, int tq, int tk) {
   const bool queries = (tq > tk ? tq : tk) <= (long long)LONG * seqs;
-  const bool keys = key_waves(dim, seqs, tk) == 1 || (dim > 64 && queries);
+  const bool keys = key_waves(dim, seqs, tk, 0) == 1 || (dim > 64 && queries);
   return (queries ? 1 : 0) | (keys ? 2 : 0);
 }
 
@@ -1076,13 +1092,13 @@ int query_parts(int kv_heads, int seqs, int tq, int tk, int group, int window, i
   return parts_of(order_queries(seqs, tq, group) * kv_heads, others_of(tk, seqs, window, sinks), TILE, seqs);
 }
 int key_parts(int kv_heads, int dim, int seqs, int tq, int tk, int group, int window) {
-  const int kw = key_waves(dim, seqs, tk);
+  const int kw = key_waves(dim, seqs, tk, window);
   return kw < 4 ? 1 : parts_of(order_keys(seqs, tk, kw) * kv_heads * (dim <= 64 ? 1 : 2), others_of(tq, seqs, window, 128) * group,
                                dim <= 64 ? 64 : 128, seqs);
 }
-size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group) {
+size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group, int window) {
   return sizeof(int) * (ORDER_HEAD + 2 * (size_t)(order_queries(seqs, tq, group) +
-                                                  order_keys(seqs, tk, key_waves(dim, seqs, tk))));
+                                                  order_keys(seqs, tk, key_waves(dim, seqs, tk, window))));
 }
 // Where the sinks' far rows are walked over apart: where there are sinks, at most four tiles of 32, and a sequence may be longer
 // than a window and half a part; not where their slots would take more than 1 GB.
@@ -1156,6 +1172,8 @@ int attend_vjp(hipStream_t st, const Attend& a) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
     k_attend_dkv_join<T, DP, WIN><<<dim3(blocks_of(a, tiles, 1), 8 * (DP / 32)), 256, 0, st>>>(a);
+  } else if (WIN && DP == 64 && a.key_waves == 2) {
+    if constexpr (WIN && DP == 64) k_attend_dkv<T, 64, 2, 4, false, true><<<blocks_of(a, tiles, 1), 256, 0, st>>>(a);
   } else if (a.key_waves == 4) {
     k_attend_dkv<T, DP, 4, DP / 16, false, WIN><<<blocks_of(a, tiles, ROLES), THREADS, 0, st>>>(a);
   } else if constexpr (DP == 64) {
@@ -1210,7 +1228,7 @@ int dk_attention_window(hipStream_t st, int type, int heads, int kv_heads, int d
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
-  a.key_waves = pol::key_waves(dim, seqs, tk);
+  a.key_waves = pol::key_waves(dim, seqs, tk, a.window);
   a.by_sequence = pol::by_sequence(dim, seqs, tq, tk);
   a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group, a.window, a.sinks), a.scratch = (float*)scratch;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.out = out, a.lse = lse, a.order = (const int*)work;
@@ -1234,7 +1252,7 @@ int dk_attention_window_vjp(hipStream_t st, int type, int heads, int kv_heads, i
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
-  a.key_waves = pol::key_waves(dim, seqs, tk);
+  a.key_waves = pol::key_waves(dim, seqs, tk, a.window);
   a.by_sequence = pol::by_sequence(dim, seqs, tq, tk);
   a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group, a.window, a.sinks), a.scratch = (float*)scratch;
   a.parts_k = pol::key_parts(kv_heads, dim, seqs, tq, tk, a.group, a.window);
@@ -1270,7 +1288,12 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
 
 long long dk_attention_work_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk) {
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || seqs < 0 || tq < 0 || tk < 0) return 0;
-  return (long long)pol::attend_work_bytes(dim, seqs, tq, tk, heads / kv_heads);
+  return (long long)pol::attend_work_bytes(dim, seqs, tq, tk, heads / kv_heads, 0);
+}
+// for every window
+long long dk_attention_window_work_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads || seqs < 0 || tq < 0 || tk < 0) return 0;
+  return (long long)pol::attend_work_bytes(dim, seqs, tq, tk, heads / kv_heads, 1);
 }
 
 long long dk_attention_scratch_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk, int vjp) {
