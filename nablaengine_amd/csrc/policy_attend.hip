@@ -636,9 +636,9 @@ __global__ __launch_bounds__(256) void k_attend_dq_join(Attend a) {
 // time. S = Q K^T here, so that a lane holds 16 rows of ONE key and P, dS are the B operands of dV^T = dO^T P and dK^T =
 // Q^T dS. KW of the waves differ in their keys, the others take every SPLIT-th subtile of 32 rows of the same keys, and
 // their sums are added at the end, in order.
-template <typename T, int DP, int WAVES>
+template <typename T, int DP, int WAVES, int KW = 4>
 struct DkvTiles {
-  static constexpr int RT = WAVES == 1 ? 32 : DP == 64 ? 64 : 128;
+  static constexpr int RT = WAVES == 1 ? 32 : DP == 64 && KW != 2 ? 64 : 128;
   alignas(16) T tiles[2][2][RT * DP];  // (turn, q or dout)
   alignas(16) float lses[2][RT], deltas[2][RT];
   alignas(16) int places_of[2][RT];  // a row's token from its tile's first
@@ -756,8 +756,8 @@ __device__ __forceinline__ void finish_dkv(const Attend& a, const Place& p, int 
   }
 }
 template <typename T, int DP, int KW, int WAVES, int ROLE, bool PARTS, int MODE>
-__device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, WAVES>& lds) {
-  constexpr int RT = DkvTiles<T, DP, WAVES>::RT;
+__device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, WAVES, KW>& lds) {
+  constexpr int RT = DkvTiles<T, DP, WAVES, KW>::RT;
   constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 64 * WAVES / CH, SPLIT = WAVES / KW;
   // of a subtile's two column operands, those read during the exponentials (heads of 128 in parts: none, no register is left)
   constexpr int AHEAD = DP == 64 ? 2 : !PARTS ? 1 : 0;
@@ -981,7 +981,7 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
 
 template <typename T, int DP, int KW, int WAVES, bool PARTS, bool WIN>
 __global__ __launch_bounds__(WAVES == 8 ? 512 : 256) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_dkv(Attend a) {
-  __shared__ DkvTiles<T, DP, WAVES> lds[WAVES == 1 ? 4 : 1];
+  __shared__ DkvTiles<T, DP, WAVES, KW> lds[WAVES == 1 ? 4 : 1];
   const int parts = PARTS ? a.parts_k : 1;
   Place p;
   if constexpr (WAVES == 1) {  // each wave a tile of its own
@@ -999,7 +999,7 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256) __attribute__((amdgpu_waves
 // the far rows' parts; WAVES waves, as many as a row tile has subtiles
 template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_far(Attend a) {
-  __shared__ DkvTiles<T, DP, WAVES> lds;
+  __shared__ DkvTiles<T, DP, WAVES, 1> lds;
   constexpr int ROLES = DP == 64 ? 1 : 2;
   int b = blockIdx.x;
   const int role = b % ROLES;
@@ -1102,7 +1102,7 @@ size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group, int windo
 }
 // Where the sinks' far rows are walked over apart: where there are sinks, at most four tiles of 32, and a sequence may be longer
 // than a window and half a part; not where their slots would take more than 1 GB.
-constexpr int FAR_TOKENS = 512;
+constexpr int FAR_TOKENS = 256;
 struct FarPlan { int tokens, least, chunks; long long slots; };
 FarPlan far_plan(int kv_heads, int dim, int tq, int tk, int window, int sinks) {
   FarPlan r = {0, window + 1 > 64 ? window + 1 : 64, (sinks + 31) / 32, 0};
