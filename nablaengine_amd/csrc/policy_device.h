@@ -73,21 +73,20 @@ __device__ __forceinline__ float sum_lanes(float x) {
 }
 
 constexpr float LOG2E_GATE = 1.4426950408889634f;
-// a = 1 / (1 + exp(-f)) and 1 - a of a gate in T, each to its own last places
+// a = 1 / (1 + exp(-f)) and 1 - a of a gate in T, each to its own last places (down to 2^-126, below which they are 0)
 template <typename T>
 __device__ __forceinline__ void gates(float f, float& keep, float& take) {
   float e;
   if constexpr (sizeof(T) == 4) {  // with the product's rounding, which is felt by far gates
-    const float z = -fminf(fabsf(f), 200.0f), t = z * LOG2E_GATE;
+    f = f > 200.0f ? 200.0f : f;
+    const float t = -f * LOG2E_GATE;
     e = __builtin_amdgcn_exp2f(t);
-    e = fmaf(e, fmaf(z, LOG2E_GATE, -t) * 0.6931472f, e);
-    if (f != f) e = f;
+    e = t > 126.0f ? INFINITY : fmaf(e, fmaf(-f, LOG2E_GATE, -t) * 0.6931472f, e);
   } else {
-    e = __builtin_amdgcn_exp2f(-fabsf(f) * LOG2E_GATE);
+    e = __builtin_amdgcn_exp2f(-f * LOG2E_GATE);
   }
-  const float r = __builtin_amdgcn_rcpf(1.0f + e), small = e * r;
-  keep = f >= 0.0f ? r : small;
-  take = f >= 0.0f ? small : r;
+  keep = __builtin_amdgcn_rcpf(1.0f + e);
+  take = f >= 0.0f ? e * keep : 1.0f - keep;
 }
 
 // the sum of x over this lane and those before it in the wave

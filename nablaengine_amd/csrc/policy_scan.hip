@@ -66,7 +66,7 @@ __device__ __forceinline__ int scan_uniform(int x) { return __builtin_amdgcn_rea
 // Where sequences start inside a chunk: at[i] is the sequence whose first token is the chunk's token i (the last of those
 // that start there; `seqs` where the tokens behind the last sequence begin), -1 where none is; i up to CHUNK, the next
 // chunk's first token. Returns the sequence that holds the chunk's first token. Every thread of the workgroup calls it. The
-// offsets are searched by all threads at once: one read up to NT sequences, two up to NT^2.
+// offsets are searched by all threads at once: one read where lengths are even enough, two more up to NT^2 sequences.
 template <int CHUNK, int NT>
 __device__ __forceinline__ int find_starts(const Scan& a, int t0, int* at) {
   auto value = [&](int s) {
@@ -75,16 +75,25 @@ __device__ __forceinline__ int find_starts(const Scan& a, int t0, int* at) {
   };
   const int tid = threadIdx.x;
   for (int i = tid; i <= CHUNK; i += NT) at[i] = -1;
-  int lo = 0, n = a.seqs + 1;  // the last start at or before t0 is one of lo .. lo + n - 1
-  while (n > NT) {
-    const int step = (n - 1) / NT + 1;
-    const long long idx = (long long)tid * step;
-    const int c = __syncthreads_count(idx < n && value(lo + (int)idx) <= t0), skip = c > 0 ? (c - 1) * step : 0;
-    n = n - skip < step ? n - skip : step;
-    lo += skip;
-  }
+  // where the chunk's first token would lie if all sequences were as long: mostly the starts are among the NT around
+  const long long guess = (long long)(a.seqs + 1) * t0 / a.tokens - NT / 2, most = (long long)a.seqs + 1 - NT;
+  int lo = guess < 0 || most < 0 ? 0 : (int)(guess < most ? guess : most), n = a.seqs + 1 - lo < NT ? a.seqs + 1 - lo : NT;
   int v = tid < n ? value(lo + tid) : 0;
-  const int c = __syncthreads_count(tid < n && v <= t0), base = lo + (c > 0 ? c : 1) - 1;
+  int c = __syncthreads_count(tid < n && v <= t0);
+  if ((c == 0 && lo > 0) || (c == n && lo + n <= a.seqs)) {  // they are not: all are searched
+    lo = 0, n = a.seqs + 1;  // the last start at or before t0 is one of lo .. lo + n - 1
+    while (n > NT) {
+      const int step = (n - 1) / NT + 1;
+      const long long idx = (long long)tid * step;
+      c = __syncthreads_count(idx < n && value(lo + (int)idx) <= t0);
+      const int skip = c > 0 ? (c - 1) * step : 0;
+      n = n - skip < step ? n - skip : step;
+      lo += skip;
+    }
+    v = tid < n ? value(lo + tid) : 0;
+    c = __syncthreads_count(tid < n && v <= t0);
+  }
+  const int base = lo + (c > 0 ? c : 1) - 1;
   bool mine = tid < n;
   for (int s = lo + tid, next = lo + n;;) {  // until a start lies behind the chunk
     if (mine && v >= t0 && v - t0 <= CHUNK) atomicMax(&at[v - t0], s);
@@ -156,27 +165,20 @@ __device__ __forceinline__ void through(const Joined<W, V>& j, int w, float* s) 
   for (int e = 0; e < V; ++e) s[e] = drops ? j.b[w][l][e] : fmaf(j.p[w][l][e], s[e], j.b[w][l][e]);
 }
 
-// sequence s's state before its first token
+// sequence s's row of a (seqs, channels) table, zeros where there is none
 template <int V>
-__device__ __forceinline__ void initial_of(const Scan& a, int s, int c, float* f) {
-  const float* p = a.initial && s >= 0 && s < a.seqs ? a.initial + (long long)s * a.channels + c : nullptr;
-#pragma unroll
-  for (int e = 0; e < V; ++e) f[e] = p ? p[e] : 0.0f;
-}
-template <int V>
-__device__ __forceinline__ void last_of(const Scan& a, int s, int c, float* f) {  // dlast
-  const float* p = a.dlast && s >= 0 && s < a.seqs ? a.dlast + (long long)s * a.channels + c : nullptr;
-#pragma unroll
-  for (int e = 0; e < V; ++e) f[e] = p ? p[e] : 0.0f;
+__device__ __forceinline__ Few<float, V> state_of(const Scan& a, const float* table, int s, int c) {
+  Few<float, V> r = {};
+  if (table && s >= 0 && s < a.seqs) r = load_few<float, V>(table + (long long)s * a.channels + (unsigned)c);
+  return r;
 }
 
 template <typename T, int V, int TOK>
 __device__ __forceinline__ void load_tokens(const void* from, long long stride, const Scan& a, int t0, int c, Few<T, V>* r) {
-  const T* p = (const T*)from + c;
 #pragma unroll
   for (int i = 0; i < TOK; ++i) {  // tokens past the end: the last one again
     const int t = t0 + i < a.tokens ? t0 + i : a.tokens - 1;
-    r[i] = load_few<T, V>(p + t * stride);
+    r[i] = load_few<T, V>((const T*)from + t * stride + (unsigned)c);  // the row is the wave's, the channel the lane's
   }
 }
 
@@ -231,7 +233,11 @@ __global__ __launch_bounds__(64 * W) void k_scan_parts(Scan a) {
     Few<T, V> f[TOK], x[TOK];
     load_tokens<T, V, TOK>(a.gate, a.g_t, a, st.t0, lane.c, f);
     load_tokens<T, V, TOK>(a.x, a.x_t, a, st.t0, lane.c, x);
-    walk<T, V, TOK>(st, f, [&](int i) { initial_of<V>(a, st.sequence_at(i), lane.c, b); },
+    walk<T, V, TOK>(st, f, [&](int i) {
+                      const auto s = state_of<V>(a, a.initial, st.sequence_at(i), lane.c);
+#pragma unroll
+                      for (int e = 0; e < V; ++e) b[e] = s.v[e];
+                    },
                     [&](int i) {
 #pragma unroll
                       for (int e = 0; e < V; ++e) {
@@ -296,10 +302,12 @@ __global__ __launch_bounds__(64 * W) void k_scan_back_parts(Scan a) {
     else
 #pragma unroll
       for (int i = 0; i < TOK; ++i) d[i] = Few<T, V>{};
-    int seq = st.seq;  // of the tokens up to the first cut after the stretch's first token, which alone matter
     const unsigned later = st.cuts >> 1;
-    const int end = later ? __builtin_ctz(later) + 1 : TOK;  // tokens 0 .. end - 1 lead to the token before
-    if (later) last_of<V>(a, seq, lane.c, b);
+    // tokens 0 .. end - 1, of the first token's sequence, lead to the token before
+    const int end = later ? __builtin_ctz(later) + 1 : TOK;
+    const auto last = state_of<V>(a, a.dlast, later ? st.seq : -1, lane.c);
+#pragma unroll
+    for (int e = 0; e < V; ++e) b[e] = last.v[e];
 #pragma unroll
     for (int i = TOK - 1; i >= 0; --i)
       if (i < end)
@@ -341,12 +349,24 @@ __global__ __launch_bounds__(1024) void k_scan_carry(Scan a) {
   const int n = a.chunks - 1, each = (n + 63) / 64;  // the maps between neighbouring chunks, in the order of the walk
   const int first = run * each < n ? run * each : n, end = first + each < n ? first + each : n;
   auto at = [&](int i) { return a.parts + (long long)(BACK ? a.chunks - 1 - i : i) * 2 * a.channels + (in ? c : 0); };
-  float p = 1.0f, b = 0.0f;
-#pragma unroll 8
-  for (int i = first; i < end; ++i) {
-    const float pi = at(i)[0], bi = at(i)[a.channels];
+  constexpr int KEPT = 16;  // maps that stay in registers for the second walk: up to 1024 chunks, which take 8 us, and 14 with two reads
+  float pk[KEPT], bk[KEPT], p = 1.0f, b = 0.0f;
+  const bool kept = each <= KEPT;
+  auto step = [&](float pi, float bi) {
     b = pi < 0.0f ? bi : fmaf(pi, b, bi);
     p = pi < 0.0f || p < 0.0f ? -1.0f : p * pi;
+  };
+  if (kept) {
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) {
+      const bool there = first + i < end;
+      pk[i] = there ? at(first + i)[0] : 1.0f, bk[i] = there ? at(first + i)[a.channels] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) step(pk[i], bk[i]);
+  } else {
+#pragma unroll 8
+    for (int i = first; i < end; ++i) step(at(i)[0], at(i)[a.channels]);
   }
   int side = 0;
   ps[0][run][threadIdx.x % 16] = p, bs[0][run][threadIdx.x % 16] = b;
@@ -364,11 +384,17 @@ __global__ __launch_bounds__(1024) void k_scan_carry(Scan a) {
   float s = run ? bs[side][run - 1][threadIdx.x % 16] : 0.0f;  // nothing enters the first chunk
   float* out = BACK ? a.back : a.carry;
   if (run == 0 && in) out[(long long)(BACK ? a.chunks - 1 : 0) * a.channels + c] = 0.0f;
-#pragma unroll 8
-  for (int i = first; i < end; ++i) {
-    const float pi = at(i)[0], bi = at(i)[a.channels];
+  auto put = [&](int i, float pi, float bi) {
     s = pi < 0.0f ? bi : fmaf(pi, s, bi);
     if (in) out[(long long)(BACK ? a.chunks - 2 - i : i + 1) * a.channels + c] = s;
+  };
+  if (kept) {
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i)
+      if (first + i < end) put(first + i, pk[i], bk[i]);
+  } else {
+#pragma unroll 8
+    for (int i = first; i < end; ++i) put(i, at(i)[0], at(i)[a.channels]);
   }
 }
 
@@ -411,13 +437,13 @@ __global__ __launch_bounds__(64 * W) void k_scan(Scan a) {
   const Stretch<TOK> st(a, at, base, chunk * CHUNK, w);
   const unsigned inside = st.cuts & ((1u << TOK) - 1);
   const int first = inside ? __builtin_ctz(inside) : 0;
-  float first_init[V];  // on its way beside the tokens; further starts in the stretch read theirs when they come
-  initial_of<V>(a, inside ? st.sequence_at(first) : -1, lane.c, first_init);
+  // on its way beside the tokens; further starts in the stretch read theirs when they come
+  const auto first_state = state_of<V>(a, a.initial, inside ? st.sequence_at(first) : -1, lane.c);
   auto start = [&](int i, float* to) {
-    if (i == first)
+    auto s = first_state;
+    if (i != first) s = state_of<V>(a, a.initial, st.sequence_at(i), lane.c);
 #pragma unroll
-      for (int e = 0; e < V; ++e) to[e] = first_init[e];
-    else initial_of<V>(a, st.sequence_at(i), lane.c, to);
+    for (int e = 0; e < V; ++e) to[e] = s.v[e];
   };
   float keep[TOK][V], bx[TOK][V], p[V], b[V];
 #pragma unroll
@@ -441,7 +467,7 @@ __global__ __launch_bounds__(64 * W) void k_scan(Scan a) {
   __syncthreads();
   for (int o = 0; o < w; ++o) through<W, V>(joined, o, s);
   if (!lane.counts) return;
-  T* h = (T*)a.h + (long long)st.t0 * a.channels + lane.c;
+  auto put = [&](int i, const float* f) { store_few<T, V>((T*)a.h + (long long)(st.t0 + i) * a.channels + (unsigned)lane.c, f); };
   int seq = st.seq;
   walk<T, V, TOK>(st, f,
                   [&](int i) {
@@ -451,9 +477,9 @@ __global__ __launch_bounds__(64 * W) void k_scan(Scan a) {
                   [&](int i) {
 #pragma unroll
                     for (int e = 0; e < V; ++e) s[e] = fmaf(keep[i][e], s[e], bx[i][e]);
-                    store_few<T, V>(h + (long long)i * a.channels, s);
+                    put(i, s);
                     if (st.cuts >> (i + 1) & 1) {
-                      float* last = a.last + (long long)seq * a.channels + lane.c;
+                      float* last = a.last + (long long)seq * a.channels + (unsigned)lane.c;
 #pragma unroll
                       for (int e = 0; e < V; ++e) last[e] = s[e];
                     }
@@ -461,11 +487,11 @@ __global__ __launch_bounds__(64 * W) void k_scan(Scan a) {
   const float none[V] = {};
 #pragma unroll
   for (int i = 0; i < TOK; ++i)
-    if (i >= st.live && i < st.there) store_few<T, V>(h + (long long)i * a.channels, none);
+    if (i >= st.live && i < st.there) put(i, none);
 }
 
 template <typename T, int V, int W, int TOK>
-__global__ __launch_bounds__(64 * W) void k_scan_vjp(Scan a) {
+__global__ __launch_bounds__(64 * W, 4) void k_scan_vjp(Scan a) {
   constexpr int CHUNK = W * TOK, NT = 64 * W;
   __shared__ int at[CHUNK + 1];
   __shared__ Joined<W, V> ahead, behind;
@@ -497,37 +523,38 @@ __global__ __launch_bounds__(64 * W) void k_scan_vjp(Scan a) {
     const unsigned starts = inside & ((1u << i) - 1);
     return starts ? st.sequence_at(31 - __builtin_clz(starts)) : st.seq;
   };
-  float first_init[V], final_d[V];
-  initial_of<V>(a, inside ? st.sequence_at(first) : -1, lane.c, first_init);
-  last_of<V>(a, later ? before(final) : -1, lane.c, final_d);
+  const auto first_state = state_of<V>(a, a.initial, inside ? st.sequence_at(first) : -1, lane.c);
+  const auto final_d = state_of<V>(a, a.dlast, later ? before(final) : -1, lane.c);
   auto start = [&](int i, float* to) {
-    if (i == first)
+    auto s = first_state;
+    if (i != first) s = state_of<V>(a, a.initial, st.sequence_at(i), lane.c);
 #pragma unroll
-      for (int e = 0; e < V; ++e) to[e] = first_init[e];
-    else initial_of<V>(a, st.sequence_at(i), lane.c, to);
+    for (int e = 0; e < V; ++e) to[e] = s.v[e];
   };
-  auto end = [&](int i, float* to) {  // the token before cut i: its sequence's last
-    if (i == final)
-#pragma unroll
-      for (int e = 0; e < V; ++e) to[e] = final_d[e];
-    else last_of<V>(a, before(i), lane.c, to);
+  auto end = [&](int i) {  // the token before cut i
+    auto s = final_d;
+    if (i != final) s = state_of<V>(a, a.dlast, before(i), lane.c);
+    return s;
   };
-  float keep[TOK][V], p[V], b[V], q[V], c[V];
+  // Both ways' P and B in one walk: the other way's B is the sum of the cotangents, each times the product of the gates up to its
+  // token, up to the first sequence's end. Gates are computed anew in each of the three walks: kept, they would take the registers
+  // of the second workgroup on a compute unit.
+  float p[V], b[V], q[V], c[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) p[e] = q[e] = 1.0f, b[e] = c[e] = 0.0f;
-  float prev[TOK][V];  // take x, then the state before each token
-#pragma unroll
-  for (int i = 0; i < TOK; ++i)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float take;
-      gates<T>((float)f[i].v[e], keep[i][e], take);
-      prev[i][e] = take * (float)x[i].v[e];
-    }
+  const int led = later ? __builtin_ctz(later) : TOK;  // tokens that lead to the stretch's first without an end between
+  auto led_d = final_d;
+  if (led != final) led_d = state_of<V>(a, a.dlast, later ? st.seq : -1, lane.c);
   walk<T, V, TOK>(st, f, [&](int i) { start(i, b); },
                   [&](int i) {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) p[e] *= keep[i][e], b[e] = fmaf(keep[i][e], b[e], prev[i][e]);
+                    for (int e = 0; e < V; ++e) {
+                      float keep, take;
+                      gates<T>((float)f[i].v[e], keep, take);
+                      p[e] *= keep;
+                      b[e] = fmaf(keep, b[e], take * (float)x[i].v[e]);
+                      if (i < led) q[e] = p[e], c[e] = fmaf(p[e], (float)d[i].v[e] + (i == led - 1 ? led_d.v[e] : 0.0f), c[e]);
+                    }
                   });
   const bool plain = st.live == TOK && !st.cuts;
   auto walk_back = [&](auto ends, auto step) {  // from the last token on
@@ -543,11 +570,6 @@ __global__ __launch_bounds__(64 * W) void k_scan_vjp(Scan a) {
         }
     }
   };
-  walk_back([&](int i) { end(i, c); },
-            [&](int i) {
-#pragma unroll
-              for (int e = 0; e < V; ++e) q[e] *= keep[i][e], c[e] = keep[i][e] * (c[e] + (float)d[i].v[e]);
-            });
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     ahead.p[w][l][e] = p[e], ahead.b[w][l][e] = b[e];
@@ -558,17 +580,25 @@ __global__ __launch_bounds__(64 * W) void k_scan_vjp(Scan a) {
   for (int o = 0; o < w; ++o) through<W, V>(ahead, o, s);
   for (int o = W - 1; o > w; --o) through<W, V>(behind, o, r);
   if (!lane.counts) return;
+  float off[TOK][V];  // how far the state before each token is from its x
   walk<T, V, TOK>(st, f, [&](int i) { start(i, s); },
                   [&](int i) {
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
-                      const float bx = prev[i][e];
-                      prev[i][e] = s[e];
-                      s[e] = fmaf(keep[i][e], s[e], bx);
+                      float keep, take;
+                      gates<T>((float)f[i].v[e], keep, take);
+                      off[i][e] = s[e] - (float)x[i].v[e];
+                      s[e] = fmaf(keep, s[e], take * (float)x[i].v[e]);
                     }
                   });
-  const long long at0 = (long long)st.t0 * a.channels + lane.c;
-  walk_back([&](int i) { end(i, r); },
+  auto put = [&](void* to, int i, const float* f) {
+    if (to) store_few<T, V>((T*)to + (long long)(st.t0 + i) * a.channels + (unsigned)lane.c, f);
+  };
+  walk_back([&](int i) {
+              const auto s = end(i);
+#pragma unroll
+              for (int e = 0; e < V; ++e) r[e] = s.v[e];
+            },
             [&](int i) {
               float dx[V], dg[V];
 #pragma unroll
@@ -578,12 +608,12 @@ __global__ __launch_bounds__(64 * W) void k_scan_vjp(Scan a) {
                 const float g = r[e] + (float)d[i].v[e];
                 dx[e] = take * g;
                 r[e] = k * g;
-                dg[e] = dx[e] * k * (prev[i][e] - (float)x[i].v[e]);
+                dg[e] = dx[e] * k * off[i][e];
               }
-              if (a.dx) store_few<T, V>((T*)a.dx + at0 + (long long)i * a.channels, dx);
-              if (a.dgate) store_few<T, V>((T*)a.dgate + at0 + (long long)i * a.channels, dg);
+              put(a.dx, i, dx);
+              put(a.dgate, i, dg);
               if ((st.cuts >> i & 1) && a.dinitial) {
-                float* to = a.dinitial + (long long)st.sequence_at(i) * a.channels + lane.c;
+                float* to = a.dinitial + (long long)st.sequence_at(i) * a.channels + (unsigned)lane.c;
 #pragma unroll
                 for (int e = 0; e < V; ++e) to[e] = r[e];
               }
@@ -591,10 +621,7 @@ __global__ __launch_bounds__(64 * W) void k_scan_vjp(Scan a) {
   const float none[V] = {};
 #pragma unroll
   for (int i = 0; i < TOK; ++i)
-    if (i >= st.live && i < st.there) {
-      if (a.dx) store_few<T, V>((T*)a.dx + at0 + (long long)i * a.channels, none);
-      if (a.dgate) store_few<T, V>((T*)a.dgate + at0 + (long long)i * a.channels, none);
-    }
+    if (i >= st.live && i < st.there) put(a.dx, i, none), put(a.dgate, i, none);
 }
 
 // ---- one token a world ----------------------------------------------------------------------------------------------
