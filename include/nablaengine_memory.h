@@ -14,7 +14,7 @@ extern "C" {
  * channels) float32, the states before the first tokens, or NULL for zeros. h (tokens, channels) contiguous, zeros behind the
  * last sequence; last (seqs, channels) float32, the states after the last tokens (of a sequence without tokens: its initial one).
  * carry: dk_recurrence_carry_bytes bytes, which the backward reads again; work: dk_recurrence_work_bytes bytes (vjp 0); both
- * NULL when 0. channels >= 1; a launch's work-items bound (tokens / 128) (channels / 64) by a little below 2^23. */
+ * NULL when 0. channels >= 1; a launch's work-items bound (tokens / 64) (channels / 64) by a little below 2^23. */
 int dk_recurrence(hipStream_t st, int type, int tokens, int channels, int seqs, const void* x, long long x_t, const void* gate,
                   long long gate_t, const int* starts, const float* initial, void* h, float* last, float* carry, void* work);
 /* Its VJP, from the forward's arguments and carry: dh (type, dh_t elements from token to token) and dlast (seqs, channels)

@@ -339,17 +339,19 @@ __global__ __launch_bounds__(64 * W) void k_scan_back_parts(Scan a) {
 
 // ---- the states that enter the chunks -------------------------------------------------------------------------------
 
-// 16 channels a workgroup and 64 runs of chunks: each run's own P and B, those joined over the runs by doubling, then each
-// run once more from the state that enters it. BACK: the chunks from the last to the first.
+// 8 channels a workgroup and 128 runs of chunks: each run's own P and B, those joined over the runs by doubling, then each
+// run once more from the state that enters it. BACK: the chunks from the last to the first. Bound by one read after another: 1400
+// chunks of 512 channels 9 us, 11 with 16 channels and 64 runs.
 template <bool BACK>
 __global__ __launch_bounds__(1024) void k_scan_carry(Scan a) {
-  __shared__ float ps[2][64][16], bs[2][64][16];
-  const int c = blockIdx.x * 16 + threadIdx.x % 16, run = threadIdx.x / 16;
+  constexpr int CH = 8, RUNS = 1024 / CH;
+  __shared__ float ps[2][RUNS][CH], bs[2][RUNS][CH];
+  const int l = threadIdx.x % CH, c = blockIdx.x * CH + l, run = threadIdx.x / CH;
   const bool in = c < a.channels;
-  const int n = a.chunks - 1, each = (n + 63) / 64;  // the maps between neighbouring chunks, in the order of the walk
+  const int n = a.chunks - 1, each = (n + RUNS - 1) / RUNS;  // the maps between neighbouring chunks, in the order of the walk
   const int first = run * each < n ? run * each : n, end = first + each < n ? first + each : n;
   auto at = [&](int i) { return a.parts + (long long)(BACK ? a.chunks - 1 - i : i) * 2 * a.channels + (in ? c : 0); };
-  constexpr int KEPT = 16;  // maps that stay in registers for the second walk: up to 1024 chunks, which take 8 us, and 14 with two reads
+  constexpr int KEPT = 16;  // maps that stay in registers for the second walk: up to 2048 chunks
   float pk[KEPT], bk[KEPT], p = 1.0f, b = 0.0f;
   const bool kept = each <= KEPT;
   auto step = [&](float pi, float bi) {
@@ -369,19 +371,19 @@ __global__ __launch_bounds__(1024) void k_scan_carry(Scan a) {
     for (int i = first; i < end; ++i) step(at(i)[0], at(i)[a.channels]);
   }
   int side = 0;
-  ps[0][run][threadIdx.x % 16] = p, bs[0][run][threadIdx.x % 16] = b;
+  ps[0][run][l] = p, bs[0][run][l] = b;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2, side ^= 1) {
+  for (int d = 1; d < RUNS; d *= 2, side ^= 1) {
     __syncthreads();
     if (run >= d) {
-      const float p0 = ps[side][run - d][threadIdx.x % 16], b0 = bs[side][run - d][threadIdx.x % 16];
+      const float p0 = ps[side][run - d][l], b0 = bs[side][run - d][l];
       b = p < 0.0f ? b : fmaf(p, b0, b);
       p = p < 0.0f || p0 < 0.0f ? -1.0f : p * p0;
     }
-    ps[side ^ 1][run][threadIdx.x % 16] = p, bs[side ^ 1][run][threadIdx.x % 16] = b;
+    ps[side ^ 1][run][l] = p, bs[side ^ 1][run][l] = b;
   }
   __syncthreads();
-  float s = run ? bs[side][run - 1][threadIdx.x % 16] : 0.0f;  // nothing enters the first chunk
+  float s = run ? bs[side][run - 1][l] : 0.0f;  // nothing enters the first chunk
   float* out = BACK ? a.back : a.carry;
   if (run == 0 && in) out[(long long)(BACK ? a.chunks - 1 : 0) * a.channels + c] = 0.0f;
   auto put = [&](int i, float pi, float bi) {
@@ -499,7 +501,7 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_vjp(Scan a) {
     if (a.dinitial) empty_sequences(a, a.dlast, a.dinitial);
     return;
   }
-  const int chunk = blockIdx.x / a.groups, w = scan_uniform(threadIdx.x / 64), l = threadIdx.x % 64;
+  const int chunk = a.chunks - 1 - blockIdx.x / a.groups, w = scan_uniform(threadIdx.x / 64), l = threadIdx.x % 64;
   const Lane<V> lane(a, blockIdx.x % a.groups);
   Few<T, V> f[TOK], x[TOK], d[TOK];
   load_tokens<T, V, TOK>(a.gate, a.g_t, a, chunk * CHUNK + w * TOK, lane.c, f);
@@ -716,7 +718,7 @@ int launch_scan(hipStream_t st, int type, const Scan& a) {
       k_scan_parts<T, V, W, SCAN_TOKENS><<<(unsigned)((a.chunks - 1) * a.groups), 64 * W, 0, st>>>(a);
       hipError_t e = hipGetLastError();
       if (e != hipSuccess) return (int)e;
-      k_scan_carry<false><<<(unsigned)((a.channels + 15) / 16), 1024, 0, st>>>(a);
+      k_scan_carry<false><<<(unsigned)((a.channels + 7) / 8), 1024, 0, st>>>(a);
       e = hipGetLastError();
       if (e != hipSuccess) return (int)e;
     }
@@ -733,12 +735,12 @@ int launch_scan_vjp(hipStream_t st, int type, const Scan& a) {
       k_scan_back_parts<T, V, W, SCAN_TOKENS><<<(unsigned)((a.chunks - 1) * a.groups), 64 * W, 0, st>>>(a);
       hipError_t e = hipGetLastError();
       if (e != hipSuccess) return (int)e;
-      k_scan_carry<true><<<(unsigned)((a.channels + 15) / 16), 1024, 0, st>>>(a);
+      k_scan_carry<true><<<(unsigned)((a.channels + 7) / 8), 1024, 0, st>>>(a);
       e = hipGetLastError();
       if (e != hipSuccess) return (int)e;
     }
     const unsigned blocks = scan_blocks(a);
-    if (blocks) k_scan_vjp<T, V, W, SCAN_TOKENS><<<blocks, 64 * W, 0, st>>>(a);
+    if (blocks) k_scan_vjp<T, V, SCAN_CHUNK / SCAN_TOKENS_VJP, SCAN_TOKENS_VJP><<<blocks, 64 * SCAN_CHUNK / SCAN_TOKENS_VJP, 0, st>>>(a);
     return (int)hipGetLastError();
   });
 }

@@ -21,7 +21,7 @@ constexpr bool attention_sizes(int heads, int kv_heads, int seqs, int tq, int tk
 // for the backward, as for rows of no more keys without a window.
 constexpr int NARROW = 64;
 
-constexpr int SCAN_TOKENS = 16, SCAN_CHUNK = 128;  // the recurrence's tokens a wave and a workgroup
+constexpr int SCAN_TOKENS = 16, SCAN_TOKENS_VJP = 8, SCAN_CHUNK = 64;  // the recurrence's tokens a wave (of its backward) and a workgroup
 
 // whether the recurrence's indices and grids hold these sizes: workgroups of 512 work-items, one a chunk and 64 channels at least
 constexpr bool scan_sizes(int tokens, int channels, int seqs) {

@@ -135,8 +135,8 @@ def _fake_recurrence(x, gate, starts, initial):
 
 
 def _carry_words(tokens, channels):
-    """dk_recurrence_carry_bytes / 4, of symbolic sizes too: a row for each chunk of 128 tokens."""
-    return (tokens + 127) // 128 * channels
+    """dk_recurrence_carry_bytes / 4, of symbolic sizes too: a row for each chunk of 64 tokens."""
+    return (tokens + 63) // 64 * channels
 
 
 def _fake_recurrence_forward(x, gate, starts, initial):
