@@ -33,10 +33,42 @@ struct Residual {
   float* part;            // (blocks, 2, n): each workgroup's m and dw', or NULL
 };
 
+// how many of vector v's first elements the vector before it holds too; elements past the row are 0 and count as nothing
+template <int E>
+__device__ __forceinline__ int repeated(int v, int n) {
+  return n >= E && v < vectors_in(n, E) ? v * E - first_of<E>(v, n) : 0;
+}
 // vector v of a row of activations that may not be there
 template <typename T>
 __device__ __forceinline__ void given(const void* p, long long row, long long stride, int v, int n, float* f) {
   row_load<Vec<T>::E>(p ? (const T*)p + row * stride : (const T*)nullptr, v, n, 0.0f, f);
+}
+// the same as it is
+template <typename T>
+__device__ __forceinline__ Vec<T> row_vector(const T* p, int v, int n) {
+  constexpr int E = Vec<T>::E;
+  Vec<T> r = {};
+  if (p && v * E < n) {
+    if (n >= E) {
+      r = load16(p + first_of<E>(v, n));
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e < n) r.v[e] = p[e];
+    }
+  }
+  return r;
+}
+// The compiler takes its 16 bytes for new ones: what was computed of them before is not kept in registers for later.
+template <typename T>
+__device__ __forceinline__ void anew(Vec<T>& v) {
+  unsigned x[4];
+  __builtin_memcpy(x, &v, 16);
+  asm("" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+  __builtin_memcpy(&v, x, 16);
+}
+__device__ __forceinline__ float of_wave(float x) {  // one for all lanes
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
 }
 template <typename T>
 __device__ __forceinline__ float open_gate(const Residual& a, float f, float& shut) {
@@ -57,6 +89,9 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void k_residual(Residual a) {
     row_load<E>((const W*)a.w, lane + c * L, n, 1.0f, w[to]);
     row_load<E>((const W*)a.s, lane + c * L, n, 1.0f, sc[to]);
   };
+  int repeats[C];  // elements of this lane's vectors that the one before has: the row's last vector ends with it
+#pragma unroll
+  for (int c = 0; c < C; ++c) repeats[c] = repeated<E>(lane + c * L, n);
   auto next_params = [&](int c, int to) { row_load<E>((const W*)a.w2, lane + c * L, n, 1.0f, w2[to]); };
   if (KEEP)
 #pragma unroll
@@ -75,7 +110,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void k_residual(Residual a) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int e = 0; e < E; ++e) q += own<E>(lane + c * L, n, e) ? u[c][e] * u[c][e] : 0.0f;
+      for (int e = 0; e < E; ++e) q += e >= repeats[c] ? u[c][e] * u[c][e] : 0.0f;
     const float r = 1.0f / sqrtf(group_sum<L>(q, red) / (float)n + a.eps);
     q = 0.0f;
 #pragma unroll
@@ -87,7 +122,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void k_residual(Residual a) {
         float shut;
         const float sg = open_gate<T>(a, g[c][e], shut);
         x[c][e] += sc[at][e] * sg * (u[c][e] * r * w[at][e]);
-        q += own<E>(lane + c * L, n, e) ? x[c][e] * x[c][e] : 0.0f;
+        q += e >= repeats[c] ? x[c][e] * x[c][e] : 0.0f;
       }
     }
     const float r2 = 1.0f / sqrtf(group_sum<L>(q, red) / (float)n + a.eps);
@@ -163,71 +198,76 @@ __global__ __launch_bounds__(WIDE) void k_residual_wide(Residual a) {
 
 // ---- backward -------------------------------------------------------------------------------------------------------
 
-template <typename T, typename W, int L, int C>
-__global__ __launch_bounds__(vjp_block(L)) void k_residual_vjp(Residual a) {
-  constexpr int E = Vec<T>::E, GROUPS = vjp_block(L) / L, CE = C * E;
+template <typename T, typename W, int L>
+__global__ __launch_bounds__(vjp_block(L), 4) void k_residual_vjp(Residual a) {
+  constexpr int E = Vec<T>::E, GROUPS = vjp_block(L) / L;
   constexpr int SLOTS = L >= 64 ? GROUPS : 8;  // the sums left after those inside each wave
   __shared__ float red[16];
-  __shared__ float add[SLOTS > 1 ? SLOTS / 2 * L * CE : 1];
+  __shared__ float add[SLOTS > 1 ? SLOTS / 2 * L * E : 1];
   const int lane = threadIdx.x % L, group = threadIdx.x / L, n = a.n;
-  float am[CE], an[CE], w[CE], w2[CE], sc[CE];
+  // the parameters as the lanes of a group use them, the same for all rows; in LDS, since a lane's 24 floats would be the
+  // registers of the second workgroup (neighbouring lanes' 16 bytes side by side: lanes 32 bytes apart conflict)
+  __shared__ __align__(16) float params[3][L * E];
+  float am[E], an[E];
 #pragma unroll
-  for (int i = 0; i < CE; ++i) am[i] = an[i] = 0.0f;
+  for (int e = 0; e < E; ++e) am[e] = an[e] = 0.0f;
+  for (int v = threadIdx.x; v < L; v += vjp_block(L)) {
+    float f[E];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    row_load<E>((const W*)a.w, lane + c * L, n, 1.0f, w + c * E);
-    row_load<E>((const W*)a.w2, lane + c * L, n, 1.0f, w2 + c * E);
-    row_load<E>((const W*)a.s, lane + c * L, n, 1.0f, sc + c * E);
+    for (int i = 0; i < 3; ++i) {
+      row_load<E>((const W*)(i == 0 ? a.w : i == 1 ? a.w2 : a.s), v, n, 1.0f, f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) params[i][(e / 4 * L + v) * 4 + e % 4] = f[e];
+    }
   }
+  __syncthreads();
+  const int repeats = repeated<E>(lane, n);
   // as in the forward, groups of several waves stay together
   for (long long row = (long long)blockIdx.x * GROUPS + group;; row += (long long)gridDim.x * GROUPS) {
     if (L > 64 ? row - group >= a.rows : row >= a.rows) break;
     const int m = row < a.rows ? n : 0;
-    float x[CE], u[CE], g[CE], dy[CE], dz[CE];
+    int place = lane;  // anew for each row, so that the parameters are not read to registers once and for all
+    asm volatile("" : "+v"(place));
+    auto param = [&](int which, int e) { return params[which][(e / 4 * L + place) * 4 + e % 4]; };
+    // What is read stays as it is, half the registers of its floats in 16 bits; of the products only those that the sums between
+    // them need are kept: 126 registers a lane instead of 163, two workgroups a compute unit instead of one.
+    const Vec<T> xr = row_vector((const T*)a.x + row * a.x_r, lane, m);
+    Vec<T> ur = row_vector((const T*)a.u + row * a.u_r, lane, m);
+    const Vec<T> gr = row_vector(a.gate ? (const T*)a.gate + row * a.g_r : nullptr, lane, m);
+    Vec<T> yr = row_vector(a.dy ? (const T*)a.dy + row * a.dy_r : nullptr, lane, m);
+    Vec<T> zr = row_vector(a.dz ? (const T*)a.dz + row * a.dz_r : nullptr, lane, m);
+    float r = m ? a.stats[row] : 0.0f, r2 = m ? a.stats[a.rows + row] : 0.0f;
+    if (L >= 64) r = of_wave(r), r2 = of_wave(r2);
+    float q = 0.0f, yh[E], sg[E], shut[E];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      given<T>(a.x, row, a.x_r, lane + c * L, m, x + c * E);
-      given<T>(a.u, row, a.u_r, lane + c * L, m, u + c * E);
-      given<T>(a.gate, row, a.g_r, lane + c * L, m, g + c * E);
-      given<T>(a.dy, row, a.dy_r, lane + c * L, m, dy + c * E);
-      given<T>(a.dz, row, a.dz_r, lane + c * L, m, dz + c * E);
-    }
-    const float r = m ? a.stats[row] : 0.0f, r2 = m ? a.stats[a.rows + row] : 0.0f;
-    float q = 0.0f;
-#pragma unroll
-    for (int i = 0; i < CE; ++i) {  // past the row's end all five were read as 0
-      float shut;
-      const float sg = open_gate<T>(a, g[i], shut);
-      u[i] *= r;                                             // uh
-      const float yh = (x[i] + sc[i] * sg * (u[i] * w[i])) * r2;
-      an[i] += dz[i] * yh;
-      dz[i] *= w2[i];
-      q += own<E>(lane + i / E * L, n, i % E) ? dz[i] * yh : 0.0f;
-      x[i] = yh;
+    for (int e = 0; e < E; ++e) {  // past the row's end all five were read as 0
+      sg[e] = open_gate<T>(a, (float)gr.v[e], shut[e]);
+      yh[e] = ((float)xr.v[e] + param(2, e) * sg[e] * ((float)ur.v[e] * r * param(0, e))) * r2;
+      const float dz = (float)zr.v[e];
+      an[e] += dz * yh[e];
+      q += e >= repeats ? dz * param(1, e) * yh[e] : 0.0f;
     }
     q = group_sum<L>(q, red) / (float)n;
-    float p = 0.0f;
+    anew(ur), anew(yr), anew(zr);
+    float p = 0.0f, c[E], dx[E], dg[E];
 #pragma unroll
-    for (int i = 0; i < CE; ++i) {
-      float shut;
-      const float sg = open_gate<T>(a, g[i], shut), e = dy[i] + r2 * (dz[i] - x[i] * q), es = e * sc[i];
-      am[i] += e * sg * u[i];
-      dy[i] = e;
-      dz[i] = es * sg * w[i];                                // c
-      g[i] = es * (u[i] * w[i]) * sg * shut;                 // dgate
-      p += own<E>(lane + i / E * L, n, i % E) ? dz[i] * u[i] : 0.0f;
+    for (int e = 0; e < E; ++e) {
+      const float uh = (float)ur.v[e] * r;
+      dx[e] = (float)yr.v[e] + r2 * ((float)zr.v[e] * param(1, e) - yh[e] * q);
+      c[e] = dx[e] * param(2, e) * sg[e] * param(0, e);
+      am[e] += dx[e] * sg[e] * uh;
+      dg[e] = c[e] * uh * shut[e];
+      p += e >= repeats ? c[e] * uh : 0.0f;
     }
-    p = group_sum<L>(p, red) / (float)n;
+    const bool mine = lane * E < m;
+    if (mine && a.dx) row_store((T*)a.dx + row * n, lane, n, dx);
+    if (mine && a.dgate) row_store((T*)a.dgate + row * n, lane, n, dg);
+    if (a.du) {
+      p = group_sum<L>(p, red) / (float)n;
+      anew(ur);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      if ((lane + c * L) * E >= m) continue;
-      if (a.dx) row_store((T*)a.dx + row * n, lane + c * L, n, dy + c * E);
-      if (a.dgate) row_store((T*)a.dgate + row * n, lane + c * L, n, g + c * E);
-      if (a.du) {
-#pragma unroll
-        for (int i = c * E; i < c * E + E; ++i) dz[i] = r * (dz[i] - u[i] * p);
-        row_store((T*)a.du + row * n, lane + c * L, n, dz + c * E);
-      }
+      for (int e = 0; e < E; ++e) c[e] = r * (c[e] - (float)ur.v[e] * r * p);
+      if (mine) row_store((T*)a.du + row * n, lane, n, c);
     }
   }
   if (!a.part) return;
@@ -237,10 +277,10 @@ __global__ __launch_bounds__(vjp_block(L)) void k_residual_vjp(Residual a) {
   for (int which = 0; which < 2; ++which) {
     float* s = which ? an : am;
 #pragma unroll
-    for (int i = 0; i < CE; ++i) {
-      if constexpr (L <= 8) s[i] += __shfl_xor(s[i], 8);
-      if constexpr (L <= 16) s[i] = add_rows(s[i]);
-      if constexpr (L <= 32) s[i] = add_halves(s[i]);
+    for (int e = 0; e < E; ++e) {
+      if constexpr (L <= 8) s[e] += __shfl_xor(s[e], 8);
+      if constexpr (L <= 16) s[e] = add_rows(s[e]);
+      if constexpr (L <= 32) s[e] = add_halves(s[e]);
     }
     const int slot = L >= 64 ? group : threadIdx.x / 64;
     const bool holds = L >= 64 || threadIdx.x % 64 < L;
@@ -249,18 +289,16 @@ __global__ __launch_bounds__(vjp_block(L)) void k_residual_vjp(Residual a) {
       __syncthreads();
       if (holds && slot >= half && slot < 2 * half)
 #pragma unroll
-        for (int i = 0; i < CE; ++i) add[((slot - half) * CE + i) * L + lane] = s[i];
+        for (int e = 0; e < E; ++e) add[((slot - half) * E + e) * L + lane] = s[e];
       __syncthreads();
       if (holds && slot < half)
 #pragma unroll
-        for (int i = 0; i < CE; ++i) s[i] += add[(slot * CE + i) * L + lane];
+        for (int e = 0; e < E; ++e) s[e] += add[(slot * E + e) * L + lane];
     }
     if (holds && slot == 0)
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (own<E>(lane + c * L, n, e)) out[(long long)which * n + first_of<E>(lane + c * L, n) + e] = s[c * E + e];
+      for (int e = 0; e < E; ++e)
+        if (own<E>(lane, n, e)) out[(long long)which * n + first_of<E>(lane, n) + e] = s[e];
   }
 }
 
@@ -376,21 +414,18 @@ __global__ __launch_bounds__(1024) void k_residual_params(int blocks, int n, con
 
 // ---- launches -------------------------------------------------------------------------------------------------------
 
-// Of by_width's groups, those whose lanes hold at most 8 elements: the backward keeps ten values for each.
-template <int E, typename F>
+// The backward's lanes hold one vector each: it keeps ten values for each element.
+template <typename F>
 bool by_width_vjp(int nv, F f) {
-  bool taken = false;
-  by_width<E>(nv, [&](auto l, auto c) {
-    if constexpr (decltype(c)::value * E <= 8) f(l, c), taken = true;
-    else if (nv <= 1024) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 1>{}), taken = true;
-  });
-  return taken;
+#define POL_CASE(L) \
+  if (nv <= L) { f(std::integral_constant<int, L>{}); return true; }
+  POL_CASE(8) POL_CASE(16) POL_CASE(32) POL_CASE(64) POL_CASE(128) POL_CASE(256) POL_CASE(512) POL_CASE(1024)
+#undef POL_CASE
+  return false;
 }
 int residual_blocks(long long rows, int n, int type) {
   int lanes = WIDE;
-  auto f = [&](auto l, auto) { lanes = decltype(l)::value; };
-  if (bytes_of(type) == 2) by_width_vjp<8>(vectors_of(n, type), f);
-  else by_width_vjp<4>(vectors_of(n, type), f);
+  by_width_vjp(vectors_of(n, type), [&](auto l) { lanes = decltype(l)::value; });
   const int groups = vjp_block(lanes) / lanes;
   const long long need = (rows + groups - 1) / groups, most = 2 * CUS;
   return (int)(need < most ? need : most);
@@ -404,7 +439,8 @@ int residual(hipStream_t st, const Residual& a, int type) {
   };
   if (!by_width<Vec<T>::E>(vectors_of(a.n, type), [&](auto l, auto c) {
         constexpr int L = decltype(l)::value, C = decltype(c)::value, BLOCK = L > 256 ? L : 256;
-        launch(k_residual<T, W, L, C>, BLOCK, BLOCK / L);
+        if constexpr (L * C * Vec<T>::E > 8192) launch(k_residual_wide<T, W>, WIDE, 1);  // the registers would not do
+        else launch(k_residual<T, W, L, C>, BLOCK, BLOCK / L);
       }))
     launch(k_residual_wide<T, W>, WIDE, 1);
   return (int)hipGetLastError();
@@ -413,9 +449,9 @@ template <typename T, typename W>
 int residual_vjp(hipStream_t st, const Residual& a, int type, void* dw, void* dw2, void* ds) {
   const int blocks = residual_blocks(a.rows, a.n, type);
   if (a.rows > 0) {
-    if (!by_width_vjp<Vec<T>::E>(vectors_of(a.n, type), [&](auto l, auto c) {
-          constexpr int L = decltype(l)::value, C = decltype(c)::value;
-          k_residual_vjp<T, W, L, C><<<blocks, vjp_block(L), 0, st>>>(a);
+    if (!by_width_vjp(vectors_of(a.n, type), [&](auto l) {
+          constexpr int L = decltype(l)::value;
+          k_residual_vjp<T, W, L><<<blocks, vjp_block(L), 0, st>>>(a);
         }))
       k_residual_vjp_wide<T, W><<<blocks, WIDE, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
