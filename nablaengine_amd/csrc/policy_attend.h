@@ -39,7 +39,7 @@ struct Attend {
   const void *q, *k, *v;
   long long q_t, q_h, k_t, k_h, v_t, v_h;  // elements from token to token, and from head to head
   int heads, kv_heads, group, dim, seqs, tq, tk;
-  int by_sequence;  // bit `list`: its order, see below
+  int by_sequence, grouped;  // bit `list`: its order, and whether its neighbours go to one XCD, see below
   int key_waves;  // 32 keys each: a tile of the keys' gradients (1 or 4)
   int parts_q, parts_k;  // workgroups (of a role) among which a query tile's keys, a key tile's rows are split
   const int *starts_q, *starts_k;

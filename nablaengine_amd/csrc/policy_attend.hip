@@ -160,7 +160,7 @@ __device__ __forceinline__ bool place(const Attend& a, int which, int at, Place&
 __device__ __forceinline__ bool place_of_block(const Attend& a, int which, int parts, Place& p) {
   const int b = blockIdx.x;
   int at;
-  if (a.by_sequence >> which & 1) {
+  if (a.grouped >> which & 1) {
     const int all = uniform(a.order[which]) * a.kv_heads * parts, base = b / (WINDOW * XCDS) * (WINDOW * XCDS);
     const int left = all - base, mine = left < WINDOW * XCDS ? (left + XCDS - 1) / XCDS : WINDOW, r = b - base;
     if (left <= 0 || r / XCDS >= mine) return false;
@@ -184,8 +184,9 @@ struct Rows {
   int pos, head, limit, all_see, any_sees, tiles;
   bool valid;
   // WIN: the workgroup's keys are the `front` sinks before its first row's window and all from that window on, `skip` keys
-  // further: their places are counted without the keys between, so that a few sinks fill no tile of their own
-  int front, skip;
+  // further: their places are counted without the keys between, so that a few sinks fill no tile of their own. A row sees the
+  // places up to hi, from lo on or before `sinks`.
+  int front, skip, hi, lo;
   __device__ __forceinline__ Rows(const Attend& a, const Place& p, int w) {
     const int rows = p.nq * a.group, off = p.nk - p.nq;
     const int row0 = p.tile * QROWS + 32 * w, row = row0 + threadIdx.x % 32;
@@ -204,19 +205,36 @@ struct Rows {
       front = skip ? a.sinks : 0;
     }
     tiles = last < 0 ? 0 : (last - skip) / TILE + 1;
+    hi = limit - skip;
+    const int own = WIN ? hi - a.window + 1 : 0;
+    lo = WIN && own < a.sinks ? a.sinks : own;
   }
   __device__ __forceinline__ int last_place() const { return any_sees - skip; }
-  // whether any of the wave's rows sees one of the 32 keys from a place on (up to last_place()), and whether some row does not see all
+  // of the 32 keys from a place on, up to last_place(): whether any of the wave's rows sees one; whether some row's last key, or
+  // its window's first, lies among them
   __device__ __forceinline__ bool sees(const Attend& a, int place) const {
-    return !WIN || place < front || place + skip + 31 > all_see - a.window || place + skip < a.sinks;
+    return !WIN || place < a.sinks || place + 31 > all_see - skip - a.window;
   }
-  __device__ __forceinline__ bool masks(const Attend& a, int place) const {
-    if (WIN && place < front) return place + 31 >= front;
-    return place + skip + 31 > all_see || (WIN && place + skip <= any_sees - a.window && place + skip + 31 >= a.sinks);
+  __device__ __forceinline__ bool ends(int place) const { return place + 31 > all_see - skip; }
+  __device__ __forceinline__ bool begins(const Attend& a, int place) const {
+    return WIN && place <= any_sees - skip - a.window && place + 31 >= a.sinks;
   }
-  __device__ __forceinline__ bool hides(const Attend& a, int place) const {  // from this lane's row
-    const int key = WIN && place >= front ? place + skip : place;
-    return key > limit || (WIN && window_hides(a, key, limit));
+  // f(j) for register j of a C of those keys where this lane's row does not see it; each border takes one comparison
+  template <typename F>
+  __device__ __forceinline__ void hidden(const Attend& a, int place, int h, F f) const {
+    if (ends(place)) {
+      const int last = hi - place - 4 * h;
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j % 4 + 8 * (j / 4) > last) f(j);
+    }
+    if (begins(a, place)) {
+      const int from = place + 4 * h - a.sinks;
+      const unsigned most = (unsigned)(lo - a.sinks);
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if ((unsigned)(from + j % 4 + 8 * (j / 4)) < most) f(j);
+    }
   }
 };
 
@@ -407,10 +425,7 @@ __global__ __launch_bounds__(256, 2) void k_attend(Attend a) {
       }
 #pragma unroll
       for (int x = 0; x < KS; ++x) s[i] = mfma(read_rows<DP>(kt, 32 * i, x, n, h), q[x], s[i]);
-      if (r.masks(a, key0 + 32 * i))
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (r.hides(a, key0 + 32 * i + j % 4 + 8 * (j / 4) + 4 * h)) s[i][j] = -INFINITY;
+      r.hidden(a, key0 + 32 * i, h, [&](int j) { s[i][j] = -INFINITY; });
     }
     float top = s[0][0];
 #pragma unroll
@@ -542,10 +557,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_dq(Attend a) {
       s = mfma(read_rows<DP>(kt, 32 * i, x, n, h), q[x], s);
       dp = mfma(read_rows<DP>(vt, 32 * i, x, n, h), g[x], dp);
     }
-    if (r.masks(a, key0 + 32 * i))
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (r.hides(a, key0 + 32 * i + j % 4 + 8 * (j / 4) + 4 * h)) s[j] = -INFINITY, dp[j] = 0.0f;
+    r.hidden(a, key0 + 32 * i, h, [&](int j) { s[j] = -INFINITY, dp[j] = 0.0f; });
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[j] = exp2_fast(fmaf(s[j], c, -lse));
   };
@@ -785,6 +797,8 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
   // that a thread's rows keep their distance from the tile's first token: RT or a little less rows are used of each.
   const RowTiles<MODE> all(a, p, KW, RT);
   const int sinks = MODE == WINDOWED ? near_sinks(a, p) : a.sinks;
+  // the first row whose window lies behind this lane's key; none for a sink (FAR: for a key that is none)
+  const int behind = (key < sinks) == (MODE == FAR) ? key + a.window : 0x7fffffff;
   const int rows = all.rows, used = all.used, first = all.first, back = used / group;  // back: tokens of a tile
   auto chunk = [&](int i) { return tid % CH ^ swizzle<DP>(tid / CH + i * STEP); };
   const T *qp[N], *gp[N];  // this thread's rows of the next tile to load, and its row's place in lse and delta
@@ -889,8 +903,10 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
           if (ROLE != VALUES) qc[x][d] = read_columns<DP>(qt, 32 * i + 16 * x, d, l);
         }
       phase();
-      const bool masked = MODE == FAR ? low - a.window < key0 + 31 || key0 + 31 >= sinks
-                                      : low < key0 + 31 || (MODE == WINDOWED && key0 <= most - a.window && key0 + 31 >= sinks);
+      // some row's last key lies before some of the wave's, or its window behind it
+      const bool ends = MODE != FAR && low < key0 + 31;
+      const bool begins = MODE == FAR ? low - a.window < key0 + 31 || key0 + 31 >= sinks
+                                      : MODE == WINDOWED && key0 <= most - a.window && key0 + 31 >= sinks;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int at = 32 * i + 8 * j + 4 * h;
@@ -902,13 +918,16 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
           s[4 * j + e] = exp2_fast(fmaf(s[4 * j + e], c, -ls[e]));
           if (ROLE != VALUES) dp[4 * j + e] = s[4 * j + e] * (dp[4 * j + e] - de[e]);
         }
-        if (masked) {
+        if (ends || begins) {
           const I4 li = *(const I4*)(places_of[turn] + at) + (token + off);
+          if (ends)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (MODE == FAR ? key > li[e] - a.window || key >= sinks
-                            : key > li[e] || (MODE == WINDOWED && key <= li[e] - a.window && key >= sinks))
-              s[4 * j + e] = dp[4 * j + e] = 0.0f;
+            for (int e = 0; e < 4; ++e)
+              if (key > li[e]) s[4 * j + e] = dp[4 * j + e] = 0.0f;
+          if (begins)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (MODE == FAR ? li[e] < behind : li[e] >= behind) s[4 * j + e] = dp[4 * j + e] = 0.0f;
         }
       }
       if (ROLE != VALUES) lift.template scale<DT>(dp, dk);
@@ -1067,8 +1086,9 @@ int key_waves(int dim, int seqs, int tk, int window) {
 // 265 and 272, 389 and 353; 1500, 297 and 308, 388 and 405, 654 and 574; heads of 128, 700, 358 and 394, 470 and 498, 929
 // and 1038; 1500, 544 and 618, 711 and 768, 1540 and 1617. 65536 tokens, mean 2048, heads of 64: forward 220 and 196, all of
 // the backward 800 and 605; of 128, 401 and 372, 1559 and 1470. A wave alone has no neighbours: the shorter listing.
-int by_sequence(int dim, int seqs, int tq, int tk) {
+int by_sequence(int dim, int seqs, int tq, int tk, int window) {
   const bool queries = (tq > tk ? tq : tk) <= (long long)LONG * seqs;
+  if (window) return queries ? 3 : 0;
   const bool keys = key_waves(dim, seqs, tk, 0) == 1 || (dim > 64 && queries);
   return (queries ? 1 : 0) | (keys ? 2 : 0);
 }
@@ -1229,7 +1249,7 @@ int dk_attention_window(hipStream_t st, int type, int heads, int kv_heads, int d
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
   a.key_waves = pol::key_waves(dim, seqs, tk, a.window);
-  a.by_sequence = pol::by_sequence(dim, seqs, tq, tk);
+  a.by_sequence = pol::by_sequence(dim, seqs, tq, tk, a.window), a.grouped = a.window ? 3 : a.by_sequence;
   a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group, a.window, a.sinks), a.scratch = (float*)scratch;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.out = out, a.lse = lse, a.order = (const int*)work;
   return a.window ? pol::launch_attend<true>(st, type, a) : pol::launch_attend<false>(st, type, a);
@@ -1253,7 +1273,7 @@ int dk_attention_window_vjp(hipStream_t st, int type, int heads, int kv_heads, i
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
   a.key_waves = pol::key_waves(dim, seqs, tk, a.window);
-  a.by_sequence = pol::by_sequence(dim, seqs, tq, tk);
+  a.by_sequence = pol::by_sequence(dim, seqs, tq, tk, a.window), a.grouped = a.window ? 3 : a.by_sequence;
   a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group, a.window, a.sinks), a.scratch = (float*)scratch;
   a.parts_k = pol::key_parts(kv_heads, dim, seqs, tq, tk, a.group, a.window);
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.order = (const int*)work;
