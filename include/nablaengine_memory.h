@@ -70,7 +70,7 @@ int dk_cache_append(hipStream_t st, int type, int worlds, int tokens, int kv_hea
 /* dk_attention and its VJP with a window: of the keys that the causal mask leaves a query, it sees the `window` last ones and the
  * `sinks` first ones of its sequence (window 0, or as long as tk: all). rest: (tq, heads, dim) in the outputs' type, contiguous:
  * what their rounding took off, which the backward adds where it is given one; worth its bytes for windows of few keys, whose
- * outputs' rounding is felt in the gradients. NULL: none. work: dk_attention_window_work_bytes bytes, whatever the window. */
+ * outputs' rounding is felt in the gradients. NULL: none. work: dk_attention_work_bytes bytes. */
 int dk_attention_window(hipStream_t st, int type, int heads, int kv_heads, int dim, int seqs, int tq, int tk, const void* q,
                         long long q_t, long long q_h, const void* k, long long k_t, long long k_h, const void* v, long long v_t,
                         long long v_h, const int* starts_q, const int* starts_k, float scale, int window, int sinks, void* out,
@@ -80,7 +80,6 @@ int dk_attention_window_vjp(hipStream_t st, int type, int heads, int kv_heads, i
                             long long v_h, const int* starts_q, const int* starts_k, float scale, int window, int sinks,
                             const void* out, const void* rest, const float* lse, const void* work, const void* dout,
                             long long do_t, long long do_h, float* delta, void* dq, void* dk, void* dv, void* scratch);
-long long dk_attention_window_work_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk);
 long long dk_attention_window_scratch_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk, int window, int sinks, int vjp);
 
 #ifdef __cplusplus

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(1024) void k_attend_order(int seqs, int tq, int tk,
   if (by_sequence < 3)
     while (ls < 1024 && ls * 2 * (long long)(seqs + 1) <= 1024) ls *= 2;
   const int lane = threadIdx.x % ls, first_seq = threadIdx.x / ls, stride = 1024 / ls;
-  const int bits[2] = {7, key_waves == 1 ? 5 : key_waves == 2 ? 6 : 7};  // of a tile's rows
+  const int bits[2] = {7, key_waves == 1 ? 5 : 7};  // of a tile's rows
   static_assert(QROWS == 128, "");
   const unsigned caps[2] = {(unsigned)order_queries(seqs, tq, group), (unsigned)order_keys(seqs, tk, key_waves)};
   int* const lists[2] = {order + ORDER_HEAD, order + ORDER_HEAD + 2LL * caps[0]};
@@ -648,9 +648,9 @@ __global__ __launch_bounds__(256) void k_attend_dq_join(Attend a) {
 // time. S = Q K^T here, so that a lane holds 16 rows of ONE key and P, dS are the B operands of dV^T = dO^T P and dK^T =
 // Q^T dS. KW of the waves differ in their keys, the others take every SPLIT-th subtile of 32 rows of the same keys, and
 // their sums are added at the end, in order.
-template <typename T, int DP, int WAVES, int KW = 4>
+template <typename T, int DP, int WAVES>
 struct DkvTiles {
-  static constexpr int RT = WAVES == 1 ? 32 : DP == 64 && KW != 2 ? 64 : 128;
+  static constexpr int RT = WAVES == 1 ? 32 : DP == 64 ? 64 : 128;
   alignas(16) T tiles[2][2][RT * DP];  // (turn, q or dout)
   alignas(16) float lses[2][RT], deltas[2][RT];
   alignas(16) int places_of[2][RT];  // a row's token from its tile's first
@@ -768,8 +768,8 @@ __device__ __forceinline__ void finish_dkv(const Attend& a, const Place& p, int 
   }
 }
 template <typename T, int DP, int KW, int WAVES, int ROLE, bool PARTS, int MODE>
-__device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, WAVES, KW>& lds) {
-  constexpr int RT = DkvTiles<T, DP, WAVES, KW>::RT;
+__device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTiles<T, DP, WAVES>& lds) {
+  constexpr int RT = DkvTiles<T, DP, WAVES>::RT;
   constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8, STEP = 64 * WAVES / CH, SPLIT = WAVES / KW;
   // of a subtile's two column operands, those read during the exponentials (heads of 128 in parts: none, no register is left)
   constexpr int AHEAD = DP == 64 ? 2 : !PARTS ? 1 : 0;
@@ -1000,7 +1000,7 @@ __device__ __forceinline__ void dkv_tile(const Attend& a, const Place& p, DkvTil
 
 template <typename T, int DP, int KW, int WAVES, bool PARTS, bool WIN>
 __global__ __launch_bounds__(WAVES == 8 ? 512 : 256) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_dkv(Attend a) {
-  __shared__ DkvTiles<T, DP, WAVES, KW> lds[WAVES == 1 ? 4 : 1];
+  __shared__ DkvTiles<T, DP, WAVES> lds[WAVES == 1 ? 4 : 1];
   const int parts = PARTS ? a.parts_k : 1;
   Place p;
   if constexpr (WAVES == 1) {  // each wave a tile of its own
@@ -1018,7 +1018,7 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256) __attribute__((amdgpu_waves
 // the far rows' parts; WAVES waves, as many as a row tile has subtiles
 template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_far(Attend a) {
-  __shared__ DkvTiles<T, DP, WAVES, 1> lds;
+  __shared__ DkvTiles<T, DP, WAVES> lds;
   constexpr int ROLES = DP == 64 ? 1 : 2;
   int b = blockIdx.x;
   const int role = b % ROLES;
@@ -1072,14 +1072,11 @@ __global__ __launch_bounds__(256) void k_attend_dkv_join(Attend a) {
 
 // ---- launches -------------------------------------------------------------------------------------------------------
 
-constexpr int NARROW_TILES = 1 << 30;
 // Keys a tile of the keys' gradients: 128; 32, a wave each, where sequences are short and heads up to 64, since most of a
 // workgroup's waves would have no keys there. Backward of 65536 tokens of 8 heads on 2, lengths 1 to twice the mean, alone
 // and together: mean 16 113 and 157 us, 32 105 and 125, 64 115 and 123, 96 120 and 146 (all of 96: 107 and 111; all of 128:
 // 121 and 114). Heads of 128 gain nothing from tiles of 64 keys (mean 32 445 us for 434, 64 413 for 363).
-int key_waves(int dim, int seqs, int tk, int window) {
-  return dim > 64 ? 4 : tk <= 96LL * seqs ? 1 : window && window <= NARROW_TILES ? 2 : 4;
-}
+int key_waves(int dim, int seqs, int tk) { return dim <= 64 && tk <= 96LL * seqs ? 1 : 4; }
 
 // The lists in the order of the sequences: bit 0 the query tiles, bit 1 the key tiles. 131072 tokens of 8 heads on 2, by
 // sequence and singly: heads of 64, mean length 100, forward 97 and 102 us, dq 136 and 141, dkv 183 and 135; 700, 194 and 206,
@@ -1089,7 +1086,7 @@ int key_waves(int dim, int seqs, int tk, int window) {
 int by_sequence(int dim, int seqs, int tq, int tk, int window) {
   const bool queries = (tq > tk ? tq : tk) <= (long long)LONG * seqs;
   if (window) return queries ? 3 : 0;
-  const bool keys = key_waves(dim, seqs, tk, 0) == 1 || (dim > 64 && queries);
+  const bool keys = key_waves(dim, seqs, tk) == 1 || (dim > 64 && queries);
   return (queries ? 1 : 0) | (keys ? 2 : 0);
 }
 
@@ -1112,13 +1109,13 @@ int query_parts(int kv_heads, int seqs, int tq, int tk, int group, int window, i
   return parts_of(order_queries(seqs, tq, group) * kv_heads, others_of(tk, seqs, window, sinks), TILE, seqs);
 }
 int key_parts(int kv_heads, int dim, int seqs, int tq, int tk, int group, int window) {
-  const int kw = key_waves(dim, seqs, tk, window);
+  const int kw = key_waves(dim, seqs, tk);
   return kw < 4 ? 1 : parts_of(order_keys(seqs, tk, kw) * kv_heads * (dim <= 64 ? 1 : 2), others_of(tq, seqs, window, 128) * group,
                                dim <= 64 ? 64 : 128, seqs);
 }
-size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group, int window) {
+size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group) {
   return sizeof(int) * (ORDER_HEAD + 2 * (size_t)(order_queries(seqs, tq, group) +
-                                                  order_keys(seqs, tk, key_waves(dim, seqs, tk, window))));
+                                                  order_keys(seqs, tk, key_waves(dim, seqs, tk))));
 }
 // Where the sinks' far rows are walked over apart: where there are sinks, at most four tiles of 32, and a sequence may be longer
 // than a window and half a part; not where their slots would take more than 1 GB.
@@ -1192,8 +1189,6 @@ int attend_vjp(hipStream_t st, const Attend& a) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
     k_attend_dkv_join<T, DP, WIN><<<dim3(blocks_of(a, tiles, 1), 8 * (DP / 32)), 256, 0, st>>>(a);
-  } else if (WIN && DP == 64 && a.key_waves == 2) {
-    if constexpr (WIN && DP == 64) k_attend_dkv<T, 64, 2, 4, false, true><<<blocks_of(a, tiles, 1), 256, 0, st>>>(a);
   } else if (a.key_waves == 4) {
     k_attend_dkv<T, DP, 4, DP / 16, false, WIN><<<blocks_of(a, tiles, ROLES), THREADS, 0, st>>>(a);
   } else if constexpr (DP == 64) {
@@ -1248,7 +1243,7 @@ int dk_attention_window(hipStream_t st, int type, int heads, int kv_heads, int d
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
-  a.key_waves = pol::key_waves(dim, seqs, tk, a.window);
+  a.key_waves = pol::key_waves(dim, seqs, tk);
   a.by_sequence = pol::by_sequence(dim, seqs, tq, tk, a.window), a.grouped = a.window ? 3 : a.by_sequence;
   a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group, a.window, a.sinks), a.scratch = (float*)scratch;
   a.starts_q = starts_q, a.starts_k = starts_k, a.scale = scale, a.out = out, a.lse = lse, a.order = (const int*)work;
@@ -1272,7 +1267,7 @@ int dk_attention_window_vjp(hipStream_t st, int type, int heads, int kv_heads, i
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;
-  a.key_waves = pol::key_waves(dim, seqs, tk, a.window);
+  a.key_waves = pol::key_waves(dim, seqs, tk);
   a.by_sequence = pol::by_sequence(dim, seqs, tq, tk, a.window), a.grouped = a.window ? 3 : a.by_sequence;
   a.parts_q = pol::query_parts(kv_heads, seqs, tq, tk, a.group, a.window, a.sinks), a.scratch = (float*)scratch;
   a.parts_k = pol::key_parts(kv_heads, dim, seqs, tq, tk, a.group, a.window);
@@ -1308,12 +1303,7 @@ int dk_attention_vjp(hipStream_t st, int type, int heads, int kv_heads, int dim,
 
 long long dk_attention_work_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk) {
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || seqs < 0 || tq < 0 || tk < 0) return 0;
-  return (long long)pol::attend_work_bytes(dim, seqs, tq, tk, heads / kv_heads, 0);
-}
-// for every window
-long long dk_attention_window_work_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk) {
-  if (heads < 1 || kv_heads < 1 || heads % kv_heads || seqs < 0 || tq < 0 || tk < 0) return 0;
-  return (long long)pol::attend_work_bytes(dim, seqs, tq, tk, heads / kv_heads, 1);
+  return (long long)pol::attend_work_bytes(dim, seqs, tq, tk, heads / kv_heads);
 }
 
 long long dk_attention_scratch_bytes(int heads, int kv_heads, int dim, int seqs, int tq, int tk, int vjp) {

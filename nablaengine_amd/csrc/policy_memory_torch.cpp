@@ -3,6 +3,7 @@
 #include "policy_torch.h"
 
 #include "../../include/nablaengine_memory.h"
+#include "../../include/nablaengine_policy.h"
 
 namespace {
 
@@ -10,7 +11,7 @@ namespace {
   X(dk_recurrence) X(dk_recurrence_vjp) X(dk_recurrence_carry_bytes) X(dk_recurrence_work_bytes) X(dk_recurrence_step) \
   X(dk_gated_residual) X(dk_gated_residual_vjp) X(dk_gated_residual_work_bytes)             \
   X(dk_attention_paged) X(dk_attention_paged_work_bytes) X(dk_cache_append)                             \
-  X(dk_attention_window) X(dk_attention_window_vjp) X(dk_attention_window_scratch_bytes) X(dk_attention_window_work_bytes)
+  X(dk_attention_window) X(dk_attention_window_vjp) X(dk_attention_window_scratch_bytes) X(dk_attention_work_bytes)
 struct Entries {
 #define X(name) decltype(&::name) name;
   ENTRIES(X)
@@ -275,7 +276,7 @@ Tensor window_scratch(const Heads& h, int seqs, const Tensor& q, const Tensor& k
   return bytes ? work_of(q, bytes) : Tensor();
 }
 long long order_words(const Heads& h, int seqs, const Tensor& q, const Tensor& k) {
-  return lib.dk_attention_window_work_bytes(h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0)) / 4;
+  return lib.dk_attention_work_bytes(h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0)) / 4;
 }
 
 // out, lse, work and rest (what the output's rounding took off, for narrow windows)

@@ -111,23 +111,22 @@ def _fake_norm(grads, *_):
     return grads[0].new_empty((), dtype=torch.float32)
 
 
-def _order_words(group, dim, seqs, tq, tk, window=False):
-    """dk_attention_work_bytes / 4 (dk_attention_window_work_bytes / 4), written out so that sizes may be symbolic (the
-    library's own takes numbers only): a head of 16, and two words each of the query tiles of 128 rows and of the key tiles of
-    128 keys, 32 or (with a window) 64."""
-    keys = 32 if dim <= 64 and tk <= 96 * seqs else 64 if window and dim <= 64 else 128
+def _order_words(group, dim, seqs, tq, tk):
+    """dk_attention_work_bytes / 4, written out so that sizes may be symbolic (the library's own takes numbers only): a
+    head of 16, and two words each of the query tiles of 128 rows and of the key tiles of 128 or 32 keys."""
+    keys = 32 if dim <= 64 and tk <= 96 * seqs else 128
     return 16 + 2 * (tq * group // 128 + tk // keys + 2 * (seqs + 1))
 
 
-def _fake_attention_forward(q, k, v, starts_q, starts_k, scale, train, window=False):
-    words = _order_words(q.shape[1] // k.shape[1], q.shape[2], starts_q.shape[0] - 1, q.shape[0], k.shape[0], window)
+def _fake_attention_forward(q, k, v, starts_q, starts_k, scale, train):
+    words = _order_words(q.shape[1] // k.shape[1], q.shape[2], starts_q.shape[0] - 1, q.shape[0], k.shape[0])
     return [q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0] if train else 0), dtype=torch.float32),
             starts_q.new_empty((words,))]
 
 
 def _fake_attention_window_forward(q, k, v, starts_q, starts_k, scale, window, sinks, train):
     rest = q.new_empty(q.shape if train and window + sinks <= 64 else (0,))
-    return _fake_attention_forward(q, k, v, starts_q, starts_k, scale, train, True) + [rest]
+    return _fake_attention_forward(q, k, v, starts_q, starts_k, scale, train) + [rest]
 
 
 def _fake_recurrence(x, gate, starts, initial):

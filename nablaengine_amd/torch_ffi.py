@@ -134,7 +134,6 @@ _MEMORY_PROTOTYPES = {
     "dk_attention_paged_work_bytes": "q:iiiiiiii",
     "dk_attention_window": "i:piiiiiii" + "pqq" * 3 + "ppfiippppp",
     "dk_attention_window_vjp": "i:piiiiiii" + "pqq" * 3 + "ppfiipppp" + "pqq" + "ppppp",
-    "dk_attention_window_work_bytes": "q:iiiiii",
     "dk_attention_window_scratch_bytes": "q:iiiiiiiii",
     "dk_cache_append": "i:p" + "i" * 8 + "pqq" * 2 + "p" + "pqqq" * 2 + "pqp",
 }
