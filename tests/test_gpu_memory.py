@@ -1116,3 +1116,147 @@ def test_window_refusals():
             policy.attention(q, k, v, starts([10]), **kw)
     with pytest.raises(TypeError):
         policy.attention(q.float(), k.float(), v.float(), starts([10]), window=3)
+
+
+# ---- streams, graphs, compilation, runs together --------------------------------------------------------------------
+
+def all_operators():
+    lq = [70, 3, 190]
+    x, f = gated(263, 40, F32, 1)
+    s0, dh, dl = rand((3, 40), F32, 3), rand((263, 40), F32, 4), rand((3, 40), F32, 5)
+    r = residual_inputs(300, 99, F32)
+    dy, dz = rand((300, 99), F32, 8), rand((300, 99), F32, 9)
+    q, k, v = heads_of(lq, lq, 4, 2, 64)
+    dout, a = rand(q.shape, BF16, 6), starts(lq)
+    table, count = paged_tables([0, 1, 600, 33, 599, 2], 16, 40)
+    n = torch.tensor([0, 1, 600, 33, 599, 2], dtype=torch.int32, device="cuda")
+    kp, vp, qs = rand((count, 16, 2, 64), BF16, 11), rand((count, 16, 2, 64), BF16, 12), rand((6, 4, 64), BF16, 13)
+    new = rand((6, 4, 64), BF16, 14)
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in (x, f, s0)]
+        out = policy.recurrence(leaves[0], leaves[1], a, leaves[2])
+        res = [*out, *torch.autograd.grad(out, leaves, (dh, dl)), *policy.recurrence_step(x, f, dh)]
+        leaves = [t.detach().requires_grad_() for t in r]
+        out = policy.gated_residual(*leaves[:4], gate=leaves[4], scale=leaves[5])
+        res += [*out, *torch.autograd.grad(out, leaves, (dy, dz))]
+        for window, sinks in ((20, 3), (100, 0)):
+            leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+            o = policy.attention(*leaves, a, window=window, sinks=sinks)
+            res += [o, *torch.autograd.grad(o, leaves, dout)]
+        policy.cache_append_(kp, vp, new[:, :2], new[:, 2:], table, n - 1)
+        res += [kp.clone(), vp.clone()] + [policy.attention_paged(qs, kp, vp, table, n, window=w, sinks=3) for w in (None, 50)]
+        return [t.detach() for t in res]
+    return run, (x, f, s0, dh, dl, *r, dy, dz, q, k, v, dout, kp, vp, qs, new)
+
+
+def test_operators_are_the_same_every_time():
+    run, _ = all_operators()
+    assert all(torch.equal(a, b) for a, b in zip(run(), run()))
+
+
+def test_operators_on_another_stream():
+    run, _ = all_operators()
+    want = run()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = run()
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_operators_on_two_streams_at_once():
+    run, _ = all_operators()
+    want = run()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    for one in got:  # (the appended tokens are the same ones)
+        assert all(torch.equal(a, b) for a, b in zip(want, one))
+
+
+def test_operators_in_graphs():
+    """Two captured graphs of the same calls, replayed in turn over new inputs with eager work between."""
+    run, inputs = all_operators()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run()
+    torch.cuda.current_stream().wait_stream(s)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held = run()
+        graphs.append((g, held))
+    for turn in range(4):
+        for i, t in enumerate(inputs):
+            t.copy_(rand(t.shape, t.dtype, 100 * turn + i))
+        want = [t.clone() for t in run()]
+        torch.cuda.synchronize()
+        for g, held in graphs:
+            g.replay()
+            torch.cuda.synchronize()
+            for i, (a, b) in enumerate(zip(want, held)):
+                assert torch.equal(a, b), (turn, i)
+
+
+def test_operators_compiled_over_sizes():
+    """torch.compile keeps each operator as one node of a full graph, forward and backward, over several batches: eager's
+    results for each."""
+    w = rand((64,), F32, 2)
+
+    def loss(x, f, heads, a, s0):
+        h, last = policy.recurrence(torch.sin(x), f, a, s0)
+        y, z = policy.gated_residual(x, h, w, None, gate=f, scale=w)
+        o = policy.attention(heads[:, :2], heads[:, 2:4], heads[:, 4:], a, window=20, sinks=2)
+        return (y * z).sum() + last.sum() + (o.float() * 3).sum()
+
+    def run(fn, lq):
+        n = sum(lq)
+        leaves = [t.detach().requires_grad_() for t in (*gated(n, 64, F32, 1), rand((n, 6, 64), BF16, 4))]
+        s0 = rand((len(lq), 64), F32, 5).requires_grad_()
+        value = fn(*leaves, starts(lq), s0)
+        return [value.detach(), *torch.autograd.grad(value, [*leaves, s0])]
+    torch._dynamo.reset()
+    compiled = torch.compile(loss, fullgraph=True, backend="aot_eager")
+    for lq in ([20, 0, 44, 11], [7, 300], [1], [500, 900, 2, 2, 2], [33] * 40):
+        for i, (e, c) in enumerate(zip(run(loss, lq), run(compiled, lq))):
+            assert torch.equal(e, c), (lq[:4], i)
+
+
+def test_appending_compiled():
+    """The pages are written under torch.compile as they are without, and read after."""
+    def step(kp, vp, k, q, table, n):
+        policy.cache_append_(kp, vp, k, k * 2, table, n)
+        return policy.attention_paged(q, kp, vp, table, n + 1, window=9) * 2
+    table, count = paged_tables([20, 5, 40], 8, 6)
+    n = torch.tensor([19, 4, 39], dtype=torch.int32, device="cuda")
+    k, q = rand((3, 2, 64), BF16, 1), rand((3, 4, 64), BF16, 2)
+    pools = [[rand((count, 8, 2, 64), BF16, i) for i in (3, 4)] for _ in range(2)]
+    compiled = torch.compile(step, fullgraph=True, backend="aot_eager")
+    assert torch.equal(step(*pools[0], k, q, table, n), compiled(*pools[1], k, q, table, n))
+    assert all(torch.equal(a, b) for a, b in zip(*pools))
+
+
+def test_gradients_in_a_graph_of_gradients():
+    """Under create_graph the gradients are those without it, and differentiating them again raises."""
+    lq = [20, 70]
+    a, r = starts(lq), residual_inputs(40, 99, F32)
+    q, k, v = heads_of(lq, lq, 4, 2, 64)
+    x, f = gated(90, 30, F32, 1)
+    for call, at in ((lambda x, f: policy.recurrence(x, f, a)[0], (x, f)),
+                     (lambda x, u, w, w2, g, s: policy.gated_residual(x, u, w, w2, gate=g, scale=s)[1], r),
+                     (lambda *t: policy.attention(*t, a, window=9, sinks=2), (q, k, v))):
+        leaves = [t.detach().requires_grad_() for t in at]
+        cot = rand(at[0].shape, at[0].dtype, 9)
+        want = torch.autograd.grad(call(*leaves), leaves, cot)
+        got = torch.autograd.grad(call(*leaves), leaves, cot, create_graph=True)
+        assert all(torch.equal(p, r) and r.requires_grad and not p.requires_grad for p, r in zip(want, got))
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            sum(g.float().square().sum() for g in got).backward()
