@@ -15,6 +15,12 @@
 // with what they compute again). At heads of 128 the products lead: 2 sequences of 8192 and 2752 tokens, 16 heads on 4,
 // forward 340 us (900 TFLOP/s; a large library product of 16 bits reaches 1200), dq 440, dkv 955. Short sequences are bound
 // by their bytes: 4096 segments of up to 32 tokens, 8 heads on 2, forward 56 us (4.0 TB/s), dq 81 (3.8), dkv 60 (4.4).
+//
+// With a window a tile's loop is short, and what a workgroup waits for before it counts: its place in the lists, its rows, its
+// first tile. The same 256 episodes with a window of 128 and 4 sinks: forward 156 us (of which 120 are left at a window of 16: 0.41
+// GB, 3.4 TB/s), dq 231, dkv 306 and 84 for the sinks' far rows; matrix instructions take 14 to 16 % of the SIMDs' cycles, vector
+// instructions 69 % in the forward and 34 % in dkv, which waits for its tiles with eight waves a compute unit. The two
+// recordings with a window of 1000 and 16 sinks, heads of 128: 145, 174, 401 and 56.
 #include "../../include/nablaengine_memory.h"
 #include "../../include/nablaengine_policy.h"
 #include "policy_attend.h"
@@ -665,7 +671,8 @@ constexpr size_t far_slot(int dp) { return 2 * 32 * (size_t)dp; }  // floats of 
 // operands here; the eight waves fill a CU's LDS, so that no other workgroup covers it.
 enum Role { BOTH, KEYS, VALUES };
 // A window's sinks are seen by all rows of their sequence, other keys by those of one window: their tiles would take many times as
-// long, most of their waves idle, and end last (two sequences of 8192 and 2752 tokens, window 1000, 16 sinks: 1121 us). The rows
+// long, most of their waves idle, and end last (two sequences of 8192 and 2752 tokens, window 1000, 16 sinks: 1121 us, now 401 and
+// 56). The rows
 // behind the window of a sequence's first key are taken from those tiles and walked over by workgroups of their own, a part of
 // far_tokens tokens each for 32 sinks, all of whose waves share the rows; their sums in float32 go to slots that the key tile's
 // workgroup adds before it rounds. A part's slot follows from where its sequence lies: a sequence of n queries from q0 and m keys
@@ -1085,7 +1092,7 @@ int key_waves(int dim, int seqs, int tk) { return dim <= 64 && tk <= 96LL * seqs
 // the backward 800 and 605; of 128, 401 and 372, 1559 and 1470. A wave alone has no neighbours: the shorter listing.
 int by_sequence(int dim, int seqs, int tq, int tk, int window) {
   const bool queries = (tq > tk ? tq : tk) <= (long long)LONG * seqs;
-  if (window) return queries ? 3 : 0;
+  if (window) return queries ? 3 : 0;  // its tiles cost alike
   const bool keys = key_waves(dim, seqs, tk) == 1 || (dim > 64 && queries);
   return (queries ? 1 : 0) | (keys ? 2 : 0);
 }
@@ -1118,7 +1125,8 @@ size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group) {
                                                   order_keys(seqs, tk, key_waves(dim, seqs, tk))));
 }
 // Where the sinks' far rows are walked over apart: where there are sinks, at most four tiles of 32, and a sequence may be longer
-// than a window and half a part; not where their slots would take more than 1 GB.
+// than a window and half a part; not where their slots would take more than 1 GB. Parts of 512 tokens: 50 us for 34, of two
+// sequences of 8192 tokens.
 constexpr int FAR_TOKENS = 256;
 struct FarPlan { int tokens, least, chunks; long long slots; };
 FarPlan far_plan(int kv_heads, int dim, int tq, int tk, int window, int sinks) {
@@ -1128,18 +1136,18 @@ FarPlan far_plan(int kv_heads, int dim, int tq, int tk, int window, int sinks) {
   if (r.slots * r.chunks * kv_heads * far_slot(dim <= 64 ? 64 : 128) <= 1LL << 28) r.tokens = FAR_TOKENS;
   return r;
 }
-size_t attend_parts_floats(int kv_heads, int dim, int seqs, int tq, int tk, int group, int window, int sinks, bool vjp);
-size_t attend_scratch_bytes(int kv_heads, int dim, int seqs, int tq, int tk, int group, int window, int sinks, bool vjp) {
-  const FarPlan far = far_plan(kv_heads, dim, tq, tk, window, sinks);
-  const size_t parts = attend_parts_floats(kv_heads, dim, seqs, tq, tk, group, window, sinks, vjp);
-  return sizeof(float) * (parts + (vjp && far.tokens ? (size_t)far.slots * far.chunks * kv_heads * far_slot(dim <= 64 ? 64 : 128) : 0));
-}
 size_t attend_parts_floats(int kv_heads, int dim, int seqs, int tq, int tk, int group, int window, int sinks, bool vjp) {
   const size_t pq = query_parts(kv_heads, seqs, tq, tk, group, window, sinks);
   const size_t pk = vjp ? key_parts(kv_heads, dim, seqs, tq, tk, group, window) : 1;
   const size_t q = pq == 1 ? 0 : pq * order_queries(seqs, tq, group) * kv_heads * (dim <= 64 ? RowsPart<64>::SIZE : RowsPart<128>::SIZE);
   const size_t k = pk == 1 ? 0 : pk * order_keys(seqs, tk, 4) * kv_heads * (dim <= 64 ? 1 : 2) * Part<KEY_PART>::SIZE;
   return q > k ? q : k;
+}
+size_t attend_scratch_bytes(int kv_heads, int dim, int seqs, int tq, int tk, int group, int window, int sinks, bool vjp) {
+  const FarPlan far = far_plan(kv_heads, dim, tq, tk, window, sinks);
+  const size_t parts = attend_parts_floats(kv_heads, dim, seqs, tq, tk, group, window, sinks, vjp);
+  const size_t slots = vjp && far.tokens ? (size_t)far.slots * far.chunks * kv_heads : 0;
+  return sizeof(float) * (parts + slots * far_slot(dim <= 64 ? 64 : 128));
 }
 
 template <typename T, int DP, bool WIN>
@@ -1199,8 +1207,8 @@ int attend_vjp(hipStream_t st, const Attend& a) {
 
 template <bool WIN>
 int launch_attend(hipStream_t st, int type, const Attend& a) {
-  k_attend_order<<<1, 1024, 0, st>>>(a.seqs, a.tq, a.tk, a.group, a.key_waves, a.by_sequence, WIN ? a.window : 0, WIN && !a.far_tokens ? a.sinks : 0,
-                                  a.starts_q, a.starts_k, (int*)a.order);
+  k_attend_order<<<1, 1024, 0, st>>>(a.seqs, a.tq, a.tk, a.group, a.key_waves, a.by_sequence, WIN ? a.window : 0,
+                                  WIN && !a.far_tokens ? a.sinks : 0, a.starts_q, a.starts_k, (int*)a.order);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.tq) return (int)e;
   if (type == BF16) return a.dim <= 64 ? attend<__bf16, 64, WIN>(st, a) : attend<__bf16, 128, WIN>(st, a);
@@ -1263,7 +1271,8 @@ int dk_attention_window_vjp(hipStream_t st, int type, int heads, int kv_heads, i
   a.window = window_of(window, tk), a.sinks = sinks_of(sinks, tk), a.rest = const_cast<void*>(rest);
   const pol::FarPlan far = pol::far_plan(kv_heads, dim, tq, tk, a.window, a.sinks);
   a.far_tokens = far.tokens, a.far_least = far.least, a.far_chunks = far.chunks;
-  if (scratch) a.far = (float*)scratch + pol::attend_parts_floats(kv_heads, dim, seqs, tq, tk, heads / kv_heads, a.window, a.sinks, true);
+  if (scratch)  // the slots behind the parts
+    a.far = (float*)scratch + pol::attend_parts_floats(kv_heads, dim, seqs, tq, tk, heads / kv_heads, a.window, a.sinks, true);
   a.q = q, a.k = k, a.v = v;
   a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
   a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim, a.seqs = seqs, a.tq = tq, a.tk = tk;

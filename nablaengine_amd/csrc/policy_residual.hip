@@ -6,8 +6,9 @@
 //   e = dy + r' (dz w' - yh mean(dz w' yh)),  dx = e,  dgate = e s n sg (1 - sg),  c = e s sg w,  du = r (c - uh mean(c uh))
 //   m = sum over rows of e sg uh:  dw = s m,  ds = w m;  dw' = sum over rows of dz yh
 //
-// Memory bounds both: the forward reads three rows and writes two, the backward reads five and writes three; in operations of
-// their own the same formulas move 12 and 24 rows and more. A row is read once into the registers of a group of L lanes and all
+// Memory bounds the forward: it reads three rows and writes two, and of 131072 rows of 512 bfloat16 takes 125 us, 5.4 TB/s, more
+// than a large copy's 5.0 to 5.2. The backward reads five and writes three, 251 us, 4.3 TB/s: beside that its vector instructions
+// take 56 % of the SIMDs' cycles (two gates' exponentials and reciprocals and some 60 others an element). A row is read once into the registers of a group of L lanes and all
 // is computed there in float32; z comes of the y that is not rounded yet, and the backward computes y again from x, u and gate,
 // which it needs anyway, instead of reading a rounded one. The backward's groups keep their columns' m and dw' in registers; at
 // the end a workgroup adds its groups' sums in LDS and writes one partial row, and a second kernel adds those in a fixed order.

@@ -14,6 +14,13 @@
 // where the next chunk starts a sequence), and a third kernel carries states over the chunks: two reads of x and gate
 // where sequences are long, one where they are short. The backward does the same from the other end; it takes the forward's
 // carried states, so the states between are computed from x and gate again and none is stored.
+//
+// Memory bounds it, and where sequences are short one read after another: where they start, then their tokens. Measured, bfloat16,
+// of the 5.0 to 5.2 TB/s of a large copy: two sequences of 65536 tokens together, 1024 channels, forward 71 us (5.7 TB/s of x, gate
+// and h, some still in the cache), the chunks' P and B 64 (4.2 TB/s), backward 157 (4.3 TB/s) and 65; 4096 sequences of up to 32
+// tokens, 512 channels, 64 and 25, 119 and 24; the states over the chunks 11 each time. Chunks of 128 tokens, two workgroups of
+// eight waves a compute unit: forward 73 and 82 us, backward 134 and 186. Stretches of 16 tokens in the backward: 127 and 168 us.
+// One token a world: 16384 worlds of 1024 channels 35 us, 6.7 TB/s.
 #include "../../include/nablaengine_memory.h"
 #include "policy_device.h"
 #include "policy_sizes.h"
@@ -539,8 +546,8 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_vjp(Scan a) {
     return s;
   };
   // Both ways' P and B in one walk: the other way's B is the sum of the cotangents, each times the product of the gates up to its
-  // token, up to the first sequence's end. Gates are computed anew in each of the three walks: kept, they would take the registers
-  // of the second workgroup on a compute unit.
+  // token, up to the first sequence's end. Gates are computed anew in each of the three walks: kept, they take the registers of
+  // other waves (94 a lane for 70; 4096 short sequences 127 us for 119, long ones the same).
   float p[V], b[V], q[V], c[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) p[e] = q[e] = 1.0f, b[e] = c[e] = 0.0f;

@@ -3,23 +3,32 @@
   layer_norm(x, weight=None, bias=None, *, eps=1e-5) -> y
   grad_norm(grads) -> norm
   clip_grads_(grads, max_norm, *, out=None) -> norm;  clip_grad_norm_(parameters, max_norm) -> norm
-  attention(q, k, v, starts_q, starts_k=None, *, scale=None) -> out
+  attention(q, k, v, starts_q, starts_k=None, *, scale=None, window=None, sinks=0) -> out
   attention_step(q, k, v, lengths, *, scale=None) -> out
+  cache_append_(k_pages, v_pages, k, v, pages, lengths, starts=None)
+  attention_paged(q, k_pages, v_pages, pages, lengths, *, scale=None, window=None, sinks=0) -> out
+  recurrence(x, gate, starts, initial=None) -> (h, last);  recurrence_step(x, gate, state) -> (h, state)
+  gated_residual(x, u, weight=None, next_weight=None, *, gate=None, scale=None, eps=1e-5) -> (y, z)
 
 A policy's hidden layers are normed over thousands of worlds (layer_norm, with its gradients); one that remembers
 attends over its own past: over whole episodes of different lengths, packed one after another, in training (attention,
-with its gradients), and over each world's cached history in the control loop (attention_step). Backpropagation
-through time gives large gradients now and then, which are clipped by their global norm before the optimizer's step
-(clip_grad_norm_).
+with its gradients), and over each world's cached history in the control loop (attention_step). One that remembers
+longer carries a state (recurrence, with its gradients; recurrence_step in the control loop) beside attention that sees
+a window of the last steps and a few first ones: over episodes in training, over pages of a shared pool in the control
+loop (attention_paged, which cache_append_ fills), so that a world needs no more than its window's pages however long it
+runs. Between its blocks lies gated_residual: a block's output normed, gated and scaled onto the residual stream, and
+that normed for the next block. Backpropagation through time gives large gradients now and then, which are clipped by
+their global norm before the optimizer's step (clip_grad_norm_).
 
 Conventions are torch_ffi's: tensors lie on one ROCm device and are never cast, copied or moved: another type, shape or
 device is a TypeError, a bad option a ValueError, a failed library call a RuntimeError; there is no CPU path. Calls only
 launch kernels on the device's current stream and take memory from torch's caching allocator: nothing synchronizes, so
-they may be captured in a HIP graph, and each is an operator of the ``nablaengine`` namespace with a fake
-implementation, which torch.compile keeps as one node (torch_ffi.init() first, as for the step: a trace cannot load the
-library). A tensor made on another stream than the call's is the caller's to synchronize and to keep alive
-(Tensor.record_stream), as with torch's own operators. Results are bitwise the same on every run. Gradients are first order
-by reverse mode: forward mode, the backward of a gradient and torch.func's derivatives raise RuntimeError.
+they may be captured in a HIP graph (a backward pass as torch captures any: with no eager graph of the same leaves left
+alive), and each is an operator of the ``nablaengine`` namespace with a fake implementation, which torch.compile keeps
+as one node (torch_ffi.init() first, as for the step: a trace cannot load the library). A tensor made on another stream
+than the call's is the caller's to synchronize and to keep alive (Tensor.record_stream), as with torch's own operators.
+Results are bitwise the same on every run. Gradients are first order by reverse mode: forward mode, the backward of a
+gradient and torch.func's derivatives raise RuntimeError.
 """
 import ctypes
 import math
@@ -312,8 +321,8 @@ def recurrence(x, gate, starts, initial=None):
 
     x, gate: (tokens, channels), float32, bfloat16 or float16, each token's elements neighbours, tokens any distance apart
     (slices of one projection's output; a gate of one row for all, expanded). starts: int32 offsets on the device, 0 first, not
-    falling, sequence s being tokens starts[s] .. starts[s + 1] - 1. initial: (sequences, channels) float32, the states before
-    the first tokens, or None for zeros. h has x's type and is zero behind the last sequence (padding, whose gradients are zero
+    falling, sequence s being tokens starts[s] .. starts[s + 1] - 1. initial: (sequences, channels) float32, contiguous, the
+    states before the first tokens, or None for zeros. h has x's type and is zero behind the last sequence (padding, whose gradients are zero
     too); the last states are float32, those of sequences without tokens their initial ones.
 
     The gate is given before its sigmoid, since 16 bits do not tell long memories apart after it: 1 - a keeps its own last

@@ -326,6 +326,24 @@ def test_recurrence_past_32_bits():
     assert all(torch.equal(a, b) for a, b in zip(run(x, f), run(big[:, 1:131], big[:, 140:270])))
 
 
+def test_recurrence_of_more_than_32_bits():
+    """Outputs of more than 2^31 elements: one token for all, sequences as long as a chunk, so that each repeats the first bit
+    for bit."""
+    n, c, seqs = 64, 1030, 33000
+    x, f = gated(1, c, BF16, 1)
+    leaves = [t.expand(n * seqs, c).detach().requires_grad_() for t in (x, f)]
+    h, last = policy.recurrence(*leaves, starts([n] * seqs))
+    dh = rand((1, c), BF16, 3).expand(n * seqs, c)
+    dx, df = torch.autograd.grad(h, leaves, dh)
+    want = recur64(x.expand(n, c), f.expand(n, c), [n], None, dh[:n], torch.zeros((1, c)))
+    for name, t in (("h", h.detach()), ("dx", dx), ("dgate", df)):
+        within(name, t[:n], *want[name])
+        t = t.view(seqs, n, c)
+        for i in range(0, seqs, 3000):
+            assert (t[i:i + 3000] == t[:1]).all(), (name, i)
+    assert (last == last[:1]).all()
+
+
 def test_recurrence_refusals():
     x, f, a, s = rand((10, 6), BF16, 1), rand((10, 6), BF16, 2), starts([4, 6]), rand((2, 6), F32, 3)
     for args in ((x.double(), f.double(), a), (x, f.float(), a), (x, f[:9], a), (x.t(), f.t(), a), (x, f, a.long()), (x, f, a[None]),
@@ -1042,6 +1060,19 @@ def test_window_what_it_hides(dtype, dim, heads, n, bad):
     got = run_window(q, k, v3, lq, lk, window, sinks, dout)
     same(got, "out", [0]), same(got, "out", slice(n, None)), same(got, "out", slice(1, n), slice(0, 5))
     assert not torch.isfinite(got["out"][1:n, :, 5]).any()
+
+
+def test_window_scores_that_are_all_minus_infinity():
+    """Rows whose every key in sight has a score of -inf give NaN, rows that see another one its value."""
+    q = torch.ones((300, 1, 64), dtype=BF16, device="cuda")
+    k, v = torch.full((300, 1, 64), -math.inf, dtype=BF16, device="cuda"), rand((300, 1, 64), BF16, 2)
+    k[100] = 1
+    out = policy.attention(q, k, v, starts([300]), window=20, sinks=2)
+    assert torch.isnan(out[:100]).all() and torch.isnan(out[120:]).all()
+    assert torch.equal(out[100:120], v[100:101].expand(20, 1, 64))
+    k[1] = 1  # a sink
+    out = policy.attention(q, k, v, starts([300]), window=20, sinks=2)
+    assert torch.isnan(out[0]).all() and torch.equal(out[120:], v[1:2].expand(180, 1, 64))
 
 
 def test_window_offsets_that_are_wrong_stay_in_bounds():
