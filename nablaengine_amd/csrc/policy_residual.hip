@@ -231,7 +231,7 @@ __global__ __launch_bounds__(vjp_block(L), 4) void k_residual_vjp(Residual a) {
     asm volatile("" : "+v"(place));
     auto param = [&](int which, int e) { return params[which][(e / 4 * L + place) * 4 + e % 4]; };
     // What is read stays as it is, half the registers of its floats in 16 bits; of the products only those that the sums between
-    // them need are kept: 126 registers a lane instead of 163, two workgroups a compute unit instead of one.
+    // them need are kept: 114 to 119 registers a lane instead of 163, two workgroups a compute unit instead of one.
     const Vec<T> xr = row_vector((const T*)a.x + row * a.x_r, lane, m);
     Vec<T> ur = row_vector((const T*)a.u + row * a.u_r, lane, m);
     const Vec<T> gr = row_vector(a.gate ? (const T*)a.gate + row * a.g_r : nullptr, lane, m);

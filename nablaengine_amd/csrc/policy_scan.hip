@@ -19,7 +19,7 @@
 // of the 5.0 to 5.2 TB/s of a large copy: two sequences of 65536 tokens together, 1024 channels, forward 71 us (5.7 TB/s of x, gate
 // and h, some still in the cache), the chunks' P and B 64 (4.2 TB/s), backward 157 (4.3 TB/s) and 65; 4096 sequences of up to 32
 // tokens, 512 channels, 64 and 25, 119 and 24; the states over the chunks 11 each time. Chunks of 128 tokens, two workgroups of
-// eight waves a compute unit: forward 73 and 82 us, backward 134 and 186. Stretches of 16 tokens in the backward: 127 and 168 us.
+// eight waves a compute unit: forward 73 and 81 us, backward 134 and 186. Stretches of 16 tokens in the backward: 127 and 168 us.
 // One token a world: 16384 worlds of 1024 channels 35 us, 6.7 TB/s.
 #include "../../include/nablaengine_memory.h"
 #include "policy_device.h"
@@ -347,8 +347,8 @@ __global__ __launch_bounds__(64 * W) void k_scan_back_parts(Scan a) {
 // ---- the states that enter the chunks -------------------------------------------------------------------------------
 
 // 8 channels a workgroup and 128 runs of chunks: each run's own P and B, those joined over the runs by doubling, then each
-// run once more from the state that enters it. BACK: the chunks from the last to the first. Bound by one read after another: 1400
-// chunks of 512 channels 9 us, 11 with 16 channels and 64 runs.
+// run once more from the state that enters it. BACK: the chunks from the last to the first. Bound by one read after another: 1340
+// chunks of 512 channels 11 us, the same with 16 channels and 64 runs.
 template <bool BACK>
 __global__ __launch_bounds__(1024) void k_scan_carry(Scan a) {
   constexpr int CH = 8, RUNS = 1024 / CH;
