@@ -289,7 +289,7 @@ std::vector<Tensor> attention_window_forward(const Tensor& q, const Tensor& k, c
   const Tensor out = at::empty(q.sizes(), q.options());
   const Tensor lse = at::empty({h.heads, train ? q.size(0) : 0}, q.options().dtype(at::kFloat));
   const Tensor work = at::empty({order_words(h, seqs, q, k)}, q.options().dtype(at::kInt));
-  const Tensor rest = at::empty(train && window + sinks <= pol::NARROW ? q.sizes() : at::IntArrayRef{0}, q.options());
+  const Tensor rest = at::empty(train && (int64_t)s.window + s.sinks <= pol::NARROW ? q.sizes() : at::IntArrayRef{0}, q.options());
   const Tensor scratch = window_scratch(h, seqs, q, k, s, 0);
   call("the windowed attention launch", q, [&](hipStream_t st) {
     return lib.dk_attention_window(st, h.type, h.heads, h.kv, h.dim, seqs, (int)q.size(0), (int)k.size(0), q.data_ptr(), q.stride(0),

@@ -271,7 +271,8 @@ def _sight(window, sinks):
     w, s = 0 if window is None else operator.index(window), operator.index(sinks)
     if w < (0 if window is None else 1) or s < 0:
         raise _err(f"window must be None or at least 1 and sinks at least 0, got {window} and {sinks}", ValueError)
-    return w, s
+    most = 1 << 30  # more tokens than any sequence has
+    return min(w, most), min(s, most)
 
 
 def attention(q, k, v, starts_q, starts_k=None, *, scale=None, window=None, sinks=0):

@@ -985,6 +985,15 @@ def test_window_as_long_as_the_keys_hides_nothing():
         assert all(torch.equal(a, b) for a, b in zip(want, got.values()))
 
 
+def test_windows_and_sinks_past_64_bits():
+    lq = [300, 7, 512]
+    q, k, v = heads_of(lq, lq, 4, 2, 64)
+    dout = rand(q.shape, BF16, 9)
+    for big, plain in (((2 ** 63 - 1, 4), (None, 0)), ((2 ** 70, 2 ** 70), (None, 0)), ((100, 2 ** 70), (100, sum(lq)))):
+        want, got = (run_window(q, k, v, lq, lq, *s, dout) for s in (plain, big))
+        assert all(torch.equal(want[name], got[name]) for name in want)
+
+
 def test_window_rounds_as_finely_as_few_keys_need():
     """A window of one key: the output is the value and the scores have no part, so their gradients are exactly 0."""
     lq = [300, 40]

@@ -151,6 +151,19 @@ def test_fake_shapes():
         assert ops.cache_append_(pages, pages, k, k, table, n, None) is None
 
 
+def test_windows_of_any_length_are_taken():
+    """A window or sinks past what an operator's integers hold are more than any sequence has."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = policy._ops(True)
+    with FakeTensorMode():
+        (_, _, a, _), (q, k), (pages, table, n) = _cpu()
+        for window, sinks in ((2 ** 63 - 1, 4), (2 ** 70, 0), (5, 2 ** 70), (2 ** 70, 2 ** 70)):
+            w, s = policy._sight(window, sinks)
+            out, _, _, rest = ops.attention_window_forward(q, k, k, a, a, 0.125, w, s, True)
+            assert out.shape == q.shape and rest.shape == (0,)
+            assert ops.attention_paged(q, pages, pages, table, n, 0.125, w, s).shape == q.shape
+
+
 def test_fake_carry_is_the_librarys():
     dll = torch_ffi.load_library()
     for tokens in (0, 1, 63, 64, 65, 1000, 2 ** 30):
