@@ -2,6 +2,8 @@
 // handed over apart (dk_memory_torch_bind): a kernels' library built before them still has the others.
 #include "policy_torch.h"
 
+#include <ATen/MemoryOverlap.h>
+
 #include "../../include/nablaengine_memory.h"
 #include "../../include/nablaengine_policy.h"
 
@@ -253,6 +255,15 @@ void cache_append_(const Tensor& k_pages, const Tensor& v_pages, const Tensor& k
   }
   CHECK_VALUE(tokens < 1 << 30 && worlds < 1 << 24 && worlds * h.kv * (h.dim / 8) < 1LL << 30, tokens, " tokens of ", worlds,
               " worlds exceed one launch");
+  // what is read beside what is written, where it can be told (pages of keys and values side by side in one buffer are apart)
+  const auto apart = [](const char* a, const Tensor& x, const char* b, const Tensor& y) {
+    const auto o = at::get_overlap_status(x, y);
+    CHECK_VALUE(x.numel() == 0 || y.numel() == 0 || (o != at::MemOverlapStatus::Full && o != at::MemOverlapStatus::Partial), a, " and ",
+                b, " lie over one another in memory");
+  };
+  apart("k_pages", k_pages, "v_pages", v_pages);
+  apart("k", k, "k_pages", k_pages), apart("k", k, "v_pages", v_pages);
+  apart("v", v, "k_pages", k_pages), apart("v", v, "v_pages", v_pages);
   call("the cache append launch", k, [&](hipStream_t st) {
     return lib.dk_cache_append(st, h.type, (int)worlds, (int)tokens, h.kv, h.dim, p.count, p.page, p.most, k.data_ptr(), k.stride(0),
                                k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), (const int*)in(starts), k_pages.data_ptr(),

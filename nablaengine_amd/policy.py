@@ -366,8 +366,9 @@ def cache_append_(k_pages, v_pages, k, v, pages, lengths, starts=None):
     its token lengths[w] + i, lengths being those without the new ones; adding them to lengths is the caller's.
 
     k_pages, v_pages: (pool, page, kv_heads, dim), bfloat16 or float16, page a power of two; pages: (worlds, most) int32 on the
-    device, the numbers of each world's pages in order. A page that is written belongs to one world alone. A token that has no
-    place, past the `most` pages or on a page whose number is none of the pool's (-1, say), is dropped. No gradients."""
+    device, the numbers of each world's pages in order. A page that is written belongs to one world alone, and the pages, k and
+    v lie apart in memory. A token that has no place, past the `most` pages or on a page whose number is none of the pool's
+    (-1, say), is dropped. No gradients."""
     for name, x in (("k_pages", k_pages), ("v_pages", v_pages), ("k", k), ("v", v), ("pages", pages), ("lengths", lengths)):
         _tensor(name, x)
     if _wants_grad(k_pages, v_pages, k, v):

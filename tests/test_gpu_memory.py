@@ -856,6 +856,21 @@ def test_paged_refusals():
         policy.cache_append_(kp, vp, k.clone().requires_grad_(), v, t, n)
 
 
+def test_append_refuses_what_lies_over_the_pages():
+    kp, vp = rand((9, 16, 2, 64), BF16, 2), rand((9, 16, 2, 64), BF16, 3)
+    t, n = torch.zeros((3, 5), dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    k, v = rand((3, 2, 64), BF16, 4), rand((3, 2, 64), BF16, 5)
+    was = kp.clone(), vp.clone()
+    for args in ((kp, kp, k, v), (kp, vp, kp[0, :3], v), (kp, vp, vp[0, :3], v), (kp, vp, k, kp[0, 5:8]), (kp, vp, k, vp[8, 13:])):
+        with pytest.raises(ValueError):
+            policy.cache_append_(*args, t, n)
+    assert torch.equal(kp, was[0]) and torch.equal(vp, was[1])
+    t = torch.arange(15, dtype=torch.int32, device="cuda").view(3, 5) % 9  # each world's first page is its own
+    for both in (rand((9, 2, 16, 2, 64), BF16, 6).unbind(1), rand((2, 9, 16, 2, 64), BF16, 7).unbind(0)):
+        policy.cache_append_(*both, k, v, t, n)
+        assert torch.equal(both[0][t[:, 0].long(), 0], k) and torch.equal(both[1][t[:, 0].long(), 0], v)
+
+
 def test_appending_marks_what_it_writes():
     """A graph that saved a pool which appending then overwrites notices."""
     w = rand((4, 16, 1, 8), BF16, 1).requires_grad_()
