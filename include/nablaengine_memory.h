@@ -26,7 +26,8 @@ int dk_recurrence_vjp(hipStream_t st, int type, int tokens, int channels, int se
 long long dk_recurrence_carry_bytes(int tokens, int channels);
 long long dk_recurrence_work_bytes(int tokens, int channels, int vjp);
 /* One token of every world: next = a state + (1 - a) x, float32, and h, its value in `type`; x, gate, state: (worlds, channels),
- * x_w, gate_w, state_w elements from world to world; h, next contiguous. next may be state where that is contiguous. */
+ * x_w, gate_w, state_w elements from world to world; h, next contiguous. next may be state where
+ * that is contiguous, and lies apart from it otherwise. */
 int dk_recurrence_step(hipStream_t st, int type, long long worlds, int channels, const void* x, long long x_w, const void* gate,
                        long long gate_w, const float* state, long long state_w, void* h, float* next);
 

@@ -645,7 +645,9 @@ struct Tick {
   float* next;
 };
 
-// Bytes bound it; a thread takes 16 bytes of x at a time, the last vector of a row ending with it
+// Bytes bound it; a thread takes 16 bytes of x at a time, the last vector of a row ending with it, so that it holds elements of
+// the one before again. Where the next states overwrite the states another thread may have written those already: there a row's
+// last elements are taken singly, each by one thread.
 template <typename T>
 __global__ __launch_bounds__(256) void k_scan_step(Tick a) {
   constexpr int E = Vec<T>::E;
@@ -653,7 +655,7 @@ __global__ __launch_bounds__(256) void k_scan_step(Tick a) {
   const long long all = a.worlds * nv;
   for (long long v = (long long)blockIdx.x * 256 + threadIdx.x; v < all; v += (long long)gridDim.x * 256) {
     const long long row = all >> 32 ? v / nv : (unsigned)v / (unsigned)nv;
-    const int i = (int)(v - row * nv) * E, c = n >= E && i > n - E ? n - E : i;
+    const int i = (int)(v - row * nv) * E, c = n >= E && i > n - E && a.next != a.state ? n - E : i;
     const T *x = (const T*)a.x + row * a.x_w + c, *g = (const T*)a.gate + row * a.g_w + c;
     const float* s = a.state + row * a.s_w + c;
     T* h = (T*)a.h + row * n + c;
@@ -663,7 +665,7 @@ __global__ __launch_bounds__(256) void k_scan_step(Tick a) {
       gates<T>(f, keep, take);
       return fmaf(keep, s, take * x);
     };
-    if (n >= E) {
+    if (c <= n - E) {
       float xf[E], gf[E], sf[E];
       load_floats<E>(xf, x);
       load_floats<E>(gf, g);
@@ -683,7 +685,7 @@ __global__ __launch_bounds__(256) void k_scan_step(Tick a) {
         store16(to + e, q);
       }
     } else {
-      for (int e = 0; e < n; ++e) {
+      for (int e = 0; e < n - c; ++e) {
         const float y = one((float)g[e], (float)x[e], s[e]);
         h[e] = rounded<T>(y);
         to[e] = y;
@@ -797,6 +799,10 @@ int dk_recurrence_step(hipStream_t st, int type, long long worlds, int channels,
   if (type < 0 || type > 2 || worlds < 0 || channels < 1) return (int)hipErrorInvalidValue;
   if (worlds == 0) return 0;
   if (!x || !gate || !state || !h || !next) return (int)hipErrorInvalidValue;
+  // the next states lie over the states row by row, or beside them
+  const bool rows = worlds == 1 || state_w == channels;
+  if (next == state ? !rows : rows && next < state + worlds * channels && state < next + worlds * channels)
+    return (int)hipErrorInvalidValue;
   pol::Tick a = {};
   a.x = x, a.gate = gate, a.x_w = x_w, a.g_w = gate_w, a.state = state, a.s_w = state_w;
   a.worlds = worlds, a.channels = channels, a.h = h, a.next = next;

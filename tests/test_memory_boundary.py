@@ -97,6 +97,17 @@ def test_c_entries_refuse_before_any_launch():
     assert size(4, 2, 64, 9, 5000, 5000, 50, 4, 1) > 0 == size(4, 2, 64, 9, 5000, 5000, 50, 0, 1)
 
 
+def test_next_states_lie_over_the_states_row_by_row_or_apart():
+    dll = torch_ffi.load_library()
+
+    def step(state, next_, worlds=3, channels=8, state_w=8):
+        return dll.dk_recurrence_step(None, 0, worlds, channels, 0x100000, 8, 0x200000, 8, state, state_w, 0x300000, next_)
+    at = 0x400000  # never dereferenced
+    for args in (dict(state=at, next_=at, state_w=9), dict(state=at, next_=at, state_w=0), dict(state=at, next_=at + 4), dict(state=at, next_=at - 92),
+                 dict(state=at, next_=at + 92), dict(state=at, next_=at - 4, worlds=1)):
+        assert step(**args) == 1, args
+
+
 def _cpu():
     """(x, gate, starts, states), heads of queries and keys, pages with their table and lengths, on the CPU or fake"""
     x, f, a, s = torch.randn(10, 6), torch.randn(10, 6), torch.tensor([0, 4, 10], dtype=I32), torch.randn(2, 6)
