@@ -72,16 +72,17 @@ __device__ __forceinline__ float sum_lanes(float x) {
   return x;
 }
 
-constexpr float LOG2E_GATE = 1.4426950408889634f;
-// a = 1 / (1 + exp(-f)) and 1 - a of a gate in T, each to its own last places (down to 2^-126, below which they are 0)
+constexpr float LOG2E_GATE = 1.4426950408889634f, LOG2E_REST = 1.925963e-8f;  // log2(e) to 24 bits, and what is left of it
+// a = 1 / (1 + exp(-f)) and 1 - a of a gate in T. In float32 the smaller one is within 7 2^-24 of itself, down to 2^-126, below which
+// they are 0; in 16 bits the exponent's own rounding stays, 1.3 |f| 2^-24 more, far below what the last place of such an f tells.
 template <typename T>
 __device__ __forceinline__ void gates(float f, float& keep, float& take) {
   float e;
-  if constexpr (sizeof(T) == 4) {  // with the product's rounding, which is felt by far gates
+  if constexpr (sizeof(T) == 4) {  // with what the exponent's rounding and the constant's take off, which is felt by far gates
     f = f > 200.0f ? 200.0f : f;
-    const float t = -f * LOG2E_GATE;
+    const float t = -f * LOG2E_GATE, rest = fmaf(-f, LOG2E_REST, fmaf(-f, LOG2E_GATE, -t));
     e = __builtin_amdgcn_exp2f(t);
-    e = t > 126.0f ? INFINITY : fmaf(e, fmaf(-f, LOG2E_GATE, -t) * 0.6931472f, e);
+    e = t > 126.0f ? INFINITY : fmaf(e, rest * 0.6931472f, e);
   } else {
     e = __builtin_amdgcn_exp2f(-f * LOG2E_GATE);
   }

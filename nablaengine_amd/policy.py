@@ -326,8 +326,8 @@ def recurrence(x, gate, starts, initial=None):
     states before the first tokens, or None for zeros. h has x's type and is zero behind the last sequence (padding, whose gradients are zero
     too); the last states are float32, those of sequences without tokens their initial ones.
 
-    The gate is given before its sigmoid, since 16 bits do not tell long memories apart after it: 1 - a keeps its own last
-    places for every a. States and all sums are float32 and each output is rounded once. Infinities and NaN stay in their
+    The gate is given before its sigmoid, since 16 bits do not tell long memories apart after it: the smaller of a and 1 - a is
+    computed of it directly, within 7 2^-24 of itself for float32 gates and 1.3 |gate| 2^-24 more for those of 16 bits. States and all sums are float32 and each output is rounded once. Infinities and NaN stay in their
     channel and sequence."""
     return _ops(True).recurrence(_tensor("x", x), _tensor("gate", gate), _tensor("starts", starts), initial)
 
