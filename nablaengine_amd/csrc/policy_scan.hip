@@ -3,24 +3,32 @@
 //   a = 1 / (1 + exp(-gate)),  h_t = a_t h_{t-1} + (1 - a_t) x_t  a channel, from each sequence's carried state
 //   g_t = dh_t + a_{t+1} g_{t+1},  dx = (1 - a) g,  dgate = g (h_{t-1} - x) a (1 - a),  dinitial = a g of the first token
 //
-// Steps compose: a stretch of tokens takes the state s that enters it to P s + B. The packed tokens are cut into chunks,
-// whatever sequences they hold, so that work is even over ragged lengths; a sequence's first token cuts the chain (a
-// choice, not a product with 0: what is not finite stays in its sequence). A workgroup takes a chunk and 64 V channels:
-// each of its waves reads TOK tokens at once into registers, a lane V channels of each, finds its stretch's P and B, gets
-// the state that enters it from the stretches before (LDS) and from the chunks before (memory), and walks over its tokens
-// once more. Sums and states are float32 throughout; each output is rounded once.
+// Steps compose: a stretch of tokens takes the state s that enters it to P s + B. A state lasts for as many steps as its gates
+// say, a million with one of 14, and what steps are off by must not add up over them: 1 - a has its own places, but a has not,
+// and a product of many, or many steps by it, is off by 2^-24 a token. So 1 - P is a sum of its own, from which P is taken
+// where it is the larger (map_of), wherever a state leaves a stretch, a chunk or a call; inside a stretch the product does.
+// 65536 tokens from a state and with inputs of 1 and gates of 12: every state 1 within 17 2^-24 (products throughout: 3.0e-3
+// off); the state's decay alone within 1.2e-6 of itself. The packed tokens are cut into chunks, whatever sequences they hold,
+// so that work is even over ragged lengths; a sequence's first token cuts the chain (a choice, not a product with 0: what is
+// not finite stays in its sequence). A workgroup takes a chunk and 64 V channels: each of its waves reads TOK tokens at once
+// into registers, a lane V channels of each, finds its stretch's P and B, gets the state that enters it from the stretches
+// before (LDS) and from the chunks before (memory), and walks over its tokens once more. Sums and states are float32
+// throughout; each output is rounded once.
 //
 // The chunks' P and B come from a kernel of their own, which reads only the tokens after a chunk's last sequence start (none
 // where the next chunk starts a sequence), and a third kernel carries states over the chunks: two reads of x and gate
 // where sequences are long, one where they are short. The backward does the same from the other end; it takes the forward's
 // carried states, so the states between are computed from x and gate again and none is stored.
 //
-// Memory bounds it, and where sequences are short one read after another: where they start, then their tokens. Measured, bfloat16,
-// of the 5.0 to 5.2 TB/s of a large copy: two sequences of 65536 tokens together, 1024 channels, forward 71 us (5.7 TB/s of x, gate
-// and h, some still in the cache), the chunks' P and B 64 (4.2 TB/s), backward 157 (4.3 TB/s) and 65; 4096 sequences of up to 32
-// tokens, 512 channels, 64 and 25, 119 and 24; the states over the chunks 11 each time. Chunks of 128 tokens, two workgroups of
-// eight waves a compute unit: forward 73 and 81 us, backward 134 and 186. Stretches of 16 tokens in the backward: 127 and 168 us.
-// One token a world: 16384 worlds of 1024 channels 35 us, 6.7 TB/s.
+// Memory bounds it, and where sequences are short one read after another: where they start, then their tokens. Measured,
+// bfloat16, of the 5.0 to 5.2 TB/s of a large copy: two sequences of 65536 tokens together, 1024 channels, forward 73 us (5.5
+// TB/s of x, gate and h, some still in the cache), the chunks' P and B 65 (4.1 TB/s), backward 160 (4.2 TB/s) and 70; 4096
+// sequences of up to 32 tokens, 512 channels, 63 and 26, 123 and 25; the states over the chunks 13 each time. 1 - P as a sum of
+// its own costs 3 % of a forward and backward (243 and 355 us a call without, 251 and 365 with). Without it: chunks of 128
+// tokens, two workgroups of eight waves a compute unit, forward 73 and 81 us for 64 and 71, backward 134 and 186 for 119 and
+// 157; stretches of 16 tokens in the backward 127 and 168. One token a world: 16384 worlds of 1024 channels 35 us, 6.7 TB/s.
+#include <cfloat>
+
 #include "../../include/nablaengine_memory.h"
 #include "policy_device.h"
 #include "policy_sizes.h"
@@ -36,7 +44,7 @@ struct Scan {
   void* h;
   float* last;   // (seqs, channels)
   float* carry;  // (chunks, channels): the state that enters each chunk
-  float* parts;  // (chunks, 2, channels): P, negative where the chunk drops what enters it, and B
+  float* parts;  // (chunks, 2, channels): the map (packed), DROPS where the chunk drops what enters it, and B
   // the backward's
   const void* dh;  // or NULL: zeros
   long long d_t;
@@ -67,6 +75,34 @@ __device__ __forceinline__ void store_few(T* p, const float* f) {
   for (int e = 0; e < V; ++e) r.v[e] = rounded<T>(f[e]);
   __builtin_memcpy(p, &r, sizeof(r));
 }
+
+// What tokens do to the state that enters them, P s + B, with what it takes for states that last long: P and Q = 1 - P are sums
+// of their own, each with its own last places. Up to a Q of 0.5, P is taken from it, and what its rounding leaves is added.
+struct Map { float p, rest; };
+__device__ __forceinline__ Map map_of(float p, float q) {
+  const float p1 = 1.0f - q;
+  return q <= 0.5f ? Map{p1, 1.0f - p1 - q} : Map{p, 0.0f};
+}
+// an infinite state is one whatever the rest's sign
+__device__ __forceinline__ float mapped(const Map& m, float b, float s) {
+  return fmaf(m.p, s, fmaf(m.rest, __builtin_amdgcn_fmed3f(s, -FLT_MAX, FLT_MAX), b));
+}
+// a token alone
+__device__ __forceinline__ float stepped(float keep, float take, float x, float s) { return mapped(map_of(keep, take), take * x, s); }
+// a map in one float: Q, or P with its sign changed
+__device__ __forceinline__ float packed(float p, float q) { return q <= 0.5f ? q : -p; }
+__device__ __forceinline__ Map unpacked(float m, float& p, float& q) {
+  const bool far = (int)__float_as_uint(m) < 0;
+  p = far ? -m : 1.0f - m;
+  const float left = 1.0f - p;
+  q = far ? left : m;
+  return {p, far ? 0.0f : left - m};
+}
+__device__ __forceinline__ Map unpacked(float m) {
+  float p, q;
+  return unpacked(m, p, q);
+}
+constexpr float DROPS = 2.0f;  // in a map's place: nothing of what enters leaves; unpacked, a P of -1
 
 __device__ __forceinline__ int scan_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
@@ -156,20 +192,29 @@ struct Lane {
   }
 };
 
-// P and B of the waves' stretches: (W, 64 V) each, and whether a stretch drops what enters it
-template <int W, int V>
+// the maps of the waves' stretches: (W, 64 V) each, and whether a stretch drops what enters it. WHOLE: with what P's rounding
+// leaves, for states that go on past the chunk.
+template <int W, int V, bool WHOLE = true>
 struct Joined {
-  float p[W][64][V], b[W][64][V];
+  float p[W][64][V], b[W][64][V], rest[WHOLE ? W : 1][64][V];
   int drops[W];
+  __device__ __forceinline__ void put(int w, int l, int e, const Map& m, float to) {
+    p[w][l][e] = m.p, b[w][l][e] = to;
+    if (WHOLE) rest[w][l][e] = m.rest;
+  }
+  __device__ __forceinline__ Map at(int w, int l, int e) const { return {p[w][l][e], rest[w][l][e]}; }
 };
 
 // the state after stretches from .. to - 1 (or, from the end, from .. to + 1 downwards) from the one that enters them
-template <int W, int V>
-__device__ __forceinline__ void through(const Joined<W, V>& j, int w, float* s) {
+template <int W, int V, bool WHOLE>
+__device__ __forceinline__ void through(const Joined<W, V, WHOLE>& j, int w, float* s) {
   const int l = threadIdx.x % 64;
-  const bool drops = j.drops[w];
+  const bool none = j.drops[w];
 #pragma unroll
-  for (int e = 0; e < V; ++e) s[e] = drops ? j.b[w][l][e] : fmaf(j.p[w][l][e], s[e], j.b[w][l][e]);
+  for (int e = 0; e < V; ++e) {
+    const float b = j.b[w][l][e];
+    s[e] = none ? b : WHOLE ? mapped(j.at(w, l, e), b, s[e]) : fmaf(j.p[w][l][e], s[e], b);
+  }
 }
 
 // sequence s's row of a (seqs, channels) table, zeros where there is none
@@ -220,7 +265,7 @@ __global__ __launch_bounds__(64 * W) void k_scan_parts(Scan a) {
   if (at[CHUNK] >= 0) {  // the next chunk takes nothing over
     if (w == 0 && lane.counts)
 #pragma unroll
-      for (int e = 0; e < V; ++e) out[e] = -1.0f, out[a.channels + e] = 0.0f;
+      for (int e = 0; e < V; ++e) out[e] = DROPS, out[a.channels + e] = 0.0f;
     return;
   }
   const Stretch<TOK> st(a, at, base, chunk * CHUNK, w);
@@ -233,44 +278,52 @@ __global__ __launch_bounds__(64 * W) void k_scan_parts(Scan a) {
     from = o > from ? o : from;
   }
   from = scan_uniform(from);
-  float p[V], b[V];
+  float p[V], q[V], b[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) p[e] = 1.0f, b[e] = 0.0f;
+  for (int e = 0; e < V; ++e) p[e] = 1.0f, q[e] = b[e] = 0.0f;
   if ((w + 1) * TOK > from) {
     Few<T, V> f[TOK], x[TOK];
     load_tokens<T, V, TOK>(a.gate, a.g_t, a, st.t0, lane.c, f);
     load_tokens<T, V, TOK>(a.x, a.x_t, a, st.t0, lane.c, x);
+    Few<float, V> s = {};
     walk<T, V, TOK>(st, f, [&](int i) {
-                      const auto s = state_of<V>(a, a.initial, st.sequence_at(i), lane.c);
+                      s = state_of<V>(a, a.initial, st.sequence_at(i), lane.c);
 #pragma unroll
-                      for (int e = 0; e < V; ++e) b[e] = s.v[e];
+                      for (int e = 0; e < V; ++e) p[e] = 1.0f, q[e] = b[e] = 0.0f;
                     },
                     [&](int i) {
 #pragma unroll
                       for (int e = 0; e < V; ++e) {
                         float keep, take;
                         gates<T>((float)f[i].v[e], keep, take);
+                        q[e] = fmaf(take, p[e], q[e]);
                         p[e] *= keep;
                         b[e] = fmaf(keep, b[e], take * (float)x[i].v[e]);
                       }
                     });
+#pragma unroll
+    for (int e = 0; e < V; ++e) b[e] = mapped(map_of(p[e], q[e]), b[e], s.v[e]);  // from the last start's state, or none
   }
 #pragma unroll
-  for (int e = 0; e < V; ++e) joined.p[w][l][e] = p[e], joined.b[w][l][e] = b[e];
+  for (int e = 0; e < V; ++e) joined.put(w, l, e, map_of(p[e], q[e]), b[e]);
   if (l == 0) joined.drops[w] = (st.cuts & ((1u << TOK) - 1)) != 0;
   __syncthreads();
   if (w || !lane.counts) return;
-  bool drops = false;
+  bool none = false;
 #pragma unroll
-  for (int e = 0; e < V; ++e) p[e] = 1.0f, b[e] = 0.0f;
+  for (int e = 0; e < V; ++e) p[e] = 1.0f, q[e] = b[e] = 0.0f;
   for (int o = 0; o < W; ++o) {
-    through<W, V>(joined, o, b);
-    drops |= joined.drops[o] != 0;
+    through(joined, o, b);
+    none |= joined.drops[o] != 0;
 #pragma unroll
-    for (int e = 0; e < V; ++e) p[e] *= joined.p[o][l][e];
+    for (int e = 0; e < V; ++e) {
+      const Map m = joined.at(o, l, e);
+      q[e] = fmaf(1.0f - m.p - m.rest, p[e], q[e]);
+      p[e] *= m.p;
+    }
   }
 #pragma unroll
-  for (int e = 0; e < V; ++e) out[e] = drops ? -1.0f : p[e], out[a.channels + e] = b[e];
+  for (int e = 0; e < V; ++e) out[e] = none ? DROPS : packed(p[e], q[e]), out[a.channels + e] = b[e];
 }
 
 // the same from the other end: what a chunk hands to the token before its first, from what the token after its last hands to
@@ -287,7 +340,7 @@ __global__ __launch_bounds__(64 * W) void k_scan_back_parts(Scan a) {
   if (at[0] >= 0) {
     if (w == 0 && lane.counts)
 #pragma unroll
-      for (int e = 0; e < V; ++e) out[e] = -1.0f, out[a.channels + e] = 0.0f;
+      for (int e = 0; e < V; ++e) out[e] = DROPS, out[a.channels + e] = 0.0f;
     return;
   }
   const Stretch<TOK> st(a, at, base, chunk * CHUNK, w);
@@ -299,9 +352,9 @@ __global__ __launch_bounds__(64 * W) void k_scan_back_parts(Scan a) {
     to = o < to ? o : to;
   }
   to = scan_uniform(to);
-  float p[V], b[V];
+  float p[V], q[V], b[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) p[e] = 1.0f, b[e] = 0.0f;
+  for (int e = 0; e < V; ++e) p[e] = 1.0f, q[e] = b[e] = 0.0f;
   if (w * TOK < to && st.live > 0) {
     Few<T, V> f[TOK], d[TOK];
     load_tokens<T, V, TOK>(a.gate, a.g_t, a, st.t0, lane.c, f);
@@ -314,34 +367,39 @@ __global__ __launch_bounds__(64 * W) void k_scan_back_parts(Scan a) {
     const int end = later ? __builtin_ctz(later) + 1 : TOK;
     const auto last = state_of<V>(a, a.dlast, later ? st.seq : -1, lane.c);
 #pragma unroll
-    for (int e = 0; e < V; ++e) b[e] = last.v[e];
-#pragma unroll
     for (int i = TOK - 1; i >= 0; --i)
       if (i < end)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           float keep, take;
           gates<T>((float)f[i].v[e], keep, take);
+          q[e] = fmaf(take, p[e], q[e]);
           p[e] *= keep;
           b[e] = keep * (b[e] + (float)d[i].v[e]);
         }
+#pragma unroll
+    for (int e = 0; e < V; ++e) b[e] = mapped(map_of(p[e], q[e]), b[e], last.v[e]);
   }
 #pragma unroll
-  for (int e = 0; e < V; ++e) joined.p[w][l][e] = p[e], joined.b[w][l][e] = b[e];
+  for (int e = 0; e < V; ++e) joined.put(w, l, e, map_of(p[e], q[e]), b[e]);
   if (l == 0) joined.drops[w] = (st.cuts >> 1) != 0;
   __syncthreads();
   if (w || !lane.counts) return;
-  bool drops = false;
+  bool none = false;
 #pragma unroll
-  for (int e = 0; e < V; ++e) p[e] = 1.0f, b[e] = 0.0f;
+  for (int e = 0; e < V; ++e) p[e] = 1.0f, q[e] = b[e] = 0.0f;
   for (int o = W - 1; o >= 0; --o) {
-    through<W, V>(joined, o, b);
-    drops |= joined.drops[o] != 0;
+    through(joined, o, b);
+    none |= joined.drops[o] != 0;
 #pragma unroll
-    for (int e = 0; e < V; ++e) p[e] *= joined.p[o][l][e];
+    for (int e = 0; e < V; ++e) {
+      const Map m = joined.at(o, l, e);
+      q[e] = fmaf(1.0f - m.p - m.rest, p[e], q[e]);
+      p[e] *= m.p;
+    }
   }
 #pragma unroll
-  for (int e = 0; e < V; ++e) out[e] = drops ? -1.0f : p[e], out[a.channels + e] = b[e];
+  for (int e = 0; e < V; ++e) out[e] = none ? DROPS : packed(p[e], q[e]), out[a.channels + e] = b[e];
 }
 
 // ---- the states that enter the chunks -------------------------------------------------------------------------------
@@ -352,58 +410,71 @@ __global__ __launch_bounds__(64 * W) void k_scan_back_parts(Scan a) {
 template <bool BACK>
 __global__ __launch_bounds__(1024) void k_scan_carry(Scan a) {
   constexpr int CH = 8, RUNS = 1024 / CH;
-  __shared__ float ps[2][RUNS][CH], bs[2][RUNS][CH];
+  __shared__ float ps[2][RUNS][CH], qs[2][RUNS][CH], bs[2][RUNS][CH];
   const int l = threadIdx.x % CH, c = blockIdx.x * CH + l, run = threadIdx.x / CH;
   const bool in = c < a.channels;
   const int n = a.chunks - 1, each = (n + RUNS - 1) / RUNS;  // the maps between neighbouring chunks, in the order of the walk
   const int first = run * each < n ? run * each : n, end = first + each < n ? first + each : n;
   auto at = [&](int i) { return a.parts + (long long)(BACK ? a.chunks - 1 - i : i) * 2 * a.channels + (in ? c : 0); };
   constexpr int KEPT = 16;  // maps that stay in registers for the second walk: up to 2048 chunks
-  float pk[KEPT], bk[KEPT], p = 1.0f, b = 0.0f;
+  Map mk[KEPT];
+  float bk[KEPT], p = 1.0f, q = 0.0f, b = 0.0f;
+  bool none = false;
   const bool kept = each <= KEPT;
-  auto step = [&](float pi, float bi) {
-    b = pi < 0.0f ? bi : fmaf(pi, b, bi);
-    p = pi < 0.0f || p < 0.0f ? -1.0f : p * pi;
+  // a map's P is below 0 where it drops what enters
+  auto from = [&](const Map& m, float bi, float s) { return m.p < 0.0f ? bi : mapped(m, bi, s); };
+  auto step = [&](float mi, float bi) {
+    float p1, q1;
+    const Map m = unpacked(mi, p1, q1);
+    b = from(m, bi, b);
+    none |= m.p < 0.0f;
+    q = fmaf(q1, p, q);
+    p *= p1;
+    return m;
   };
   if (kept) {
+    float in[KEPT];
 #pragma unroll
     for (int i = 0; i < KEPT; ++i) {
       const bool there = first + i < end;
-      pk[i] = there ? at(first + i)[0] : 1.0f, bk[i] = there ? at(first + i)[a.channels] : 0.0f;
+      in[i] = there ? at(first + i)[0] : 0.0f, bk[i] = there ? at(first + i)[a.channels] : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < KEPT; ++i) step(pk[i], bk[i]);
+    for (int i = 0; i < KEPT; ++i)
+      if (i < each) mk[i] = step(in[i], bk[i]);
   } else {
 #pragma unroll 8
     for (int i = first; i < end; ++i) step(at(i)[0], at(i)[a.channels]);
   }
   int side = 0;
-  ps[0][run][l] = p, bs[0][run][l] = b;
+  if (none) p = -1.0f;
+  ps[0][run][l] = p, qs[0][run][l] = q, bs[0][run][l] = b;
 #pragma unroll
   for (int d = 1; d < RUNS; d *= 2, side ^= 1) {
     __syncthreads();
-    if (run >= d) {
-      const float p0 = ps[side][run - d][l], b0 = bs[side][run - d][l];
-      b = p < 0.0f ? b : fmaf(p, b0, b);
-      p = p < 0.0f || p0 < 0.0f ? -1.0f : p * p0;
+    if (run >= d && !(p < 0.0f)) {
+      const float p0 = ps[side][run - d][l];
+      b = mapped(map_of(p, q), b, bs[side][run - d][l]);
+      q = fmaf(q, p0, qs[side][run - d][l]);
+      p = p0 < 0.0f ? p0 : p * p0;
     }
-    ps[side ^ 1][run][l] = p, bs[side ^ 1][run][l] = b;
+    ps[side ^ 1][run][l] = p, qs[side ^ 1][run][l] = q, bs[side ^ 1][run][l] = b;
   }
   __syncthreads();
   float s = run ? bs[side][run - 1][l] : 0.0f;  // nothing enters the first chunk
   float* out = BACK ? a.back : a.carry;
   if (run == 0 && in) out[(long long)(BACK ? a.chunks - 1 : 0) * a.channels + c] = 0.0f;
-  auto put = [&](int i, float pi, float bi) {
-    s = pi < 0.0f ? bi : fmaf(pi, s, bi);
+  auto put = [&](int i, const Map& m, float bi) {
+    s = from(m, bi, s);
     if (in) out[(long long)(BACK ? a.chunks - 2 - i : i + 1) * a.channels + c] = s;
   };
   if (kept) {
 #pragma unroll
     for (int i = 0; i < KEPT; ++i)
-      if (first + i < end) put(first + i, pk[i], bk[i]);
+      if (first + i < end) put(first + i, mk[i], bk[i]);
   } else {
 #pragma unroll 8
-    for (int i = first; i < end; ++i) put(i, at(i)[0], at(i)[a.channels]);
+    for (int i = first; i < end; ++i) put(i, unpacked(at(i)[0]), at(i)[a.channels]);
   }
 }
 
@@ -454,27 +525,40 @@ __global__ __launch_bounds__(64 * W) void k_scan(Scan a) {
 #pragma unroll
     for (int e = 0; e < V; ++e) to[e] = s.v[e];
   };
-  float keep[TOK][V], bx[TOK][V], p[V], b[V];
+  // What leads to each token from the state that enters its sequence in this stretch: P s + B, P as the gates' product, whose TOK
+  // roundings at most end there; at a sequence's end, whose state goes on to other calls, the whole map.
+  float to_p[TOK][V], to_b[TOK][V], p[V], q[V], b[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) p[e] = 1.0f, b[e] = 0.0f;
+  for (int e = 0; e < V; ++e) p[e] = 1.0f, q[e] = b[e] = 0.0f;
 #pragma unroll
-  for (int i = 0; i < TOK; ++i)
+  for (int i = 0; i < TOK; ++i) {  // tokens past the last sequence's end too: nothing takes what they lead to
+    if (st.cuts >> i & 1)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (i) to_p[i - 1][e] = packed(p[e], q[e]);
+        p[e] = 1.0f, q[e] = b[e] = 0.0f;
+      }
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      float take;
-      gates<T>((float)f[i].v[e], keep[i][e], take);
-      bx[i][e] = take * (float)x[i].v[e];
+      float keep, take;
+      gates<T>((float)f[i].v[e], keep, take);
+      q[e] = fmaf(take, p[e], q[e]);
+      p[e] *= keep;
+      b[e] = fmaf(keep, b[e], take * (float)x[i].v[e]);
+      to_p[i][e] = p[e], to_b[i][e] = b[e];
     }
-  walk<T, V, TOK>(st, f, [&](int i) { start(i, b); },
-                  [&](int i) {
+  }
+  float s0[V] = {};  // the last start's state
+  if (inside) start(31 - __builtin_clz(inside), s0);
+  Map whole[V];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) p[e] *= keep[i][e], b[e] = fmaf(keep[i][e], b[e], bx[i][e]);
-                  });
-#pragma unroll
-  for (int e = 0; e < V; ++e) joined.p[w][l][e] = p[e], joined.b[w][l][e] = b[e];
+  for (int e = 0; e < V; ++e) {
+    whole[e] = map_of(p[e], q[e]);
+    joined.put(w, l, e, whole[e], mapped(whole[e], b[e], s0[e]));
+  }
   if (l == 0) joined.drops[w] = inside != 0;
   __syncthreads();
-  for (int o = 0; o < w; ++o) through<W, V>(joined, o, s);
+  for (int o = 0; o < w; ++o) through(joined, o, s);
   if (!lane.counts) return;
   auto put = [&](int i, const float* f) { store_few<T, V>((T*)a.h + (long long)(st.t0 + i) * a.channels + (unsigned)lane.c, f); };
   int seq = st.seq;
@@ -484,14 +568,17 @@ __global__ __launch_bounds__(64 * W) void k_scan(Scan a) {
                     seq = st.sequence_at(i);
                   },
                   [&](int i) {
-#pragma unroll
-                    for (int e = 0; e < V; ++e) s[e] = fmaf(keep[i][e], s[e], bx[i][e]);
-                    put(i, s);
+                    float h[V];
                     if (st.cuts >> (i + 1) & 1) {
                       float* last = a.last + (long long)seq * a.channels + (unsigned)lane.c;
 #pragma unroll
-                      for (int e = 0; e < V; ++e) last[e] = s[e];
+                      for (int e = 0; e < V; ++e)
+                        last[e] = h[e] = mapped(i + 1 == TOK ? whole[e] : unpacked(to_p[i][e]), to_b[i][e], s[e]);
+                    } else {
+#pragma unroll
+                      for (int e = 0; e < V; ++e) h[e] = fmaf(to_p[i][e], s[e], to_b[i][e]);
                     }
+                    put(i, h);
                   });
   const float none[V] = {};
 #pragma unroll
@@ -503,7 +590,8 @@ template <typename T, int V, int W, int TOK>
 __global__ __launch_bounds__(64 * W, 4) void k_scan_vjp(Scan a) {
   constexpr int CHUNK = W * TOK, NT = 64 * W;
   __shared__ int at[CHUNK + 1];
-  __shared__ Joined<W, V> ahead, behind;
+  __shared__ Joined<W, V, false> ahead;  // to the gates' gradients alone
+  __shared__ Joined<W, V> behind;
   if ((int)blockIdx.x >= a.chunks * a.groups) {
     if (a.dinitial) empty_sequences(a, a.dlast, a.dinitial);
     return;
@@ -548,46 +636,61 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_vjp(Scan a) {
   // Both ways' P and B in one walk: the other way's B is the sum of the cotangents, each times the product of the gates up to its
   // token, up to the first sequence's end. Gates are computed anew in each of the three walks: kept, they take the registers of
   // other waves (94 a lane for 70; 4096 short sequences 127 us for 119, long ones the same).
-  float p[V], b[V], q[V], c[V];
+  float p[V], q[V], b[V], c[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) p[e] = q[e] = 1.0f, b[e] = c[e] = 0.0f;
+  for (int e = 0; e < V; ++e) p[e] = 1.0f, q[e] = b[e] = c[e] = 0.0f;
   const int led = later ? __builtin_ctz(later) : TOK;  // tokens that lead to the stretch's first without an end between
   auto led_d = final_d;
   if (led != final) led_d = state_of<V>(a, a.dlast, later ? st.seq : -1, lane.c);
-  walk<T, V, TOK>(st, f, [&](int i) { start(i, b); },
+  auto put_behind = [&] {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const Map m = map_of(p[e], q[e]);
+      behind.put(w, l, e, m, mapped(m, c[e], led_d.v[e]));
+    }
+  };
+  walk<T, V, TOK>(st, f,
+                  [&](int i) {
+                    if (i == led) put_behind();
+#pragma unroll
+                    for (int e = 0; e < V; ++e) p[e] = 1.0f, q[e] = b[e] = 0.0f;
+                  },
                   [&](int i) {
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
                       float keep, take;
                       gates<T>((float)f[i].v[e], keep, take);
+                      q[e] = fmaf(take, p[e], q[e]);
                       p[e] *= keep;
                       b[e] = fmaf(keep, b[e], take * (float)x[i].v[e]);
-                      if (i < led) q[e] = p[e], c[e] = fmaf(p[e], (float)d[i].v[e] + (i == led - 1 ? led_d.v[e] : 0.0f), c[e]);
+                      c[e] = fmaf(p[e], (float)d[i].v[e], c[e]);
                     }
                   });
   const bool plain = st.live == TOK && !st.cuts;
   auto walk_back = [&](auto ends, auto step) {  // from the last token on
     if (plain) {
 #pragma unroll
-      for (int i = TOK - 1; i >= 0; --i) step(i);
+      for (int i = TOK - 1; i >= 0; --i) step(i, std::false_type());
     } else {
 #pragma unroll
       for (int i = TOK - 1; i >= 0; --i)
         if (i < st.live) {
           if (st.cuts >> (i + 1) & 1) ends(i + 1);
-          step(i);
+          step(i, std::true_type());
         }
     }
   };
+  if (led >= st.live) put_behind();  // no sequence has started behind those
+  float s0[V] = {};  // the last start's state
+  if (inside) start(31 - __builtin_clz(inside), s0);
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    ahead.p[w][l][e] = p[e], ahead.b[w][l][e] = b[e];
-    behind.p[w][l][e] = q[e], behind.b[w][l][e] = c[e];
+    ahead.put(w, l, e, {p[e], 0.0f}, fmaf(p[e], s0[e], b[e]));
   }
   if (l == 0) ahead.drops[w] = inside != 0, behind.drops[w] = later != 0;
   __syncthreads();
-  for (int o = 0; o < w; ++o) through<W, V>(ahead, o, s);
-  for (int o = W - 1; o > w; --o) through<W, V>(behind, o, r);
+  for (int o = 0; o < w; ++o) through(ahead, o, s);
+  for (int o = W - 1; o > w; --o) through(behind, o, r);
   if (!lane.counts) return;
   float off[TOK][V];  // how far the state before each token is from its x
   walk<T, V, TOK>(st, f, [&](int i) { start(i, s); },
@@ -608,7 +711,7 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_vjp(Scan a) {
 #pragma unroll
               for (int e = 0; e < V; ++e) r[e] = s.v[e];
             },
-            [&](int i) {
+            [&](int i, auto cut) {  // cut: a sequence may start here, whose dinitial goes on to other calls
               float dx[V], dg[V];
 #pragma unroll
               for (int e = 0; e < V; ++e) {
@@ -616,7 +719,7 @@ __global__ __launch_bounds__(64 * W, 4) void k_scan_vjp(Scan a) {
                 gates<T>((float)f[i].v[e], k, take);
                 const float g = r[e] + (float)d[i].v[e];
                 dx[e] = take * g;
-                r[e] = k * g;
+                r[e] = cut ? stepped(k, take, 0.0f, g) : k * g;
                 dg[e] = dx[e] * k * off[i][e];
               }
               put(a.dx, i, dx);
@@ -663,7 +766,7 @@ __global__ __launch_bounds__(256) void k_scan_step(Tick a) {
     auto one = [](float f, float x, float s) {
       float keep, take;
       gates<T>(f, keep, take);
-      return fmaf(keep, s, take * x);
+      return stepped(keep, take, x, s);
     };
     if (c <= n - E) {
       float xf[E], gf[E], sf[E];
