@@ -406,12 +406,12 @@ __global__ __launch_bounds__(64 * W) void k_scan_back_parts(Scan a) {
 
 // 8 channels a workgroup and 128 runs of chunks: each run's own P and B, those joined over the runs by doubling, then each
 // run once more from the state that enters it. BACK: the chunks from the last to the first. Bound by one read after another: 1340
-// chunks of 512 channels 11 us, the same with 16 channels and 64 runs.
+// chunks of 512 channels 12.5 us; 11 before 1 - P was a sum of its own, the same with 16 channels and 64 runs.
 template <bool BACK>
-__global__ __launch_bounds__(1024) void k_scan_carry(Scan a) {
+__global__ __launch_bounds__(1024) void k_scan_carry(Scan a, int c0) {
   constexpr int CH = 8, RUNS = 1024 / CH;
   __shared__ float ps[2][RUNS][CH], qs[2][RUNS][CH], bs[2][RUNS][CH];
-  const int l = threadIdx.x % CH, c = blockIdx.x * CH + l, run = threadIdx.x / CH;
+  const int l = threadIdx.x % CH, c = c0 + blockIdx.x * CH + l, run = threadIdx.x / CH;
   const bool in = c < a.channels;
   const int n = a.chunks - 1, each = (n + RUNS - 1) / RUNS;  // the maps between neighbouring chunks, in the order of the walk
   const int first = run * each < n ? run * each : n, end = first + each < n ? first + each : n;
@@ -822,17 +822,29 @@ unsigned scan_blocks(const Scan& a) {  // the chunks', and those that look for e
   return (unsigned)(a.chunks * a.groups + (extra < 256 ? extra : 256));
 }
 
+// 8 channels a workgroup, in as many launches as keep the work-items of each below 2^32: one up to 2^24 channels
+template <bool BACK>
+int launch_carry(hipStream_t st, const Scan& a) {
+  constexpr int MOST = 1 << 24;
+  for (int c0 = 0; c0 < a.channels; c0 += MOST) {
+    const int n = a.channels - c0 < MOST ? a.channels - c0 : MOST;
+    k_scan_carry<BACK><<<(unsigned)((n + 7) / 8), 1024, 0, st>>>(a, c0);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  return 0;
+}
+
 int launch_scan(hipStream_t st, int type, const Scan& a) {
   return scan_by_type(type, a.channels, [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value, W = SCAN_CHUNK / SCAN_TOKENS;
     if (a.chunks > 1) {
       k_scan_parts<T, V, W, SCAN_TOKENS><<<(unsigned)((a.chunks - 1) * a.groups), 64 * W, 0, st>>>(a);
-      hipError_t e = hipGetLastError();
+      const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return (int)e;
-      k_scan_carry<false><<<(unsigned)((a.channels + 7) / 8), 1024, 0, st>>>(a);
-      e = hipGetLastError();
-      if (e != hipSuccess) return (int)e;
+      const int rc = launch_carry<false>(st, a);
+      if (rc) return rc;
     }
     const unsigned blocks = scan_blocks(a);
     if (blocks) k_scan<T, V, W, SCAN_TOKENS><<<blocks, 64 * W, 0, st>>>(a);
@@ -845,11 +857,10 @@ int launch_scan_vjp(hipStream_t st, int type, const Scan& a) {
     constexpr int V = decltype(v)::value, W = SCAN_CHUNK / SCAN_TOKENS;
     if (a.chunks > 1) {
       k_scan_back_parts<T, V, W, SCAN_TOKENS><<<(unsigned)((a.chunks - 1) * a.groups), 64 * W, 0, st>>>(a);
-      hipError_t e = hipGetLastError();
+      const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return (int)e;
-      k_scan_carry<true><<<(unsigned)((a.channels + 7) / 8), 1024, 0, st>>>(a);
-      e = hipGetLastError();
-      if (e != hipSuccess) return (int)e;
+      const int rc = launch_carry<true>(st, a);
+      if (rc) return rc;
     }
     const unsigned blocks = scan_blocks(a);
     if (blocks) k_scan_vjp<T, V, SCAN_CHUNK / SCAN_TOKENS_VJP, SCAN_TOKENS_VJP><<<blocks, 64 * SCAN_CHUNK / SCAN_TOKENS_VJP, 0, st>>>(a);
