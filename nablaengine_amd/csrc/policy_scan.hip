@@ -6,9 +6,10 @@
 // Steps compose: a stretch of tokens takes the state s that enters it to P s + B. A state lasts for as many steps as its gates
 // say, a million with one of 14, and what steps are off by must not add up over them: 1 - a has its own places, but a has not,
 // and a product of many, or many steps by it, is off by 2^-24 a token. So 1 - P is a sum of its own, from which P is taken
-// where it is the larger (map_of), wherever a state leaves a stretch, a chunk or a call; inside a stretch the product does.
-// 65536 tokens from a state and with inputs of 1 and gates of 12: every state 1 within 17 2^-24 (products throughout: 3.0e-3
-// off); the state's decay alone within 1.2e-6 of itself. The packed tokens are cut into chunks, whatever sequences they hold,
+// where it is the larger (map_of, join), wherever a state leaves a stretch, a chunk or a call; inside a stretch the product
+// does. 65536 tokens from a state and with inputs of 1: every state 1 within 30 2^-24 at any gate (products throughout: 3.0e-3
+// off at a gate of 12; of chunks: 104 2^-24), and over 2^25 tokens within 23; the state's decay alone within 1.4e-6 of itself
+// from gates of 8 on. The packed tokens are cut into chunks, whatever sequences they hold,
 // so that work is even over ragged lengths; a sequence's first token cuts the chain (a choice, not a product with 0: what is
 // not finite stays in its sequence). A workgroup takes a chunk and 64 V channels: each of its waves reads TOK tokens at once
 // into registers, a lane V channels of each, finds its stretch's P and B, gets the state that enters it from the stretches
@@ -86,6 +87,11 @@ __device__ __forceinline__ Map map_of(float p, float q) {
 // an infinite state is one whatever the rest's sign
 __device__ __forceinline__ float mapped(const Map& m, float b, float s) {
   return fmaf(m.p, s, fmaf(m.rest, __builtin_amdgcn_fmed3f(s, -FLT_MAX, FLT_MAX), b));
+}
+// p and q of what (p1, q1) makes of what they are already
+__device__ __forceinline__ void join(float& p, float& q, float p1, float q1) {
+  q = fmaf(q1, p, q);
+  p = q <= 0.5f ? 1.0f - q : p * p1;  // the product's factors are off by 2^-25 each
 }
 // a token alone
 __device__ __forceinline__ float stepped(float keep, float take, float x, float s) { return mapped(map_of(keep, take), take * x, s); }
@@ -318,8 +324,7 @@ __global__ __launch_bounds__(64 * W) void k_scan_parts(Scan a) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const Map m = joined.at(o, l, e);
-      q[e] = fmaf(1.0f - m.p - m.rest, p[e], q[e]);
-      p[e] *= m.p;
+      join(p[e], q[e], m.p, 1.0f - m.p - m.rest);
     }
   }
 #pragma unroll
@@ -394,8 +399,7 @@ __global__ __launch_bounds__(64 * W) void k_scan_back_parts(Scan a) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const Map m = joined.at(o, l, e);
-      q[e] = fmaf(1.0f - m.p - m.rest, p[e], q[e]);
-      p[e] *= m.p;
+      join(p[e], q[e], m.p, 1.0f - m.p - m.rest);
     }
   }
 #pragma unroll
@@ -428,8 +432,7 @@ __global__ __launch_bounds__(1024) void k_scan_carry(Scan a, int c0) {
     const Map m = unpacked(mi, p1, q1);
     b = from(m, bi, b);
     none |= m.p < 0.0f;
-    q = fmaf(q1, p, q);
-    p *= p1;
+    join(p, q, p1, q1);
     return m;
   };
   if (kept) {
@@ -455,8 +458,10 @@ __global__ __launch_bounds__(1024) void k_scan_carry(Scan a, int c0) {
     if (run >= d && !(p < 0.0f)) {
       const float p0 = ps[side][run - d][l];
       b = mapped(map_of(p, q), b, bs[side][run - d][l]);
-      q = fmaf(q, p0, qs[side][run - d][l]);
-      p = p0 < 0.0f ? p0 : p * p0;
+      const float p1 = p, q1 = q;
+      p = p0, q = qs[side][run - d][l];
+      join(p, q, p1, q1);
+      if (p0 < 0.0f) p = p0;
     }
     ps[side ^ 1][run][l] = p, qs[side ^ 1][run][l] = q, bs[side ^ 1][run][l] = b;
   }

@@ -50,6 +50,28 @@ def test_a_state_that_its_input_repeats_stays(n, gate):
         assert off <= roundings(n) * U, (name, off)
 
 
+@pytest.mark.parametrize("gate", [12.0, 15.0, 17.0])
+def test_a_state_that_its_input_repeats_stays_over_many_chunks(gate):
+    """2^25 tokens, 4096 chunks a run of the chain: the maps of many chunks, too, are no products of roundings."""
+    n = 2 ** 25
+    print("many chunks", gate, flush=True)
+    value = torch.tensor([1.0, -0.7], device="cuda")
+    h, last = policy.recurrence(value.expand(n, 2), torch.tensor([[gate]], device="cuda").expand(n, 2).contiguous(), one_sequence(n),
+                                value[None].clone())
+    off = (h / value - 1).abs().max().item()
+    assert off <= (roundings(n) + 1) * U, off
+
+
+def test_a_state_that_its_input_repeats_stays_at_any_gate():
+    """Gates 0.01 apart from 0 to 20, a channel each."""
+    n, gates = 65536, torch.linspace(0, 20, 2001, device="cuda")
+    print("gates", flush=True)
+    x = torch.full((n, 2001), -0.7, device="cuda")
+    h, _ = policy.recurrence(x, gates.expand(n, 2001), one_sequence(n), x[:1].clone())
+    off = (h.double() / x.double() - 1).abs().amax(0)
+    assert (off <= roundings(n) * U).all(), (off.max().item(), gates[off.argmax()].item())
+
+
 @pytest.mark.parametrize("n", [100, 5000, 65536])
 @pytest.mark.parametrize("gate", [2.0, 5.5, 8.0, 9.3, 12.0, 15.0, 17.0, 20.0])
 def test_decay_and_its_gradients(n, gate):
