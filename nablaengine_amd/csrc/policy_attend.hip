@@ -1126,7 +1126,9 @@ size_t attend_work_bytes(int dim, int seqs, int tq, int tk, int group) {
 }
 // Where the sinks' far rows are walked over apart: where there are sinks, at most four tiles of 32, and a sequence may be longer
 // than a window and half a part; not where their slots would take more than 1 GB. Parts of 512 tokens: 50 us for 34, of two
-// sequences of 8192 tokens.
+// sequences of 8192 tokens. Forward and backward with 128 sinks, with 129 as they are, and with five tiles apart: 256 sequences of up
+// to 1000, window 128, 817, 746 and 847 us; 8192 and 2752 tokens, window 1000, 761, 1150 and 822; four of 16384, window 512, 643, 2647
+// and 643: past the limit long sequences pay for all their rows.
 constexpr int FAR_TOKENS = 256;
 struct FarPlan { int tokens, least, chunks; long long slots; };
 FarPlan far_plan(int kv_heads, int dim, int tq, int tk, int window, int sinks) {

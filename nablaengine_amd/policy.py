@@ -288,7 +288,7 @@ def attention(q, k, v, starts_q, starts_k=None, *, scale=None, window=None, sink
     sequence (padding), whose gradients are zero too. scale (> 0) defaults to 1 / sqrt(dim).
 
     window: of those keys a query sees the `window` last ones only, and the `sinks` first ones of its sequence; the time goes by
-    the keys in sight then. A window that no sequence is longer than hides nothing; without one, sinks have no part.
+    the keys in sight then, but with more than 128 sinks the gradients of the first keys by all of a sequence's rows. A window that no sequence is longer than hides nothing; without one, sinks have no part.
 
     Scores, softmax statistics and all sums are float32; probabilities and score gradients are rounded to q's type for
     the matrix instructions, as the inputs are (float16: brought inside its range first). A query whose every score is -inf
@@ -327,8 +327,10 @@ def recurrence(x, gate, starts, initial=None):
     too); the last states are float32, those of sequences without tokens their initial ones.
 
     The gate is given before its sigmoid, since 16 bits do not tell long memories apart after it: the smaller of a and 1 - a is
-    computed of it directly, within 7 2^-24 of itself for float32 gates and 1.3 |gate| 2^-24 more for those of 16 bits. States and all sums are float32 and each output is rounded once. Infinities and NaN stay in their
-    channel and sequence."""
+    computed of it directly, within 7 2^-24 of itself for float32 gates and 1.3 |gate| 2^-24 more for those of 16 bits. States and
+    all sums are float32 and each output is rounded once. What steps are off by does not add up token by token: a state that its
+    inputs repeat stays itself within 2^-18, whatever the gate and the tokens' number. Infinities and NaN stay in their channel and
+    sequence; whether an infinite state or input gives infinities or NaN further on depends on where in a chunk it lies."""
     return _ops(True).recurrence(_tensor("x", x), _tensor("gate", gate), _tensor("starts", starts), initial)
 
 
