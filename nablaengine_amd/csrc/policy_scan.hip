@@ -9,12 +9,11 @@
 // where it is the larger (map_of, join), wherever a state leaves a stretch, a chunk or a call; inside a stretch the product
 // does. 65536 tokens from a state and with inputs of 1: every state 1 within 30 2^-24 at any gate (products throughout: 3.0e-3
 // off at a gate of 12; of chunks: 104 2^-24), and over 2^25 tokens within 23; the state's decay alone within 1.4e-6 of itself
-// from gates of 8 on. The packed tokens are cut into chunks, whatever sequences they hold,
-// so that work is even over ragged lengths; a sequence's first token cuts the chain (a choice, not a product with 0: what is
-// not finite stays in its sequence). A workgroup takes a chunk and 64 V channels: each of its waves reads TOK tokens at once
-// into registers, a lane V channels of each, finds its stretch's P and B, gets the state that enters it from the stretches
-// before (LDS) and from the chunks before (memory), and walks over its tokens once more. Sums and states are float32
-// throughout; each output is rounded once.
+// from gates of 8 on. The packed tokens are cut into chunks, whatever sequences they hold, so that work is even over ragged
+// lengths; a sequence's first token cuts the chain (a choice, not a product with 0: what is not finite stays in its sequence).
+// A workgroup takes a chunk and 64 V channels: each of its waves reads TOK tokens at once into registers, a lane V channels of
+// each, finds its stretch's P and B, gets the state that enters it from the stretches before (LDS) and from the chunks before
+// (memory), and walks over its tokens once more. Sums and states are float32 throughout; each output is rounded once.
 //
 // The chunks' P and B come from a kernel of their own, which reads only the tokens after a chunk's last sequence start (none
 // where the next chunk starts a sequence), and a third kernel carries states over the chunks: two reads of x and gate

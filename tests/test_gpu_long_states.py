@@ -100,9 +100,8 @@ def test_decay_and_its_gradients(n, gate):
 
 @pytest.mark.parametrize("gate", [8.0, 12.0, 17.0])
 def test_segments_carried_on_are_the_sequence(gate):
-    """A long sequence in segments of 37 tokens, each from the state of the one before: a constant stays, and the states are
-    the whole sequence's. Each segment adds the roundings of its own maps at most; those of 37 tokens' states that move by less than
-    their last place (1 - a below 2^-11 here) would add up without sight of the true value, U a token."""
+    """A long sequence in segments of 37 tokens, each from the state of the one before: a constant stays. Each segment adds the
+    roundings of its own maps at most."""
     print("segments", gate, flush=True)
     n, most = 37, 100
     value = torch.tensor([1.0, -0.7, 3.3], device="cuda")
